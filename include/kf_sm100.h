@@ -47,7 +47,9 @@ const char* kf_last_error(void);
  * device). 0 = no kernel has failed since the last reset; otherwise the code
  * of the first failure: 1-4 a bounded wait gave up (1 TMA producer, 2 MMA
  * issuer, 3 GEMM epilogue, 4 attention softmax), 5 an ordered attention
- * call got a batch_order entry outside [0, B). `reset` != 0 clears it. */
+ * call got a batch_order entry outside [0, B), 6 an 8-bit cache call found a
+ * length beyond its table or a page number outside its pool. `reset` != 0
+ * clears it. */
 int kf_device_status(int reset);
 
 /* The same status word copied into host_dst (pinned host memory, one int32)
@@ -334,6 +336,99 @@ int kf_flash_fwd_tf32_keep_noalloc(const float* q, int64_t q_sb, int64_t q_sh, i
                                    const uint8_t* keep, int64_t ld_keep, int64_t B, int64_t H,
                                    int64_t S, int dh, int dh_out, float sm_scale, int flags,
                                    void* stream);
+
+/* ----------------------------------------------------------- 8-bit key/value cache */
+
+#define KF_DT_F32 0  /* element types of q, k, v, out */
+#define KF_DT_BF16 1
+#define KF_DT_F16 2
+
+#define KF_KV8_INT8 0 /* codes are int8, scale = amax / 127 */
+#define KF_KV8_E4M3 1 /* codes are e4m3 floats, scale = amax / 448 */
+
+/* One layer's cache of B sequences. Tokens live in pages of `block` tokens;
+ * token t of sequence b is slot t % block of page table[b * ld_table + t / block].
+ * A pool holds `pages` pages of codes [kv_heads][block][head_dim] (contiguous,
+ * 16-byte aligned), their scales [kv_heads][2] (K, V; fp32) and, optionally,
+ * their attention-weight record [kv_heads][block] (fp32). A block of tokens
+ * and head is the unit that shares a scale. No reference counterpart (the
+ * reference recomputes the whole sequence, kernelforge/optimized.py:397-458).
+ * head_dim 16, 32, 64 or 128; block 16, 32, 64 or 128. All pointers are
+ * device pointers owned by the caller. A sequence's pages must not be shared
+ * with a sequence that is appended to. */
+typedef struct kf_kv8_cache {
+  void* k;
+  void* v;
+  float* scale;
+  float* weight; /* null: no record */
+  const int32_t* table;
+  const int32_t* lens; /* [batch] tokens held */
+  int64_t pages;
+  int64_t ld_table;
+  int32_t blocks; /* usable columns of the table */
+  int32_t batch;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t block;
+  int32_t format; /* KF_KV8_* */
+} kf_kv8_cache;
+
+/* Quantise new tokens into the cache: token t < counts[b] (counts null: T) of
+ * k and v [batch, kv_heads, T, head_dim] (strides in elements, unit stride on
+ * head_dim) goes to position lens[b] + t. Per page, head and K|V:
+ *     s = max(s_old, max|x| * fl(1/Qmax))   Qmax 127 or 448; s_old = 0 for a
+ *         page that holds no earlier token; NaN when an infinity or NaN comes
+ *         in; 0 when below 2^-126
+ *     code = rn(clamp(x * (1/s)));  earlier tokens of a page whose scale grew
+ *     are rescaled in place: rn(clamp(code * (s_old * (1/s))))
+ * The weight record of the new tokens is set to 0. lens is not changed. */
+int kf_kv8_append(const kf_kv8_cache* cache, const void* k, int64_t k_sb, int64_t k_sh,
+                  int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype,
+                  const int32_t* counts, int64_t T, void* stream);
+
+/* Read values back: k_out and v_out [batch, kv_heads, n, head_dim]
+ * (contiguous, 16-byte aligned) get code * s of positions start[b] + i (start
+ * null: 0) below lens[b] + counts[b] (counts null: 0), and 0 past them. */
+int kf_kv8_read(const kf_kv8_cache* cache, const int32_t* start, const int32_t* counts, int64_t n,
+                void* k_out, void* v_out, int dtype, void* stream);
+
+#define KF_KV8_CAUSAL 1 /* query i sees positions <= lens[b] + i */
+#define KF_KV8_TRACK 2  /* add each key's attention weight to cache->weight */
+
+/* Attention of the newest tokens over the cache that holds them: query i <
+ * counts[b] (counts null: T) of q [batch, q_heads, T, head_dim] stands at
+ * position lens[b] + i and sees positions below lens[b] + counts[b] (with
+ * KF_KV8_CAUSAL: up to its own). q_heads is a multiple of kv_heads; query
+ * head h reads kv head h / (q_heads / kv_heads).
+ *     out = softmax(sm_scale * q K^T) V,  lse = log of the softmax's sum
+ * Scores, sums, maxima and the accumulators are fp32. q and the weights enter
+ * the products as fp16 for 16-bit q, as two fp16 planes (22 bits) for fp32.
+ * out has q's type; rows without a visible key, and rows i >= counts[b], are 0
+ * (lse -inf). lse (may be null) is fp32 [batch, q_heads, T]. With KF_KV8_TRACK
+ * cache->weight[key] += the key's weight summed over the queries and the query
+ * heads of its kv head, in a fixed order. max_len: an upper bound of lens[b] +
+ * counts[b] known to the caller (0: the table's reach); longer sequences are
+ * cut there and recorded in the device status. `workspace`: at least
+ * kf_kv8_attention_workspace_bytes of the same arguments, 256-byte aligned;
+ * calls that overlap on the GPU must not share it. */
+int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_t q_sb, int64_t q_sh,
+                     int64_t q_st, void* out, int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype,
+                     const int32_t* counts, int64_t T, int64_t q_heads, int64_t max_len,
+                     float sm_scale, int flags, float* lse, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+int64_t kf_kv8_attention_workspace_bytes(const kf_kv8_cache* cache, int dtype, int64_t T,
+                                         int64_t q_heads, int64_t max_len, int flags);
+
+/* Cut every sequence to n = min(lens[b], budget) tokens, per kv head: the last
+ * min(recent, lens[b]) tokens and, of the others, those of the largest weight
+ * (ties: the lowest position; NaN counts as the largest), in their order. They
+ * are requantised by blocks (s' = max|code * s| * fl(1/Qmax)) into the pages
+ * of table_out [batch, ld_out] (ceil(budget / block) columns; pages of the
+ * same pool that no sequence of `cache` uses), their weights moved along;
+ * lens_out[b] = n. kept (may not be null) is int32 [batch, kv_heads, budget]:
+ * the kept positions in order, then -1. 0 <= recent <= budget, budget > 0. */
+int kf_kv8_evict(const kf_kv8_cache* cache, const int32_t* table_out, int64_t ld_out,
+                 int64_t budget, int64_t recent, int32_t* kept, int32_t* lens_out, void* stream);
 
 /* ----------------------------------------------------------- utilities */
 

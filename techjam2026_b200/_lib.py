@@ -18,6 +18,18 @@ _c_int = ctypes.c_int
 _c_float = ctypes.c_float
 _c_ptr = ctypes.c_void_p
 
+
+class KV8CacheStruct(ctypes.Structure):
+    """kf_kv8_cache of include/kf_sm100.h."""
+    _fields_ = [("k", _c_ptr), ("v", _c_ptr), ("scale", _c_ptr), ("weight", _c_ptr),
+                ("table", _c_ptr), ("lens", _c_ptr), ("pages", _c_i64), ("ld_table", _c_i64),
+                ("blocks", ctypes.c_int32), ("batch", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("block", ctypes.c_int32), ("format", ctypes.c_int32)]
+
+
+_c_cache = ctypes.POINTER(KV8CacheStruct)
+
 # name -> (restype, argtypes); must mirror include/kf_sm100.h exactly.
 SIGNATURES = {
     "kf_version": (_c_int, []),
@@ -74,6 +86,15 @@ SIGNATURES = {
                                                 _c_ptr, _c_i64, _c_i64, _c_i64,
                                                 _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64,
                                                 _c_int, _c_int, _c_float, _c_int, _c_ptr]),
+    "kf_kv8_append": (_c_int, [_c_cache, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64,
+                               _c_i64, _c_int, _c_ptr, _c_i64, _c_ptr]),
+    "kf_kv8_read": (_c_int, [_c_cache, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_int, _c_ptr]),
+    "kf_kv8_attention": (_c_int, [_c_cache, _c_ptr, _c_i64, _c_i64, _c_i64,
+                                  _c_ptr, _c_i64, _c_i64, _c_i64, _c_int, _c_ptr, _c_i64, _c_i64,
+                                  _c_i64, _c_float, _c_int, _c_ptr, _c_ptr, _c_i64, _c_ptr]),
+    "kf_kv8_attention_workspace_bytes": (_c_i64, [_c_cache, _c_int, _c_i64, _c_i64, _c_i64,
+                                                  _c_int]),
+    "kf_kv8_evict": (_c_int, [_c_cache, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr]),
 }
 
 # C-ABI constants (include/kf_sm100.h)
@@ -105,6 +126,13 @@ KF_GEMM_OUT_BF16X2 = 8
 KF_GEMM_PAIR = 32
 KF_GEMM_W_STATIC = 64
 KF_NOALLOC_KEEP_WORDS_MAX = 262144
+KF_DT_F32 = 0
+KF_DT_BF16 = 1
+KF_DT_F16 = 2
+KF_KV8_INT8 = 0
+KF_KV8_E4M3 = 1
+KF_KV8_CAUSAL = 1
+KF_KV8_TRACK = 2
 
 _lib = None
 _lock = threading.Lock()

@@ -40,6 +40,7 @@ enum : int {
   KF_DEV_WAIT_TIMEOUT_EPI = 3,
   KF_DEV_WAIT_TIMEOUT_SOFTMAX = 4,
   KF_DEV_BAD_BATCH_ORDER = 5,  // a batch_order entry outside [0, B)
+  KF_DEV_BAD_KV_PAGE = 6,      // a cache length or page number outside its table or pool
 };
 
 // Time limit of every bounded wait on work (mbarrier phases, the producer's

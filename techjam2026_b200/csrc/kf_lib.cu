@@ -6,3 +6,5 @@
 #include "flash_sm100.cu"
 #include "flash_persist_sm100.cu"
 #include "noalloc_sm100.cu"
+#include "kv8_cache_sm100.cu"
+#include "kv8_attn_sm100.cu"

@@ -1,0 +1,779 @@
+// Attention of a few query rows over the 8-bit cache (single tokens, short
+// chunks), split along the keys, and the kernels that join the parts.
+//
+// What bounds it: the codes. A token of a kv head is 2 * D bytes and serves
+// only the G = q_heads / kv_heads query rows of its group, so the arithmetic
+// per byte is small and the kernel is a stream over K and V.
+//
+// One CTA = one chunk of keys of one (sequence, kv head) for a tile of 16 query
+// rows (row = token * G + head of the group). Its four warps take the chunk's
+// groups of 16 keys in turn, each with its own running reference and sums,
+// joined in shared memory at the end. Codes go from global memory straight to
+// the registers of the lane that feeds them to the tensor core: a contraction
+// may order its terms freely, so the lane that holds k-slots {2t, 2t+1, 2t+8,
+// 2t+9} of mma.m16n8k16 simply owns the consecutive bytes of a K row (the
+// same ones of q), and consecutive bytes of four V rows, and no shared memory
+// or shuffle sits between the load and the product. 16 rows fill the m16
+// tile; the 128-row tensor-memory products would waste 7/8 of theirs here.
+//
+// Numbers. Codes are exact in fp16. A q row is scaled by a power of two to
+// [2^14, 2^15) before it becomes one fp16 plane (16-bit q: nothing is lost
+// until 2^-28 of the row's largest) or two (fp32 q: 22 bits). P is relative to
+// a reference 2^9 below the running maximum, so it uses fp16 up to 2^15 and
+// loses precision only below 2^-23 of the largest weight; for fp32 output it
+// is two planes as well. The V scale of a page is folded into P as the ratio
+// to the chunk's largest (<= 1, so P stays in range). The sum l adds the
+// unrounded fp32 weights.
+#include "kv8_common.cuh"
+
+namespace kf {
+
+constexpr int KV8_ROWS = 16;            // query rows of a CTA
+constexpr int KV8_CHUNK_MAX = 4096;     // keys of a CTA: at most 256 pages of 16
+constexpr float KV8_BIAS = 9.f;         // log2 of P's largest value after a rescale
+constexpr float KV8_SLACK = 6.f;        // growth of the maximum that needs no rescale
+
+// Layout of the workspace: per (sequence, kv head, padded row, chunk) the
+// reference and the sum, then the partial outputs, then (track) the scores.
+struct KV8Work {
+  float* ref;     // [B*H][rows][chunks]
+  float* sum;     // [B*H][rows][chunks]
+  float* part;    // [B*H][rows][chunks][D]
+  float* lse;     // [B*H][rows]: log2 of the softmax's sum
+  float* score;   // [B*H][rows][ld_score] (rows <= 16 and track), in log2 units
+  int64_t ld_score;
+  int rows;       // T * G
+  int chunks;
+  int chunk;      // keys of a chunk
+};
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+  if constexpr (BYTES == 16) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x; w[1] = v.y;
+  } else if constexpr (BYTES == 4) {
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  } else {
+    w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The rest of a and b after pack_half2, as a second fp16 plane.
+__device__ __forceinline__ uint32_t pack_half2_rest(float a, float b, uint32_t hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return pack_half2(a - f.x, b - f.y);
+}
+
+// Power of two that brings a row whose largest magnitude is `amax` to
+// [2^14, 2^15), as a biased exponent pattern; 1 for a row of zeros or one that
+// holds an infinity or a NaN.
+__device__ __forceinline__ float kv8_row_scale(float amax, float* inverse) {
+  const uint32_t ex = __float_as_uint(amax) >> 23;
+  if (amax == 0.f || ex == 255u) {
+    *inverse = 1.f;
+    return 1.f;
+  }
+  const int e = min(max(268 - static_cast<int>(ex), 1), 253);
+  *inverse = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+  return __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+
+// The q fragments of 16 rows: lane (g, t) holds rows g and g + 8, the K bytes
+// it owns (see above). qf[r]: factor from the products to log2 units.
+template <int DH, int PL>
+struct QFrag {
+  static constexpr int EPT = DH / 4 < 16 ? DH / 4 : 16;  // consecutive elements of a piece
+  static constexpr int NPC = DH / 4 / EPT;               // pieces (64 elements apart)
+  static constexpr int KS = DH / 16;                     // k-steps
+  uint32_t a[PL][KS][4];
+  float qf[2];
+
+  __device__ __forceinline__ void load(const KV8& c, const void* q, int64_t q_sb, int64_t q_sh,
+                                       int64_t q_st, int dtype, bool vec, int b, int h, int G,
+                                       int row0, int rows, float scale_log2) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = row0 + g + 8 * r;
+      float x[NPC * EPT];
+      float amax = 0.f;
+      if (row < rows) {
+        const int tok = row / G;
+        const int64_t base = b * q_sb + static_cast<int64_t>(h * G + row - tok * G) * q_sh +
+                             tok * q_st;
+#pragma unroll
+        for (int p = 0; p < NPC; ++p)
+#pragma unroll
+          for (int e = 0; e < EPT; e += 4) {
+            float y[4];
+            kv8_load4(q, base + p * 64 + t * EPT + e, dtype, vec, y);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[p * EPT + e + u] = y[u];
+          }
+      } else {
+#pragma unroll
+        for (int e = 0; e < NPC * EPT; ++e) x[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < NPC * EPT; ++e)
+        amax = __uint_as_float(max(__float_as_uint(amax), __float_as_uint(fabsf(x[e]))));
+#pragma unroll
+      for (int d = 1; d <= 2; d <<= 1)
+        amax = __uint_as_float(
+            max(__float_as_uint(amax), __shfl_xor_sync(0xffffffffu, __float_as_uint(amax), d)));
+      float inv;
+      const float sc = kv8_row_scale(amax, &inv);
+      qf[r] = inv * scale_log2;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        float y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) y[u] = x[4 * s + u] * sc;
+        a[0][s][r] = pack_half2(y[0], y[1]);
+        a[0][s][2 + r] = pack_half2(y[2], y[3]);
+        if constexpr (PL == 2) {
+          a[1][s][r] = pack_half2_rest(y[0], y[1], a[0][s][r]);
+          a[1][s][2 + r] = pack_half2_rest(y[2], y[3], a[0][s][2 + r]);
+        }
+      }
+    }
+  }
+};
+
+// Codes of K for 16 keys as one lane owns them: two n8 tiles of keys.
+template <int DH>
+struct KBytes {
+  static constexpr int EPT = DH / 4 < 16 ? DH / 4 : 16;
+  static constexpr int NPC = DH / 4 / EPT;
+  uint32_t w[2][DH / 16];
+  __device__ __forceinline__ void load(const uint8_t* base) {  // base: the group's first row
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int p = 0; p < NPC; ++p)
+        load_bytes<EPT>(base + (8 * n + g) * DH + p * 64 + t * EPT, &w[n][p * (EPT / 4)]);
+  }
+};
+template <int DH>
+struct VBytes {
+  static constexpr int VB = DH / 8;            // consecutive bytes of a row
+  static constexpr int W = VB < 4 ? 1 : VB / 4;
+  uint32_t w[4][W];                            // keys 2t, 2t+1, 8+2t, 9+2t
+  __device__ __forceinline__ void load(const uint8_t* base) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      load_bytes<VB>(base + ((i >> 1) * 8 + 2 * t + (i & 1)) * DH + g * VB, w[i]);
+  }
+};
+
+// Products of 16 q rows with 16 keys: d[n][.] in the m16n8 accumulator layout.
+template <int DH, int FMT, int PL>
+__device__ __forceinline__ void score_tile(const QFrag<DH, PL>& q, const KBytes<DH>& kb,
+                                           float (&d)[2][4]) {
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+#pragma unroll
+    for (int s = 0; s < DH / 16; ++s) {
+      uint32_t b0, b1;
+      kv8_cvt4<FMT>(kb.w[n][s], b0, b1);
+      if constexpr (PL == 2)
+        mma_f16_16816(d[n], q.a[1][s][0], q.a[1][s][1], q.a[1][s][2], q.a[1][s][3], b0, b1);
+      mma_f16_16816(d[n], q.a[0][s][0], q.a[0][s][1], q.a[0][s][2], q.a[0][s][3], b0, b1);
+    }
+  }
+}
+
+template <int DH, int FMT, int PL>
+__global__ void __launch_bounds__(128)
+    kv8_split_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+                     void* __restrict__ out, int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype,
+                     int vec, const int32_t* __restrict__ counts, int T, int G, int max_len,
+                     float scale_log2, int flags, float* __restrict__ lse_out, KV8Work w) {
+  constexpr int NT = DH / 8;  // n8 tiles of the output
+  __shared__ int s_page[KV8_CHUNK_MAX / 16];
+  __shared__ float s_ks[KV8_CHUNK_MAX / 16];
+  __shared__ float s_vs[KV8_CHUNK_MAX / 16];
+  __shared__ float s_vmax[4];
+  __shared__ float s_o[4][KV8_ROWS][DH];
+  __shared__ float s_ref[4][KV8_ROWS], s_sum[4][KV8_ROWS];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int chunk = blockIdx.x;
+  const int row0 = blockIdx.y * KV8_ROWS;
+  const int bh = blockIdx.z;
+  const int b = bh / c.H, h = bh - b * c.H;
+  const int len = kv8_len(c, b);
+  const int count = kv8_count(counts, b, T);
+  int end = kv8_end(c, len, count);
+  if (end > max_len) {
+    if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
+    end = max_len;
+  }
+  const bool causal = (flags & KF_KV8_CAUSAL) != 0;
+  // Last key that any row of this tile sees, and the rows' own limits.
+  int limit[2];
+  int reach = 0;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = row0 + g + 8 * r;
+    const int tok = row / G;
+    limit[r] = (row < w.rows && tok < count) ? (causal ? min(len + tok + 1, end) : end) : 0;
+  }
+  {
+    const int last_row = min(row0 + KV8_ROWS, w.rows) - 1;
+    const int last_tok = min(last_row / G, count - 1);
+    reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
+  }
+  const int k0 = chunk * w.chunk;
+  const int k1 = min(k0 + w.chunk, reach);
+  const bool alone = w.chunks == 1;
+  if (k0 >= k1 && !alone) {
+    // nothing here: the join reads this chunk's sums all the same
+    for (int r = tid; r < KV8_ROWS; r += 128)
+      if (row0 + r < w.rows) {
+        const int64_t at = (static_cast<int64_t>(bh) * w.rows + row0 + r) * w.chunks + chunk;
+        w.ref[at] = -INFINITY;
+        w.sum[at] = 0.f;
+      }
+    return;
+  }
+  const int j0 = k0 >> c.p_shift;
+  float vmax = 0.f;
+  for (int j = j0 + tid; (j << c.p_shift) < k1; j += 128) {
+    const int page = kv8_page(c, b, j);
+    s_page[j - j0] = page;
+    float2 s = make_float2(0.f, 0.f);
+    if (page >= 0) s = *reinterpret_cast<const float2*>(c.scale + 2 * (static_cast<int64_t>(page) * c.H + h));
+    s_ks[j - j0] = s.x;
+    s_vs[j - j0] = s.y;
+    vmax = fmaxf(vmax, s.y);
+  }
+  QFrag<DH, PL> qa;
+  qa.load(c, q, q_sb, q_sh, q_st, dtype, vec != 0, b, h, G, row0, w.rows, scale_log2);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
+  if (lane == 0) s_vmax[warp] = vmax;
+  __syncthreads();
+  vmax = fmaxf(fmaxf(s_vmax[0], s_vmax[1]), fmaxf(s_vmax[2], s_vmax[3]));
+  const float inv_vmax = vmax > 0.f ? 1.f / vmax : 0.f;
+
+  float o[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+
+  const int page_bytes = c.P * DH;
+  auto group_at = [&](int key) -> int64_t {  // byte offset of a group of 16 keys
+    const int page = s_page[(key >> c.p_shift) - j0];
+    return (static_cast<int64_t>(page < 0 ? 0 : page) * c.H + h) * page_bytes +
+           (key & (c.P - 1)) * DH;
+  };
+  KBytes<DH> kb;
+  VBytes<DH> vb;
+  int key = k0 + 16 * warp;
+  if (key < k1) {
+    const int64_t at = group_at(key);
+    kb.load(c.k + at);
+    vb.load(c.v + at);
+  }
+  for (; key < k1; key += 64) {
+    KBytes<DH> kn;
+    VBytes<DH> vn;
+    const bool more = key + 64 < k1;
+    if (more) {
+      const int64_t at = group_at(key + 64);
+      kn.load(c.k + at);
+      vn.load(c.v + at);
+    }
+    const int pj = (key >> c.p_shift) - j0;
+    const float ks = s_page[pj] < 0 ? 0.f : s_ks[pj];
+    const float ratio = s_vs[pj] * inv_vmax;
+    const int bad = s_page[pj] < 0 ? 0 : 0x7fffffff;  // a refused page has no visible key
+
+    float f[2][4];
+    score_tile<DH, FMT, PL>(qa, kb, f);
+    float top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int kk = key + 8 * n + 2 * t + (e & 1);
+        const float x = f[n][e] * (qa.qf[e >> 1] * ks);
+        f[n][e] = kk < min(limit[e >> 1], bad) ? x : -INFINITY;
+      }
+    if (w.score) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        if (row0 + g + 8 * r < w.rows) {
+          float* sp = w.score + (static_cast<int64_t>(bh) * w.rows + row0 + g + 8 * r) * w.ld_score +
+                      key + 2 * t;
+          *reinterpret_cast<float2*>(sp) = make_float2(f[0][2 * r], f[0][2 * r + 1]);
+          *reinterpret_cast<float2*>(sp + 8) = make_float2(f[1][2 * r], f[1][2 * r + 1]);
+        }
+    }
+    // A row's reference moves only when its maximum has outgrown it by more
+    // than the slack; all lanes of the warp look at once.
+    float m2[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      m2[r] = fmaxf(fmaxf(f[0][2 * r], f[0][2 * r + 1]), fmaxf(f[1][2 * r], f[1][2 * r + 1]));
+      top = fmaxf(top, m2[r] - (ref[r] == -INFINITY ? 0.f : ref[r]) >
+                               (ref[r] == -INFINITY ? -INFINITY : KV8_BIAS + KV8_SLACK)
+                           ? 1.f
+                           : -INFINITY);
+    }
+    if (__any_sync(0xffffffffu, top > 0.f)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float m = m2[r];
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        if (m - KV8_BIAS > ref[r]) {
+          const float old = ref[r];
+          ref[r] = m - KV8_BIAS;
+          const float alpha = old == -INFINITY ? 0.f : fast_exp2(old - ref[r]);
+          if (old != -INFINITY) {
+            sum[r] *= alpha;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              o[n][2 * r] *= alpha;
+              o[n][2 * r + 1] *= alpha;
+            }
+          }
+        }
+      }
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float neg = ref[r] == -INFINITY ? 0.f : -ref[r];
+        float p[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float x = f[n][2 * r + u];
+          const float e = fast_exp2(x + neg);
+          sum[r] += e;
+          p[u] = x == -INFINITY ? 0.f : e * ratio;
+        }
+        hi[2 * n + r] = pack_half2(p[0], p[1]);
+        if constexpr (PL == 2) lo[2 * n + r] = pack_half2_rest(p[0], p[1], hi[2 * n + r]);
+      }
+    // Slots past the end hold whatever was there (an e4m3 NaN among it): as
+    // zeros they cannot reach the product.
+    if (key + 16 > end) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (key + (i >> 1) * 8 + 2 * t + (i & 1) >= end) {
+#pragma unroll
+          for (int u = 0; u < VBytes<DH>::W; ++u) vb.w[i][u] = 0u;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < VBytes<DH>::W; ++u) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (4 * u + 2 * half >= NT) continue;
+        const uint32_t sel = half ? 0x7362 : 0x5140;
+        uint32_t b00, b01, b10, b11;
+        kv8_cvt4<FMT>(__byte_perm(vb.w[0][u], vb.w[1][u], sel), b00, b01);
+        kv8_cvt4<FMT>(__byte_perm(vb.w[2][u], vb.w[3][u], sel), b10, b11);
+        const int n = 4 * u + 2 * half;
+        if constexpr (PL == 2) {
+          mma_f16_16816(o[n], lo[0], lo[1], lo[2], lo[3], b00, b10);
+          mma_f16_16816(o[n + 1], lo[0], lo[1], lo[2], lo[3], b01, b11);
+        }
+        mma_f16_16816(o[n], hi[0], hi[1], hi[2], hi[3], b00, b10);
+        mma_f16_16816(o[n + 1], hi[0], hi[1], hi[2], hi[3], b01, b11);
+      }
+    }
+    if (more) {
+      kb = kn;
+      vb = vn;
+    }
+  }
+
+  // Join the four warps. Column of accumulator (n, e): (2t + (e & 1)) * NT + n.
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float l = sum[r];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t == 0) {
+      s_ref[warp][g + 8 * r] = ref[r];
+      s_sum[warp][g + 8 * r] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      s_o[warp][g + 8 * r][(2 * t) * NT + n] = o[n][2 * r];
+      s_o[warp][g + 8 * r][(2 * t + 1) * NT + n] = o[n][2 * r + 1];
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < KV8_ROWS * DH; i += 128) {
+    const int r = i / DH, d = i - r * DH;
+    const int row = row0 + r;
+    if (row >= w.rows) break;
+    float top = s_ref[0][r];
+#pragma unroll
+    for (int u = 1; u < 4; ++u) top = fmaxf(top, s_ref[u][r]);
+    float l = 0.f, x = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float a = top == -INFINITY ? 1.f : fast_exp2(s_ref[u][r] - top);
+      l += a * s_sum[u][r];
+      x += a * s_o[u][r][d];
+    }
+    x *= vmax;
+    const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
+    if (alone) {
+      const int tok = row / G;
+      const int hq = h * G + row - tok * G;
+      kv8_store1(out, b * o_sb + hq * o_sh + tok * o_st + d, dtype, l == 0.f ? 0.f : x / l);
+      if (d == 0) {
+        const float l2 = l == 0.f ? -INFINITY : top + log2f(l);
+        if (lse_out)
+          lse_out[(static_cast<int64_t>(b) * c.H * G + hq) * T + tok] = l2 * 0.6931471805599453f;
+        if (w.lse) w.lse[at] = l2;
+      }
+    } else {
+      w.part[(at * w.chunks + chunk) * DH + d] = x;
+      if (d == 0) {
+        w.ref[at * w.chunks + chunk] = top;
+        w.sum[at * w.chunks + chunk] = l;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- join
+
+// One CTA per query row: the chunks' parts in chunk order.
+__global__ void __launch_bounds__(128)
+    kv8_join_kernel(KV8 c, void* __restrict__ out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+                    int dtype, int T, int G, float* __restrict__ lse_out, KV8Work w) {
+  __shared__ float s_x[128], s_l[4];
+  __shared__ float s_m[4];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.x;
+  const int bh = blockIdx.y;
+  const int b = bh / c.H, h = bh - b * c.H;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t at = (static_cast<int64_t>(bh) * w.rows + row) * w.chunks;
+  float top = -INFINITY;
+  for (int i = tid; i < w.chunks; i += 128) top = fmaxf(top, w.ref[at + i]);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (lane == 0) s_m[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  float l = 0.f;
+  for (int i = tid; i < w.chunks; i += 128)
+    l += (top == -INFINITY ? 1.f : fast_exp2(w.ref[at + i] - top)) * w.sum[at + i];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (lane == 0) s_l[warp] = l;
+  const int parts = 128 / c.D, d = tid & (c.D - 1), part = tid / c.D;
+  float x = 0.f;
+  for (int i = part; i < w.chunks; i += parts) {
+    const float r = w.ref[at + i];
+    // an empty chunk wrote no part (its sum is 0; a NaN sum has a part)
+    if (r == -INFINITY && w.sum[at + i] == 0.f) continue;
+    x += (top == -INFINITY ? 1.f : fast_exp2(r - top)) * w.part[(at + i) * c.D + d];
+  }
+  s_x[tid] = x;
+  __syncthreads();
+  if (part == 0) {
+    for (int u = 1; u < parts; ++u) x += s_x[u * c.D + d];
+    l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    const int tok = row / G;
+    const int hq = h * G + row - tok * G;
+    kv8_store1(out, b * o_sb + hq * o_sh + tok * o_st + d, dtype, l == 0.f ? 0.f : x / l);
+    if (d == 0) {
+      const float l2 = l == 0.f ? -INFINITY : top + log2f(l);
+      if (lse_out)
+        lse_out[(static_cast<int64_t>(b) * c.H * G + hq) * T + tok] = l2 * 0.6931471805599453f;
+      if (w.lse) w.lse[static_cast<int64_t>(bh) * w.rows + row] = l2;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- weights
+
+// Adds each key's weight to the record, from the scores the split kernel left
+// (at most 16 rows). One thread per key; the rows are added in order.
+__global__ void __launch_bounds__(256)
+    kv8_weights_kernel(KV8 c, const int32_t* __restrict__ counts, int T, int G, int max_len,
+                       int flags, KV8Work w) {
+  __shared__ float s_lse[KV8_ROWS];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int bh = blockIdx.y;
+  const int b = bh / c.H, h = bh - b * c.H;
+  if (threadIdx.x < w.rows) s_lse[threadIdx.x] = w.lse[static_cast<int64_t>(bh) * w.rows + threadIdx.x];
+  __syncthreads();
+  const int len = kv8_len(c, b);
+  const int count = kv8_count(counts, b, T);
+  const int end = min(kv8_end(c, len, count), max_len);
+  const int key = blockIdx.x * 256 + threadIdx.x;
+  if (key >= end) return;
+  const int page = kv8_page(c, b, key >> c.p_shift);
+  if (page < 0) return;
+  float x = 0.f;
+  for (int r = 0; r < w.rows; ++r) {
+    const int tok = r / G;
+    if (tok >= count || ((flags & KF_KV8_CAUSAL) && key > len + tok)) continue;
+    const float l = s_lse[r];
+    if (l == -INFINITY) continue;
+    x += fast_exp2(w.score[(static_cast<int64_t>(bh) * w.rows + r) * w.ld_score + key] - l);
+  }
+  float* at = c.weight + (static_cast<int64_t>(page) * c.H + h) * c.P + (key & (c.P - 1));
+  *at += x;
+}
+
+// The same for more rows: the scores are computed again. One CTA per 64 keys;
+// a warp takes 16 of them against all rows, 16 at a time.
+template <int DH, int FMT, int PL>
+__global__ void __launch_bounds__(128)
+    kv8_reweigh_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh,
+                       int64_t q_st, int dtype, int vec, const int32_t* __restrict__ counts,
+                       int T, int G, int max_len, float scale_log2, int flags, KV8Work w) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int bh = blockIdx.y;
+  const int b = bh / c.H, h = bh - b * c.H;
+  const int len = kv8_len(c, b);
+  const int count = kv8_count(counts, b, T);
+  const int end = min(kv8_end(c, len, count), max_len);
+  const int key = blockIdx.x * 64 + warp * 16;
+  if (key >= end) return;
+  const int page = kv8_page(c, b, key >> c.p_shift);
+  if (page < 0) return;
+  const int64_t block = static_cast<int64_t>(page) * c.H + h;
+  const float ks = c.scale[2 * block];
+  KBytes<DH> kb;
+  kb.load(c.k + block * c.P * DH + (key & (c.P - 1)) * DH);
+  const bool causal = (flags & KF_KV8_CAUSAL) != 0;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};  // keys 2t, 2t+1, 8+2t, 9+2t
+  // the first row that sees the group's first key
+  const int first = causal && key > len ? (key - len) * G : 0;
+  const int rows = min(w.rows, count * G);
+  for (int row0 = first & ~(KV8_ROWS - 1); row0 < rows; row0 += KV8_ROWS) {
+    QFrag<DH, PL> qa;
+    qa.load(c, q, q_sb, q_sh, q_st, dtype, vec != 0, b, h, G, row0, rows, scale_log2);
+    float f[2][4];
+    score_tile<DH, FMT, PL>(qa, kb, f);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = row0 + g + 8 * r;
+      if (row >= rows) continue;
+      const float l = w.lse[static_cast<int64_t>(bh) * w.rows + row];
+      const int limit = causal ? min(len + row / G + 1, end) : end;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = f[i >> 1][2 * r + (i & 1)] * (qa.qf[r] * ks);
+        if (key + (i >> 1) * 8 + 2 * t + (i & 1) < limit && l != -INFINITY)
+          x[i] += fast_exp2(y - l);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int d = 4; d <= 16; d <<= 1) x[i] += __shfl_xor_sync(0xffffffffu, x[i], d);
+    const int kk = key + (i >> 1) * 8 + 2 * t + (i & 1);
+    if (g == 0 && kk < end) c.weight[block * c.P + (kk & (c.P - 1))] += x[i];
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+// How a call is cut: chunks of keys so that there are a few CTAs per SM, each
+// with work enough to pay for its start.
+static void kv8_plan(const KV8& c, int64_t T, int G, int64_t max_len, int flags, KV8Work* w) {
+  const int64_t rows = T * G;
+  const int64_t tiles = (rows + KV8_ROWS - 1) / KV8_ROWS;
+  const int64_t items = tiles * c.B * c.H;
+  const int64_t want = 148 * 8;
+  int64_t chunks = (want + items - 1) / items;
+  const int64_t most = (max_len + 127) / 128;    // at least 128 keys a chunk
+  if (chunks > most) chunks = most;
+  const int64_t least = (max_len + KV8_CHUNK_MAX - 1) / KV8_CHUNK_MAX;
+  if (chunks < least) chunks = least;
+  if (chunks < 1) chunks = 1;
+  int64_t chunk = (max_len + chunks - 1) / chunks;
+  chunk = (chunk + 127) / 128 * 128;             // whole pages, whatever the page
+  if (chunk < 128) chunk = 128;
+  w->chunk = static_cast<int>(chunk);
+  w->chunks = static_cast<int>((max_len + chunk - 1) / chunk);
+  if (w->chunks < 1) w->chunks = 1;
+  w->rows = static_cast<int>(rows);
+  w->ld_score = (flags & KF_KV8_TRACK) && rows <= KV8_ROWS ? (max_len + 15) / 16 * 16 : 0;
+}
+
+// Splits the workspace; returns the bytes it takes.
+static int64_t kv8_carve(const KV8& c, int flags, uint8_t* base, KV8Work* w) {
+  int64_t at = 0;
+  auto take = [&](int64_t floats) -> float* {
+    float* p = reinterpret_cast<float*>(base + at);
+    at += (floats * 4 + 255) / 256 * 256;
+    return p;
+  };
+  const int64_t n = static_cast<int64_t>(c.B) * c.H * w->rows;
+  w->ref = w->sum = w->part = w->lse = w->score = nullptr;
+  if (w->chunks > 1) {
+    w->ref = take(n * w->chunks);
+    w->sum = take(n * w->chunks);
+    w->part = take(n * w->chunks * c.D);
+  }
+  if (flags & KF_KV8_TRACK) w->lse = take(n);
+  if (w->ld_score) w->score = take(n * w->ld_score);
+  return at;
+}
+
+static int kv8_attention_check(const char* what, const kf_kv8_cache* cache, int dtype, int64_t T,
+                               int64_t q_heads, int64_t* max_len, int flags, KV8* c) {
+  int rc = kv8_view(what, cache, c);
+  if (!rc) rc = kv8_dtype(what, dtype);
+  if (rc) return rc;
+  if (T < 0 || q_heads <= 0 || q_heads % c->H || (flags & ~(KF_KV8_CAUSAL | KF_KV8_TRACK)) ||
+      *max_len < 0) {
+    set_last_error("%s: needs T >= 0, q_heads a multiple of kv_heads and known flags", what);
+    return KF_E_INVALID;
+  }
+  if ((flags & KF_KV8_TRACK) && !c->weight) {
+    set_last_error("%s: KF_KV8_TRACK needs a cache with a weight record", what);
+    return KF_E_INVALID;
+  }
+  const int64_t reach = static_cast<int64_t>(c->blocks) * c->P;
+  if (*max_len == 0 || *max_len > reach) *max_len = reach;
+  if (static_cast<int64_t>(c->B) * c->H > 65535 || T * (q_heads / c->H) > 65535LL * KV8_ROWS) {
+    set_last_error("%s: needs batch * kv_heads <= 65535 and at most 2^20 query rows a kv head",
+                   what);
+    return KF_E_UNSUPPORTED;
+  }
+  return KF_OK;
+}
+
+}  // namespace kf
+
+using namespace kf;
+
+extern "C" int64_t kf_kv8_attention_workspace_bytes(const kf_kv8_cache* cache, int dtype,
+                                                    int64_t T, int64_t q_heads, int64_t max_len,
+                                                    int flags) {
+  KV8 c;
+  if (kv8_attention_check("kf_kv8_attention_workspace_bytes", cache, dtype, T, q_heads, &max_len,
+                          flags, &c))
+    return -1;
+  KV8Work w;
+  kv8_plan(c, T, static_cast<int>(q_heads / c.H), max_len, flags, &w);
+  return kv8_carve(c, flags, nullptr, &w);
+}
+
+extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_t q_sb,
+                                int64_t q_sh, int64_t q_st, void* out, int64_t o_sb, int64_t o_sh,
+                                int64_t o_st, int dtype, const int32_t* counts, int64_t T,
+                                int64_t q_heads, int64_t max_len, float sm_scale, int flags,
+                                float* lse, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
+  KV8 c;
+  int rc = kv8_attention_check("kf_kv8_attention", cache, dtype, T, q_heads, &max_len, flags, &c);
+  if (rc) return rc;
+  if (!q || !out) {
+    set_last_error("kf_kv8_attention: q and out must not be null");
+    return KF_E_INVALID;
+  }
+  if (T == 0 || c.B == 0) return KF_OK;
+  const int G = static_cast<int>(q_heads / c.H);
+  KV8Work w;
+  kv8_plan(c, T, G, max_len, flags, &w);
+  const int64_t need = kv8_carve(c, flags, static_cast<uint8_t*>(workspace), &w);
+  if (need > 0 && (!workspace || workspace_bytes < need || !kv8_aligned(workspace, 256))) {
+    set_last_error("kf_kv8_attention: needs a 256-byte aligned workspace of %lld bytes",
+                   (long long)need);
+    return KF_E_INVALID;
+  }
+  const int64_t es = dtype_size(dtype);
+  const int vec = kv8_aligned(q, 4 * es) && q_sb % 4 == 0 && q_sh % 4 == 0 && q_st % 4 == 0;
+  const float scale_log2 = sm_scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int Ti = static_cast<int>(T), cap = static_cast<int>(max_len);
+  const unsigned bh = static_cast<unsigned>(c.B * c.H);
+  const dim3 grid(static_cast<unsigned>(w.chunks),
+                  static_cast<unsigned>((w.rows + KV8_ROWS - 1) / KV8_ROWS), bh);
+  const bool reweigh = (flags & KF_KV8_TRACK) && !w.score;
+  cudaError_t e = cudaSuccess, e2 = cudaSuccess;
+#define KF_KV8_SPLIT(DH, FMT, PL)                                                               \
+  e = launch_chained(kv8_split_kernel<DH, FMT, PL>, grid, dim3(128), 0, st, c, q, q_sb, q_sh,   \
+                     q_st, out, o_sb, o_sh, o_st, dtype, vec, counts, Ti, G, cap, scale_log2,   \
+                     flags, lse, w)
+#define KF_KV8_REWEIGH(DH, FMT, PL)                                                             \
+  e2 = launch_chained(kv8_reweigh_kernel<DH, FMT, PL>,                                          \
+                      dim3(static_cast<unsigned>((max_len + 63) / 64), bh), dim3(128), 0, st, c, \
+                      q, q_sb, q_sh, q_st, dtype, vec, counts, Ti, G, cap, scale_log2, flags, w)
+#define KF_KV8_PICK(WHAT, DH)                        \
+  do {                                               \
+    const bool i8 = c.fmt == KF_KV8_INT8;            \
+    const bool two = dtype == KF_DT_F32;             \
+    if (i8 && two)                                   \
+      WHAT(DH, KF_KV8_INT8, 2);                      \
+    else if (i8)                                     \
+      WHAT(DH, KF_KV8_INT8, 1);                      \
+    else if (two)                                    \
+      WHAT(DH, KF_KV8_E4M3, 2);                      \
+    else                                             \
+      WHAT(DH, KF_KV8_E4M3, 1);                      \
+  } while (0)
+#define KF_KV8_PICK_DH(WHAT)              \
+  switch (c.D) {                          \
+    case 16: KF_KV8_PICK(WHAT, 16); break; \
+    case 32: KF_KV8_PICK(WHAT, 32); break; \
+    case 64: KF_KV8_PICK(WHAT, 64); break; \
+    default: KF_KV8_PICK(WHAT, 128); break; \
+  }
+  KF_KV8_PICK_DH(KF_KV8_SPLIT)
+  if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention launch");
+  if (w.chunks > 1) {
+    e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(128), 0, st,
+                       c, out, o_sb, o_sh, o_st, dtype, Ti, G, lse, w);
+    if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention join launch");
+  }
+  if (max_len == 0 || !(flags & KF_KV8_TRACK)) return KF_OK;
+  if (reweigh) {
+    KF_KV8_PICK_DH(KF_KV8_REWEIGH)
+  } else {
+    e2 = launch_chained(kv8_weights_kernel,
+                        dim3(static_cast<unsigned>((max_len + 255) / 256), bh), dim3(256), 0, st,
+                        c, counts, Ti, G, cap, flags, w);
+  }
+  return cuda_status(e2, "kf_kv8_attention weights launch");
+#undef KF_KV8_SPLIT
+#undef KF_KV8_REWEIGH
+#undef KF_KV8_PICK
+#undef KF_KV8_PICK_DH
+}
