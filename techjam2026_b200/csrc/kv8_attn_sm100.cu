@@ -690,6 +690,7 @@ extern "C" int64_t kf_kv8_attention_workspace_bytes(const kf_kv8_cache* cache, i
   if (kv8_attention_check("kf_kv8_attention_workspace_bytes", cache, dtype, T, q_heads, &max_len,
                           flags, &c))
     return -1;
+  if (T == 0 || c.B == 0) return 0;
   KV8Work w;
   kv8_plan(c, T, static_cast<int>(q_heads / c.H), max_len, flags, &w);
   return kv8_carve(c, flags, nullptr, &w);
@@ -704,11 +705,11 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
   KV8 c;
   int rc = kv8_attention_check("kf_kv8_attention", cache, dtype, T, q_heads, &max_len, flags, &c);
   if (rc) return rc;
+  if (T == 0 || c.B == 0) return KF_OK;
   if (!q || !out) {
     set_last_error("kf_kv8_attention: q and out must not be null");
     return KF_E_INVALID;
   }
-  if (T == 0 || c.B == 0) return KF_OK;
   const int G = static_cast<int>(q_heads / c.H);
   KV8Work w;
   kv8_plan(c, T, G, max_len, flags, &w);

@@ -388,11 +388,11 @@ extern "C" int kf_kv8_append(const kf_kv8_cache* cache, const void* k, int64_t k
   int rc = kv8_view("kf_kv8_append", cache, &c);
   if (!rc) rc = kv8_dtype("kf_kv8_append", dtype);
   if (rc) return rc;
+  if (T == 0 || c.B == 0) return KF_OK;
   if (!k || !v || T < 0 || T > INT32_MAX / 2) {
     set_last_error("kf_kv8_append: invalid arguments (T = %lld)", (long long)T);
     return KF_E_INVALID;
   }
-  if (T == 0 || c.B == 0) return KF_OK;
   const int64_t es = dtype_size(dtype);
   const int64_t strides[6] = {k_sb, k_sh, k_st, v_sb, v_sh, v_st};
   int vec = kv8_aligned(k, 4 * es) && kv8_aligned(v, 4 * es);
@@ -426,7 +426,8 @@ extern "C" int kf_kv8_read(const kf_kv8_cache* cache, const int32_t* start, cons
   int rc = kv8_view("kf_kv8_read", cache, &c);
   if (!rc) rc = kv8_dtype("kf_kv8_read", dtype);
   if (rc) return rc;
-  if (!k_out || !v_out || n < 0 || n * c.D > INT32_MAX) {
+  if (n == 0 || c.B == 0) return KF_OK;
+  if (!k_out || !v_out || n < 0 || n > INT32_MAX / c.D) {
     set_last_error("kf_kv8_read: invalid arguments (n = %lld)", (long long)n);
     return KF_E_INVALID;
   }
@@ -434,7 +435,6 @@ extern "C" int kf_kv8_read(const kf_kv8_cache* cache, const int32_t* start, cons
     set_last_error("kf_kv8_read: outputs must be 16-byte aligned");
     return KF_E_UNSUPPORTED;
   }
-  if (n == 0 || c.B == 0) return KF_OK;
   const int64_t groups = n * c.D / 4;
   const dim3 grid(static_cast<unsigned>((groups + KV8_THREADS - 1) / KV8_THREADS),
                   static_cast<unsigned>(c.H), static_cast<unsigned>(c.B));
