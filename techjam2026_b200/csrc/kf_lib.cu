@@ -8,3 +8,5 @@
 #include "noalloc_sm100.cu"
 #include "kv8_cache_sm100.cu"
 #include "kv8_attn_sm100.cu"
+#include "kv8_prompt_sm100.cu"
+#include "kv8_entry_sm100.cu"

@@ -1,0 +1,268 @@
+// Host side of kf_kv8_attention: which kernels run, how the work is cut, and
+// the workspace.
+#include "kv8_common.cuh"
+
+namespace kf {
+
+// Query rows of a kv head from which the tensor-memory kernel runs.
+constexpr int KV8_PROMPT_ROWS = 17;
+
+// How a call is cut: chunks of keys so that there are a few CTAs per SM, each
+// with work enough to pay for its start.
+static void kv8_plan(const KV8& c, int64_t T, int G, int64_t max_len, int flags, KV8Work* w) {
+  const int64_t rows = T * G;
+  if (rows >= KV8_PROMPT_ROWS) {
+    const int64_t ctas = (rows + 255) / 256 * c.B * c.H;
+    int64_t chunks = (2 * 148 + ctas - 1) / ctas;
+    const int64_t most = (max_len + 2047) / 2048;
+    if (chunks > most) chunks = most;
+    if (chunks < 1) chunks = 1;
+    const int64_t chunk = ((max_len + chunks - 1) / chunks + 127) / 128 * 128;
+    w->chunk = static_cast<int>(chunk < 128 ? 128 : chunk);
+    w->chunks = static_cast<int>((max_len + w->chunk - 1) / w->chunk);
+    if (w->chunks < 1) w->chunks = 1;
+    w->rows = static_cast<int>(rows);
+    w->ld_score = 0;
+    return;
+  }
+  const int64_t tiles = (rows + KV8_ROWS - 1) / KV8_ROWS;
+  const int64_t items = tiles * c.B * c.H;
+  const int64_t want = 148 * 8;
+  int64_t chunks = (want + items - 1) / items;
+  const int64_t most = (max_len + 127) / 128;    // at least 128 keys a chunk
+  if (chunks > most) chunks = most;
+  const int64_t least = (max_len + KV8_CHUNK_MAX - 1) / KV8_CHUNK_MAX;
+  if (chunks < least) chunks = least;
+  if (chunks < 1) chunks = 1;
+  int64_t chunk = (max_len + chunks - 1) / chunks;
+  chunk = (chunk + 127) / 128 * 128;             // whole pages, whatever the page
+  if (chunk < 128) chunk = 128;
+  w->chunk = static_cast<int>(chunk);
+  w->chunks = static_cast<int>((max_len + chunk - 1) / chunk);
+  if (w->chunks < 1) w->chunks = 1;
+  w->rows = static_cast<int>(rows);
+  w->ld_score = (flags & KF_KV8_TRACK) && rows <= KV8_ROWS ? (max_len + 15) / 16 * 16 : 0;
+}
+
+// Splits the workspace; returns the bytes it takes.
+static int64_t kv8_carve(const KV8& c, int dtype, int flags, uint8_t* base, KV8Work* w) {
+  int64_t at = 0;
+  auto take = [&](int64_t floats) -> float* {
+    float* p = reinterpret_cast<float*>(base + at);
+    at += (floats * 4 + 255) / 256 * 256;
+    return p;
+  };
+  const int64_t n = static_cast<int64_t>(c.B) * c.H * w->rows;
+  w->ref = w->sum = w->part = w->lse = w->score = nullptr;
+  if (w->chunks > 1) {
+    w->ref = take(n * w->chunks);
+    w->sum = take(n * w->chunks);
+    w->part = take(n * w->chunks * c.D);
+  }
+  if (flags & KF_KV8_TRACK) w->lse = take(n);
+  if (w->ld_score) w->score = take(n * w->ld_score);
+  w->planes = nullptr;
+  w->qf = nullptr;
+  if (w->rows >= KV8_PROMPT_ROWS) {
+    const int64_t planes = dtype == KF_DT_F32 ? 2 : 1;
+    w->planes = reinterpret_cast<uint16_t*>(take((planes * n * c.D + 1) / 2));
+    w->qf = take(n);
+  }
+  return at;
+}
+
+static int kv8_attention_check(const char* what, const kf_kv8_cache* cache, int dtype, int64_t T,
+                               int64_t q_heads, int64_t* max_len, int flags, KV8* c) {
+  int rc = kv8_view(what, cache, c);
+  if (!rc) rc = kv8_dtype(what, dtype);
+  if (rc) return rc;
+  if (T < 0 || q_heads <= 0 || q_heads % c->H || (flags & ~(KF_KV8_CAUSAL | KF_KV8_TRACK)) ||
+      *max_len < 0) {
+    set_last_error("%s: needs T >= 0, q_heads a multiple of kv_heads and known flags", what);
+    return KF_E_INVALID;
+  }
+  if ((flags & KF_KV8_TRACK) && !c->weight) {
+    set_last_error("%s: KF_KV8_TRACK needs a cache with a weight record", what);
+    return KF_E_INVALID;
+  }
+  const int64_t reach = static_cast<int64_t>(c->blocks) * c->P;
+  if (*max_len == 0 || *max_len > reach) *max_len = reach;
+  if (static_cast<int64_t>(c->B) * c->H > 65535 || T * (q_heads / c->H) > 65535LL * KV8_ROWS) {
+    set_last_error("%s: needs batch * kv_heads <= 65535 and at most 2^20 query rows a kv head",
+                   what);
+    return KF_E_UNSUPPORTED;
+  }
+  return KF_OK;
+}
+
+// Arguments of a call, for the kernels' launchers.
+struct KV8Call {
+  const void* q;
+  int64_t q_sb, q_sh, q_st;
+  void* out;
+  int64_t o_sb, o_sh, o_st;
+  int dtype, q_vec, o_vec;
+  const int32_t* counts;
+  int T, G, max_len;
+  float scale_log2;
+  int flags;
+  float* lse;
+  cudaStream_t st;
+};
+
+template <int DH, int PL>
+static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
+  using Cfg = PromptCfg<DH, PL>;
+  using Wei = WeighCfg<DH, PL>;
+  const unsigned bh = static_cast<unsigned>(c.B * c.H);
+  const bool track = (a.flags & KF_KV8_TRACK) != 0;
+  CUtensorMap map;
+  const uint64_t dims[3] = {DH, static_cast<uint64_t>(w.rows), static_cast<uint64_t>(PL) * bh};
+  const uint64_t strides[2] = {DH * 2, static_cast<uint64_t>(w.rows) * DH * 2};
+  const uint32_t box[3] = {64, 128, 1};
+  int rc = encode_tensor_map(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, w.planes, dims, strides, box,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  auto kern = kv8_prompt_kernel<DH, PL>;
+  auto kern_w = kv8_prompt_weights_kernel<DH, PL>;
+  static DeviceOnce once;
+  rc = once.run("kf_kv8_attention", nullptr, [&](int) {
+    cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kern_w, cudaFuncAttributeMaxDynamicSharedMemorySize, Wei::SMEM);
+    return cuda_status(e, "kf_kv8_attention: set smem attribute");
+  });
+  if (rc) return rc;
+  cudaError_t e = launch_chained(kv8_prep_q_kernel<DH, PL>,
+                                 dim3(static_cast<unsigned>((w.rows + 63) / 64), bh), dim3(256), 0,
+                                 a.st, c, a.q, a.q_sb, a.q_sh, a.q_st, a.dtype, a.q_vec, a.counts,
+                                 a.T, a.G, a.scale_log2, w);
+  if (e == cudaSuccess)
+    e = launch_chained(kern,
+                       dim3(static_cast<unsigned>((w.rows + 255) / 256),
+                            static_cast<unsigned>(w.chunks), bh),
+                       dim3(Cfg::THREADS), Cfg::SMEM, a.st, map, c, a.out, a.o_sb, a.o_sh, a.o_st,
+                       a.dtype, a.o_vec, a.counts, a.T, a.G, a.max_len, a.flags, a.lse, w);
+  if (e == cudaSuccess && w.chunks > 1)
+    e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(128), 0, a.st,
+                       c, a.out, a.o_sb, a.o_sh, a.o_st, a.dtype, a.T, a.G, a.lse, w);
+  if (e == cudaSuccess && track && a.max_len > 0)
+    e = launch_chained(kern_w, dim3(static_cast<unsigned>((a.max_len + 127) / 128), bh),
+                       dim3(Wei::THREADS), Wei::SMEM, a.st, map, c, a.counts, a.T, a.G, a.max_len,
+                       a.flags, w);
+  return cuda_status(e, "kf_kv8_attention launch");
+}
+
+}  // namespace kf
+
+using namespace kf;
+
+extern "C" int64_t kf_kv8_attention_workspace_bytes(const kf_kv8_cache* cache, int dtype,
+                                                    int64_t T, int64_t q_heads, int64_t max_len,
+                                                    int flags) {
+  KV8 c;
+  if (kv8_attention_check("kf_kv8_attention_workspace_bytes", cache, dtype, T, q_heads, &max_len,
+                          flags, &c))
+    return -1;
+  if (T == 0 || c.B == 0) return 0;
+  KV8Work w;
+  kv8_plan(c, T, static_cast<int>(q_heads / c.H), max_len, flags, &w);
+  return kv8_carve(c, dtype, flags, nullptr, &w);
+}
+
+extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_t q_sb,
+                                int64_t q_sh, int64_t q_st, void* out, int64_t o_sb, int64_t o_sh,
+                                int64_t o_st, int dtype, const int32_t* counts, int64_t T,
+                                int64_t q_heads, int64_t max_len, float sm_scale, int flags,
+                                float* lse, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
+  KV8 c;
+  int rc = kv8_attention_check("kf_kv8_attention", cache, dtype, T, q_heads, &max_len, flags, &c);
+  if (rc) return rc;
+  if (T == 0 || c.B == 0) return KF_OK;
+  if (!q || !out) {
+    set_last_error("kf_kv8_attention: q and out must not be null");
+    return KF_E_INVALID;
+  }
+  const int G = static_cast<int>(q_heads / c.H);
+  KV8Work w;
+  kv8_plan(c, T, G, max_len, flags, &w);
+  const int64_t need = kv8_carve(c, dtype, flags, static_cast<uint8_t*>(workspace), &w);
+  if (need > 0 && (!workspace || workspace_bytes < need || !kv8_aligned(workspace, 256))) {
+    set_last_error("kf_kv8_attention: needs a 256-byte aligned workspace of %lld bytes",
+                   (long long)need);
+    return KF_E_INVALID;
+  }
+  const int64_t es = dtype_size(dtype);
+  const int vec = kv8_aligned(q, 4 * es) && q_sb % 4 == 0 && q_sh % 4 == 0 && q_st % 4 == 0;
+  const float scale_log2 = sm_scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int Ti = static_cast<int>(T), cap = static_cast<int>(max_len);
+  const unsigned bh = static_cast<unsigned>(c.B * c.H);
+  const dim3 grid(static_cast<unsigned>(w.chunks),
+                  static_cast<unsigned>((w.rows + KV8_ROWS - 1) / KV8_ROWS), bh);
+  const bool reweigh = (flags & KF_KV8_TRACK) && !w.score;
+  if (w.rows >= KV8_PROMPT_ROWS) {
+    const int64_t per = 16 / es;
+    const int o_vec = kv8_aligned(out, 16) && o_sb % per == 0 && o_sh % per == 0 && o_st % per == 0;
+    const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, o_vec, counts, Ti, G,
+                       cap, scale_log2, flags, lse, st};
+    const bool two = dtype == KF_DT_F32;
+    switch (c.D) {
+      case 16: return two ? kv8_prompt<16, 2>(c, a, w) : kv8_prompt<16, 1>(c, a, w);
+      case 32: return two ? kv8_prompt<32, 2>(c, a, w) : kv8_prompt<32, 1>(c, a, w);
+      case 64: return two ? kv8_prompt<64, 2>(c, a, w) : kv8_prompt<64, 1>(c, a, w);
+      default: return two ? kv8_prompt<128, 2>(c, a, w) : kv8_prompt<128, 1>(c, a, w);
+    }
+  }
+  cudaError_t e = cudaSuccess, e2 = cudaSuccess;
+#define KF_KV8_SPLIT(DH, FMT, PL)                                                               \
+  e = launch_chained(kv8_split_kernel<DH, FMT, PL>, grid, dim3(128), 0, st, c, q, q_sb, q_sh,   \
+                     q_st, out, o_sb, o_sh, o_st, dtype, vec, counts, Ti, G, cap, scale_log2,   \
+                     flags, lse, w)
+#define KF_KV8_REWEIGH(DH, FMT, PL)                                                             \
+  e2 = launch_chained(kv8_reweigh_kernel<DH, FMT, PL>,                                          \
+                      dim3(static_cast<unsigned>((max_len + 63) / 64), bh), dim3(128), 0, st, c, \
+                      q, q_sb, q_sh, q_st, dtype, vec, counts, Ti, G, cap, scale_log2, flags, w)
+#define KF_KV8_PICK(WHAT, DH)                        \
+  do {                                               \
+    const bool i8 = c.fmt == KF_KV8_INT8;            \
+    const bool two = dtype == KF_DT_F32;             \
+    if (i8 && two)                                   \
+      WHAT(DH, KF_KV8_INT8, 2);                      \
+    else if (i8)                                     \
+      WHAT(DH, KF_KV8_INT8, 1);                      \
+    else if (two)                                    \
+      WHAT(DH, KF_KV8_E4M3, 2);                      \
+    else                                             \
+      WHAT(DH, KF_KV8_E4M3, 1);                      \
+  } while (0)
+#define KF_KV8_PICK_DH(WHAT)              \
+  switch (c.D) {                          \
+    case 16: KF_KV8_PICK(WHAT, 16); break; \
+    case 32: KF_KV8_PICK(WHAT, 32); break; \
+    case 64: KF_KV8_PICK(WHAT, 64); break; \
+    default: KF_KV8_PICK(WHAT, 128); break; \
+  }
+  KF_KV8_PICK_DH(KF_KV8_SPLIT)
+  if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention launch");
+  if (w.chunks > 1) {
+    e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(128), 0, st,
+                       c, out, o_sb, o_sh, o_st, dtype, Ti, G, lse, w);
+    if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention join launch");
+  }
+  if (max_len == 0 || !(flags & KF_KV8_TRACK)) return KF_OK;
+  if (reweigh) {
+    KF_KV8_PICK_DH(KF_KV8_REWEIGH)
+  } else {
+    e2 = launch_chained(kv8_weights_kernel,
+                        dim3(static_cast<unsigned>((max_len + 255) / 256), bh), dim3(256), 0, st,
+                        c, counts, Ti, G, cap, flags, w);
+  }
+  return cuda_status(e2, "kf_kv8_attention weights launch");
+#undef KF_KV8_SPLIT
+#undef KF_KV8_REWEIGH
+#undef KF_KV8_PICK
+#undef KF_KV8_PICK_DH
+}
