@@ -72,10 +72,14 @@ static int64_t kv8_carve(const KV8& c, int dtype, int flags, uint8_t* base, KV8W
 }
 
 static int kv8_attention_check(const char* what, const kf_kv8_cache* cache, int dtype, int64_t T,
-                               int64_t q_heads, int64_t* max_len, int flags, KV8* c) {
+                               int64_t q_heads, int64_t* max_len, float sm_scale, int flags, KV8* c) {
   int rc = kv8_view(what, cache, c);
   if (!rc) rc = kv8_dtype(what, dtype);
   if (rc) return rc;
+  if (!(sm_scale >= 0.f) || sm_scale > 3.0e38f) {
+    set_last_error("%s: sm_scale must be finite and not negative", what);
+    return KF_E_INVALID;
+  }
   if (T < 0 || q_heads <= 0 || q_heads % c->H || (flags & ~(KF_KV8_CAUSAL | KF_KV8_TRACK)) ||
       *max_len < 0) {
     set_last_error("%s: needs T >= 0, q_heads a multiple of kv_heads and known flags", what);
@@ -140,7 +144,7 @@ static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
                                  a.T, a.G, a.scale_log2, w);
   if (e == cudaSuccess)
     e = launch_chained(kern,
-                       dim3(static_cast<unsigned>((w.rows + 255) / 256),
+                       dim3(static_cast<unsigned>((w.rows + Cfg::ROWS - 1) / Cfg::ROWS),
                             static_cast<unsigned>(w.chunks), bh),
                        dim3(Cfg::THREADS), Cfg::SMEM, a.st, map, c, a.out, a.o_sb, a.o_sh, a.o_st,
                        a.dtype, a.o_vec, a.counts, a.T, a.G, a.max_len, a.flags, a.lse, w);
@@ -162,7 +166,7 @@ extern "C" int64_t kf_kv8_attention_workspace_bytes(const kf_kv8_cache* cache, i
                                                     int64_t T, int64_t q_heads, int64_t max_len,
                                                     int flags) {
   KV8 c;
-  if (kv8_attention_check("kf_kv8_attention_workspace_bytes", cache, dtype, T, q_heads, &max_len,
+  if (kv8_attention_check("kf_kv8_attention_workspace_bytes", cache, dtype, T, q_heads, &max_len, 1.f,
                           flags, &c))
     return -1;
   if (T == 0 || c.B == 0) return 0;
@@ -178,7 +182,8 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
                                 float* lse, void* workspace, int64_t workspace_bytes,
                                 void* stream) {
   KV8 c;
-  int rc = kv8_attention_check("kf_kv8_attention", cache, dtype, T, q_heads, &max_len, flags, &c);
+  int rc = kv8_attention_check("kf_kv8_attention", cache, dtype, T, q_heads, &max_len, sm_scale,
+                               flags, &c);
   if (rc) return rc;
   if (T == 0 || c.B == 0) return KF_OK;
   if (!q || !out) {

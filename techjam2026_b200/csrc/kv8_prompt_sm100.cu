@@ -5,15 +5,17 @@
 // kv8_prompt_kernel: one CTA = two tiles of 128 query rows (row = token * G +
 // head of the group, so the query heads of a kv head share its K and V) of one
 // (sequence, kv head), over a range of keys. Roles:
-//   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row: reads its S
-//                   row from TMEM in halves of 64, writes P over it as fp16;
-//   warps 8-11      load the codes of the next 128 keys into registers while
-//                   the current ones are in use, and write them as fp16 into
-//                   128-byte-swizzled tiles (K: K-major, V: MN-major, the same
-//                   bytes: rows are keys); codes are exact in fp16;
-//   warp 12         (of 12-15) allocates TMEM, loads Q by TMA and issues the products
+//   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row: reads its 128
+//                   scores from TMEM, writes P over them as fp16;
+//   warp 8          allocates TMEM, loads Q by TMA and issues the products
 //                   S = Q K^T (operands in shared memory) and O += P V (P read
-//                   from TMEM).
+//                   from TMEM);
+//   warps 9-11      loaders: copy pages of codes to shared memory with bulk
+//                   copies a step or two ahead, and expand them to fp16 in
+//                   128-byte-swizzled tiles (K: K-major, V: MN-major, the same
+//                   bytes: rows are keys); they also stage the scales. (Codes
+//                   fetched through registers with a page lookup per piece held
+//                   the whole kernel at 6000 clocks a step.)
 // TMEM: S0 | S1 (128 columns each, P in place), O0 | O1. For each tile the
 // order is P V(j), then S(j + 1): the pipe runs in issue order, so a softmax
 // that sees S(j + 1) knows O holds P V(j) and may rescale it at once, and while
@@ -48,16 +50,6 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-
-// Registers a thread of this warpgroup may use from here on (all of its warps
-// execute it).
-template <bool INC, int N>
-__device__ __forceinline__ void set_max_registers() {
-  if constexpr (INC)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-  else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // ---------------------------------------------------------------- q planes
@@ -172,82 +164,140 @@ __device__ __forceinline__ void kv8_store_run(void* out, int64_t at, int dtype, 
   }
 }
 
+// A tile of 128 rows of raw codes to fp16 in the 128-byte-swizzled layout
+// (64-column halves one after the other), by three warps, 16 codes at a time.
+// Rows from `rows` on, and groups of 16 rows in `bad`, become zeros (ZERO).
+template <int DH, int FMT, bool ZERO>
+__device__ __forceinline__ void kv8_expand(const uint8_t* raw, uint8_t* tile, int lt, int rows,
+                                           uint32_t bad) {
+  constexpr int RC = DH / 16, RP = 96 / RC;  // pieces of a row, rows of a pass
+  static_assert(RP % 4 == 0, "swizzle phase");
+  const int c16 = lt % RC, r0 = lt / RC;
+  uint8_t* dst = tile + (c16 >> 2) * 128 * 128 + r0 * 128;
+  const uint32_t ch = static_cast<uint32_t>((c16 & 3) * 2 ^ (r0 & 7)) << 4;
+#pragma unroll
+  for (int i = 0; i < (128 + RP - 1) / RP; ++i) {
+    const int r = r0 + i * RP;
+    if (128 % RP && r >= 128) break;
+    uint4 w = *reinterpret_cast<const uint4*>(raw + (lt + i * 96) * 16);
+    if (ZERO && (r >= rows || ((bad >> (r >> 4)) & 1u))) w = make_uint4(0u, 0u, 0u, 0u);
+    uint32_t h[8];
+    kv8_cvt4<FMT>(w.x, h[0], h[1]);
+    kv8_cvt4<FMT>(w.y, h[2], h[3]);
+    kv8_cvt4<FMT>(w.z, h[4], h[5]);
+    kv8_cvt4<FMT>(w.w, h[6], h[7]);
+    // r & 7 moves by RP & 7, which is 0 or 4: the swizzle flips one bit
+    const uint32_t at = ch ^ (((i * RP) & 4) << 4);
+    *reinterpret_cast<uint4*>(dst + i * RP * 128 + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(dst + i * RP * 128 + (at ^ 16u)) = make_uint4(h[4], h[5], h[6], h[7]);
+  }
+}
+
+// Named barrier over `count` threads that tells all of them whether any came
+// with `flag` set.
+__device__ __forceinline__ bool named_bar_or(int id, int count, bool flag) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(count), "r"(static_cast<uint32_t>(flag))
+      : "memory");
+  return r != 0;
+}
+
+// Untiled copy global -> shared, completion counted on an mbarrier; 16-byte
+// aligned addresses and size.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 template <int DH, int PL>
 struct PromptCfg {
-  static constexpr int BM = 128;                           // query rows of a tile
-  static constexpr int BN = (DH == 128 && PL == 2) ? 64 : 128;  // keys of a step
+  // Tiles of 128 query rows. fp32 at head_dim 128 takes one: its Q planes fill
+  // shared memory and its second accumulator TMEM.
+  static constexpr int NT = (DH == 128 && PL == 2) ? 1 : 2;
+  static constexpr int BM = 128;
+  static constexpr int BN = 128;                           // keys of a step
   static constexpr int CH = DH > 64 ? 2 : 1;               // 64-column halves of a row
   static constexpr int Q_PLANE = BM * 128 * CH;            // bytes of one tile's plane
-  static constexpr int Q_BYTES = 2 * PL * Q_PLANE;
+  static constexpr int Q_BYTES = NT * PL * Q_PLANE;
   static constexpr int KV_BYTES = BN * 128 * CH;
   static constexpr int ST = 2;                             // stages of K and of V
+  static constexpr int RAW = BN * DH;                      // bytes of a tile's codes
+  static constexpr int RS = DH > 64 ? 1 : 2;               // raw tiles of K and of V
   static constexpr int K_OFF = Q_BYTES;
   static constexpr int V_OFF = K_OFF + ST * KV_BYTES;
-  static constexpr int BAR_OFF = V_OFF + ST * KV_BYTES;
-  static constexpr int SC_OFF = BAR_OFF + 256;             // page scales of each stage
+  static constexpr int RAWK_OFF = V_OFF + ST * KV_BYTES;
+  static constexpr int RAWV_OFF = RAWK_OFF + RS * RAW;
+  static constexpr int BAR_OFF = RAWV_OFF + RS * RAW;
+  static constexpr int SC_OFF = BAR_OFF + 256;             // page scales of each step
   // Four slots, each read by step j's softmax and rewritten for step j + 4: by
   // then every softmax warp has begun step j + 2.
   static constexpr int SLOTS = 4;
   static constexpr int USED = SC_OFF + SLOTS * 128 + 1024;
   // One CTA per SM (all of TMEM): ask for more than half of shared memory.
   static constexpr int SMEM = USED > 120 * 1024 ? USED : 120 * 1024;
-  static constexpr int GROUPS = BN / 16;                   // scale entries of a stage
-  static constexpr int LOADS = BN * DH / 16 / 128;         // 16-byte loads a loader thread
-  static constexpr int O_COL = 256;
-  static constexpr int O_STRIDE = DH < 32 ? 32 : DH;       // columns between O0 and O1
-  // Four warpgroups launched with 128 registers a thread; the softmax ones
-  // take 176 (a row of 64 scores and its packed P), the loaders keep 96, the
-  // issuer's 64: 8 * 176 + 4 * 96 + 4 * 64 = 16 * 128.
-  static constexpr int THREADS = 16 * 32;
+  static constexpr int GROUPS = BN / 16;                   // scale entries of a step
+  static constexpr int O_STRIDE = DH < 32 ? 32 : DH;
+  static constexpr int O_COL = 256;                        // O of tile t
+  // fp32 output: O collects FLUSH steps and is then added to a second
+  // accumulator with ordinary fp32 additions. The tensor core's own
+  // accumulation drops the bits below the running sum: measured against
+  // float64, 2e-9 of relative error per key, 4e-6 after 2048 keys; 5e-7 after 256.
+  static constexpr int FLUSH = 2;
+  static constexpr int M_COL = O_COL + NT * O_STRIDE;
+  static constexpr int ROWS = NT * BM;
+  // Twelve warps leave 168 registers a thread: a softmax row's 128 scores and
+  // what goes with them.
+  static constexpr int THREADS = 12 * 32;
   static_assert(SMEM <= 232448, "smem");
-  static_assert(O_COL + 2 * O_STRIDE <= 512, "TMEM");
+  static_assert((PL == 2 ? M_COL : O_COL) + NT * O_STRIDE <= 512, "TMEM");
 };
 
-// Scales of the keys of one stage, by groups of 16 keys.
+// Scales of the keys of one step, by groups of 16 keys.
 struct alignas(16) PromptScales {
   float ks[8];
-  float ratio[8];   // V scale over the range's largest
-  uint32_t bad;      // groups on a refused page
-  uint32_t spoiled;  // groups on a page whose V scale is NaN (their ratio is 0)
+  float ratio[8];     // V scale over the range's largest
+  uint32_t bad;       // groups on a refused page
+  uint32_t spoiled_k; // groups on a page whose K scale is NaN (its ks is 0 here)
+  uint32_t spoiled_v; // the same of V
 };
 
-// One row's 64 scores of a half tile: loaded, scaled to log2 units, masked.
-template <int BN>
-__device__ __forceinline__ void prompt_scores(uint32_t t_addr, float qf, const float* ks,
-                                              uint32_t bad, bool mask, int limit, float (&s)[64]) {
-  tmem_ld64(t_addr, s);
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const float f = qf * ks[g];
-    const uint64_t f2 = f2_pack(f, f);
-#pragma unroll
-    for (int u = 0; u < 16; u += 2)
-      f2_unpack(f2_mul(f2_pack(s[16 * g + u], s[16 * g + u + 1]), f2), s[16 * g + u],
-                s[16 * g + u + 1]);
-  }
-  if (mask) {
-    uint32_t kw[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-      kw[w] = ((bad >> (2 * w)) & 1u ? 0u : 0x0000ffffu) |
-              ((bad >> (2 * w + 1)) & 1u ? 0u : 0xffff0000u);
-    mask_scores<64>(s, kw, limit);
-  }
+// 128 consecutive columns of this thread's lane, and the wait. The first half's
+// registers pass through the last statement, so nothing reads them before it.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]), "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+               : "r"(taddr)
+               : "memory");
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=f"(v[64]), "=f"(v[65]), "=f"(v[66]), "=f"(v[67]), "=f"(v[68]), "=f"(v[69]), "=f"(v[70]), "=f"(v[71]), "=f"(v[72]), "=f"(v[73]), "=f"(v[74]), "=f"(v[75]), "=f"(v[76]), "=f"(v[77]), "=f"(v[78]), "=f"(v[79]), "=f"(v[80]), "=f"(v[81]), "=f"(v[82]), "=f"(v[83]), "=f"(v[84]), "=f"(v[85]), "=f"(v[86]), "=f"(v[87]), "=f"(v[88]), "=f"(v[89]), "=f"(v[90]), "=f"(v[91]), "=f"(v[92]), "=f"(v[93]), "=f"(v[94]), "=f"(v[95]), "=f"(v[96]), "=f"(v[97]), "=f"(v[98]), "=f"(v[99]), "=f"(v[100]), "=f"(v[101]), "=f"(v[102]), "=f"(v[103]), "=f"(v[104]), "=f"(v[105]), "=f"(v[106]), "=f"(v[107]), "=f"(v[108]), "=f"(v[109]), "=f"(v[110]), "=f"(v[111]), "=f"(v[112]), "=f"(v[113]), "=f"(v[114]), "=f"(v[115]), "=f"(v[116]), "=f"(v[117]), "=f"(v[118]), "=f"(v[119]), "=f"(v[120]), "=f"(v[121]), "=f"(v[122]), "=f"(v[123]), "=f"(v[124]), "=f"(v[125]), "=f"(v[126]), "=f"(v[127])
+               : "r"(taddr + 64)
+               : "memory");
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]), "+f"(v[32]), "+f"(v[33]), "+f"(v[34]), "+f"(v[35]), "+f"(v[36]), "+f"(v[37]), "+f"(v[38]), "+f"(v[39]), "+f"(v[40]), "+f"(v[41]), "+f"(v[42]), "+f"(v[43]), "+f"(v[44]), "+f"(v[45]), "+f"(v[46]), "+f"(v[47]), "+f"(v[48]), "+f"(v[49]), "+f"(v[50]), "+f"(v[51]), "+f"(v[52]), "+f"(v[53]), "+f"(v[54]), "+f"(v[55]), "+f"(v[56]), "+f"(v[57]), "+f"(v[58]), "+f"(v[59]), "+f"(v[60]), "+f"(v[61]), "+f"(v[62]), "+f"(v[63]) :: "memory");
 }
-
-__device__ __forceinline__ float max64(const float (&s)[64]) {
-  float m[8];
-#pragma unroll
-  for (int u = 0; u < 8; ++u) m[u] = fmaxf(s[u], s[u + 8]);
-#pragma unroll
-  for (int c = 16; c < 64; c += 16) {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) m[u] = fmax3(m[u], s[c + u], s[c + 8 + u]);
-  }
-  return fmax3(fmax3(m[0], m[1], m[2]), fmax3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
+// 16 consecutive columns of this thread's lane, and the wait.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
-
-// Store 16 consecutive TMEM columns of this thread's lane (no wait).
+// Store 16 consecutive columns (no wait).
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -261,35 +311,15 @@ __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// P of 64 scores: fp16 words (and the second plane's), the unrounded sum.
-template <int PL>
-__device__ __forceinline__ float prompt_weights(const float (&s)[64], float neg_ref,
-                                                const float* ratio, uint32_t t_addr) {
-  uint64_t acc[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-  const uint64_t nr = f2_pack(neg_ref, neg_ref);
-#pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    uint32_t hi[16], lo[16];
-#pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      const int k = 32 * part + 2 * u;
-      float a, b;
-      f2_unpack(f2_add(f2_pack(s[k], s[k + 1]), nr), a, b);
-      a = fast_exp2(a);
-      b = fast_exp2(b);
-      acc[u & 1] = f2_add(acc[u & 1], f2_pack(a, b));
-      const float r = ratio[k >> 4];
-      f2_unpack(f2_mul(f2_pack(a, b), f2_pack(r, r)), a, b);
-      hi[u] = pack_half2(a, b);
-      if constexpr (PL == 2) lo[u] = pack_half2_rest(a, b, hi[u]);
-    }
-    tmem_st16(t_addr + 16 * part, hi);
-    if constexpr (PL == 2) tmem_st16(t_addr + 32 + 16 * part, lo);
-  }
-  float x0, x1, x2, x3;
-  f2_unpack(acc[0], x0, x1);
-  f2_unpack(acc[1], x2, x3);
-  return (x0 + x1) + (x2 + x3);
+// Largest of 16 consecutive scores.
+__device__ __forceinline__ float max16(const float* s) {
+  float m = fmax3(s[0], s[1], s[2]);
+  float n = fmax3(s[3], s[4], s[5]);
+  m = fmax3(m, s[6], s[7]);
+  n = fmax3(n, s[8], s[9]);
+  m = fmax3(m, s[10], s[11]);
+  n = fmax3(n, s[12], s[13]);
+  return fmax3(fmaxf(m, n), s[14], s[15]);
 }
 
 template <int DH, int PL>
@@ -299,7 +329,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
                       const int32_t* __restrict__ counts, int T, int G, int max_len, int flags,
                       float* __restrict__ lse_out, KV8Work w) {
   using Cfg = PromptCfg<DH, PL>;
-  constexpr int BM = Cfg::BM, BN = Cfg::BN;
+  constexpr int BM = Cfg::BM, BN = Cfg::BN, NT = Cfg::NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -308,17 +338,20 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   uint8_t* sV = smem + Cfg::V_OFF;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::BAR_OFF);
   uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;    // [ST] 4 loader warps
+  uint64_t* k_full = bars + 1;    // [ST] fp16 tile written, scales staged
   uint64_t* v_full = bars + 3;    // [ST]
-  uint64_t* k_empty = bars + 5;   // [ST] S of both tiles done, 8 softmax warps at that step
-  uint64_t* v_empty = bars + 7;   // [ST] P V of both tiles done
-  uint64_t* s_full = bars + 9;    // [2]
-  uint64_t* p_full = bars + 11;   // [2] 4 warps
-  uint64_t* o_final = bars + 13;  // [2]
-  uint64_t* drain = bars + 15;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  uint64_t* k_empty = bars + 5;   // [ST] S of all tiles done, softmax warps at that step
+  uint64_t* v_empty = bars + 7;   // [ST] P V of all tiles done
+  uint64_t* s_full = bars + 9;    // [2] by S buffer
+  uint64_t* p_full = bars + 11;   // [2] by S buffer, 4 warps
+  uint64_t* o_done = bars + 13;   // one tile: P V of a step done
+  uint64_t* o_final = bars + 14;  // [2]
+  uint64_t* drain = bars + 16;
+  uint64_t* rk_full = bars + 17;  // [RS] raw codes of K, of V: their bytes
+  uint64_t* rv_full = bars + 19;  // [RS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* s_vmax = reinterpret_cast<float*>(tmem_slot + 2);  // [16]
+  float* s_vmax = reinterpret_cast<float*>(tmem_slot + 2);  // [12]
   PromptScales* s_sc = reinterpret_cast<PromptScales*>(smem + Cfg::SC_OFF);
   static_assert(sizeof(PromptScales) <= 128, "scale ring");
 
@@ -327,7 +360,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   const int bh = blockIdx.z;
   const int b = bh / c.H, h = bh - b * c.H;
   const int chunk = blockIdx.y;
-  const int row0 = static_cast<int>(gridDim.x - 1 - blockIdx.x) * 2 * BM;  // heaviest first
+  const int row0 = static_cast<int>(gridDim.x - 1 - blockIdx.x) * Cfg::ROWS;  // heaviest first
   const int len = kv8_len(c, b);
   const int count = kv8_count(counts, b, T);
   int end = kv8_end(c, len, count);
@@ -336,7 +369,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
     end = max_len;
   }
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
-  const int last_row = min(row0 + 2 * BM, w.rows) - 1;
+  const int last_row = min(row0 + Cfg::ROWS, w.rows) - 1;
   const int last_tok = min(last_row / G, count - 1);
   const int reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
   const int k0 = chunk * w.chunk;
@@ -344,7 +377,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   const bool alone = w.chunks == 1;
   if (k0 >= k1) {
     // No key: zeros, or an empty part for the join.
-    for (int i = tid; i < 2 * BM; i += Cfg::THREADS) {
+    for (int i = tid; i < Cfg::ROWS; i += Cfg::THREADS) {
       const int row = row0 + i;
       if (row >= w.rows) break;
       const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
@@ -354,7 +387,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         continue;
       }
       const int tok = row / G, hq = h * G + row - tok * G;
-      for (int d = 0; d < DH; ++d) kv8_store1(out, b * o_sb + hq * o_sh + tok * o_st + d, dtype, 0.f);
+      for (int d = 0; d < DH; ++d)
+        kv8_store1(out, b * o_sb + hq * o_sh + tok * o_st + d, dtype, 0.f);
       if (lse_out) lse_out[(static_cast<int64_t>(b) * c.H * G + hq) * T + tok] = -INFINITY;
       if (w.lse) w.lse[at] = -INFINITY;
     }
@@ -365,20 +399,23 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   if (tid == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 4);
-      mbar_init(&v_full[s], 4);
-      mbar_init(&k_empty[s], 1 + 8);
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&rk_full[s], 1);
+      mbar_init(&rv_full[s], 1);
+      mbar_init(&k_empty[s], 1 + 4 * NT);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
       mbar_init(&o_final[s], 1);
     }
+    mbar_init(o_done, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmQ);
   }
-  if (warp == 12) {
+  if (warp == 8) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -387,7 +424,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
     float vmax = 0.f;
     for (int j = (k0 >> c.p_shift) + tid; (j << c.p_shift) < k1; j += Cfg::THREADS) {
       const int page = kv8_page(c, b, j);
-      if (page >= 0) vmax = fmaxf(vmax, __ldg(c.scale + 2 * (static_cast<int64_t>(page) * c.H + h) + 1));
+      if (page >= 0)
+        vmax = fmaxf(vmax, __ldg(c.scale + 2 * (static_cast<int64_t>(page) * c.H + h) + 1));
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
@@ -400,14 +438,13 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   pdl_launch_dependents();  // every CTA that runs holds its TMEM by now
   float vmax = s_vmax[0];
 #pragma unroll
-  for (int i = 1; i < 16; ++i) vmax = fmaxf(vmax, s_vmax[i]);
+  for (int i = 1; i < 12; ++i) vmax = fmaxf(vmax, s_vmax[i]);
 
-  if (warp >= 12) {
-    set_max_registers<false, 64>();
-    if (warp == 12 && lane == 0) {
+  if (warp == 8) {
+    if (lane == 0) {
       // ------------------------------------------------ Q, products
       mbar_arrive_expect_tx(q_full, Cfg::Q_BYTES);
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NT; ++t)
         for (int pl = 0; pl < PL; ++pl)
           for (int ch = 0; ch < Cfg::CH; ++ch)
             tma_load_3d(sQ + (t * PL + pl) * Cfg::Q_PLANE + ch * BM * 128, &tmQ, q_full, ch * 64,
@@ -415,7 +452,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       constexpr uint32_t idesc_s = make_idesc_f16(BM, BN, 0);
       constexpr uint32_t idesc_o = make_idesc_f16(BM, DH, 1);
       const uint32_t sQa = smem_u32(sQ), sKa = smem_u32(sK), sVa = smem_u32(sV);
-      auto issue_s = [&](int t, int stage) {
+      // S of tile t and the K tile of `stage` into S buffer `buf`.
+      auto issue_s = [&](int t, int buf, int stage) {
 #pragma unroll
         for (int pl = PL - 1; pl >= 0; --pl)  // the small plane first
 #pragma unroll
@@ -426,91 +464,108 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
             const uint64_t bd =
                 make_smem_desc(sKa + stage * Cfg::KV_BYTES + (kk >> 2) * BN * 128 + (kk & 3) * 32,
                                16, 1024, KF_SWIZZLE_128B);
-            mma_bf16_ss(tmem_base + t * 128, ad, bd, idesc_s, (pl < PL - 1 || kk > 0) ? 1u : 0u);
+            mma_bf16_ss(tmem_base + buf * 128, ad, bd, idesc_s, (pl < PL - 1 || kk > 0) ? 1u : 0u);
           }
-        mma_commit(&s_full[t]);
+        mma_commit(&s_full[buf]);
+      };
+      // O of tile t += P in S buffer `buf` times the V tile of `stage`.
+      auto issue_o = [&](int t, int buf, int stage, bool fresh) {
+#pragma unroll
+        for (int pl = PL - 1; pl >= 0; --pl)
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk) {
+            const uint64_t bd = make_smem_desc(sVa + stage * Cfg::KV_BYTES + kk * 16 * 128, BN * 128,
+                                               1024, KF_SWIZZLE_128B);
+            mma_f16_ts(tmem_base + Cfg::O_COL + t * Cfg::O_STRIDE,
+                       tmem_base + buf * 128 + (kk >> 2) * 64 + pl * 32 + (kk & 3) * 8, bd, idesc_o,
+                       (!fresh || pl < PL - 1 || kk > 0) ? 1u : 0u);
+          }
       };
       bool ok = mbar_wait(q_full, 0, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA) &&
                 mbar_wait(&k_full[0], 0, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA);
       if (ok) {
         tc_fence_after();
-        issue_s(0, 0);
-        issue_s(1, 0);
+        for (int t = 0; t < NT; ++t) issue_s(t, t, 0);
         mma_commit(&k_empty[0]);
       }
       for (int j = 0; j < n_steps && ok; ++j) {
-        const int st = j & 1, nx = (j + 1) & 1;
+        const int st = j & 1, nx = st ^ 1;
         const uint32_t ph = (j >> 1) & 1, nph = ((j + 1) >> 1) & 1;
-        ok = mbar_wait(&v_full[st], ph, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA);
-        for (int t = 0; t < 2 && ok; ++t) {
-          ok = mbar_wait(&p_full[t], j & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA);
+        const bool fresh = PL == 2 ? j % Cfg::FLUSH == 0 : j == 0;
+        const bool more = j + 1 < n_steps;
+        if (NT == 1) {
+          // S runs one step ahead of the softmax, in the other buffer: the P
+          // there (step j - 1) was consumed by a product issued earlier.
+          if (more) {
+            ok = mbar_wait(&k_full[nx], nph, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(0, nx, nx);
+            mma_commit(&k_empty[nx]);
+          }
+          ok = mbar_wait(&v_full[st], ph, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA) &&
+               mbar_wait(&p_full[st], ph, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA);
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
-          for (int pl = PL - 1; pl >= 0; --pl)
-#pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk) {
-              const uint64_t bd = make_smem_desc(sVa + st * Cfg::KV_BYTES + kk * 16 * 128, BN * 128,
-                                                 1024, KF_SWIZZLE_128B);
-              mma_f16_ts(tmem_base + Cfg::O_COL + t * Cfg::O_STRIDE,
-                         tmem_base + t * 128 + (kk >> 2) * 64 + pl * 32 + (kk & 3) * 8, bd,
-                         idesc_o, (j > 0 || pl < PL - 1 || kk > 0) ? 1u : 0u);
+          issue_o(0, st, st, fresh);
+          mma_commit(more ? o_done : &o_final[0]);
+          mma_commit(&v_empty[st]);
+        } else {
+          ok = mbar_wait(&v_full[st], ph, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA);
+          for (int t = 0; t < 2 && ok; ++t) {
+            ok = mbar_wait(&p_full[t], j & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA);
+            if (!ok) break;
+            tc_fence_after();
+            issue_o(t, t, st, fresh);
+            if (!more) {
+              mma_commit(&o_final[t]);
+              continue;
             }
-          if (j + 1 < n_steps) {
             if (t == 0) {
               ok = mbar_wait(&k_full[nx], nph, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA);
               if (!ok) break;
               tc_fence_after();
             }
-            issue_s(t, nx);
-          } else {
-            mma_commit(&o_final[t]);
+            issue_s(t, t, nx);
           }
-        }
-        if (ok) {
+          if (!ok) break;
           mma_commit(&v_empty[st]);
-          if (j + 1 < n_steps) mma_commit(&k_empty[nx]);
+          if (more) mma_commit(&k_empty[nx]);
         }
       }
       mma_commit(drain);
       mbar_wait_drain(drain, 0, KF_DEV_WAIT_TIMEOUT_MMA);
       mbar_wait_drain(q_full, 0, KF_DEV_WAIT_TIMEOUT_MMA);
     }
-  } else if (warp >= 8) {
-    // -------------------------------------------------- loaders
-    set_max_registers<false, 96>();
-    const int lt = tid - 256;
+  } else if (warp > 8) {
+    // -------------------------------------------------- loaders (3 warps)
+    const int lt = tid - 9 * 32;
     const float inv_vmax = vmax > 0.f ? 1.f / vmax : 0.f;
-    constexpr int RC = DH / 16;  // 16-byte pieces of a row
-    uint4 kr[Cfg::LOADS], vr[Cfg::LOADS];
+    uint8_t* rawk = smem + Cfg::RAWK_OFF;
+    uint8_t* rawv = smem + Cfg::RAWV_OFF;
+    const int segs = BN >> c.p_shift;              // pages of a tile (1 to 8)
+    const uint32_t seg_bytes = static_cast<uint32_t>(c.P) * DH;
+    // Warp 9 copies the codes of step j's pages into raw slot j % RS. A page is
+    // copied whole: its slots past the end exist, whatever they hold.
+    auto fetch = [&](const uint8_t* pool, uint8_t* raw, uint64_t* full, int j) {
+      const int key = k0 + j * BN + (lane << c.p_shift);
+      int page = -1;
+      if (lane < segs && key < k1) page = kv8_page(c, b, key >> c.p_shift);
+      const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
+      const int slot = j % Cfg::RS;
+      if (lane == 0) mbar_arrive_expect_tx(&full[slot], __popc(live) * seg_bytes);
+      __syncwarp();
+      if (page >= 0)
+        bulk_load(raw + slot * Cfg::RAW + lane * seg_bytes,
+                  pool + (static_cast<int64_t>(page) * c.H + h) * seg_bytes, seg_bytes,
+                  &full[slot]);
+    };
+    // Lanes 0-7 of warp 9 hold the scales of the next step's groups of 16 keys.
     float sc_k = 0.f, sc_r = 0.f;
     bool sc_bad = false;
-    auto load = [&](const uint8_t* pool, int key0, uint4 (&r)[Cfg::LOADS]) {
-#pragma unroll
-      for (int i = 0; i < Cfg::LOADS; ++i) {
-        const int id = i * 128 + lt;
-        const int key = key0 + id / RC;
-        r[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (key < k1) {
-          const int page = kv8_page(c, b, key >> c.p_shift);
-          if (page >= 0)
-            r[i] = __ldg(reinterpret_cast<const uint4*>(
-                       pool + ((static_cast<int64_t>(page) * c.H + h) * c.P + (key & (c.P - 1))) * DH) +
-                   id % RC);
-        }
-      }
-    };
-    auto put = [&](uint8_t* tile, const uint4 (&r)[Cfg::LOADS]) {
-#pragma unroll
-      for (int i = 0; i < Cfg::LOADS; ++i) {
-        const int id = i * 128 + lt;
-        kv8_put16(tile, BN, id / RC, id % RC, r[i], c.fmt);
-      }
-      fence_proxy_async_smem();
-    };
     auto load_scale = [&](int key0) {
-      if (lt >= Cfg::GROUPS) return;
-      const int key = key0 + lt * 16;
+      if (lane >= Cfg::GROUPS) return;
+      const int key = key0 + lane * 16;
       sc_k = sc_r = 0.f;
       sc_bad = false;
       if (key < k1) {
@@ -524,42 +579,83 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         }
       }
     };
-    load_scale(k0);
-    load(c.k, k0, kr);
-    load(c.v, k0, vr);
-    for (int j = 0; j < n_steps; ++j) {
-      const int st = j & 1;
-      const uint32_t eph = ((j >> 1) & 1) ^ 1;  // phase of the release two steps back
-      if (j >= 2 && !mbar_wait(&k_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)) break;
-      put(sK + st * Cfg::KV_BYTES, kr);
-      if (lt < 32) {
-        const uint32_t bad = __ballot_sync(0xffffffffu, sc_bad);
-        const uint32_t spoiled = __ballot_sync(0xffffffffu, sc_r != sc_r);
-        if (lt < Cfg::GROUPS) {
-          s_sc[j & 3].ks[lt] = sc_k;
-          s_sc[j & 3].ratio[lt] = sc_r == sc_r ? sc_r : 0.f;
-        }
-        if (lt == 0) {
-          s_sc[j & 3].bad = bad;
-          s_sc[j & 3].spoiled = spoiled;
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[st]);
-      const int next = k0 + (j + 1) * BN;
-      if (j + 1 < n_steps) {
-        load_scale(next);
-        load(c.k, next, kr);
-      }
-      if (j >= 2 && !mbar_wait(&v_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)) break;
-      put(sV + st * Cfg::KV_BYTES, vr);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[st]);
-      if (j + 1 < n_steps) load(c.v, next, vr);
+    int fetched_k = 0, fetched_v = 0;
+    if (warp == 9) {
+      load_scale(k0);
+      for (; fetched_k < Cfg::RS && fetched_k < n_steps; ++fetched_k)
+        fetch(c.k, rawk, rk_full, fetched_k);
+      for (; fetched_v < Cfg::RS && fetched_v < n_steps; ++fetched_v)
+        fetch(c.v, rawv, rv_full, fetched_v);
     }
-  } else {
+    for (int j = 0; j < n_steps; ++j) {
+      const int st = j & 1, slot = j % Cfg::RS;
+      const uint32_t eph = ((j >> 1) & 1) ^ 1;  // phase of the release two steps back
+      const uint32_t rph = (j / Cfg::RS) & 1;
+      bool ok = mbar_wait(&rk_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) &&
+                (j < 2 || mbar_wait(&k_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA));
+      if (ok) {
+        if (c.fmt == KF_KV8_INT8)
+          kv8_expand<DH, KF_KV8_INT8, false>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
+        else
+          kv8_expand<DH, KF_KV8_E4M3, false>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
+        fence_proxy_async_smem();
+      }
+      PromptScales& sc = s_sc[j & 3];
+      if (warp == 9 && ok) {
+        const uint32_t bad = __ballot_sync(0xffffffffu, sc_bad);
+        const uint32_t spoiled_k = __ballot_sync(0xffffffffu, sc_k != sc_k);
+        const uint32_t spoiled_v = __ballot_sync(0xffffffffu, sc_r != sc_r);
+        if (lane < Cfg::GROUPS) {
+          sc.ks[lane] = sc_k == sc_k ? sc_k : 0.f;
+          sc.ratio[lane] = sc_r == sc_r ? sc_r : 0.f;
+        }
+        if (lane == 0) {
+          sc.bad = bad;
+          sc.spoiled_k = spoiled_k;
+          sc.spoiled_v = spoiled_v;
+        }
+      }
+      if (named_bar_or(1, 96, !ok)) break;  // all three warps leave together
+      if (lt == 0) mbar_arrive(&k_full[st]);
+      if (warp == 9) {
+        if (fetched_k < n_steps) fetch(c.k, rawk, rk_full, fetched_k++);
+        if (j + 1 < n_steps) load_scale(k0 + (j + 1) * BN);
+      }
+      ok = mbar_wait(&rv_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) &&
+           (j < 2 || mbar_wait(&v_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA));
+      if (ok) {
+        // An e4m3 NaN in a slot past the end must not meet a weight of 0.
+        const int rows = k1 - (k0 + j * BN);
+        const uint32_t bad = sc.bad;
+        const bool whole = rows >= BN && bad == 0;
+        const uint8_t* raw = rawv + slot * Cfg::RAW;
+        uint8_t* tile = sV + st * Cfg::KV_BYTES;
+        if (c.fmt == KF_KV8_INT8) {
+          if (whole)
+            kv8_expand<DH, KF_KV8_INT8, false>(raw, tile, lt, 0, 0);
+          else
+            kv8_expand<DH, KF_KV8_INT8, true>(raw, tile, lt, rows, bad);
+        } else {
+          if (whole)
+            kv8_expand<DH, KF_KV8_E4M3, false>(raw, tile, lt, 0, 0);
+          else
+            kv8_expand<DH, KF_KV8_E4M3, true>(raw, tile, lt, rows, bad);
+        }
+        fence_proxy_async_smem();
+      }
+      if (named_bar_or(1, 96, !ok)) break;
+      if (lt == 0) mbar_arrive(&v_full[st]);
+      if (warp == 9 && fetched_v < n_steps) fetch(c.v, rawv, rv_full, fetched_v++);
+    }
+    if (warp == 9 && lane == 0) {
+      // no copy may be in flight when the CTA leaves
+      for (int j = fetched_k > Cfg::RS ? fetched_k - Cfg::RS : 0; j < fetched_k; ++j)
+        mbar_wait_drain(&rk_full[j % Cfg::RS], (j / Cfg::RS) & 1, KF_DEV_WAIT_TIMEOUT_TMA);
+      for (int j = fetched_v > Cfg::RS ? fetched_v - Cfg::RS : 0; j < fetched_v; ++j)
+        mbar_wait_drain(&rv_full[j % Cfg::RS], (j / Cfg::RS) & 1, KF_DEV_WAIT_TIMEOUT_TMA);
+    }
+  } else if (warp < 4 * NT) {
     // -------------------------------------------------- softmax
-    set_max_registers<true, 176>();
     const int t = warp >> 2;
     const int quarter = warp & 3;
     const int row = row0 + t * BM + quarter * 32 + lane;
@@ -567,42 +663,89 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
     const int limit = (row < w.rows && tok < count) ? (causal ? min(len + tok + 1, end) : end) : 0;
     const float qf = row < w.rows ? __ldg(w.qf + static_cast<int64_t>(bh) * w.rows + row) : 0.f;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t t_s = t_row + t * 128;
     const uint32_t t_o = t_row + Cfg::O_COL + t * Cfg::O_STRIDE;
+    const uint32_t t_m = t_row + Cfg::M_COL + t * Cfg::O_STRIDE;
     float ref = -INFINITY, sum = 0.f;
-    bool ok = true, nan_row = false;
+    bool ok = true, nan_k = false, nan_v = false;
+    auto scale_cols = [&](uint32_t at, float alpha) {
+#pragma unroll 1
+      for (int cc = 0; cc < Cfg::O_STRIDE / 16; ++cc) {
+        uint32_t o[16];
+        tmem_ld16(at + cc * 16, o);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * alpha);
+        tmem_st16(at + cc * 16, o);
+      }
+      tmem_wait_st();
+    };
+#pragma unroll 1
     for (int j = 0; j < n_steps; ++j) {
       const int st = j & 1;
+      const int buf = NT == 1 ? st : t;
+      const uint32_t t_s = t_row + buf * 128;
+      const uint32_t sph = NT == 1 ? (j >> 1) & 1 : j & 1;
       if (!mbar_wait(&k_full[st], (j >> 1) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX) ||
-          !mbar_wait(&s_full[t], j & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX)) {
+          !mbar_wait(&s_full[buf], sph, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX)) {
         ok = false;
         break;
       }
       tc_fence_after();
       if (lane == 0) mbar_arrive(&k_empty[st]);
-      const PromptScales& sc = s_sc[j & 3];
-      const float* ks = sc.ks;
-      const float* ratio = sc.ratio;
-      const uint32_t bad = sc.bad;
-      const uint32_t spoiled = sc.spoiled;
-      const int key0 = k0 + j * BN;
-      const int lim = min(limit, k1) - key0;
-      const bool mask = __any_sync(0xffffffffu, lim < BN) || bad;
-      // Only rows that see a token of a spoiled page are NaN: decided per row,
-      // since 0 * NaN in the product would reach rows that do not.
-      if (spoiled && lim > 16 * (__ffs(static_cast<int>(spoiled)) - 1)) nan_row = true;
-      float s[64];
-      float mx = -INFINITY;
-      if constexpr (BN == 128) {
-        prompt_scores<BN>(t_s, qf, ks, bad, mask, lim, s);
-        mx = max64(s);
-        prompt_scores<BN>(t_s + 64, qf, ks + 4, bad >> 4, mask, lim - 64, s);
-      } else {
-        prompt_scores<BN>(t_s, qf, ks, bad, mask, lim, s);
+      // Two tiles: S of this step was issued after P V of the last one, so O is
+      // at rest. One tile: S runs ahead, so wait for that product.
+      auto at_rest = [&]() -> bool {
+        if (NT == 2) return true;
+        ok = mbar_wait(o_done, (j - 1) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX);
+        tc_fence_after();
+        return ok;
+      };
+      const bool flush = PL == 2 && j > 0 && j % Cfg::FLUSH == 0;
+      const bool have_m = PL == 2 && j >= Cfg::FLUSH;  // M holds something
+      if (flush) {
+        if (!at_rest()) break;
+#pragma unroll
+        for (int cc = 0; cc < Cfg::O_STRIDE / 16; ++cc) {
+          uint32_t o[16], m[16];
+          tmem_ld16(t_o + cc * 16, o);
+          if (j > Cfg::FLUSH) {
+            tmem_ld16(t_m + cc * 16, m);
+#pragma unroll
+            for (int u = 0; u < 16; ++u)
+              o[u] = __float_as_uint(__uint_as_float(o[u]) + __uint_as_float(m[u]));
+          }
+          tmem_st16(t_m + cc * 16, o);
+        }
+        tmem_wait_st();
       }
-      mx = fmaxf(mx, max64(s));
+      float s[128];
+      tmem_ld128(t_s, s);
+      const PromptScales& sc = s_sc[j & 3];
+      const int lim = min(limit, k1) - (k0 + j * BN);
+      const uint32_t bad = sc.bad;
+      if (__any_sync(0xffffffffu, lim < BN) || bad) {
+        uint32_t kw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          kw[i] = ((bad >> (2 * i)) & 1u ? 0u : 0x0000ffffu) |
+                  ((bad >> (2 * i + 1)) & 1u ? 0u : 0xffff0000u);
+        mask_scores<128>(s, kw, lim);
+      }
+      if (sc.spoiled_k | sc.spoiled_v) {
+        // Rows that see a token of a page whose scale is NaN are NaN: decided
+        // per row, since NaN in a product would reach rows that do not.
+        if (sc.spoiled_k && lim > 16 * (__ffs(static_cast<int>(sc.spoiled_k)) - 1)) nan_k = true;
+        if (sc.spoiled_v && lim > 16 * (__ffs(static_cast<int>(sc.spoiled_v)) - 1)) nan_v = true;
+      }
+      // Factors to log2 units, never 0: a masked score times 0 would be NaN.
+      float f[8];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) f[g] = fmaxf(qf * sc.ks[g], 1e-38f);
+      // Page scales are positive, so a group's maximum scales with it.
+      float mx = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) mx = fmaxf(mx, max16(s + 16 * g) * f[g]);
       // The reference moves when the maximum has outgrown it by more than the
-      // slack. S of this step was issued after P V of the last, so O is at rest.
+      // slack.
       float alpha = 1.f;
       const bool move = mx > ref + (KV8_BIAS + KV8_SLACK);
       if (move) {
@@ -611,36 +754,62 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         sum *= alpha;
       }
       if (j > 0 && __any_sync(0xffffffffu, move)) {
-#pragma unroll
-        for (int cc = 0; cc < (DH + 31) / 32; ++cc) {
-          float o[32];  // head_dim 16: the columns past O are unused
-          tmem_ld32(t_o + cc * 32, o);
-#pragma unroll
-          for (int u = 0; u < 32; ++u) o[u] *= alpha;
-          tmem_st32(t_o + cc * 32, o);
-        }
+        if (!at_rest()) break;
+        if (!flush) scale_cols(t_o, alpha);
+        if (have_m) scale_cols(t_m, alpha);
       }
       const float neg = ref == -INFINITY ? 0.f : -ref;
-      if constexpr (BN == 128) {
-        sum += prompt_weights<PL>(s, neg, ratio + 4, t_s + 64);
-        prompt_scores<BN>(t_s, qf, ks, bad, mask, lim, s);
+      const uint64_t nr = f2_pack(neg, neg);
+      uint64_t acc[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+      for (int part = 0; part < 4; ++part) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const int k = 32 * part + 2 * u;
+          const float fg = f[k >> 4];
+          float x, y;
+          f2_unpack(f2_fma(f2_pack(s[k], s[k + 1]), f2_pack(fg, fg), nr), x, y);
+          x = fast_exp2(x);
+          y = fast_exp2(y);
+          acc[u & 1] = f2_add(acc[u & 1], f2_pack(x, y));
+          const float r = sc.ratio[k >> 4];
+          f2_unpack(f2_mul(f2_pack(x, y), f2_pack(r, r)), x, y);
+          hi[u] = pack_half2(x, y);
+          if constexpr (PL == 2) lo[u] = pack_half2_rest(x, y, hi[u]);
+        }
+        const uint32_t at = t_s + (part >> 1) * 64 + (part & 1) * 16;
+        tmem_st16(at, hi);
+        if constexpr (PL == 2) tmem_st16(at + 32, lo);
       }
-      sum += prompt_weights<PL>(s, neg, ratio, t_s);
+      float x0, x1, x2, x3;
+      f2_unpack(acc[0], x0, x1);
+      f2_unpack(acc[1], x2, x3);
+      sum += (x0 + x1) + (x2 + x3);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
+      if (lane == 0) mbar_arrive(&p_full[buf]);
     }
     if (ok && mbar_wait(&o_final[t], 0, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX)) {
       tc_fence_after();
       const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
       const int hq = h * G + row - tok * G;
+      const float nan = __uint_as_float(0x7fc00000u);
+      if (nan_k) sum = nan;
       float f = alone ? vmax / sum : vmax;  // not used where sum is 0
-      if (nan_row) f = __uint_as_float(0x7fc00000u);
+      if (nan_v) f = nan;
+      const bool have_m = PL == 2 && n_steps > Cfg::FLUSH;
 #pragma unroll
       for (int cc = 0; cc < (DH + 31) / 32; ++cc) {
         float o[32];
         tmem_ld32(t_o + cc * 32, o);
+        if (have_m) {
+          float m[32];
+          tmem_ld32(t_m + cc * 32, m);
+#pragma unroll
+          for (int u = 0; u < 32; ++u) o[u] += m[u];
+        }
         if (row >= w.rows) continue;
 #pragma unroll
         for (int u = 0; u < 32; ++u) o[u] = sum == 0.f ? 0.f : o[u] * f;
@@ -650,7 +819,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         } else {
           float4* p = reinterpret_cast<float4*>(w.part + (at * w.chunks + chunk) * DH + cc * 32);
 #pragma unroll
-          for (int u = 0; u < NC; u += 4) p[u >> 2] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+          for (int u = 0; u < NC; u += 4)
+            p[u >> 2] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
         }
       }
       if (row < w.rows) {
@@ -669,7 +839,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) {
+  if (warp == 8) {
     __syncwarp();
     tmem_dealloc(tmem_base, 512);
   }
