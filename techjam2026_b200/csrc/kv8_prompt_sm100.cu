@@ -16,10 +16,13 @@
 //                   bytes: rows are keys); they also stage the scales. (Codes
 //                   fetched through registers with a page lookup per piece held
 //                   the whole kernel at 6000 clocks a step.)
-// TMEM: S0 | S1 (128 columns each, P in place), O0 | O1. For each tile the
-// order is P V(j), then S(j + 1): the pipe runs in issue order, so a softmax
-// that sees S(j + 1) knows O holds P V(j) and may rescale it at once, and while
-// one tile's products run the other tile's softmax has the exponential unit.
+// TMEM: S0 | S1 (128 columns each), O0 | O1, and P. At head_dim <= 64 with 16-bit
+// q, P has 64 columns of its own per tile, and S(j + 1) is issued as soon as
+// step j's scores are in registers, so it is there when their softmax ends.
+// Elsewhere P overwrites S and each tile's order is P V(j), then S(j + 1): the
+// pipe runs in issue order, so a softmax that sees S(j + 1) knows O holds P V(j)
+// and may rescale it at once, and while one tile's products run the other
+// tile's softmax has the exponential unit.
 // What bounds it: the exponentials, 16 a clock and SM: 2048 clocks for two
 // tiles against 128 keys, where the products take 1024 at head_dim 64.
 //
@@ -170,26 +173,38 @@ __device__ __forceinline__ void kv8_store_run(void* out, int64_t at, int dtype, 
 template <int DH, int FMT, bool ZERO>
 __device__ __forceinline__ void kv8_expand(const uint8_t* raw, uint8_t* tile, int lt, int rows,
                                            uint32_t bad) {
-  constexpr int RC = DH / 16, RP = 96 / RC;  // pieces of a row, rows of a pass
-  static_assert(RP % 4 == 0, "swizzle phase");
+  constexpr int CW = DH < 64 ? DH : 64;        // columns of a half
+  constexpr int RC = CW / 16, RP = 96 / RC;    // pieces of a row of a half, rows of a pass
+  constexpr int N = (128 + RP - 1) / RP;
+  static_assert(RP % 8 == 0, "swizzle phase");
   const int c16 = lt % RC, r0 = lt / RC;
-  uint8_t* dst = tile + (c16 >> 2) * 128 * 128 + r0 * 128;
-  const uint32_t ch = static_cast<uint32_t>((c16 & 3) * 2 ^ (r0 & 7)) << 4;
+  const uint32_t ch = static_cast<uint32_t>((c16 * 2) ^ (r0 & 7)) << 4;
+  const bool last = r0 + (N - 1) * RP < 128;   // the last pass has rows for some lanes only
 #pragma unroll
-  for (int i = 0; i < (128 + RP - 1) / RP; ++i) {
-    const int r = r0 + i * RP;
-    if (128 % RP && r >= 128) break;
-    uint4 w = *reinterpret_cast<const uint4*>(raw + (lt + i * 96) * 16);
-    if (ZERO && (r >= rows || ((bad >> (r >> 4)) & 1u))) w = make_uint4(0u, 0u, 0u, 0u);
-    uint32_t h[8];
-    kv8_cvt4<FMT>(w.x, h[0], h[1]);
-    kv8_cvt4<FMT>(w.y, h[2], h[3]);
-    kv8_cvt4<FMT>(w.z, h[4], h[5]);
-    kv8_cvt4<FMT>(w.w, h[6], h[7]);
-    // r & 7 moves by RP & 7, which is 0 or 4: the swizzle flips one bit
-    const uint32_t at = ch ^ (((i * RP) & 4) << 4);
-    *reinterpret_cast<uint4*>(dst + i * RP * 128 + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(dst + i * RP * 128 + (at ^ 16u)) = make_uint4(h[4], h[5], h[6], h[7]);
+  for (int x = 0; x < DH / CW; ++x) {
+    // Two halves: even rows take half x, odd rows the other one, so that eight
+    // lanes touch all banks both when they read and when they write.
+    const int half = DH > 64 ? x ^ (r0 & 1) : 0;
+    const uint8_t* src = raw + r0 * DH + half * 64 + c16 * 16;
+    uint8_t* dst = tile + half * 128 * 128 + r0 * 128;
+    uint4 w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < N - 1 || last) w[i] = *reinterpret_cast<const uint4*>(src + i * RP * DH);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i == N - 1 && !last) break;
+      const int r = r0 + i * RP;
+      if (ZERO && (r >= rows || ((bad >> (r >> 4)) & 1u))) w[i] = make_uint4(0u, 0u, 0u, 0u);
+      uint32_t h[8];
+      kv8_cvt4<FMT>(w[i].x, h[0], h[1]);
+      kv8_cvt4<FMT>(w[i].y, h[2], h[3]);
+      kv8_cvt4<FMT>(w[i].z, h[4], h[5]);
+      kv8_cvt4<FMT>(w[i].w, h[6], h[7]);
+      *reinterpret_cast<uint4*>(dst + i * RP * 128 + ch) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(dst + i * RP * 128 + (ch ^ 16u)) =
+          make_uint4(h[4], h[5], h[6], h[7]);
+    }
   }
 }
 
@@ -254,12 +269,17 @@ struct PromptCfg {
   // float64, 2e-9 of relative error per key, 4e-6 after 2048 keys; 5e-7 after 256.
   static constexpr int FLUSH = 2;
   static constexpr int M_COL = O_COL + NT * O_STRIDE;
+  // With room in TMEM P has columns of its own, and S of the next step is
+  // computed while this step's softmax runs; otherwise P overwrites S.
+  static constexpr bool SEP = NT == 2 && PL == 1 && DH <= 64;
+  static constexpr int P_COL = O_COL + NT * O_STRIDE;
   static constexpr int ROWS = NT * BM;
   // Twelve warps leave 168 registers a thread: a softmax row's 128 scores and
   // what goes with them.
   static constexpr int THREADS = 12 * 32;
   static_assert(SMEM <= 232448, "smem");
   static_assert((PL == 2 ? M_COL : O_COL) + NT * O_STRIDE <= 512, "TMEM");
+  static_assert(!SEP || P_COL + 128 <= 512, "TMEM");
 };
 
 // Scales of the keys of one step, by groups of 16 keys.
@@ -344,12 +364,13 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   uint64_t* v_empty = bars + 7;   // [ST] P V of all tiles done
   uint64_t* s_full = bars + 9;    // [2] by S buffer
   uint64_t* p_full = bars + 11;   // [2] by S buffer, 4 warps
-  uint64_t* o_done = bars + 13;   // one tile: P V of a step done
-  uint64_t* o_final = bars + 14;  // [2]
-  uint64_t* drain = bars + 16;
-  uint64_t* rk_full = bars + 17;  // [RS] raw codes of K, of V: their bytes
-  uint64_t* rv_full = bars + 19;  // [RS]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  uint64_t* o_done = bars + 13;   // [2] P V of a step done (not in place: by tile)
+  uint64_t* o_final = bars + 15;  // [2]
+  uint64_t* drain = bars + 17;
+  uint64_t* rk_full = bars + 18;  // [RS] raw codes of K, of V: their bytes
+  uint64_t* rv_full = bars + 20;  // [RS]
+  uint64_t* s_free = bars + 22;   // [2] S read into registers (P apart), 4 warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_vmax = reinterpret_cast<float*>(tmem_slot + 2);  // [12]
   PromptScales* s_sc = reinterpret_cast<PromptScales*>(smem + Cfg::SC_OFF);
@@ -408,8 +429,9 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
       mbar_init(&o_final[s], 1);
+      mbar_init(&o_done[s], 1);
+      mbar_init(&s_free[s], 4);
     }
-    mbar_init(o_done, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -470,6 +492,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       };
       // O of tile t += P in S buffer `buf` times the V tile of `stage`.
       auto issue_o = [&](int t, int buf, int stage, bool fresh) {
+        const uint32_t p_base = tmem_base + (Cfg::SEP ? Cfg::P_COL + t * 64 : buf * 128);
 #pragma unroll
         for (int pl = PL - 1; pl >= 0; --pl)
 #pragma unroll
@@ -477,7 +500,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
             const uint64_t bd = make_smem_desc(sVa + stage * Cfg::KV_BYTES + kk * 16 * 128, BN * 128,
                                                1024, KF_SWIZZLE_128B);
             mma_f16_ts(tmem_base + Cfg::O_COL + t * Cfg::O_STRIDE,
-                       tmem_base + buf * 128 + (kk >> 2) * 64 + pl * 32 + (kk & 3) * 8, bd, idesc_o,
+                       p_base + (Cfg::SEP ? kk * 8 : (kk >> 2) * 64 + pl * 32 + (kk & 3) * 8), bd, idesc_o,
                        (!fresh || pl < PL - 1 || kk > 0) ? 1u : 0u);
           }
       };
@@ -488,7 +511,47 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         for (int t = 0; t < NT; ++t) issue_s(t, t, 0);
         mma_commit(&k_empty[0]);
       }
-      for (int j = 0; j < n_steps && ok; ++j) {
+      if (Cfg::SEP && ok) {
+        // Whatever is ready goes next: P V of a tile whose P is written, S of the
+        // next step of a tile whose scores are in registers. The last of the two
+        // tiles to use a K or V stage releases it.
+        int s_next[2] = {1, 1}, p_next[2] = {0, 0};
+        long long idle = clock64();
+        while (p_next[0] < n_steps || p_next[1] < n_steps) {
+          bool progress = false;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int js = s_next[t], jp = p_next[t];
+            if (js < n_steps && mbar_test_wait(&s_free[t], (js - 1) & 1) &&
+                mbar_test_wait(&k_full[js & 1], (js >> 1) & 1)) {
+              tc_fence_after();
+              issue_s(t, t, js & 1);
+              s_next[t] = js + 1;
+              if (s_next[t ^ 1] > js) mma_commit(&k_empty[js & 1]);
+              progress = true;
+            }
+            if (jp < n_steps && mbar_test_wait(&p_full[t], jp & 1) &&
+                mbar_test_wait(&v_full[jp & 1], (jp >> 1) & 1)) {
+              tc_fence_after();
+              issue_o(t, t, jp & 1, jp == 0);
+              mma_commit(jp + 1 < n_steps ? &o_done[t] : &o_final[t]);
+              p_next[t] = jp + 1;
+              if (p_next[t ^ 1] > jp) mma_commit(&v_empty[jp & 1]);
+              progress = true;
+            }
+          }
+          if (progress) {
+            idle = clock64();
+          } else if (*abort_flag) {
+            break;
+          } else if (clock64() - idle > wait_limit()) {
+            *abort_flag = 1;
+            record_device_status(KF_DEV_WAIT_TIMEOUT_MMA);
+            break;
+          }
+        }
+      }
+      for (int j = 0; j < n_steps && ok && !Cfg::SEP; ++j) {
         const int st = j & 1, nx = st ^ 1;
         const uint32_t ph = (j >> 1) & 1, nph = ((j + 1) >> 1) & 1;
         const bool fresh = PL == 2 ? j % Cfg::FLUSH == 0 : j == 0;
@@ -545,47 +608,63 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
     uint8_t* rawv = smem + Cfg::RAWV_OFF;
     const int segs = BN >> c.p_shift;              // pages of a tile (1 to 8)
     const uint32_t seg_bytes = static_cast<uint32_t>(c.P) * DH;
-    // Warp 9 copies the codes of step j's pages into raw slot j % RS. A page is
-    // copied whole: its slots past the end exist, whatever they hold.
-    auto fetch = [&](const uint8_t* pool, uint8_t* raw, uint64_t* full, int j) {
-      const int key = k0 + j * BN + (lane << c.p_shift);
-      int page = -1;
-      if (lane < segs && key < k1) page = kv8_page(c, b, key >> c.p_shift);
-      const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
-      const int slot = j % Cfg::RS;
-      if (lane == 0) mbar_arrive_expect_tx(&full[slot], __popc(live) * seg_bytes);
-      __syncwarp();
-      if (page >= 0)
-        bulk_load(raw + slot * Cfg::RAW + lane * seg_bytes,
-                  pool + (static_cast<int64_t>(page) * c.H + h) * seg_bytes, seg_bytes,
-                  &full[slot]);
+    // Lane g < 8 of warp 9 keeps the pages of group g (16 keys) of the steps
+    // ahead: the table entry of step j + RS + 1 is loaded while step j runs, so
+    // no copy waits for it. pg[i]: step j + i, -1 where there is no key or the
+    // entry is no page (recorded).
+    int pg[Cfg::RS + 1];
+    int entry = -1;
+    auto load_entry = [&](int j) {
+      const int key = k0 + j * BN + lane * 16;
+      entry = -2;
+      if (lane < Cfg::GROUPS && key < k1) entry = __ldg(c.table + b * c.ld_table + (key >> c.p_shift));
     };
-    // Lanes 0-7 of warp 9 hold the scales of the next step's groups of 16 keys.
-    float sc_k = 0.f, sc_r = 0.f;
-    bool sc_bad = false;
-    auto load_scale = [&](int key0) {
-      if (lane >= Cfg::GROUPS) return;
-      const int key = key0 + lane * 16;
-      sc_k = sc_r = 0.f;
-      sc_bad = false;
-      if (key < k1) {
-        const int page = kv8_page(c, b, key >> c.p_shift);
-        sc_bad = page < 0;
-        if (page >= 0) {
-          const float2 s = __ldg(reinterpret_cast<const float2*>(
-              c.scale + 2 * (static_cast<int64_t>(page) * c.H + h)));
-          sc_k = s.x;
-          sc_r = s.y * inv_vmax;
-        }
-      }
+    auto take_entry = [&]() -> int {
+      if (entry == -2) return -2;                       // no key
+      if (entry >= 0 && entry < c.pages) return entry;
+      record_device_status(KF_DEV_BAD_KV_PAGE);
+      return -1;                                        // a refused page
+    };
+    // Copies the codes of the pages in lanes 0-7 into a raw slot. A page is
+    // copied whole: its slots past the end exist, whatever they hold.
+    auto fetch = [&](const uint8_t* pool, uint8_t* raw, uint64_t* full, int page8) {
+      const int page = __shfl_sync(0xffffffffu, page8, (lane << (c.p_shift - 4)) & 31);
+      const bool live = lane < segs && page >= 0;
+      const uint32_t n = __popc(__ballot_sync(0xffffffffu, live));
+      if (lane == 0) mbar_arrive_expect_tx(full, n * seg_bytes);
+      __syncwarp();
+      if (live)
+        bulk_load(raw + lane * seg_bytes, pool + (static_cast<int64_t>(page) * c.H + h) * seg_bytes,
+                  seg_bytes, full);
+    };
+    float2 scale = make_float2(0.f, 0.f);
+    auto load_scale = [&](int page8) {
+      scale = make_float2(0.f, 0.f);
+      if (page8 >= 0)
+        scale = __ldg(reinterpret_cast<const float2*>(
+            c.scale + 2 * (static_cast<int64_t>(page8) * c.H + h)));
     };
     int fetched_k = 0, fetched_v = 0;
     if (warp == 9) {
-      load_scale(k0);
-      for (; fetched_k < Cfg::RS && fetched_k < n_steps; ++fetched_k)
-        fetch(c.k, rawk, rk_full, fetched_k);
-      for (; fetched_v < Cfg::RS && fetched_v < n_steps; ++fetched_v)
-        fetch(c.v, rawv, rv_full, fetched_v);
+#pragma unroll
+      for (int i = 0; i <= Cfg::RS; ++i) {
+        load_entry(i);
+        pg[i] = take_entry();
+      }
+      load_entry(Cfg::RS + 1);
+      load_scale(pg[0]);
+#pragma unroll
+      for (int i = 0; i < Cfg::RS; ++i)
+        if (i < n_steps) {
+          fetch(c.k, rawk + i * Cfg::RAW, &rk_full[i], pg[i]);
+          ++fetched_k;
+        }
+#pragma unroll
+      for (int i = 0; i < Cfg::RS; ++i)
+        if (i < n_steps) {
+          fetch(c.v, rawv + i * Cfg::RAW, &rv_full[i], pg[i]);
+          ++fetched_v;
+        }
     }
     for (int j = 0; j < n_steps; ++j) {
       const int st = j & 1, slot = j % Cfg::RS;
@@ -602,7 +681,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       }
       PromptScales& sc = s_sc[j & 3];
       if (warp == 9 && ok) {
-        const uint32_t bad = __ballot_sync(0xffffffffu, sc_bad);
+        const float sc_k = scale.x, sc_r = scale.y * inv_vmax;
+        const uint32_t bad = __ballot_sync(0xffffffffu, lane < Cfg::GROUPS && pg[0] == -1);
         const uint32_t spoiled_k = __ballot_sync(0xffffffffu, sc_k != sc_k);
         const uint32_t spoiled_v = __ballot_sync(0xffffffffu, sc_r != sc_r);
         if (lane < Cfg::GROUPS) {
@@ -618,8 +698,11 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       if (named_bar_or(1, 96, !ok)) break;  // all three warps leave together
       if (lt == 0) mbar_arrive(&k_full[st]);
       if (warp == 9) {
-        if (fetched_k < n_steps) fetch(c.k, rawk, rk_full, fetched_k++);
-        if (j + 1 < n_steps) load_scale(k0 + (j + 1) * BN);
+        if (fetched_k < n_steps) {
+          fetch(c.k, rawk + slot * Cfg::RAW, &rk_full[slot], pg[Cfg::RS]);
+          ++fetched_k;
+        }
+        load_scale(pg[1]);
       }
       ok = mbar_wait(&rv_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) &&
            (j < 2 || mbar_wait(&v_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA));
@@ -645,7 +728,16 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       }
       if (named_bar_or(1, 96, !ok)) break;
       if (lt == 0) mbar_arrive(&v_full[st]);
-      if (warp == 9 && fetched_v < n_steps) fetch(c.v, rawv, rv_full, fetched_v++);
+      if (warp == 9) {
+        if (fetched_v < n_steps) {
+          fetch(c.v, rawv + slot * Cfg::RAW, &rv_full[slot], pg[Cfg::RS]);
+          ++fetched_v;
+        }
+#pragma unroll
+        for (int i = 0; i < Cfg::RS; ++i) pg[i] = pg[i + 1];
+        pg[Cfg::RS] = take_entry();
+        load_entry(j + Cfg::RS + 2);
+      }
     }
     if (warp == 9 && lane == 0) {
       // no copy may be in flight when the CTA leaves
@@ -691,11 +783,11 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       }
       tc_fence_after();
       if (lane == 0) mbar_arrive(&k_empty[st]);
-      // Two tiles: S of this step was issued after P V of the last one, so O is
-      // at rest. One tile: S runs ahead, so wait for that product.
+      // In place with two tiles, S of this step was issued after P V of the last
+      // one, so O is at rest. Otherwise S runs ahead: wait for that product.
       auto at_rest = [&]() -> bool {
-        if (NT == 2) return true;
-        ok = mbar_wait(o_done, (j - 1) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX);
+        if (NT == 2 && !Cfg::SEP) return true;
+        ok = mbar_wait(&o_done[t], (j - 1) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX);
         tc_fence_after();
         return ok;
       };
@@ -719,6 +811,11 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       }
       float s[128];
       tmem_ld128(t_s, s);
+      if (Cfg::SEP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);
+      }
       const PromptScales& sc = s_sc[j & 3];
       const int lim = min(limit, k1) - (k0 + j * BN);
       const uint32_t bad = sc.bad;
@@ -753,8 +850,10 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         ref = mx - KV8_BIAS;
         sum *= alpha;
       }
-      if (j > 0 && __any_sync(0xffffffffu, move)) {
-        if (!at_rest()) break;
+      const bool rescale = j > 0 && __any_sync(0xffffffffu, move);
+      if (Cfg::SEP ? j > 0 : rescale)
+        if (!at_rest()) break;       // (P apart: its columns are free then, too)
+      if (rescale) {
         if (!flush) scale_cols(t_o, alpha);
         if (have_m) scale_cols(t_m, alpha);
       }
@@ -778,7 +877,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
           hi[u] = pack_half2(x, y);
           if constexpr (PL == 2) lo[u] = pack_half2_rest(x, y, hi[u]);
         }
-        const uint32_t at = t_s + (part >> 1) * 64 + (part & 1) * 16;
+        const uint32_t at = Cfg::SEP ? t_row + Cfg::P_COL + t * 64 + part * 16
+                                     : t_s + (part >> 1) * 64 + (part & 1) * 16;
         tmem_st16(at, hi);
         if constexpr (PL == 2) tmem_st16(at + 32, lo);
       }
