@@ -7,14 +7,18 @@
 //
 // One CTA = one chunk of keys of one (sequence, kv head) for a tile of 16 query
 // rows (row = token * G + head of the group). Its four warps take the chunk's
-// groups of 16 keys in turn, each with its own running reference and sums,
-// joined in shared memory at the end. Codes go from global memory straight to
-// the registers of the lane that feeds them to the tensor core: a contraction
-// may order its terms freely, so the lane that holds k-slots {2t, 2t+1, 2t+8,
-// 2t+9} of mma.m16n8k16 simply owns the consecutive bytes of a K row (the
-// same ones of q), and consecutive bytes of four V rows, and no shared memory
-// or shuffle sits between the load and the product. 16 rows fill the m16
-// tile; the 128-row tensor-memory products would waste 7/8 of theirs here.
+// groups of 16 keys in turn, each with its own ring of groups in shared memory,
+// filled by asynchronous copies a few groups ahead, and its own running
+// reference and sums, joined in shared memory at the end. The lane that feeds a
+// code to the tensor core reads it: a contraction may order its terms freely,
+// so the lane that holds k-slots {2t, 2t+1, 2t+8, 2t+9} of mma.m16n8k16 owns
+// consecutive bytes of a K row (the same ones of q) and consecutive bytes of
+// four V rows; the 16-byte pieces of the ring are placed so that those reads
+// touch all banks. 16 rows fill the m16 tile; the 128-row tensor-memory
+// products would waste 7/8 of theirs here. RH = 1 serves at most 8 rows and
+// skips the softmax of the upper half of the tile.
+// (Codes loaded straight into registers, one group ahead, left 8 warps an SM
+// and 2.5 TB/s on 16 x 24k tokens of 8 kv heads of 128.)
 //
 // Numbers. Codes are exact in fp16. A q row is scaled by a power of two to
 // [2^14, 2^15) before it becomes one fp16 plane (16-bit q: nothing is lost
@@ -59,18 +63,28 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
 }
 
 template <int BYTES>
-__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+__device__ __forceinline__ void read_bytes(const uint8_t* p, uint32_t* w) {
   if constexpr (BYTES == 16) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   } else if constexpr (BYTES == 8) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x; w[1] = v.y;
   } else if constexpr (BYTES == 4) {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   } else {
-    w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
   }
+}
+
+__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -99,20 +113,26 @@ __device__ __forceinline__ float kv8_row_scale(float amax, float* inverse) {
 
 // The q fragments of 16 rows: lane (g, t) holds rows g and g + 8, the K bytes
 // it owns (see above). qf[r]: factor from the products to log2 units.
-template <int DH, int PL>
+template <int DH, int PL, int RH>
 struct QFrag {
   static constexpr int EPT = DH / 4 < 16 ? DH / 4 : 16;  // consecutive elements of a piece
   static constexpr int NPC = DH / 4 / EPT;               // pieces (64 elements apart)
   static constexpr int KS = DH / 16;                     // k-steps
-  uint32_t a[PL][KS][4];
-  float qf[2];
+  uint32_t a[PL][KS][4];  // RH = 1: rows g + 8 are zeros
+  float qf[RH];
 
   __device__ __forceinline__ void load(const KV8& c, const void* q, int64_t q_sb, int64_t q_sh,
                                        int64_t q_st, int dtype, bool vec, int b, int h, int G,
                                        int row0, int rows, float scale_log2) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if constexpr (RH == 1) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int pl = 0; pl < PL; ++pl) a[pl][s][1] = a[pl][s][3] = 0u;
+    }
+#pragma unroll
+    for (int r = 0; r < RH; ++r) {
       const int row = row0 + g + 8 * r;
       float x[NPC * EPT];
       float amax = 0.f;
@@ -159,19 +179,39 @@ struct QFrag {
   }
 };
 
+// A ring slot holds 16 keys: K rows, then V rows, as 16-byte pieces. Piece
+// `p` (row-major over 16 rows of DH bytes) goes to these places, so that the
+// eight lanes (16-byte reads) or sixteen (8-byte) of a read's phase fall on
+// different banks: K, 128-byte rows: odd rows swap their halves; V, 128-byte
+// rows: pieces are xored with row & 7 (a read takes rows 0, 2, 4, 6), 64-byte
+// rows: with twice the number of the 128-byte line.
+template <int DH>
+__device__ __forceinline__ int k_place(int p) {
+  if constexpr (DH == 128) return p ^ (((p >> 3) & 1) << 2);
+  return p;
+}
+template <int DH>
+__device__ __forceinline__ int v_place(int p) {
+  if constexpr (DH == 128) return p ^ ((p >> 3) & 7);
+  if constexpr (DH == 64) return p ^ (((p >> 3) & 3) << 1);
+  return p;
+}
+
 // Codes of K for 16 keys as one lane owns them: two n8 tiles of keys.
 template <int DH>
 struct KBytes {
   static constexpr int EPT = DH / 4 < 16 ? DH / 4 : 16;
   static constexpr int NPC = DH / 4 / EPT;
   uint32_t w[2][DH / 16];
-  __device__ __forceinline__ void load(const uint8_t* base) {  // base: the group's first row
+  __device__ __forceinline__ void read(const uint8_t* slot) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int p = 0; p < NPC; ++p)
-        load_bytes<EPT>(base + (8 * n + g) * DH + p * 64 + t * EPT, &w[n][p * (EPT / 4)]);
+      for (int p = 0; p < NPC; ++p) {
+        const int at = (8 * n + g) * DH + p * 64 + t * EPT;  // byte
+        read_bytes<EPT>(slot + k_place<DH>(at >> 4) * 16 + (at & 15), &w[n][p * (EPT / 4)]);
+      }
   }
 };
 template <int DH>
@@ -179,17 +219,30 @@ struct VBytes {
   static constexpr int VB = DH / 8;            // consecutive bytes of a row
   static constexpr int W = VB < 4 ? 1 : VB / 4;
   uint32_t w[4][W];                            // keys 2t, 2t+1, 8+2t, 9+2t
-  __device__ __forceinline__ void load(const uint8_t* base) {
+  __device__ __forceinline__ void read(const uint8_t* slot) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      load_bytes<VB>(base + ((i >> 1) * 8 + 2 * t + (i & 1)) * DH + g * VB, w[i]);
+    for (int i = 0; i < 4; ++i) {
+      const int at = ((i >> 1) * 8 + 2 * t + (i & 1)) * DH + g * VB;
+      read_bytes<VB>(slot + 16 * DH + v_place<DH>(at >> 4) * 16 + (at & 15), w[i]);
+    }
   }
 };
 
+template <int DH>
+struct SplitCfg {
+  static constexpr int SLOT = 32 * DH;              // bytes of 16 keys, K and V
+  static constexpr int DEPTH = DH == 128 ? 4 : 6;   // slots of a warp's ring
+  static constexpr int RING = 4 * DEPTH * SLOT;
+  static constexpr int JOIN = 4 * KV8_ROWS * DH * 4;
+  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+  // CTAs an SM is to hold: what the rings (and, at 128, the registers) allow.
+  static constexpr int min_blocks(int planes) { return DH == 128 ? (planes == 1 ? 3 : 2) : 4; }
+};
+
 // Products of 16 q rows with 16 keys: d[n][.] in the m16n8 accumulator layout.
-template <int DH, int FMT, int PL>
-__device__ __forceinline__ void score_tile(const QFrag<DH, PL>& q, const KBytes<DH>& kb,
+template <int DH, int FMT, int PL, int RH>
+__device__ __forceinline__ void score_tile(const QFrag<DH, PL, RH>& q, const KBytes<DH>& kb,
                                            float (&d)[2][4]) {
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -205,8 +258,8 @@ __device__ __forceinline__ void score_tile(const QFrag<DH, PL>& q, const KBytes<
   }
 }
 
-template <int DH, int FMT, int PL>
-__global__ void __launch_bounds__(128)
+template <int DH, int FMT, int PL, int RH>
+__global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
     kv8_split_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh, int64_t q_st,
                      void* __restrict__ out, int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype,
                      int vec, const int32_t* __restrict__ counts, int T, int G, int max_len,
@@ -216,7 +269,7 @@ __global__ void __launch_bounds__(128)
   __shared__ float s_ks[KV8_CHUNK_MAX / 16];
   __shared__ float s_vs[KV8_CHUNK_MAX / 16];
   __shared__ float s_vmax[4];
-  __shared__ float s_o[4][KV8_ROWS][DH];
+  extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ float s_ref[4][KV8_ROWS], s_sum[4][KV8_ROWS];
   pdl_launch_dependents();
   pdl_wait();
@@ -234,10 +287,10 @@ __global__ void __launch_bounds__(128)
   }
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
   // Last key that any row of this tile sees, and the rows' own limits.
-  int limit[2];
+  int limit[RH];
   int reach = 0;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
+  for (int r = 0; r < RH; ++r) {
     const int row = row0 + g + 8 * r;
     const int tok = row / G;
     limit[r] = (row < w.rows && tok < count) ? (causal ? min(len + tok + 1, end) : end) : 0;
@@ -271,7 +324,7 @@ __global__ void __launch_bounds__(128)
     s_vs[j - j0] = s.y;
     vmax = fmaxf(vmax, s.y);
   }
-  QFrag<DH, PL> qa;
+  QFrag<DH, PL, RH> qa;
   qa.load(c, q, q_sb, q_sh, q_st, dtype, vec != 0, b, h, G, row0, w.rows, scale_log2);
 #pragma unroll
   for (int d = 16; d; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
@@ -283,30 +336,50 @@ __global__ void __launch_bounds__(128)
   float o[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-
-  const int page_bytes = c.P * DH;
-  auto group_at = [&](int key) -> int64_t {  // byte offset of a group of 16 keys
-    const int page = s_page[(key >> c.p_shift) - j0];
-    return (static_cast<int64_t>(page < 0 ? 0 : page) * c.H + h) * page_bytes +
-           (key & (c.P - 1)) * DH;
-  };
-  KBytes<DH> kb;
-  VBytes<DH> vb;
-  int key = k0 + 16 * warp;
-  if (key < k1) {
-    const int64_t at = group_at(key);
-    kb.load(c.k + at);
-    vb.load(c.v + at);
+  float ref[RH], sum[RH];
+#pragma unroll
+  for (int r = 0; r < RH; ++r) {
+    ref[r] = -INFINITY;
+    sum[r] = 0.f;
   }
+
+  // The warp's ring: group i of this warp is keys k0 + 64 i + 16 warp and up.
+  using Cfg = SplitCfg<DH>;
+  uint8_t* ring = s_ring + warp * Cfg::DEPTH * Cfg::SLOT;
+  const int page_bytes = c.P * DH;
+  auto fetch = [&](int key, int slot) {
+    if (key < k1) {
+      const int page = s_page[(key >> c.p_shift) - j0];
+      const int64_t at = (static_cast<int64_t>(page < 0 ? 0 : page) * c.H + h) * page_bytes +
+                         (key & (c.P - 1)) * DH;
+      uint8_t* dst = ring + slot * Cfg::SLOT;
+#pragma unroll
+      for (int i = 0; i < (DH + 31) / 32; ++i) {
+        const int p = i * 32 + lane;
+        if (DH >= 32 || p < DH) {
+          copy16_async(dst + k_place<DH>(p) * 16, c.k + at + p * 16);
+          copy16_async(dst + 16 * DH + v_place<DH>(p) * 16, c.v + at + p * 16);
+        }
+      }
+    }
+    copy_commit();  // a group past the end commits nothing, and counts all the same
+  };
+  int key = k0 + 16 * warp;
+#pragma unroll
+  for (int i = 0; i < Cfg::DEPTH - 1; ++i) fetch(key + 64 * i, i);
+  int slot = 0;
   for (; key < k1; key += 64) {
-    KBytes<DH> kn;
-    VBytes<DH> vn;
-    const bool more = key + 64 < k1;
-    if (more) {
-      const int64_t at = group_at(key + 64);
-      kn.load(c.k + at);
-      vn.load(c.v + at);
+    copy_wait<Cfg::DEPTH - 2>();
+    __syncwarp();
+    KBytes<DH> kb;
+    VBytes<DH> vb;
+    kb.read(ring + slot * Cfg::SLOT);
+    vb.read(ring + slot * Cfg::SLOT);
+    {
+      // the slot read one group ago is free: every lane has read it
+      const int into = slot == 0 ? Cfg::DEPTH - 1 : slot - 1;
+      fetch(key + 64 * (Cfg::DEPTH - 1), into);
+      slot = slot + 1 == Cfg::DEPTH ? 0 : slot + 1;
     }
     const int pj = (key >> c.p_shift) - j0;
     const float ks = s_page[pj] < 0 ? 0.f : s_ks[pj];
@@ -314,19 +387,19 @@ __global__ void __launch_bounds__(128)
     const int bad = s_page[pj] < 0 ? 0 : 0x7fffffff;  // a refused page has no visible key
 
     float f[2][4];
-    score_tile<DH, FMT, PL>(qa, kb, f);
+    score_tile<DH, FMT, PL, RH>(qa, kb, f);
     float top = -INFINITY;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2 * RH; ++e) {
         const int kk = key + 8 * n + 2 * t + (e & 1);
         const float x = f[n][e] * (qa.qf[e >> 1] * ks);
         f[n][e] = kk < min(limit[e >> 1], bad) ? x : -INFINITY;
       }
     if (w.score) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < RH; ++r)
         if (row0 + g + 8 * r < w.rows) {
           float* sp = w.score + (static_cast<int64_t>(bh) * w.rows + row0 + g + 8 * r) * w.ld_score +
                       key + 2 * t;
@@ -336,9 +409,9 @@ __global__ void __launch_bounds__(128)
     }
     // A row's reference moves only when its maximum has outgrown it by more
     // than the slack; all lanes of the warp look at once.
-    float m2[2];
+    float m2[RH];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < RH; ++r) {
       m2[r] = fmaxf(fmaxf(f[0][2 * r], f[0][2 * r + 1]), fmaxf(f[1][2 * r], f[1][2 * r + 1]));
       top = fmaxf(top, m2[r] - (ref[r] == -INFINITY ? 0.f : ref[r]) >
                                (ref[r] == -INFINITY ? -INFINITY : KV8_BIAS + KV8_SLACK)
@@ -347,7 +420,7 @@ __global__ void __launch_bounds__(128)
     }
     if (__any_sync(0xffffffffu, top > 0.f)) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < RH; ++r) {
         float m = m2[r];
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
@@ -366,11 +439,11 @@ __global__ void __launch_bounds__(128)
         }
       }
     }
-    uint32_t hi[4], lo[4];
+    uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < RH; ++r) {
         const float neg = ref[r] == -INFINITY ? 0.f : -ref[r];
         float p[2];
 #pragma unroll
@@ -411,15 +484,15 @@ __global__ void __launch_bounds__(128)
         mma_f16_16816(o[n + 1], hi[0], hi[1], hi[2], hi[3], b01, b11);
       }
     }
-    if (more) {
-      kb = kn;
-      vb = vn;
-    }
   }
 
-  // Join the four warps. Column of accumulator (n, e): (2t + (e & 1)) * NT + n.
+  // Join the four warps, in the rings' place. Column of accumulator (n, e):
+  // (2t + (e & 1)) * NT + n.
+  copy_wait<0>();
+  __syncthreads();
+  float* s_o = reinterpret_cast<float*>(s_ring);  // [4][KV8_ROWS][DH]
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
+  for (int r = 0; r < RH; ++r) {
     float l = sum[r];
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -427,10 +500,11 @@ __global__ void __launch_bounds__(128)
       s_ref[warp][g + 8 * r] = ref[r];
       s_sum[warp][g + 8 * r] = l;
     }
+    float* row = s_o + (warp * KV8_ROWS + g + 8 * r) * DH;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      s_o[warp][g + 8 * r][(2 * t) * NT + n] = o[n][2 * r];
-      s_o[warp][g + 8 * r][(2 * t + 1) * NT + n] = o[n][2 * r + 1];
+      row[(2 * t) * NT + n] = o[n][2 * r];
+      row[(2 * t + 1) * NT + n] = o[n][2 * r + 1];
     }
   }
   __syncthreads();
@@ -446,7 +520,7 @@ __global__ void __launch_bounds__(128)
     for (int u = 0; u < 4; ++u) {
       const float a = top == -INFINITY ? 1.f : fast_exp2(s_ref[u][r] - top);
       l += a * s_sum[u][r];
-      x += a * s_o[u][r][d];
+      x += a * s_o[(u * KV8_ROWS + r) * DH + d];
     }
     x *= vmax;
     const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
@@ -526,11 +600,11 @@ __global__ void __launch_bounds__(128)
 // ---------------------------------------------------------------- weights
 
 // Adds each key's weight to the record, from the scores the split kernel left
-// (at most 16 rows). One thread per key; the rows are added in order.
+// (at most 32 rows). One thread per key; the rows are added in order.
 __global__ void __launch_bounds__(256)
     kv8_weights_kernel(KV8 c, const int32_t* __restrict__ counts, int T, int G, int max_len,
                        int flags, KV8Work w) {
-  __shared__ float s_lse[KV8_ROWS];
+  __shared__ float s_lse[2 * KV8_ROWS];
   pdl_launch_dependents();
   pdl_wait();
   const int bh = blockIdx.y;
@@ -554,62 +628,6 @@ __global__ void __launch_bounds__(256)
   }
   float* at = c.weight + (static_cast<int64_t>(page) * c.H + h) * c.P + (key & (c.P - 1));
   *at += x;
-}
-
-// The same for more rows: the scores are computed again. One CTA per 64 keys;
-// a warp takes 16 of them against all rows, 16 at a time.
-template <int DH, int FMT, int PL>
-__global__ void __launch_bounds__(128)
-    kv8_reweigh_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh,
-                       int64_t q_st, int dtype, int vec, const int32_t* __restrict__ counts,
-                       int T, int G, int max_len, float scale_log2, int flags, KV8Work w) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int bh = blockIdx.y;
-  const int b = bh / c.H, h = bh - b * c.H;
-  const int len = kv8_len(c, b);
-  const int count = kv8_count(counts, b, T);
-  const int end = min(kv8_end(c, len, count), max_len);
-  const int key = blockIdx.x * 64 + warp * 16;
-  if (key >= end) return;
-  const int page = kv8_page(c, b, key >> c.p_shift);
-  if (page < 0) return;
-  const int64_t block = static_cast<int64_t>(page) * c.H + h;
-  const float ks = c.scale[2 * block];
-  KBytes<DH> kb;
-  kb.load(c.k + block * c.P * DH + (key & (c.P - 1)) * DH);
-  const bool causal = (flags & KF_KV8_CAUSAL) != 0;
-  float x[4] = {0.f, 0.f, 0.f, 0.f};  // keys 2t, 2t+1, 8+2t, 9+2t
-  // the first row that sees the group's first key
-  const int first = causal && key > len ? (key - len) * G : 0;
-  const int rows = min(w.rows, count * G);
-  for (int row0 = first & ~(KV8_ROWS - 1); row0 < rows; row0 += KV8_ROWS) {
-    QFrag<DH, PL> qa;
-    qa.load(c, q, q_sb, q_sh, q_st, dtype, vec != 0, b, h, G, row0, rows, scale_log2);
-    float f[2][4];
-    score_tile<DH, FMT, PL>(qa, kb, f);
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = row0 + g + 8 * r;
-      if (row >= rows) continue;
-      const float l = w.lse[static_cast<int64_t>(bh) * w.rows + row];
-      const int limit = causal ? min(len + row / G + 1, end) : end;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = f[i >> 1][2 * r + (i & 1)] * (qa.qf[r] * ks);
-        if (key + (i >> 1) * 8 + 2 * t + (i & 1) < limit && l != -INFINITY)
-          x[i] += fast_exp2(y - l);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int d = 4; d <= 16; d <<= 1) x[i] += __shfl_xor_sync(0xffffffffu, x[i], d);
-    const int kk = key + (i >> 1) * 8 + 2 * t + (i & 1);
-    if (g == 0 && kk < end) c.weight[block * c.P + (kk & (c.P - 1))] += x[i];
-  }
 }
 
 }  // namespace kf

@@ -6,9 +6,10 @@ namespace kf {
 // ---------------------------------------------------------------- append
 //
 // One CTA per (page a chunk can reach, kv head, sequence and K|V). It loads the
-// page's new tokens into registers, takes max|x| as the largest bit pattern
-// (so an infinity or a NaN wins), fixes the scale, rescales the page's earlier
-// codes if the scale grew, and writes the new codes.
+// page's new tokens into registers (16 bytes a thread and load), takes max|x|
+// as the largest bit pattern (so an infinity or a NaN wins), fixes the scale,
+// rescales the page's earlier codes if the scale grew, and writes the new
+// codes. Bound by memory: one read and one write of the chunk.
 
 constexpr int KV8_THREADS = 256;
 
@@ -22,25 +23,27 @@ __device__ __forceinline__ uint32_t block_max_u32(uint32_t x, uint32_t* red) {
   return m;
 }
 
-// 4 values to 4 codes, one word.
-__device__ __forceinline__ uint32_t kv8_encode4(const float (&x)[4], float inv, int fmt) {
-  uint32_t w = 0;
+// N values (4, 8 or 16) to N codes.
+template <int FMT, int N>
+__device__ __forceinline__ void kv8_put_codes(uint8_t* p, const float* x, float inv) {
+  uint32_t w[N / 4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    w |= static_cast<uint32_t>(kv8_encode(__fmul_rn(x[u], inv), fmt)) << (8 * u);
-  return w;
-}
-__device__ __forceinline__ void kv8_decode4(uint32_t w, int fmt, float (&x)[4]) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u) x[u] = kv8_decode(static_cast<uint8_t>(w >> (8 * u)), fmt);
+  for (int u = 0; u < N / 4; ++u) w[u] = kv8_encode4<FMT>(x + 4 * u, inv);
+  if constexpr (N == 16)
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (N == 8)
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
-// NG: groups of four values a thread holds (a page has P * D / 4 groups).
-template <int NG>
+// NG: runs of 16 bytes of input that a thread holds (a page has P * D / N).
+template <int DT, int NG>
 __global__ void __launch_bounds__(KV8_THREADS)
     kv8_append_kernel(KV8 c, const void* __restrict__ k, int64_t k_sb, int64_t k_sh, int64_t k_st,
                       const void* __restrict__ v, int64_t v_sb, int64_t v_sh, int64_t v_st,
-                      int dtype, int vec, const int32_t* __restrict__ counts, int T) {
+                      int vec, const int32_t* __restrict__ counts, int T) {
+  constexpr int N = KV8Type<DT>::N;
   __shared__ uint32_t red[KV8_THREADS / 32];
   pdl_launch_dependents();
   pdl_wait();
@@ -61,39 +64,60 @@ __global__ void __launch_bounds__(KV8_THREADS)
   const int64_t base = b * (is_v ? v_sb : k_sb) + h * (is_v ? v_sh : k_sh);
   const int64_t st = is_v ? v_st : k_st;
   const int64_t block = static_cast<int64_t>(page) * c.H + h;
-  uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + block * c.P * c.D);
+  uint8_t* codes = (is_v ? c.v : c.k) + block * c.P * c.D;
   float* sp = c.scale + 2 * block + (is_v ? 1 : 0);
   const float was = lo > p0 ? *sp : 0.f;
-  const int row_groups = c.D >> 2;
-  const int first = (lo - p0) * row_groups, last = (hi - p0) * row_groups;
+  const int row_shift = c.d_shift - (N == 8 ? 3 : 2);  // runs of a row, as a power of two
+  const int first = (lo - p0) << row_shift, last = (hi - p0) << row_shift;
 
-  float x[NG][4];
+  float x[NG][N];
   uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = first + threadIdx.x + i * KV8_THREADS;
-    x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-    if (g < last) {
-      const int r = g / row_groups;
-      kv8_load4(src, base + (p0 + r - len) * st + 4 * (g - r * row_groups), dtype, vec, x[i]);
-    }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) amax = max(amax, __float_as_uint(x[i][u]) & 0x7fffffffu);
+    for (int u = 0; u < N; ++u) x[i][u] = 0.f;
+    if (g < last) {
+      const int r = g >> row_shift;
+      KV8Type<DT>::load(src, base + (p0 + r - len) * st + N * (g - (r << row_shift)), vec != 0,
+                        x[i]);
+    }
   }
+#pragma unroll
+  for (int i = 0; i < NG; ++i)
+#pragma unroll
+    for (int u = 0; u < N; ++u) amax = max(amax, __float_as_uint(x[i][u]) & 0x7fffffffu);
   const float mine = kv8_scale(block_max_u32(amax, red), c.fmt);
   const float s = (was != was || mine != mine) ? __uint_as_float(0x7fc00000u) : fmaxf(was, mine);
   const float inv = kv8_inverse(s);
+  if (s != s) {  // codes of a page whose scale is NaN mean nothing: keep them finite
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+#pragma unroll
+      for (int u = 0; u < N; ++u) x[i][u] = 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = first + threadIdx.x + i * KV8_THREADS;
-    if (g < last) codes[g] = kv8_encode4(x[i], inv, c.fmt);
+    if (g < last) {
+      if (c.fmt == KF_KV8_INT8)
+        kv8_put_codes<KF_KV8_INT8, N>(codes + g * N, x[i], inv);
+      else
+        kv8_put_codes<KF_KV8_E4M3, N>(codes + g * N, x[i], inv);
+    }
   }
   if (first > 0 && !(s == was)) {
     const float ratio = __fmul_rn(was, inv);
-    for (int g = threadIdx.x; g < first; g += KV8_THREADS) {
+    for (int g = threadIdx.x; g < first * (N / 4); g += KV8_THREADS) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(codes) + g;
       float y[4];
-      kv8_decode4(codes[g], c.fmt, y);
-      codes[g] = kv8_encode4(y, ratio, c.fmt);
+      if (c.fmt == KF_KV8_INT8) {
+        kv8_decode4<KF_KV8_INT8>(*w, y);
+        *w = s != s ? 0u : kv8_encode4<KF_KV8_INT8>(y, ratio);
+      } else {
+        kv8_decode4<KF_KV8_E4M3>(*w, y);
+        *w = s != s ? 0u : kv8_encode4<KF_KV8_E4M3>(y, ratio);
+      }
     }
   }
   if (threadIdx.x == 0) *sp = s;
@@ -104,55 +128,93 @@ __global__ void __launch_bounds__(KV8_THREADS)
 
 // ---------------------------------------------------------------- read
 
-// One thread per four codes of K or V.
+// One thread per N codes of K and of V (16 bytes of output each), four rows
+// apart in flight. Bound by memory, mostly by what it writes.
+constexpr int KV8_READ_UNROLL = 4;
+
+template <int DT>
 __global__ void __launch_bounds__(KV8_THREADS)
     kv8_read_kernel(KV8 c, const int32_t* __restrict__ start, const int32_t* __restrict__ counts,
-                    int n, void* __restrict__ k_out, void* __restrict__ v_out, int dtype) {
+                    int n, void* __restrict__ k_out, void* __restrict__ v_out) {
+  constexpr int N = KV8Type<DT>::N;
+  constexpr int W = N / 4;
   pdl_launch_dependents();
   pdl_wait();
-  const int row_groups = c.D >> 2;
+  const int row_shift = c.d_shift - (N == 8 ? 3 : 2);
   const int h = blockIdx.y;
   const int b = blockIdx.z;
   const int len = kv8_len(c, b);
   const int end = counts ? kv8_end(c, len, max(__ldg(counts + b), 0)) : len;
   const int from = start ? max(__ldg(start + b), 0) : 0;
   const int64_t out0 = (static_cast<int64_t>(b) * c.H + h) * n * c.D;
-  const int total = n * row_groups;
-  for (int g = blockIdx.x * KV8_THREADS + threadIdx.x; g < total; g += gridDim.x * KV8_THREADS) {
-    const int i = g / row_groups;
-    const int64_t pos = static_cast<int64_t>(from) + i;
-    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-    if (pos < end) {
+  const int total = n << row_shift;
+  const int g0 = blockIdx.x * (KV8_THREADS * KV8_READ_UNROLL) + threadIdx.x;
+  uint32_t kw[KV8_READ_UNROLL][W], vw[KV8_READ_UNROLL][W];
+  float2 s[KV8_READ_UNROLL];
+#pragma unroll
+  for (int i = 0; i < KV8_READ_UNROLL; ++i) {
+    const int g = g0 + i * KV8_THREADS;
+    const int64_t pos = static_cast<int64_t>(from) + (g >> row_shift);
+    s[i] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < W; ++u) kw[i][u] = vw[i][u] = 0u;
+    if (g < total && pos < end) {
       const int page = kv8_page(c, b, static_cast<int>(pos >> c.p_shift));
       if (page >= 0) {
         const int64_t block = static_cast<int64_t>(page) * c.H + h;
-        const int64_t at = (block * c.P + (pos & (c.P - 1))) * row_groups + (g - i * row_groups);
-        const float2 s = *reinterpret_cast<const float2*>(c.scale + 2 * block);
-        kv8_decode4(reinterpret_cast<const uint32_t*>(c.k)[at], c.fmt, x);
-        kv8_decode4(reinterpret_cast<const uint32_t*>(c.v)[at], c.fmt, y);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          x[u] = __fmul_rn(x[u], s.x);
-          y[u] = __fmul_rn(y[u], s.y);
+        const int64_t at = (((block << c.p_shift) + (pos & (c.P - 1))) << c.d_shift) +
+                           N * (g & ((1 << row_shift) - 1));
+        s[i] = __ldg(reinterpret_cast<const float2*>(c.scale + 2 * block));
+        if constexpr (W == 2) {
+          const uint2 a = __ldg(reinterpret_cast<const uint2*>(c.k + at));
+          const uint2 d = __ldg(reinterpret_cast<const uint2*>(c.v + at));
+          kw[i][0] = a.x; kw[i][W - 1] = a.y;
+          vw[i][0] = d.x; vw[i][W - 1] = d.y;
+        } else {
+          kw[i][0] = __ldg(reinterpret_cast<const uint32_t*>(c.k + at));
+          vw[i][0] = __ldg(reinterpret_cast<const uint32_t*>(c.v + at));
         }
       }
     }
+  }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      kv8_store1(k_out, out0 + 4 * static_cast<int64_t>(g) + u, dtype, x[u]);
-      kv8_store1(v_out, out0 + 4 * static_cast<int64_t>(g) + u, dtype, y[u]);
+  for (int i = 0; i < KV8_READ_UNROLL; ++i) {
+    const int g = g0 + i * KV8_THREADS;
+    if (g >= total) return;
+    float x[N], y[N];
+#pragma unroll
+    for (int u = 0; u < W; ++u) {
+      if (c.fmt == KF_KV8_INT8) {
+        kv8_decode4<KF_KV8_INT8>(kw[i][u], x + 4 * u);
+        kv8_decode4<KF_KV8_INT8>(vw[i][u], y + 4 * u);
+      } else {
+        kv8_decode4<KF_KV8_E4M3>(kw[i][u], x + 4 * u);
+        kv8_decode4<KF_KV8_E4M3>(vw[i][u], y + 4 * u);
+      }
     }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      x[u] = __fmul_rn(x[u], s[i].x);
+      y[u] = __fmul_rn(y[u], s[i].y);
+    }
+    const int64_t at = out0 + static_cast<int64_t>(N) * g;
+    KV8Type<DT>::store(k_out, at, x);
+    KV8Type<DT>::store(v_out, at, y);
   }
 }
 
 // ---------------------------------------------------------------- evict
 //
-// Two kernels. The first picks, per (sequence, kv head), the tokens to keep:
-// a radix search, eight bits a pass, for the need-th largest weight among the
-// tokens that are not protected, then one pass in order that lists the kept
-// positions. The second moves one destination block per CTA.
+// Two kernels. The first picks, per (sequence, kv head), the tokens to keep: a
+// radix search, eleven bits a pass, for the need-th largest weight among the
+// tokens that are not protected, then a pass in order that lists the kept
+// positions. The weights are read from memory once and kept as sortable keys
+// in shared memory as far as they fit. The second moves one destination block
+// per CTA.
 
 constexpr int KV8_SELECT_THREADS = 1024;
+constexpr int KV8_SELECT_KEYS = 48 * 1024;  // keys that shared memory holds
+constexpr int KV8_SELECT_SMEM = KV8_SELECT_KEYS * 4;
 
 // Weights in an order of unsigned integers; NaN counts as the largest, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -164,7 +226,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 __global__ void __launch_bounds__(KV8_SELECT_THREADS)
     kv8_select_kernel(KV8 c, int budget, int recent, int32_t* __restrict__ kept,
                       int32_t* __restrict__ lens_out) {
-  __shared__ uint32_t hist[256];
+  extern __shared__ uint32_t s_key[];  // [KV8_SELECT_KEYS]
+  __shared__ uint32_t hist[2048];
+  __shared__ uint32_t s_part[32];
   __shared__ uint32_t s_prefix, s_need;
   __shared__ uint32_t w_more[32], w_tie[32];
   pdl_launch_dependents();
@@ -182,78 +246,116 @@ __global__ void __launch_bounds__(KV8_SELECT_THREADS)
   }
   const int cand = len - recent;           // positions [0, cand) compete
   const int need = budget - recent;        // for this many places (need < cand)
-  auto key_at = [&](int pos) -> uint32_t {
+  for (int i = tid; i < recent; i += KV8_SELECT_THREADS) out[need + i] = cand + i;
+  if (need == 0) return;
+  auto load_key = [&](int pos) -> uint32_t {
     const int page = kv8_page(c, b, pos >> c.p_shift);
     if (page < 0) return 0u;
     return weight_key(
         c.weight[(static_cast<int64_t>(page) * c.H + h) * c.P + (pos & (c.P - 1))]);
   };
-  // The need-th largest key, eight bits at a time: s_prefix holds the bits
+  for (int base = tid; base < cand && base < KV8_SELECT_KEYS; base += 4 * KV8_SELECT_THREADS) {
+    uint32_t key[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = base + i * KV8_SELECT_THREADS;
+      key[i] = pos < cand && pos < KV8_SELECT_KEYS ? load_key(pos) : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = base + i * KV8_SELECT_THREADS;
+      if (pos < cand && pos < KV8_SELECT_KEYS) s_key[pos] = key[i];
+    }
+  }
+  auto key_at = [&](int pos) -> uint32_t {
+    return pos < KV8_SELECT_KEYS ? s_key[pos] : load_key(pos);
+  };
+  // The need-th largest key, eleven bits at a time: s_prefix holds the bits
   // found, s_need how many keys with that prefix still have to be taken.
   if (tid == 0) {
     s_prefix = 0;
     s_need = need;
   }
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  int left_bits = 32;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int bits = pass < 2 ? 11 : 10;
+    const int shift = left_bits - bits;
+    const uint32_t above = pass == 0 ? 0u : (0xffffffffu << left_bits);
+    hist[tid] = 0;
+    hist[tid + 1024] = 0;
     __syncthreads();
-    const uint32_t prefix = s_prefix;
-    const uint32_t above = shift == 24 ? 0u : (0xffffffffu << (shift + 8));
+    const uint32_t prefix = s_prefix, want = s_need;
     for (int pos = tid; pos < cand; pos += KV8_SELECT_THREADS) {
       const uint32_t key = key_at(pos);
-      if ((key & above) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+      if ((key & above) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
     }
     __syncthreads();
-    if (tid == 0) {
-      uint32_t left = s_need;
-      int d = 255;
-      while (d > 0 && hist[d] < left) left -= hist[d--];
-      s_prefix = prefix | (static_cast<uint32_t>(d) << shift);
-      s_need = left;
+    // Thread i looks at digits 2047 - 2i and 2046 - 2i: a scan over the threads
+    // counts the keys with larger digits; one thread finds its digit is it.
+    const uint32_t h0 = hist[2047 - 2 * tid], h1 = hist[2046 - 2 * tid];
+    uint32_t sum = h0 + h1;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
     }
+    if (lane == 31) s_part[warp] = sum;
     __syncthreads();
+    uint32_t before = sum - h0 - h1;
+    for (int w = 0; w < warp; ++w) before += s_part[w];
+    if (before < want && before + h0 >= want) {
+      s_prefix = prefix | (static_cast<uint32_t>(2047 - 2 * tid) << shift);
+      s_need = want - before;
+    } else if (before + h0 < want && before + h0 + h1 >= want) {
+      s_prefix = prefix | (static_cast<uint32_t>(2046 - 2 * tid) << shift);
+      s_need = want - before - h0;
+    }
+    left_bits = shift;
+    __syncthreads();
+  }
+  const uint32_t cut = s_prefix;
+  const uint32_t ties = s_need;  // keys equal to cut that are kept, lowest position first
+  // Every warp takes a run of positions: it counts, then lists, what it keeps.
+  const int run = ((cand + 31) / 32 + 31) / 32 * 32;
+  const int begin = warp * run, stop = min(begin + run, cand);
+  uint32_t more = 0, tie = 0;
+  for (int pos = begin + lane; pos < begin + run; pos += 32) {
+    const uint32_t key = pos < stop ? key_at(pos) : 0u;
+    more += __popc(__ballot_sync(0xffffffffu, pos < stop && key > cut));
+    tie += __popc(__ballot_sync(0xffffffffu, pos < stop && key == cut));
+  }
+  if (lane == 0) {
+    w_more[warp] = more;
+    w_tie[warp] = tie;
   }
   __syncthreads();
-  const uint32_t cut = s_prefix;
-  const uint32_t ties = need > 0 ? s_need : 0u;  // keys equal to cut that are kept, lowest first
-  uint32_t more_before = 0, tie_before = 0;
-  for (int base = 0; base < cand && need > 0; base += KV8_SELECT_THREADS) {
-    const int pos = base + tid;
-    const uint32_t key = pos < cand ? key_at(pos) : 0u;
-    const bool more = pos < cand && key > cut;
-    const bool tie = pos < cand && key == cut;
-    const uint32_t bm = __ballot_sync(0xffffffffu, more), bt = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) {
-      w_more[warp] = __popc(bm);
-      w_tie[warp] = __popc(bt);
-    }
-    __syncthreads();
-    uint32_t pm = more_before, pt = tie_before, all_m = 0, all_t = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w == warp) {
-        pm += all_m;
-        pt += all_t;
-      }
-      all_m += w_more[w];
-      all_t += w_tie[w];
-    }
-    const uint32_t below = (1u << lane) - 1u;
-    pm += __popc(bm & below);
-    pt += __popc(bt & below);
-    if (more || (tie && pt < ties)) out[pm + (pt < ties ? pt : ties)] = pos;
-    more_before += all_m;
-    tie_before += all_t;
-    __syncthreads();
+  uint32_t pm = 0, pt = 0;
+  for (int w = 0; w < warp; ++w) {
+    pm += w_more[w];
+    pt += w_tie[w];
   }
-  for (int i = tid; i < recent; i += KV8_SELECT_THREADS) out[need + i] = cand + i;
+  const uint32_t below = (1u << lane) - 1u;
+  for (int pos = begin + lane; pos < begin + run; pos += 32) {
+    const uint32_t key = pos < stop ? key_at(pos) : 0u;
+    const bool is_more = pos < stop && key > cut, is_tie = pos < stop && key == cut;
+    const uint32_t bm = __ballot_sync(0xffffffffu, is_more);
+    const uint32_t bt = __ballot_sync(0xffffffffu, is_tie);
+    const uint32_t m = pm + __popc(bm & below), t = pt + __popc(bt & below);
+    if (is_more || (is_tie && t < ties)) out[m + min(t, ties)] = pos;
+    pm += __popc(bm);
+    pt += __popc(bt);
+  }
 }
 
-template <int NG>
+// NG: pieces of 16 codes that a thread moves.
+template <int FMT, int NG>
 __global__ void __launch_bounds__(KV8_THREADS)
     kv8_move_kernel(KV8 c, const int32_t* __restrict__ table_out, int64_t ld_out, int budget,
                     const int32_t* __restrict__ kept) {
   __shared__ uint32_t red[KV8_THREADS / 32];
   __shared__ int64_t s_row[128];     // source row (block * P + slot) of each destination slot
+  __shared__ float s_scale[128];
   pdl_launch_dependents();
   pdl_wait();
   const int j = blockIdx.x;
@@ -271,40 +373,54 @@ __global__ void __launch_bounds__(KV8_THREADS)
   if (threadIdx.x < rows) {
     const int pos = mine[threadIdx.x];
     const int sp = kv8_page(c, b, pos >> c.p_shift);
-    s_row[threadIdx.x] =
-        sp < 0 ? -1 : (static_cast<int64_t>(sp) * c.H + h) * c.P + (pos & (c.P - 1));
+    const int64_t block = static_cast<int64_t>(sp) * c.H + h;
+    s_row[threadIdx.x] = sp < 0 ? -1 : block * c.P + (pos & (c.P - 1));
+    s_scale[threadIdx.x] = sp < 0 ? 0.f : c.scale[2 * block + (is_v ? 1 : 0)];
   }
   __syncthreads();
-  const int row_groups = c.D >> 2;
-  const uint32_t* src = reinterpret_cast<const uint32_t*>(is_v ? c.v : c.k);
-  const int last = rows * row_groups;
-  float x[NG][4];
+  const int row_shift = c.d_shift - 4;
+  const uint8_t* src = is_v ? c.v : c.k;
+  const int last = rows << row_shift;
+  uint4 w[NG];
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    const int g = threadIdx.x + i * KV8_THREADS;
+    w[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (g < last) {
+      const int64_t row = s_row[g >> row_shift];
+      if (row >= 0)
+        w[i] = *reinterpret_cast<const uint4*>(src + (row << c.d_shift) +
+                                               16 * (g & ((1 << row_shift) - 1)));
+    }
+  }
+  float x[NG][16];
   uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = threadIdx.x + i * KV8_THREADS;
-    x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-    if (g < last) {
-      const int r = g / row_groups;
-      const int64_t row = s_row[r];
-      if (row >= 0) {
-        const float s = c.scale[2 * (row >> c.p_shift) + (is_v ? 1 : 0)];
-        kv8_decode4(src[row * row_groups + (g - r * row_groups)], c.fmt, x[i]);
+    const float s = g < last ? s_scale[g >> row_shift] : 0.f;
+    kv8_decode4<FMT>(w[i].x, x[i]);
+    kv8_decode4<FMT>(w[i].y, x[i] + 4);
+    kv8_decode4<FMT>(w[i].z, x[i] + 8);
+    kv8_decode4<FMT>(w[i].w, x[i] + 12);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[i][u] = __fmul_rn(x[i][u], s);
-      }
+    for (int u = 0; u < 16; ++u) {
+      x[i][u] = __fmul_rn(x[i][u], s);
+      amax = max(amax, __float_as_uint(x[i][u]) & 0x7fffffffu);
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) amax = max(amax, __float_as_uint(x[i][u]) & 0x7fffffffu);
   }
   const float s = kv8_scale(block_max_u32(amax, red), c.fmt);
   const float inv = kv8_inverse(s);
   const int64_t block = static_cast<int64_t>(page) * c.H + h;
-  uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + block * c.P * c.D);
+  uint8_t* codes = (is_v ? c.v : c.k) + ((block << c.p_shift) << c.d_shift);
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = threadIdx.x + i * KV8_THREADS;
-    if (g < last) codes[g] = kv8_encode4(x[i], inv, c.fmt);
+    if (s != s) {
+#pragma unroll
+      for (int u = 0; u < 16; ++u) x[i][u] = 0.f;
+    }
+    if (g < last) kv8_put_codes<FMT, 16>(codes + 16 * g, x[i], inv);
   }
   if (threadIdx.x == 0) c.scale[2 * block + (is_v ? 1 : 0)] = s;
   if (!is_v && threadIdx.x < rows) {
@@ -366,6 +482,7 @@ static int kv8_view(const char* what, const kf_kv8_cache* c, KV8* out) {
   v.P = c->block;
   v.fmt = c->format;
   v.p_shift = log2_exact(c->block);
+  v.d_shift = log2_exact(c->head_dim);
   *out = v;
   return KF_OK;
 }
@@ -393,29 +510,41 @@ extern "C" int kf_kv8_append(const kf_kv8_cache* cache, const void* k, int64_t k
     set_last_error("kf_kv8_append: invalid arguments (T = %lld)", (long long)T);
     return KF_E_INVALID;
   }
-  const int64_t es = dtype_size(dtype);
+  const int64_t es = dtype_size(dtype), per = 16 / es;
   const int64_t strides[6] = {k_sb, k_sh, k_st, v_sb, v_sh, v_st};
-  int vec = kv8_aligned(k, 4 * es) && kv8_aligned(v, 4 * es);
-  for (int i = 0; i < 6; ++i) vec = vec && strides[i] % 4 == 0;
+  int vec = kv8_aligned(k, 16) && kv8_aligned(v, 16);
+  for (int i = 0; i < 6; ++i) vec = vec && strides[i] % per == 0;
   const unsigned n = static_cast<unsigned>((c.P + T - 2) / c.P + 1);
   const dim3 grid(n, static_cast<unsigned>(c.H), static_cast<unsigned>(2 * c.B));
-  const int groups = c.P * c.D / 4 / KV8_THREADS;
+  // runs of 16 bytes that a thread holds: of a page, or of a chunk that is shorter
+  const int64_t rows = T < c.P ? T : c.P;
+  const int64_t groups = (rows * c.D / per + KV8_THREADS - 1) / KV8_THREADS;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int Ti = static_cast<int>(T);
   cudaError_t e;
-#define KF_KV8_APPEND(NG)                                                                        \
-  e = launch_chained(kv8_append_kernel<NG>, grid, dim3(KV8_THREADS), 0, st, c, k, k_sb, k_sh,    \
-                     k_st, v, v_sb, v_sh, v_st, dtype, vec, counts, Ti)
-  if (groups <= 1)
-    KF_KV8_APPEND(1);
-  else if (groups <= 2)
-    KF_KV8_APPEND(2);
-  else if (groups <= 4)
-    KF_KV8_APPEND(4);
-  else if (groups <= 8)
-    KF_KV8_APPEND(8);
+#define KF_KV8_APPEND(DT, NG)                                                                    \
+  e = launch_chained(kv8_append_kernel<DT, NG>, grid, dim3(KV8_THREADS), 0, st, c, k, k_sb, k_sh, \
+                     k_st, v, v_sb, v_sh, v_st, vec, counts, Ti)
+#define KF_KV8_APPEND_NG(DT)      \
+  do {                            \
+    if (groups <= 1)              \
+      KF_KV8_APPEND(DT, 1);       \
+    else if (groups <= 2)         \
+      KF_KV8_APPEND(DT, 2);       \
+    else if (groups <= 4)         \
+      KF_KV8_APPEND(DT, 4);       \
+    else                          \
+      KF_KV8_APPEND(DT, 8);       \
+  } while (0)
+  if (dtype == KF_DT_F32 && groups > 8)  // a whole page of 128 x 128
+    KF_KV8_APPEND(KF_DT_F32, 16);
+  else if (dtype == KF_DT_F32)
+    KF_KV8_APPEND_NG(KF_DT_F32);
+  else if (dtype == KF_DT_BF16)
+    KF_KV8_APPEND_NG(KF_DT_BF16);
   else
-    KF_KV8_APPEND(16);
+    KF_KV8_APPEND_NG(KF_DT_F16);
+#undef KF_KV8_APPEND_NG
 #undef KF_KV8_APPEND
   return cuda_status(e, "kf_kv8_append launch");
 }
@@ -435,12 +564,16 @@ extern "C" int kf_kv8_read(const kf_kv8_cache* cache, const int32_t* start, cons
     set_last_error("kf_kv8_read: outputs must be 16-byte aligned");
     return KF_E_UNSUPPORTED;
   }
-  const int64_t groups = n * c.D / 4;
-  const dim3 grid(static_cast<unsigned>((groups + KV8_THREADS - 1) / KV8_THREADS),
+  const int64_t groups = n * c.D * dtype_size(dtype) / 16;
+  constexpr int64_t per_cta = KV8_THREADS * KV8_READ_UNROLL;
+  const dim3 grid(static_cast<unsigned>((groups + per_cta - 1) / per_cta),
                   static_cast<unsigned>(c.H), static_cast<unsigned>(c.B));
-  return cuda_status(launch_chained(kv8_read_kernel, grid, dim3(KV8_THREADS), 0,
+  auto kern = dtype == KF_DT_F32    ? kv8_read_kernel<KF_DT_F32>
+              : dtype == KF_DT_BF16 ? kv8_read_kernel<KF_DT_BF16>
+                                    : kv8_read_kernel<KF_DT_F16>;
+  return cuda_status(launch_chained(kern, grid, dim3(KV8_THREADS), 0,
                                     static_cast<cudaStream_t>(stream), c, start, counts,
-                                    static_cast<int>(n), k_out, v_out, dtype),
+                                    static_cast<int>(n), k_out, v_out),
                      "kf_kv8_read launch");
 }
 
@@ -468,26 +601,41 @@ extern "C" int kf_kv8_evict(const kf_kv8_cache* cache, const int32_t* table_out,
   if (c.B == 0) return KF_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int bud = static_cast<int>(budget), rec = static_cast<int>(recent);
+  static DeviceOnce once;
+  rc = once.run("kf_kv8_evict", nullptr, [&](int) {
+    return cuda_status(cudaFuncSetAttribute(kv8_select_kernel,
+                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            KV8_SELECT_SMEM),
+                       "kf_kv8_evict: set smem attribute");
+  });
+  if (rc) return rc;
+  // no more keys in shared memory than a table can hold
+  const int64_t reach = static_cast<int64_t>(c.blocks) * c.P;
+  const size_t smem = reach < KV8_SELECT_KEYS ? static_cast<size_t>(reach) * 4 : KV8_SELECT_SMEM;
   cudaError_t e = launch_chained(kv8_select_kernel,
                                  dim3(static_cast<unsigned>(c.H), static_cast<unsigned>(c.B)),
-                                 dim3(KV8_SELECT_THREADS), 0, st, c, bud, rec, kept, lens_out);
+                                 dim3(KV8_SELECT_THREADS), smem, st, c, bud, rec, kept, lens_out);
   if (e != cudaSuccess) return cuda_status(e, "kf_kv8_evict select launch");
   const dim3 grid(static_cast<unsigned>((budget + c.P - 1) / c.P), static_cast<unsigned>(c.H),
                   static_cast<unsigned>(2 * c.B));
-  const int groups = c.P * c.D / 4 / KV8_THREADS;
-#define KF_KV8_MOVE(NG)                                                                        \
-  e = launch_chained(kv8_move_kernel<NG>, grid, dim3(KV8_THREADS), 0, st, c, table_out, ld_out, \
-                     bud, static_cast<const int32_t*>(kept))
-  if (groups <= 1)
-    KF_KV8_MOVE(1);
-  else if (groups <= 2)
-    KF_KV8_MOVE(2);
-  else if (groups <= 4)
-    KF_KV8_MOVE(4);
-  else if (groups <= 8)
-    KF_KV8_MOVE(8);
+  const int groups = c.P * c.D / 16 / KV8_THREADS;
+#define KF_KV8_MOVE(FMT, NG)                                                                    \
+  e = launch_chained(kv8_move_kernel<FMT, NG>, grid, dim3(KV8_THREADS), 0, st, c, table_out,     \
+                     ld_out, bud, static_cast<const int32_t*>(kept))
+#define KF_KV8_MOVE_NG(FMT)    \
+  do {                         \
+    if (groups <= 1)           \
+      KF_KV8_MOVE(FMT, 1);     \
+    else if (groups <= 2)      \
+      KF_KV8_MOVE(FMT, 2);     \
+    else                       \
+      KF_KV8_MOVE(FMT, 4);     \
+  } while (0)
+  if (c.fmt == KF_KV8_INT8)
+    KF_KV8_MOVE_NG(KF_KV8_INT8);
   else
-    KF_KV8_MOVE(16);
+    KF_KV8_MOVE_NG(KF_KV8_E4M3);
+#undef KF_KV8_MOVE_NG
 #undef KF_KV8_MOVE
   return cuda_status(e, "kf_kv8_evict move launch");
 }

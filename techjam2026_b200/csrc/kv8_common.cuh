@@ -26,6 +26,7 @@ struct KV8 {
   int blocks;     // usable table columns
   int B, H, D, P, fmt;
   int p_shift;    // log2 P
+  int d_shift;    // log2 D
 };
 
 constexpr float KV8_TINY = 1.1754943508222875e-38f;  // 2^-126: smaller scales mean a zero block
@@ -112,6 +113,53 @@ __device__ __forceinline__ void kv8_load4(const void* p, int64_t i, int dtype, b
   }
 }
 
+// N consecutive values of type DT (16 bytes); `vec`: the address is aligned.
+template <int DT>
+struct KV8Type {
+  static constexpr int N = DT == KF_DT_F32 ? 4 : 8;
+  __device__ __forceinline__ static void load(const void* p, int64_t i, bool vec, float* x) {
+    if (!vec) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) x[u] = kv8_load1(p, i + u, DT);
+      return;
+    }
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) +
+                                                         i * (DT == KF_DT_F32 ? 4 : 2)));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if constexpr (DT == KF_DT_F32) {
+        x[u] = __uint_as_float(w[u]);
+      } else if constexpr (DT == KF_DT_BF16) {
+        x[2 * u] = __uint_as_float(w[u] << 16);
+        x[2 * u + 1] = __uint_as_float(w[u] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[u]));
+        x[2 * u] = f.x;
+        x[2 * u + 1] = f.y;
+      }
+    }
+  }
+  // N values to a 16-byte aligned address.
+  __device__ __forceinline__ static void store(void* p, int64_t i, const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if constexpr (DT == KF_DT_F32) {
+        w[u] = __float_as_uint(x[u]);
+      } else if constexpr (DT == KF_DT_BF16) {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(x[2 * u], x[2 * u + 1]);
+        w[u] = *reinterpret_cast<const uint32_t*>(&y);
+      } else {
+        const __half2 y = __floats2half2_rn(x[2 * u], x[2 * u + 1]);
+        w[u] = *reinterpret_cast<const uint32_t*>(&y);
+      }
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + i * (DT == KF_DT_F32 ? 4 : 2)) =
+        make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
 // ---------------------------------------------------------------- codes
 
 // Four codes (one word) to two fp16 pairs: exact for both code types.
@@ -137,18 +185,34 @@ __device__ __forceinline__ void kv8_cvt4(uint32_t w, uint32_t& h01, uint32_t& h2
   }
 }
 
-// One code to fp32 and back (round to nearest even, saturating).
-__device__ __forceinline__ float kv8_decode(uint8_t b, int fmt) {
-  if (fmt == KF_KV8_INT8) return static_cast<float>(static_cast<int8_t>(b));
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
-}
-__device__ __forceinline__ uint8_t kv8_encode(float x, int fmt) {
-  x = x == x ? x : 0.f;  // only in a block whose scale is NaN already
-  if (fmt == KF_KV8_INT8) {
-    x = fminf(fmaxf(x, -127.f), 127.f);
-    return static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(x)));
+// Four values to four codes, one word. |x * inv| is at most the largest code
+// (but for rounding): inv is 1 / s with s >= max|x| / Qmax, or 0.
+template <int FMT>
+__device__ __forceinline__ uint32_t kv8_encode4(const float* x, float inv) {
+  if constexpr (FMT == KF_KV8_INT8) {
+    // x * inv + 1.5 * 2^23: the sum's last place is 1, so it is rounded to the
+    // nearest integer (ties to even), whose low byte is the code
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      u[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
+    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+  } else {
+    const uint32_t a = __nv_cvt_float2_to_fp8x2(
+        make_float2(__fmul_rn(x[0], inv), __fmul_rn(x[1], inv)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t b = __nv_cvt_float2_to_fp8x2(
+        make_float2(__fmul_rn(x[2], inv), __fmul_rn(x[3], inv)), __NV_SATFINITE, __NV_E4M3);
+    return a | (b << 16);
   }
-  return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+}
+// Four codes (one word) to fp32.
+template <int FMT>
+__device__ __forceinline__ void kv8_decode4(uint32_t w, float* x) {
+  uint32_t a, b;
+  kv8_cvt4<FMT>(w, a, b);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&b));
+  x[0] = f.x; x[1] = f.y; x[2] = g.x; x[3] = g.y;
 }
 // Scale of a block whose largest magnitude has the fp32 bits `amax`.
 __device__ __forceinline__ float kv8_scale(uint32_t amax, int fmt) {

@@ -5,7 +5,7 @@
 namespace kf {
 
 // Query rows of a kv head from which the tensor-memory kernel runs.
-constexpr int KV8_PROMPT_ROWS = 17;
+constexpr int KV8_PROMPT_ROWS = 33;
 
 // How a call is cut: chunks of keys so that there are a few CTAs per SM, each
 // with work enough to pay for its start.
@@ -41,7 +41,7 @@ static void kv8_plan(const KV8& c, int64_t T, int G, int64_t max_len, int flags,
   w->chunks = static_cast<int>((max_len + chunk - 1) / chunk);
   if (w->chunks < 1) w->chunks = 1;
   w->rows = static_cast<int>(rows);
-  w->ld_score = (flags & KF_KV8_TRACK) && rows <= KV8_ROWS ? (max_len + 15) / 16 * 16 : 0;
+  w->ld_score = (flags & KF_KV8_TRACK) ? (max_len + 15) / 16 * 16 : 0;
 }
 
 // Splits the workspace; returns the bytes it takes.
@@ -113,6 +113,38 @@ struct KV8Call {
   float* lse;
   cudaStream_t st;
 };
+
+template <int DH, int FMT, int PL, int RH>
+static cudaError_t kv8_split(const KV8& c, const KV8Call& a, const KV8Work& w) {
+  auto kern = kv8_split_kernel<DH, FMT, PL, RH>;
+  constexpr int smem = SplitCfg<DH>::SMEM;
+  static DeviceOnce once;
+  cudaError_t attr = cudaSuccess;
+  once.run("kf_kv8_attention", nullptr, [&](int) {
+    attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return attr == cudaSuccess ? KF_OK : KF_E_CUDA;
+  });
+  if (attr != cudaSuccess) return attr;
+  const dim3 grid(static_cast<unsigned>(w.chunks),
+                  static_cast<unsigned>((w.rows + KV8_ROWS - 1) / KV8_ROWS),
+                  static_cast<unsigned>(c.B * c.H));
+  return launch_chained(kern, grid, dim3(128), smem, a.st, c, a.q, a.q_sb, a.q_sh, a.q_st, a.out,
+                        a.o_sb, a.o_sh, a.o_st, a.dtype, a.q_vec, a.counts, a.T, a.G, a.max_len,
+                        a.scale_log2, a.flags, a.lse, w);
+}
+template <int DH, int FMT, int PL>
+static cudaError_t kv8_split_rows(const KV8& c, const KV8Call& a, const KV8Work& w, bool half) {
+  return half ? kv8_split<DH, FMT, PL, 1>(c, a, w) : kv8_split<DH, FMT, PL, 2>(c, a, w);
+}
+template <int DH>
+static cudaError_t kv8_split_any(const KV8& c, const KV8Call& a, const KV8Work& w, bool half) {
+  const bool two = a.dtype == KF_DT_F32;
+  if (c.fmt == KF_KV8_INT8)
+    return two ? kv8_split_rows<DH, KF_KV8_INT8, 2>(c, a, w, half)
+               : kv8_split_rows<DH, KF_KV8_INT8, 1>(c, a, w, half);
+  return two ? kv8_split_rows<DH, KF_KV8_E4M3, 2>(c, a, w, half)
+             : kv8_split_rows<DH, KF_KV8_E4M3, 1>(c, a, w, half);
+}
 
 template <int DH, int PL>
 static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
@@ -205,14 +237,11 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int Ti = static_cast<int>(T), cap = static_cast<int>(max_len);
   const unsigned bh = static_cast<unsigned>(c.B * c.H);
-  const dim3 grid(static_cast<unsigned>(w.chunks),
-                  static_cast<unsigned>((w.rows + KV8_ROWS - 1) / KV8_ROWS), bh);
-  const bool reweigh = (flags & KF_KV8_TRACK) && !w.score;
+  const int64_t per = 16 / es;
+  const int o_vec = kv8_aligned(out, 16) && o_sb % per == 0 && o_sh % per == 0 && o_st % per == 0;
+  const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, o_vec, counts, Ti, G,
+                     cap, scale_log2, flags, lse, st};
   if (w.rows >= KV8_PROMPT_ROWS) {
-    const int64_t per = 16 / es;
-    const int o_vec = kv8_aligned(out, 16) && o_sb % per == 0 && o_sh % per == 0 && o_st % per == 0;
-    const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, o_vec, counts, Ti, G,
-                       cap, scale_log2, flags, lse, st};
     const bool two = dtype == KF_DT_F32;
     switch (c.D) {
       case 16: return two ? kv8_prompt<16, 2>(c, a, w) : kv8_prompt<16, 1>(c, a, w);
@@ -221,36 +250,14 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
       default: return two ? kv8_prompt<128, 2>(c, a, w) : kv8_prompt<128, 1>(c, a, w);
     }
   }
-  cudaError_t e = cudaSuccess, e2 = cudaSuccess;
-#define KF_KV8_SPLIT(DH, FMT, PL)                                                               \
-  e = launch_chained(kv8_split_kernel<DH, FMT, PL>, grid, dim3(128), 0, st, c, q, q_sb, q_sh,   \
-                     q_st, out, o_sb, o_sh, o_st, dtype, vec, counts, Ti, G, cap, scale_log2,   \
-                     flags, lse, w)
-#define KF_KV8_REWEIGH(DH, FMT, PL)                                                             \
-  e2 = launch_chained(kv8_reweigh_kernel<DH, FMT, PL>,                                          \
-                      dim3(static_cast<unsigned>((max_len + 63) / 64), bh), dim3(128), 0, st, c, \
-                      q, q_sb, q_sh, q_st, dtype, vec, counts, Ti, G, cap, scale_log2, flags, w)
-#define KF_KV8_PICK(WHAT, DH)                        \
-  do {                                               \
-    const bool i8 = c.fmt == KF_KV8_INT8;            \
-    const bool two = dtype == KF_DT_F32;             \
-    if (i8 && two)                                   \
-      WHAT(DH, KF_KV8_INT8, 2);                      \
-    else if (i8)                                     \
-      WHAT(DH, KF_KV8_INT8, 1);                      \
-    else if (two)                                    \
-      WHAT(DH, KF_KV8_E4M3, 2);                      \
-    else                                             \
-      WHAT(DH, KF_KV8_E4M3, 1);                      \
-  } while (0)
-#define KF_KV8_PICK_DH(WHAT)              \
-  switch (c.D) {                          \
-    case 16: KF_KV8_PICK(WHAT, 16); break; \
-    case 32: KF_KV8_PICK(WHAT, 32); break; \
-    case 64: KF_KV8_PICK(WHAT, 64); break; \
-    default: KF_KV8_PICK(WHAT, 128); break; \
+  cudaError_t e = cudaSuccess;
+  const bool half = w.rows <= 8;
+  switch (c.D) {
+    case 16: e = kv8_split_any<16>(c, a, w, half); break;
+    case 32: e = kv8_split_any<32>(c, a, w, half); break;
+    case 64: e = kv8_split_any<64>(c, a, w, half); break;
+    default: e = kv8_split_any<128>(c, a, w, half); break;
   }
-  KF_KV8_PICK_DH(KF_KV8_SPLIT)
   if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention launch");
   if (w.chunks > 1) {
     e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(128), 0, st,
@@ -258,16 +265,7 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
     if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention join launch");
   }
   if (max_len == 0 || !(flags & KF_KV8_TRACK)) return KF_OK;
-  if (reweigh) {
-    KF_KV8_PICK_DH(KF_KV8_REWEIGH)
-  } else {
-    e2 = launch_chained(kv8_weights_kernel,
-                        dim3(static_cast<unsigned>((max_len + 255) / 256), bh), dim3(256), 0, st,
-                        c, counts, Ti, G, cap, flags, w);
-  }
-  return cuda_status(e2, "kf_kv8_attention weights launch");
-#undef KF_KV8_SPLIT
-#undef KF_KV8_REWEIGH
-#undef KF_KV8_PICK
-#undef KF_KV8_PICK_DH
+  e = launch_chained(kv8_weights_kernel, dim3(static_cast<unsigned>((max_len + 255) / 256), bh),
+                     dim3(256), 0, st, c, counts, Ti, G, cap, flags, w);
+  return cuda_status(e, "kf_kv8_attention weights launch");
 }
