@@ -16,7 +16,8 @@
 // four V rows; the 16-byte pieces of the ring are placed so that those reads
 // touch all banks. 16 rows fill the m16 tile; the 128-row tensor-memory
 // products would waste 7/8 of theirs here. RH = 1 serves at most 8 rows and
-// skips the softmax of the upper half of the tile.
+// skips the softmax of the upper half of the tile; with two planes (fp32 q) the
+// second plane then takes that half, so one product does both.
 // (Codes loaded straight into registers, one group ahead, left 8 warps an SM
 // and 2.5 TB/s on 16 x 24k tokens of 8 kv heads of 128.)
 //
@@ -33,6 +34,7 @@
 namespace kf {
 
 constexpr int KV8_ROWS = 16;            // query rows of a CTA
+constexpr int KV8_SPLIT_ROWS = 64;      // query rows of a kv head that this path serves
 constexpr int KV8_CHUNK_MAX = 4096;     // keys of a CTA: at most 256 pages of 16
 constexpr float KV8_BIAS = 9.f;         // log2 of P's largest value after a rescale
 constexpr float KV8_SLACK = 6.f;        // growth of the maximum that needs no rescale
@@ -51,6 +53,7 @@ struct KV8Work {
   int rows;       // T * G
   int chunks;
   int chunk;      // keys of a chunk
+  bool prompt;    // the tensor-memory kernel runs
 };
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -118,18 +121,18 @@ struct QFrag {
   static constexpr int EPT = DH / 4 < 16 ? DH / 4 : 16;  // consecutive elements of a piece
   static constexpr int NPC = DH / 4 / EPT;               // pieces (64 elements apart)
   static constexpr int KS = DH / 16;                     // k-steps
-  uint32_t a[PL][KS][4];  // RH = 1: rows g + 8 are zeros
+  // RH = 1: rows g + 8 are zeros, or with two planes the second plane.
+  static constexpr int NP = RH == 1 ? 1 : PL;            // products per k-step
+  uint32_t a[NP][KS][4];
   float qf[RH];
 
   __device__ __forceinline__ void load(const KV8& c, const void* q, int64_t q_sb, int64_t q_sh,
                                        int64_t q_st, int dtype, bool vec, int b, int h, int G,
                                        int row0, int rows, float scale_log2) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    if constexpr (RH == 1) {
+    if constexpr (RH == 1 && PL == 1) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int pl = 0; pl < PL; ++pl) a[pl][s][1] = a[pl][s][3] = 0u;
+      for (int s = 0; s < KS; ++s) a[0][s][1] = a[0][s][3] = 0u;
     }
 #pragma unroll
     for (int r = 0; r < RH; ++r) {
@@ -171,8 +174,8 @@ struct QFrag {
         a[0][s][r] = pack_half2(y[0], y[1]);
         a[0][s][2 + r] = pack_half2(y[2], y[3]);
         if constexpr (PL == 2) {
-          a[1][s][r] = pack_half2_rest(y[0], y[1], a[0][s][r]);
-          a[1][s][2 + r] = pack_half2_rest(y[2], y[3], a[0][s][2 + r]);
+          a[NP - 1][s][RH == 1 ? 1 : r] = pack_half2_rest(y[0], y[1], a[0][s][r]);
+          a[NP - 1][s][RH == 1 ? 3 : 2 + r] = pack_half2_rest(y[2], y[3], a[0][s][2 + r]);
         }
       }
     }
@@ -251,9 +254,13 @@ __device__ __forceinline__ void score_tile(const QFrag<DH, PL, RH>& q, const KBy
     for (int s = 0; s < DH / 16; ++s) {
       uint32_t b0, b1;
       kv8_cvt4<FMT>(kb.w[n][s], b0, b1);
-      if constexpr (PL == 2)
+      if constexpr (PL == 2 && RH == 2)
         mma_f16_16816(d[n], q.a[1][s][0], q.a[1][s][1], q.a[1][s][2], q.a[1][s][3], b0, b1);
       mma_f16_16816(d[n], q.a[0][s][0], q.a[0][s][1], q.a[0][s][2], q.a[0][s][3], b0, b1);
+    }
+    if constexpr (PL == 2 && RH == 1) {
+      d[n][0] += d[n][2];
+      d[n][1] += d[n][3];
     }
   }
 }
@@ -434,6 +441,10 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
             for (int n = 0; n < NT; ++n) {
               o[n][2 * r] *= alpha;
               o[n][2 * r + 1] *= alpha;
+              if (PL == 2 && RH == 1) {
+                o[n][2] *= alpha;
+                o[n][3] *= alpha;
+              }
             }
           }
         }
@@ -454,7 +465,8 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
           p[u] = x == -INFINITY ? 0.f : e * ratio;
         }
         hi[2 * n + r] = pack_half2(p[0], p[1]);
-        if constexpr (PL == 2) lo[2 * n + r] = pack_half2_rest(p[0], p[1], hi[2 * n + r]);
+        if constexpr (PL == 2)
+          (RH == 1 ? hi[2 * n + 1] : lo[2 * n + r]) = pack_half2_rest(p[0], p[1], hi[2 * n + r]);
       }
     // Slots past the end hold whatever was there (an e4m3 NaN among it): as
     // zeros they cannot reach the product.
@@ -476,7 +488,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
         kv8_cvt4<FMT>(__byte_perm(vb.w[0][u], vb.w[1][u], sel), b00, b01);
         kv8_cvt4<FMT>(__byte_perm(vb.w[2][u], vb.w[3][u], sel), b10, b11);
         const int n = 4 * u + 2 * half;
-        if constexpr (PL == 2) {
+        if constexpr (PL == 2 && RH == 2) {
           mma_f16_16816(o[n], lo[0], lo[1], lo[2], lo[3], b00, b10);
           mma_f16_16816(o[n + 1], lo[0], lo[1], lo[2], lo[3], b01, b11);
         }
@@ -503,8 +515,9 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
     float* row = s_o + (warp * KV8_ROWS + g + 8 * r) * DH;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      row[(2 * t) * NT + n] = o[n][2 * r];
-      row[(2 * t + 1) * NT + n] = o[n][2 * r + 1];
+      const bool both = PL == 2 && RH == 1;
+      row[(2 * t) * NT + n] = both ? o[n][0] + o[n][2] : o[n][2 * r];
+      row[(2 * t + 1) * NT + n] = both ? o[n][1] + o[n][3] : o[n][2 * r + 1];
     }
   }
   __syncthreads();
@@ -600,11 +613,11 @@ __global__ void __launch_bounds__(128)
 // ---------------------------------------------------------------- weights
 
 // Adds each key's weight to the record, from the scores the split kernel left
-// (at most 32 rows). One thread per key; the rows are added in order.
+// (at most KV8_SPLIT_ROWS rows). One thread per key; the rows are added in order.
 __global__ void __launch_bounds__(256)
     kv8_weights_kernel(KV8 c, const int32_t* __restrict__ counts, int T, int G, int max_len,
                        int flags, KV8Work w) {
-  __shared__ float s_lse[2 * KV8_ROWS];
+  __shared__ float s_lse[KV8_SPLIT_ROWS];
   pdl_launch_dependents();
   pdl_wait();
   const int bh = blockIdx.y;

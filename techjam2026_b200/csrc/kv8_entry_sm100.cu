@@ -4,19 +4,41 @@
 
 namespace kf {
 
-// Query rows of a kv head from which the tensor-memory kernel runs.
-constexpr int KV8_PROMPT_ROWS = 33;
+// Which kernel serves a call of `rows` query rows per kv head. Measured (us,
+// split / tensor-memory kernel; 8 x 8 heads of 128 over 8k tokens bf16, 16 x 12
+// heads of 64 over 1k fp32): 32 rows 94 / 137 and 38 / 81, 64 rows 140 / 146 and
+// 56 / 83, 128 rows 260 / 158 and 101 / 85. With weights the split kernel keeps every score for
+// the last pass; where that takes too much memory, 17 rows and more go to the
+// other kernel, which computes the scores again.
+static bool kv8_is_prompt(const KV8& c, int64_t rows, int64_t max_len, int flags) {
+  if (rows > KV8_SPLIT_ROWS) return true;
+  const int64_t scores = static_cast<int64_t>(c.B) * c.H * rows * max_len * 4;
+  return (flags & KF_KV8_TRACK) && rows > KV8_ROWS && scores > (512LL << 20);
+}
 
 // How a call is cut: chunks of keys so that there are a few CTAs per SM, each
 // with work enough to pay for its start.
-static void kv8_plan(const KV8& c, int64_t T, int G, int64_t max_len, int flags, KV8Work* w) {
+static void kv8_plan(const KV8& c, int dtype, int64_t T, int G, int64_t max_len, int flags,
+                     KV8Work* w) {
   const int64_t rows = T * G;
-  if (rows >= KV8_PROMPT_ROWS) {
-    const int64_t ctas = (rows + 255) / 256 * c.B * c.H;
-    int64_t chunks = (2 * 148 + ctas - 1) / ctas;
-    const int64_t most = (max_len + 2047) / 2048;
-    if (chunks > most) chunks = most;
-    if (chunks < 1) chunks = 1;
+  w->prompt = kv8_is_prompt(c, rows, max_len, flags);
+  if (w->prompt) {
+    // One CTA per SM: as many parts of the keys as make the waves of CTAs cost
+    // least, in steps of 128 keys. A CTA's start and end cost about four steps,
+    // a part's share of the join about one. (8 heads of 128, a chunk of 1000 over 62k
+    // tokens: 32 CTAs a part, 5 parts 575 us, 10 parts 472, 14 parts 423.)
+    const int64_t tile = 128 * (c.D == 128 && dtype == KF_DT_F32 ? 1 : 2);
+    const int64_t ctas = (rows + tile - 1) / tile * c.B * c.H;
+    const int64_t steps = (max_len + 127) / 128;
+    const int sms = sm_count();
+    int64_t chunks = 1, best = INT64_MAX;
+    for (int64_t n = 1; n <= 64 && n * 16 <= steps + 15; ++n) {
+      const int64_t cost = (ctas * n + sms - 1) / sms * ((steps + n - 1) / n + 4) + n - 1;
+      if (cost < best) {
+        best = cost;
+        chunks = n;
+      }
+    }
     const int64_t chunk = ((max_len + chunks - 1) / chunks + 127) / 128 * 128;
     w->chunk = static_cast<int>(chunk < 128 ? 128 : chunk);
     w->chunks = static_cast<int>((max_len + w->chunk - 1) / w->chunk);
@@ -27,7 +49,12 @@ static void kv8_plan(const KV8& c, int64_t T, int G, int64_t max_len, int flags,
   }
   const int64_t tiles = (rows + KV8_ROWS - 1) / KV8_ROWS;
   const int64_t items = tiles * c.B * c.H;
-  const int64_t want = 148 * 8;
+  // One wave of the CTAs that an SM holds. (A 65k sequence of 16 heads of 64: 42
+  // us with four CTAs an SM, 50 with eight; 16 long sequences of 8 heads of 128:
+  // 146 with three, 164 with eight. More parts also make the join longer.)
+  const int64_t want =
+      static_cast<int64_t>(sm_count()) *
+      (c.D == 128 ? SplitCfg<128>::min_blocks(dtype == KF_DT_F32 ? 2 : 1) : SplitCfg<64>::min_blocks(1));
   int64_t chunks = (want + items - 1) / items;
   const int64_t most = (max_len + 127) / 128;    // at least 128 keys a chunk
   if (chunks > most) chunks = most;
@@ -63,7 +90,7 @@ static int64_t kv8_carve(const KV8& c, int dtype, int flags, uint8_t* base, KV8W
   if (w->ld_score) w->score = take(n * w->ld_score);
   w->planes = nullptr;
   w->qf = nullptr;
-  if (w->rows >= KV8_PROMPT_ROWS) {
+  if (w->prompt) {
     const int64_t planes = dtype == KF_DT_F32 ? 2 : 1;
     w->planes = reinterpret_cast<uint16_t*>(take((planes * n * c.D + 1) / 2));
     w->qf = take(n);
@@ -203,7 +230,7 @@ extern "C" int64_t kf_kv8_attention_workspace_bytes(const kf_kv8_cache* cache, i
     return -1;
   if (T == 0 || c.B == 0) return 0;
   KV8Work w;
-  kv8_plan(c, T, static_cast<int>(q_heads / c.H), max_len, flags, &w);
+  kv8_plan(c, dtype, T, static_cast<int>(q_heads / c.H), max_len, flags, &w);
   return kv8_carve(c, dtype, flags, nullptr, &w);
 }
 
@@ -224,7 +251,7 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
   }
   const int G = static_cast<int>(q_heads / c.H);
   KV8Work w;
-  kv8_plan(c, T, G, max_len, flags, &w);
+  kv8_plan(c, dtype, T, G, max_len, flags, &w);
   const int64_t need = kv8_carve(c, dtype, flags, static_cast<uint8_t*>(workspace), &w);
   if (need > 0 && (!workspace || workspace_bytes < need || !kv8_aligned(workspace, 256))) {
     set_last_error("kf_kv8_attention: needs a 256-byte aligned workspace of %lld bytes",
@@ -241,7 +268,7 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
   const int o_vec = kv8_aligned(out, 16) && o_sb % per == 0 && o_sh % per == 0 && o_st % per == 0;
   const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, o_vec, counts, Ti, G,
                      cap, scale_log2, flags, lse, st};
-  if (w.rows >= KV8_PROMPT_ROWS) {
+  if (w.prompt) {
     const bool two = dtype == KF_DT_F32;
     switch (c.D) {
       case 16: return two ? kv8_prompt<16, 2>(c, a, w) : kv8_prompt<16, 1>(c, a, w);

@@ -64,7 +64,8 @@ class KV8Cache:
              token has received (needed by `track` and kv8_evict)
     """
 
-    __slots__ = ("k", "v", "scale", "table", "lens", "weight", "struct", "_ref")
+    __slots__ = ("k", "v", "scale", "table", "lens", "weight", "struct", "batch", "kv_heads",
+                 "head_dim", "block", "device", "_ref", "_work")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, scale: torch.Tensor, table: torch.Tensor,
                  lens: torch.Tensor, weight: Optional[torch.Tensor] = None):
@@ -97,6 +98,9 @@ class KV8Cache:
             pages, table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1],
             table.shape[0], heads, head_dim, block, CODE_DTYPES[k.dtype])
         self._ref = ctypes.byref(self.struct)
+        self.batch, self.kv_heads, self.block, self.head_dim = table.shape[0], heads, block, head_dim
+        self.device = k.device
+        self._work = {}              # workspace bytes by (type, T, heads, max_len, flags)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, block: int, head_dim: int, table: torch.Tensor,
@@ -109,11 +113,6 @@ class KV8Cache:
                    torch.zeros((pages, kv_heads, block), dtype=torch.float32, device=dev)
                    if weight else None)
 
-    batch = property(lambda self: self.struct.batch)
-    kv_heads = property(lambda self: self.struct.kv_heads)
-    head_dim = property(lambda self: self.struct.head_dim)
-    block = property(lambda self: self.struct.block)
-
 
 def _dtype_code(t: torch.Tensor, what: str) -> int:
     code = VALUE_DTYPES.get(t.dtype)
@@ -122,23 +121,26 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _check_call(what: str, cache: KV8Cache, counts: Optional[torch.Tensor], *tensors) -> None:
-    device = cache.k.device
+def _check_call(what: str, cache: KV8Cache, counts: Optional[torch.Tensor], *tensors) -> int:
+    """Checks that a call's tensors are where the cache is; its stream."""
+    device = cache.device
     for t in tensors:
         if t.device != device:
             raise ValueError(f"{what}: tensors must be on the cache's device {device}, "
                              f"got {t.device}")
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         raise RuntimeError(f"{what}: the cache is on {device}, which is not the current device")
     if counts is not None:
         _check_index(what, "counts", counts, cache)
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _check_index(what: str, name: str, t: torch.Tensor, cache: KV8Cache) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != (cache.batch,) or not t.is_contiguous() \
-            or t.device != cache.k.device:
+    if t.dtype is not torch.int32 or t.shape != cache.lens.shape or not t.is_contiguous() \
+            or t.device != cache.device:
         raise ValueError(f"{what}: {name} must be a contiguous int32 tensor [{cache.batch}] on "
-                         f"{cache.k.device}")
+                         f"{cache.device}")
 
 
 def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor,
@@ -166,11 +168,10 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor,
         raise TypeError(f"{what}: k and v must have one type")
     if k.stride(3) != 1 or v.stride(3) != 1:
         raise ValueError(f"{what}: k and v need unit stride along head_dim")
-    _check_call(what, cache, counts, k, v)
+    stream = _check_call(what, cache, counts, k, v)
     rc = _lib.lib().kf_kv8_append(
-        cache._ref, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-        v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), code,
-        counts.data_ptr() if counts is not None else None, T, _lib.stream_ptr())
+        cache._ref, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], code,
+        counts.data_ptr() if counts is not None else None, T, stream)
     _lib.check(rc, "kf_kv8_append")
 
 
@@ -185,16 +186,16 @@ def kv8_read(cache: KV8Cache, n: int, start: Optional[torch.Tensor] = None,
         raise ValueError(f"{what}: n must not be negative")
     if dtype not in VALUE_DTYPES:
         raise TypeError(f"{what}: dtype must be float32, bfloat16 or float16, got {dtype}")
-    _check_call(what, cache, counts)
+    stream = _check_call(what, cache, counts)
     if start is not None:
         _check_index(what, "start", start, cache)
     shape = (cache.batch, cache.kv_heads, n, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=cache.k.device)
-    v = torch.empty(shape, dtype=dtype, device=cache.k.device)
+    k = torch.empty(shape, dtype=dtype, device=cache.device)
+    v = torch.empty(shape, dtype=dtype, device=cache.device)
     rc = _lib.lib().kf_kv8_read(
         cache._ref, start.data_ptr() if start is not None else None,
         counts.data_ptr() if counts is not None else None, n, k.data_ptr(), v.data_ptr(),
-        VALUE_DTYPES[dtype], _lib.stream_ptr())
+        VALUE_DTYPES[dtype], stream)
     _lib.check(rc, "kf_kv8_read")
     return k, v
 
@@ -237,21 +238,24 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, counts: Optional[torch.Tenso
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
         raise ValueError(f"{what}: out must have q's shape and type and unit stride along "
                          "head_dim")
-    _check_call(what, cache, counts, q, out)
+    stream = _check_call(what, cache, counts, q, out)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
     flags = (_lib.KF_KV8_CAUSAL if causal else 0) | (_lib.KF_KV8_TRACK if track else 0)
     L = _lib.lib()
-    need = L.kf_kv8_attention_workspace_bytes(cache._ref, code, T, Hq, max_len, flags)
-    if need < 0:
-        raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
+    key = (code, T, Hq, max_len, flags)
+    need = cache._work.get(key)
+    if need is None:
+        need = L.kf_kv8_attention_workspace_bytes(cache._ref, *key)
+        if need < 0:
+            raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
+        cache._work[key] = need
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     rc = L.kf_kv8_attention(
-        cache._ref, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
-        out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), code,
+        cache._ref, q.data_ptr(), *q.stride()[:3], out.data_ptr(), *out.stride()[:3], code,
         counts.data_ptr() if counts is not None else None, T, Hq, max_len,
         float(sm_scale) if sm_scale is not None else D ** -0.5, flags,
         lse.data_ptr() if lse is not None else None,
-        work.data_ptr() if work is not None else None, need, _lib.stream_ptr())
+        work.data_ptr() if work is not None else None, need, stream)
     _lib.check(rc, "kf_kv8_attention")
     return (out, lse) if return_lse else out
 
@@ -281,10 +285,10 @@ def kv8_evict(cache: KV8Cache, table_out: torch.Tensor, budget: int, recent: int
     if new.batch != cache.batch or table_out.shape[1] * cache.block < budget:
         raise ValueError(f"{what}: table_out must be [{cache.batch}, at least "
                          f"{-(-budget // cache.block)}]")
-    _check_call(what, cache, None)
+    stream = _check_call(what, cache, None)
     kept = torch.empty((cache.batch, cache.kv_heads, budget), dtype=torch.int32,
-                       device=cache.k.device)
+                       device=cache.device)
     rc = _lib.lib().kf_kv8_evict(cache._ref, table_out.data_ptr(), new.struct.ld_table, budget,
-                                 recent, kept.data_ptr(), new.lens.data_ptr(), _lib.stream_ptr())
+                                 recent, kept.data_ptr(), new.lens.data_ptr(), stream)
     _lib.check(rc, "kf_kv8_evict")
     return kept, new

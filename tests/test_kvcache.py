@@ -1,0 +1,30 @@
+"""The page pool's host side. CPU only."""
+from __future__ import annotations
+
+import pytest
+
+from techjam2026_b200.kvcache import PagePool
+
+
+def test_pages_are_handed_out_once_and_come_back():
+    pool = PagePool(pages=7, batch=2, blocks=3, block=16, device="cpu")
+    pool.reserve([1, 33])
+    assert [len(r) for r in pool.rows] == [1, 3] and len(pool.free) == 3
+    pool.reserve([16, 40])                        # still the same pages
+    assert [len(r) for r in pool.rows] == [1, 3]
+    used = [p for r in pool.rows for p in r]
+    assert len(set(used + pool.free)) == 7
+    assert pool.table[0, 0] == pool.rows[0][0]
+    assert pool.table[1].tolist() == pool.rows[1]
+    rows = [pool.take(1), pool.take(2)]
+    pool.replace(rows)
+    assert pool.rows == rows and len(pool.free) == 4
+    assert sorted(pool.free + rows[0] + rows[1]) == list(range(7))
+
+
+def test_a_full_pool_and_a_long_sequence_are_refused():
+    pool = PagePool(pages=3, batch=2, blocks=3, block=16, device="cpu")
+    with pytest.raises(RuntimeError):
+        pool.reserve([0, 49])
+    with pytest.raises(RuntimeError):
+        pool.reserve([33, 17])

@@ -1,0 +1,92 @@
+"""The layer stack over the 8-bit cache against the CPU oracle. The cache's
+own rounding is what separates them: a code step is 1/127 of a block's largest
+magnitude (about 4 standard deviations), so int8 K and V carry about 1 %, e4m3
+about 2.5 % of relative error, a share of which reaches the outputs."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import oracle
+from techjam2026_b200.configs import TransformerConfig, make_state_dict
+from techjam2026_b200.kvcache import CachedStack
+from techjam2026_b200.model import LayerStack
+
+pytestmark = pytest.mark.gpu
+
+
+def setup(S, d, H, layers=2, B=3):
+    cfg = TransformerConfig(B, S, d, H, 2 * d, layers, True)
+    sd = make_state_dict(cfg, 0)
+    stack = LayerStack(cfg)
+    stack.load_state_dict(sd, strict=True)
+    x = torch.randn(B, S, d, generator=torch.Generator().manual_seed(3))
+    want = oracle.forward(sd, layers, H, x, torch.ones(B, S, dtype=torch.bool), causal=True)
+    return stack, x, want
+
+
+def rel(a, b):
+    return float((a.cpu() - b).norm() / b.norm())
+
+
+@pytest.mark.parametrize("code,bound", [(torch.int8, 0.02), (torch.float8_e4m3fn, 0.05)])
+@pytest.mark.parametrize("d,H", [(128, 4), (256, 4), (256, 2), (64, 4)])
+def test_prompt_then_tokens_match_the_whole_sequence(d, H, code, bound):
+    stack, x, want = setup(90, d, H)
+    model = CachedStack(stack, 3, 90, code, block=16)
+    got = [model(x[:, :70].cuda())] + [model(x[:, i:i + 1].cuda()) for i in range(70, 90)]
+    assert rel(torch.cat(got, 1), want) < bound
+    assert model.lens.tolist() == [90] * 3
+
+
+def test_ragged_chunks_match_the_whole_sequences():
+    stack, x, want = setup(120, 128, 2)
+    model = CachedStack(stack, 3, 120, block=32)
+    at = [0, 0, 0]
+    got = torch.zeros_like(x)
+    for counts in ([40, 1, 0], [0, 37, 50], [40, 40, 17], [40, 42, 53]):
+        T = max(counts)
+        chunk = torch.full((3, T, 128), float("nan"))
+        for b, n in enumerate(counts):
+            chunk[b, :n] = x[b, at[b]:at[b] + n]
+        chunk = chunk.nan_to_num(7.0)            # what stands past a count must not matter
+        out = model(chunk.cuda(), counts=counts).cpu()
+        for b, n in enumerate(counts):
+            got[b, at[b]:at[b] + n] = out[b, :n]
+            assert not out[b, n:].any()
+            at[b] += n
+    assert at == [120] * 3
+    assert rel(got, want) < 0.02
+
+
+def test_a_budget_bounds_the_cache_and_keeps_the_outputs_near():
+    stack, x, want = setup(200, 128, 2, layers=1)
+    model = CachedStack(stack, 3, 224, block=16, budget=160, recent=32)
+    got = [model(x[:, :150].cuda())]
+    for i in range(150, 200, 5):
+        got.append(model(x[:, i:i + 5].cuda()))
+        assert max(model.held) <= 160
+        assert model.lens.tolist() == model.held
+    used = [p for r in model.pool.rows for p in r]
+    assert len(used) == len(set(used)) and not set(used) & set(model.pool.free)
+    got = torch.cat(got, 1)
+    assert rel(got[:, :160], want[:, :160]) < 0.02       # nothing was cut before
+    # a fifth of the tokens are gone: the attention branch moves, the stream less
+    assert rel(got, want) < 0.15 and torch.isfinite(got).all()
+
+
+def test_refusals():
+    stack, x, _ = setup(16, 64, 4, layers=1)
+    with pytest.raises(ValueError):
+        CachedStack(stack, 3, 16, budget=32)
+    model = CachedStack(stack, 3, 16, block=16)
+    with pytest.raises(ValueError):
+        model(x[:2].cuda())
+    with pytest.raises(ValueError):
+        model(x.cuda(), counts=[1, 2, 17])
+    with pytest.raises(RuntimeError):
+        model(torch.cat([x, x], 1).cuda())               # 32 tokens into 16
+    assert model.lens.tolist() == [0, 0, 0]
+    cfg = TransformerConfig(1, 8, 64, 4, 64, 1, False)
+    with pytest.raises(ValueError):
+        CachedStack(LayerStack(cfg), 1, 8)
