@@ -559,12 +559,18 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
 
 // ---------------------------------------------------------------- join
 
-// One CTA per query row: the chunks' parts in chunk order.
-__global__ void __launch_bounds__(128)
+// One CTA per query row: the parts of its chunks, in an order that depends on
+// their number only. Latency is what it costs, so every loop has its loads in
+// flight together.
+constexpr int KV8_JOIN_THREADS = 256;
+constexpr int KV8_JOIN_TILE = 1024;  // chunks whose factors shared memory holds
+
+__global__ void __launch_bounds__(KV8_JOIN_THREADS)
     kv8_join_kernel(KV8 c, void* __restrict__ out, int64_t o_sb, int64_t o_sh, int64_t o_st,
                     int dtype, int T, int G, float* __restrict__ lse_out, KV8Work w) {
-  __shared__ float s_x[128], s_l[4];
-  __shared__ float s_m[4];
+  __shared__ float s_a[KV8_JOIN_TILE];   // a chunk's factor; 0: it wrote no part
+  __shared__ float s_x[KV8_JOIN_THREADS];
+  __shared__ float s_m[KV8_JOIN_THREADS / 32], s_l[KV8_JOIN_THREADS / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int row = blockIdx.x;
@@ -573,31 +579,42 @@ __global__ void __launch_bounds__(128)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t at = (static_cast<int64_t>(bh) * w.rows + row) * w.chunks;
   float top = -INFINITY;
-  for (int i = tid; i < w.chunks; i += 128) top = fmaxf(top, w.ref[at + i]);
+  for (int i = tid; i < w.chunks; i += KV8_JOIN_THREADS) top = fmaxf(top, w.ref[at + i]);
 #pragma unroll
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (lane == 0) s_m[warp] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float l = 0.f;
-  for (int i = tid; i < w.chunks; i += 128)
-    l += (top == -INFINITY ? 1.f : fast_exp2(w.ref[at + i] - top)) * w.sum[at + i];
 #pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  if (lane == 0) s_l[warp] = l;
-  const int parts = 128 / c.D, d = tid & (c.D - 1), part = tid / c.D;
-  float x = 0.f;
-  for (int i = part; i < w.chunks; i += parts) {
-    const float r = w.ref[at + i];
-    // an empty chunk wrote no part (its sum is 0; a NaN sum has a part)
-    if (r == -INFINITY && w.sum[at + i] == 0.f) continue;
-    x += (top == -INFINITY ? 1.f : fast_exp2(r - top)) * w.part[(at + i) * c.D + d];
+  for (int u = 0; u < KV8_JOIN_THREADS / 32; ++u) top = fmaxf(top, s_m[u]);
+  const int parts = KV8_JOIN_THREADS / c.D, d = tid & (c.D - 1), part = tid / c.D;
+  float l = 0.f, x = 0.f;
+  for (int base = 0; base < w.chunks; base += KV8_JOIN_TILE) {
+    const int n = min(w.chunks - base, KV8_JOIN_TILE);
+    __syncthreads();
+    for (int i = tid; i < n; i += KV8_JOIN_THREADS) {
+      const float r = w.ref[at + base + i], sum = w.sum[at + base + i];
+      const float a = top == -INFINITY ? 1.f : fast_exp2(r - top);
+      l += a * sum;
+      // an empty chunk wrote no part (its sum is 0; a NaN sum has a part)
+      s_a[i] = r == -INFINITY && sum == 0.f ? 0.f : a;
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int i = part; i < n; i += parts) {
+      const float a = s_a[i];
+      if (a != 0.f) x += a * w.part[(at + base + i) * c.D + d];
+    }
   }
+#pragma unroll
+  for (int u = 16; u; u >>= 1) l += __shfl_xor_sync(0xffffffffu, l, u);
+  if (lane == 0) s_l[warp] = l;
   s_x[tid] = x;
   __syncthreads();
   if (part == 0) {
     for (int u = 1; u < parts; ++u) x += s_x[u * c.D + d];
-    l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    l = 0.f;
+#pragma unroll
+    for (int u = 0; u < KV8_JOIN_THREADS / 32; ++u) l += s_l[u];
     const int tok = row / G;
     const int hq = h * G + row - tok * G;
     kv8_store1(out, b * o_sb + hq * o_sh + tok * o_st + d, dtype, l == 0.f ? 0.f : x / l);
@@ -613,8 +630,11 @@ __global__ void __launch_bounds__(128)
 // ---------------------------------------------------------------- weights
 
 // Adds each key's weight to the record, from the scores the split kernel left
-// (at most KV8_SPLIT_ROWS rows). One thread per key; the rows are added in order.
-__global__ void __launch_bounds__(256)
+// (at most KV8_SPLIT_ROWS rows). One thread per four keys (a page is at least
+// 16); the rows are added in order.
+constexpr int KV8_WEIGHTS_KEYS = 4 * 128;  // keys of a CTA
+
+__global__ void __launch_bounds__(128)
     kv8_weights_kernel(KV8 c, const int32_t* __restrict__ counts, int T, int G, int max_len,
                        int flags, KV8Work w) {
   __shared__ float s_lse[KV8_SPLIT_ROWS];
@@ -622,25 +642,37 @@ __global__ void __launch_bounds__(256)
   pdl_wait();
   const int bh = blockIdx.y;
   const int b = bh / c.H, h = bh - b * c.H;
-  if (threadIdx.x < w.rows) s_lse[threadIdx.x] = w.lse[static_cast<int64_t>(bh) * w.rows + threadIdx.x];
-  __syncthreads();
   const int len = kv8_len(c, b);
   const int count = kv8_count(counts, b, T);
   const int end = min(kv8_end(c, len, count), max_len);
-  const int key = blockIdx.x * 256 + threadIdx.x;
+  if (static_cast<int>(blockIdx.x) * KV8_WEIGHTS_KEYS >= end) return;
+  if (threadIdx.x < w.rows)
+    s_lse[threadIdx.x] = w.lse[static_cast<int64_t>(bh) * w.rows + threadIdx.x];
+  __syncthreads();
+  const int key = blockIdx.x * KV8_WEIGHTS_KEYS + 4 * threadIdx.x;
   if (key >= end) return;
   const int page = kv8_page(c, b, key >> c.p_shift);
   if (page < 0) return;
-  float x = 0.f;
+  float* at = c.weight + (static_cast<int64_t>(page) * c.H + h) * c.P + (key & (c.P - 1));
+  const bool causal = (flags & KF_KV8_CAUSAL) != 0;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int r = 0; r < w.rows; ++r) {
     const int tok = r / G;
-    if (tok >= count || ((flags & KF_KV8_CAUSAL) && key > len + tok)) continue;
     const float l = s_lse[r];
-    if (l == -INFINITY) continue;
-    x += fast_exp2(w.score[(static_cast<int64_t>(bh) * w.rows + r) * w.ld_score + key] - l);
+    // keys of this row: below `limit` (a score past it may not have been written)
+    const int limit = tok >= count || l == -INFINITY ? 0 : (causal ? min(len + tok + 1, end) : end);
+    if (key >= limit) continue;
+    const float4 s = *reinterpret_cast<const float4*>(
+        w.score + (static_cast<int64_t>(bh) * w.rows + r) * w.ld_score + key);
+    x[0] += fast_exp2(s.x - l);
+    if (key + 1 < limit) x[1] += fast_exp2(s.y - l);
+    if (key + 2 < limit) x[2] += fast_exp2(s.z - l);
+    if (key + 3 < limit) x[3] += fast_exp2(s.w - l);
   }
-  float* at = c.weight + (static_cast<int64_t>(page) * c.H + h) * c.P + (key & (c.P - 1));
-  *at += x;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (key + u < end) at[u] += x[u];
 }
 
 }  // namespace kf

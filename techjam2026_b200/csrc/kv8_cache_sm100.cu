@@ -5,22 +5,27 @@ namespace kf {
 
 // ---------------------------------------------------------------- append
 //
-// One CTA per (page a chunk can reach, kv head, sequence and K|V). It loads the
-// page's new tokens into registers (16 bytes a thread and load), takes max|x|
-// as the largest bit pattern (so an infinity or a NaN wins), fixes the scale,
-// rescales the page's earlier codes if the scale grew, and writes the new
-// codes. Bound by memory: one read and one write of the chunk.
+// One CTA per (page a chunk can reach, kv head, sequence). It loads the page's
+// new tokens of K and V as they are into registers (16 bytes a thread and
+// load), takes max|x| of each as the largest bit pattern (so an infinity or a
+// NaN wins), fixes the scales, rescales the page's earlier codes if a scale
+// grew, and writes the new codes. Bound by memory, one read and one write of
+// the chunk, and by the loads in flight: K and V in CTAs of their own, held
+// as fp32, were 127 us for 400 MB of bf16 prompts and 52 for ragged fp32.
 
 constexpr int KV8_THREADS = 256;
 
-__device__ __forceinline__ uint32_t block_max_u32(uint32_t x, uint32_t* red) {
+// The larger of every thread's two numbers, each in one word.
+__device__ __forceinline__ void block_max2(uint32_t& x, uint32_t& y, uint2* red) {
   x = __reduce_max_sync(0xffffffffu, x);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+  y = __reduce_max_sync(0xffffffffu, y);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_uint2(x, y);
   __syncthreads();
-  uint32_t m = red[0];
 #pragma unroll
-  for (int w = 1; w < KV8_THREADS / 32; ++w) m = max(m, red[w]);
-  return m;
+  for (int w = 0; w < KV8_THREADS / 32; ++w) {
+    x = max(x, red[w].x);
+    y = max(y, red[w].y);
+  }
 }
 
 // N values (4, 8 or 16) to N codes.
@@ -37,73 +42,27 @@ __device__ __forceinline__ void kv8_put_codes(uint8_t* p, const float* x, float 
     *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
-// NG: runs of 16 bytes of input that a thread holds (a page has P * D / N).
-template <int DT, int NG>
-__global__ void __launch_bounds__(KV8_THREADS)
-    kv8_append_kernel(KV8 c, const void* __restrict__ k, int64_t k_sb, int64_t k_sh, int64_t k_st,
-                      const void* __restrict__ v, int64_t v_sb, int64_t v_sh, int64_t v_st,
-                      int vec, const int32_t* __restrict__ counts, int T) {
+// Scale of a page: what it was, raised to `mine`; NaN if either is.
+__device__ __forceinline__ float kv8_raise(float was, float mine) {
+  return (was != was || mine != mine) ? __uint_as_float(0x7fc00000u) : fmaxf(was, mine);
+}
+
+// Codes of runs [first, last) of a page (held by the threads in turn), and the
+// earlier ones rescaled from `was` to `s`.
+template <int DT, int FMT, int NG>
+__device__ __forceinline__ void kv8_write_page(uint8_t* codes, const uint4 (&x)[NG], int first,
+                                               int last, float was, float s) {
   constexpr int N = KV8Type<DT>::N;
-  __shared__ uint32_t red[KV8_THREADS / 32];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int h = blockIdx.y;
-  const int b = blockIdx.z >> 1;
-  const bool is_v = blockIdx.z & 1;
-  const int len = kv8_len(c, b);
-  const int end = kv8_end(c, len, kv8_count(counts, b, T));
-  const int j = (len >> c.p_shift) + static_cast<int>(blockIdx.x);
-  const int p0 = j << c.p_shift;                    // the page's first position
-  const int lo = p0 > len ? p0 : len;               // its new tokens are [lo, hi)
-  const int hi = p0 + c.P < end ? p0 + c.P : end;
-  if (lo >= hi) return;
-  const int page = kv8_page(c, b, j);
-  if (page < 0) return;
-
-  const void* src = is_v ? v : k;
-  const int64_t base = b * (is_v ? v_sb : k_sb) + h * (is_v ? v_sh : k_sh);
-  const int64_t st = is_v ? v_st : k_st;
-  const int64_t block = static_cast<int64_t>(page) * c.H + h;
-  uint8_t* codes = (is_v ? c.v : c.k) + block * c.P * c.D;
-  float* sp = c.scale + 2 * block + (is_v ? 1 : 0);
-  const float was = lo > p0 ? *sp : 0.f;
-  const int row_shift = c.d_shift - (N == 8 ? 3 : 2);  // runs of a row, as a power of two
-  const int first = (lo - p0) << row_shift, last = (hi - p0) << row_shift;
-
-  float x[NG][N];
-  uint32_t amax = 0;
-#pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    const int g = first + threadIdx.x + i * KV8_THREADS;
-#pragma unroll
-    for (int u = 0; u < N; ++u) x[i][u] = 0.f;
-    if (g < last) {
-      const int r = g >> row_shift;
-      KV8Type<DT>::load(src, base + (p0 + r - len) * st + N * (g - (r << row_shift)), vec != 0,
-                        x[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NG; ++i)
-#pragma unroll
-    for (int u = 0; u < N; ++u) amax = max(amax, __float_as_uint(x[i][u]) & 0x7fffffffu);
-  const float mine = kv8_scale(block_max_u32(amax, red), c.fmt);
-  const float s = (was != was || mine != mine) ? __uint_as_float(0x7fc00000u) : fmaxf(was, mine);
   const float inv = kv8_inverse(s);
-  if (s != s) {  // codes of a page whose scale is NaN mean nothing: keep them finite
-#pragma unroll
-    for (int i = 0; i < NG; ++i)
-#pragma unroll
-      for (int u = 0; u < N; ++u) x[i][u] = 0.f;
-  }
+  // codes of a page whose scale is NaN mean nothing: keep them finite
+  const bool spoiled = s != s;
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = first + threadIdx.x + i * KV8_THREADS;
     if (g < last) {
-      if (c.fmt == KF_KV8_INT8)
-        kv8_put_codes<KF_KV8_INT8, N>(codes + g * N, x[i], inv);
-      else
-        kv8_put_codes<KF_KV8_E4M3, N>(codes + g * N, x[i], inv);
+      float y[N];
+      KV8Type<DT>::values(spoiled ? make_uint4(0u, 0u, 0u, 0u) : x[i], y);
+      kv8_put_codes<FMT, N>(codes + g * N, y, inv);
     }
   }
   if (first > 0 && !(s == was)) {
@@ -111,17 +70,75 @@ __global__ void __launch_bounds__(KV8_THREADS)
     for (int g = threadIdx.x; g < first * (N / 4); g += KV8_THREADS) {
       uint32_t* w = reinterpret_cast<uint32_t*>(codes) + g;
       float y[4];
-      if (c.fmt == KF_KV8_INT8) {
-        kv8_decode4<KF_KV8_INT8>(*w, y);
-        *w = s != s ? 0u : kv8_encode4<KF_KV8_INT8>(y, ratio);
-      } else {
-        kv8_decode4<KF_KV8_E4M3>(*w, y);
-        *w = s != s ? 0u : kv8_encode4<KF_KV8_E4M3>(y, ratio);
-      }
+      kv8_decode4<FMT>(*w, y);
+      *w = spoiled ? 0u : kv8_encode4<FMT>(y, ratio);
     }
   }
-  if (threadIdx.x == 0) *sp = s;
-  if (c.weight && !is_v)
+}
+
+// NG: runs of 16 bytes of K, and of V, that a thread holds.
+template <int DT, int NG>
+__global__ void __launch_bounds__(KV8_THREADS)
+    kv8_append_kernel(KV8 c, const void* __restrict__ k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                      const void* __restrict__ v, int64_t v_sb, int64_t v_sh, int64_t v_st,
+                      int vec, const int32_t* __restrict__ counts, int T) {
+  constexpr int N = KV8Type<DT>::N;
+  __shared__ uint2 red[KV8_THREADS / 32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int h = blockIdx.y;
+  const int b = blockIdx.z;
+  const int len = kv8_len(c, b);
+  const int end = kv8_end(c, len, kv8_count(counts, b, T));
+  const int j = (len >> c.p_shift) + static_cast<int>(blockIdx.x);
+  const int p0 = j << c.p_shift;                    // the page's first position
+  const int lo = p0 > len ? p0 : len;               // its new tokens are [lo, hi)
+  const int hi = p0 + c.P < end ? p0 + c.P : end;
+  if (lo >= hi) return;
+  const int row_shift = c.d_shift - (N == 8 ? 3 : 2);  // runs of a row, as a power of two
+  const int first = (lo - p0) << row_shift, last = (hi - p0) << row_shift;
+
+  // (the loads do not wait for the table)
+  uint4 xk[NG], xv[NG];
+  const int64_t k0 = b * k_sb + h * k_sh, v0 = b * v_sb + h * v_sh;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    const int g = first + threadIdx.x + i * KV8_THREADS;
+    xk[i] = xv[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (g < last) {
+      const int r = g >> row_shift, col = N * (g - (r << row_shift));
+      const int64_t tok = p0 + r - len;
+      xk[i] = KV8Type<DT>::load(k, k0 + tok * k_st + col, vec != 0);
+      xv[i] = KV8Type<DT>::load(v, v0 + tok * v_st + col, vec != 0);
+    }
+  }
+  const int page = kv8_page(c, b, j);
+  if (page < 0) return;
+  const int64_t block = static_cast<int64_t>(page) * c.H + h;
+  float2* sp = reinterpret_cast<float2*>(c.scale + 2 * block);
+  const float2 was = lo > p0 ? *sp : make_float2(0.f, 0.f);
+  uint32_t mk = 0, mv = 0;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    KV8Type<DT>::collect(xk[i], mk);
+    KV8Type<DT>::collect(xv[i], mv);
+  }
+  mk = KV8Type<DT>::bits(mk);
+  mv = KV8Type<DT>::bits(mv);
+  block_max2(mk, mv, red);
+  const float sk = kv8_raise(was.x, kv8_scale(mk, c.fmt));
+  const float sv = kv8_raise(was.y, kv8_scale(mv, c.fmt));
+  uint8_t* ck = c.k + ((block << c.p_shift) << c.d_shift);
+  uint8_t* cv = c.v + ((block << c.p_shift) << c.d_shift);
+  if (c.fmt == KF_KV8_INT8) {
+    kv8_write_page<DT, KF_KV8_INT8, NG>(ck, xk, first, last, was.x, sk);
+    kv8_write_page<DT, KF_KV8_INT8, NG>(cv, xv, first, last, was.y, sv);
+  } else {
+    kv8_write_page<DT, KF_KV8_E4M3, NG>(ck, xk, first, last, was.x, sk);
+    kv8_write_page<DT, KF_KV8_E4M3, NG>(cv, xv, first, last, was.y, sv);
+  }
+  if (threadIdx.x == 0) *sp = make_float2(sk, sv);
+  if (c.weight)
     for (int r = lo - p0 + threadIdx.x; r < hi - p0; r += KV8_THREADS)
       c.weight[block * c.P + r] = 0.f;
 }
@@ -254,15 +271,15 @@ __global__ void __launch_bounds__(KV8_SELECT_THREADS)
     return weight_key(
         c.weight[(static_cast<int64_t>(page) * c.H + h) * c.P + (pos & (c.P - 1))]);
   };
-  for (int base = tid; base < cand && base < KV8_SELECT_KEYS; base += 4 * KV8_SELECT_THREADS) {
-    uint32_t key[4];
+  for (int base = tid; base < cand && base < KV8_SELECT_KEYS; base += 8 * KV8_SELECT_THREADS) {
+    uint32_t key[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const int pos = base + i * KV8_SELECT_THREADS;
       key[i] = pos < cand && pos < KV8_SELECT_KEYS ? load_key(pos) : 0u;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const int pos = base + i * KV8_SELECT_THREADS;
       if (pos < cand && pos < KV8_SELECT_KEYS) s_key[pos] = key[i];
     }
@@ -348,20 +365,49 @@ __global__ void __launch_bounds__(KV8_SELECT_THREADS)
   }
 }
 
-// NG: pieces of 16 codes that a thread moves.
+// Largest |code| of 16 codes, as fp16 (exact).
+template <int FMT>
+__device__ __forceinline__ float kv8_top16(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  __half2 m = __half2half2(__ushort_as_half(0));
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    uint32_t a, b;
+    kv8_cvt4<FMT>(w[u], a, b);
+    m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&a)));
+    m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&b)));
+  }
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
+// The values of 16 codes under scale s, quantised with 1 / scale `inv`.
+template <int FMT>
+__device__ __forceinline__ void kv8_recode16(uint8_t* p, const uint4& v, float s, float inv) {
+  float x[16];
+  kv8_decode4<FMT>(v.x, x);
+  kv8_decode4<FMT>(v.y, x + 4);
+  kv8_decode4<FMT>(v.z, x + 8);
+  kv8_decode4<FMT>(v.w, x + 12);
+#pragma unroll
+  for (int u = 0; u < 16; ++u) x[u] = __fmul_rn(x[u], s);
+  kv8_put_codes<FMT, 16>(p, x, inv);
+}
+
+// NG: pieces of 16 codes of K, and of V, that a thread moves. A row's scale is
+// the same along it, so the largest value of a piece is its largest code
+// times that (rounding keeps the order): the codes are decoded once.
 template <int FMT, int NG>
 __global__ void __launch_bounds__(KV8_THREADS)
     kv8_move_kernel(KV8 c, const int32_t* __restrict__ table_out, int64_t ld_out, int budget,
                     const int32_t* __restrict__ kept) {
-  __shared__ uint32_t red[KV8_THREADS / 32];
+  __shared__ uint2 red[KV8_THREADS / 32];
   __shared__ int64_t s_row[128];     // source row (block * P + slot) of each destination slot
-  __shared__ float s_scale[128];
+  __shared__ float2 s_scale[128];
   pdl_launch_dependents();
   pdl_wait();
   const int j = blockIdx.x;
   const int h = blockIdx.y;
-  const int b = blockIdx.z >> 1;
-  const bool is_v = blockIdx.z & 1;
+  const int b = blockIdx.z;
   const int len = kv8_len(c, b);
   const int n = len < budget ? len : budget;
   const int p0 = j << c.p_shift;
@@ -369,64 +415,58 @@ __global__ void __launch_bounds__(KV8_THREADS)
   if (rows <= 0) return;
   const int page = kv8_page(c, table_out, ld_out, b, j);
   if (page < 0) return;
+  const int64_t block = static_cast<int64_t>(page) * c.H + h;
   const int32_t* mine = kept + (static_cast<int64_t>(b) * c.H + h) * budget + p0;
   if (threadIdx.x < rows) {
     const int pos = mine[threadIdx.x];
     const int sp = kv8_page(c, b, pos >> c.p_shift);
-    const int64_t block = static_cast<int64_t>(sp) * c.H + h;
-    s_row[threadIdx.x] = sp < 0 ? -1 : block * c.P + (pos & (c.P - 1));
-    s_scale[threadIdx.x] = sp < 0 ? 0.f : c.scale[2 * block + (is_v ? 1 : 0)];
+    const int64_t from = static_cast<int64_t>(sp) * c.H + h;
+    const int64_t row = sp < 0 ? -1 : from * c.P + (pos & (c.P - 1));
+    s_row[threadIdx.x] = row;
+    s_scale[threadIdx.x] =
+        sp < 0 ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(c.scale + 2 * from);
+    c.weight[block * c.P + threadIdx.x] = row >= 0 ? c.weight[row] : 0.f;
   }
   __syncthreads();
   const int row_shift = c.d_shift - 4;
-  const uint8_t* src = is_v ? c.v : c.k;
   const int last = rows << row_shift;
-  uint4 w[NG];
+  uint4 wk[NG], wv[NG];
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = threadIdx.x + i * KV8_THREADS;
-    w[i] = make_uint4(0u, 0u, 0u, 0u);
+    wk[i] = wv[i] = make_uint4(0u, 0u, 0u, 0u);
     if (g < last) {
       const int64_t row = s_row[g >> row_shift];
-      if (row >= 0)
-        w[i] = *reinterpret_cast<const uint4*>(src + (row << c.d_shift) +
-                                               16 * (g & ((1 << row_shift) - 1)));
+      const int64_t at = (row << c.d_shift) + 16 * (g & ((1 << row_shift) - 1));
+      if (row >= 0) {
+        wk[i] = *reinterpret_cast<const uint4*>(c.k + at);
+        wv[i] = *reinterpret_cast<const uint4*>(c.v + at);
+      }
     }
   }
-  float x[NG][16];
-  uint32_t amax = 0;
+  uint32_t mk = 0, mv = 0;
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = threadIdx.x + i * KV8_THREADS;
-    const float s = g < last ? s_scale[g >> row_shift] : 0.f;
-    kv8_decode4<FMT>(w[i].x, x[i]);
-    kv8_decode4<FMT>(w[i].y, x[i] + 4);
-    kv8_decode4<FMT>(w[i].z, x[i] + 8);
-    kv8_decode4<FMT>(w[i].w, x[i] + 12);
-#pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      x[i][u] = __fmul_rn(x[i][u], s);
-      amax = max(amax, __float_as_uint(x[i][u]) & 0x7fffffffu);
-    }
+    const float2 s = g < last ? s_scale[g >> row_shift] : make_float2(0.f, 0.f);
+    mk = max(mk, __float_as_uint(__fmul_rn(kv8_top16<FMT>(wk[i]), s.x)) & 0x7fffffffu);
+    mv = max(mv, __float_as_uint(__fmul_rn(kv8_top16<FMT>(wv[i]), s.y)) & 0x7fffffffu);
   }
-  const float s = kv8_scale(block_max_u32(amax, red), c.fmt);
-  const float inv = kv8_inverse(s);
-  const int64_t block = static_cast<int64_t>(page) * c.H + h;
-  uint8_t* codes = (is_v ? c.v : c.k) + ((block << c.p_shift) << c.d_shift);
+  block_max2(mk, mv, red);
+  const float sk = kv8_scale(mk, c.fmt), sv = kv8_scale(mv, c.fmt);
+  const float ik = kv8_inverse(sk), iv = kv8_inverse(sv);
+  const int64_t base = (block << c.p_shift) << c.d_shift;
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = threadIdx.x + i * KV8_THREADS;
-    if (s != s) {
-#pragma unroll
-      for (int u = 0; u < 16; ++u) x[i][u] = 0.f;
+    if (g < last) {
+      const float2 s = s_scale[g >> row_shift];
+      // (a NaN scale makes the block's NaN: its codes are 0)
+      kv8_recode16<FMT>(c.k + base + 16 * g, wk[i], sk == sk ? s.x : 0.f, ik);
+      kv8_recode16<FMT>(c.v + base + 16 * g, wv[i], sv == sv ? s.y : 0.f, iv);
     }
-    if (g < last) kv8_put_codes<FMT, 16>(codes + 16 * g, x[i], inv);
   }
-  if (threadIdx.x == 0) c.scale[2 * block + (is_v ? 1 : 0)] = s;
-  if (!is_v && threadIdx.x < rows) {
-    const int64_t row = s_row[threadIdx.x];
-    c.weight[block * c.P + threadIdx.x] = row >= 0 ? c.weight[row] : 0.f;
-  }
+  if (threadIdx.x == 0) *reinterpret_cast<float2*>(c.scale + 2 * block) = make_float2(sk, sv);
 }
 
 // ---------------------------------------------------------------- host
@@ -515,7 +555,7 @@ extern "C" int kf_kv8_append(const kf_kv8_cache* cache, const void* k, int64_t k
   int vec = kv8_aligned(k, 16) && kv8_aligned(v, 16);
   for (int i = 0; i < 6; ++i) vec = vec && strides[i] % per == 0;
   const unsigned n = static_cast<unsigned>((c.P + T - 2) / c.P + 1);
-  const dim3 grid(n, static_cast<unsigned>(c.H), static_cast<unsigned>(2 * c.B));
+  const dim3 grid(n, static_cast<unsigned>(c.H), static_cast<unsigned>(c.B));
   // runs of 16 bytes that a thread holds: of a page, or of a chunk that is shorter
   const int64_t rows = T < c.P ? T : c.P;
   const int64_t groups = (rows * c.D / per + KV8_THREADS - 1) / KV8_THREADS;
@@ -617,7 +657,7 @@ extern "C" int kf_kv8_evict(const kf_kv8_cache* cache, const int32_t* table_out,
                                  dim3(KV8_SELECT_THREADS), smem, st, c, bud, rec, kept, lens_out);
   if (e != cudaSuccess) return cuda_status(e, "kf_kv8_evict select launch");
   const dim3 grid(static_cast<unsigned>((budget + c.P - 1) / c.P), static_cast<unsigned>(c.H),
-                  static_cast<unsigned>(2 * c.B));
+                  static_cast<unsigned>(c.B));
   const int groups = c.P * c.D / 16 / KV8_THREADS;
 #define KF_KV8_MOVE(FMT, NG)                                                                    \
   e = launch_chained(kv8_move_kernel<FMT, NG>, grid, dim3(KV8_THREADS), 0, st, c, table_out,     \

@@ -113,18 +113,28 @@ __device__ __forceinline__ void kv8_load4(const void* p, int64_t i, int dtype, b
   }
 }
 
-// N consecutive values of type DT (16 bytes); `vec`: the address is aligned.
+// N consecutive values of type DT: 16 bytes.
 template <int DT>
 struct KV8Type {
   static constexpr int N = DT == KF_DT_F32 ? 4 : 8;
-  __device__ __forceinline__ static void load(const void* p, int64_t i, bool vec, float* x) {
-    if (!vec) {
+  // The run at element i; `vec`: the address is aligned.
+  __device__ __forceinline__ static uint4 load(const void* p, int64_t i, bool vec) {
+    if (vec)
+      return __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) +
+                                                  i * (DT == KF_DT_F32 ? 4 : 2)));
+    uint32_t w[4];
 #pragma unroll
-      for (int u = 0; u < N; ++u) x[u] = kv8_load1(p, i + u, DT);
-      return;
+    for (int u = 0; u < 4; ++u) {
+      if constexpr (DT == KF_DT_F32) {
+        w[u] = static_cast<const uint32_t*>(p)[i + u];
+      } else {
+        const uint16_t* q = static_cast<const uint16_t*>(p) + i + 2 * u;
+        w[u] = q[0] | (static_cast<uint32_t>(q[1]) << 16);
+      }
     }
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) +
-                                                         i * (DT == KF_DT_F32 ? 4 : 2)));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ static void values(const uint4& v, float* x) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -139,6 +149,22 @@ struct KV8Type {
         x[2 * u + 1] = f.y;
       }
     }
+  }
+  // The largest magnitude of runs as a bit pattern (an infinity or a NaN is
+  // larger than any number): collect() gathers it in a word (two halves for
+  // the 16-bit types), bits() turns that into fp32 bits.
+  __device__ __forceinline__ static void collect(const uint4& v, uint32_t& m) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      m = DT == KF_DT_F32 ? max(m, w[u] & 0x7fffffffu) : __vmaxu2(m, w[u] & 0x7fff7fffu);
+  }
+  __device__ __forceinline__ static uint32_t bits(uint32_t m) {
+    if constexpr (DT == KF_DT_F32) return m;
+    const uint32_t top = max(m & 0xffffu, m >> 16);
+    if constexpr (DT == KF_DT_BF16) return top << 16;
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top)))) &
+           0x7fffffffu;
   }
   // N values to a 16-byte aligned address.
   __device__ __forceinline__ static void store(void* p, int64_t i, const float* x) {

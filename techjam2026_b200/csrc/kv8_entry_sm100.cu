@@ -208,7 +208,7 @@ static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
                        dim3(Cfg::THREADS), Cfg::SMEM, a.st, map, c, a.out, a.o_sb, a.o_sh, a.o_st,
                        a.dtype, a.o_vec, a.counts, a.T, a.G, a.max_len, a.flags, a.lse, w);
   if (e == cudaSuccess && w.chunks > 1)
-    e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(128), 0, a.st,
+    e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(KV8_JOIN_THREADS), 0, a.st,
                        c, a.out, a.o_sb, a.o_sh, a.o_st, a.dtype, a.T, a.G, a.lse, w);
   if (e == cudaSuccess && track && a.max_len > 0)
     e = launch_chained(kern_w, dim3(static_cast<unsigned>((a.max_len + 127) / 128), bh),
@@ -287,12 +287,14 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
   }
   if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention launch");
   if (w.chunks > 1) {
-    e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(128), 0, st,
+    e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(KV8_JOIN_THREADS), 0, st,
                        c, out, o_sb, o_sh, o_st, dtype, Ti, G, lse, w);
     if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention join launch");
   }
   if (max_len == 0 || !(flags & KF_KV8_TRACK)) return KF_OK;
-  e = launch_chained(kv8_weights_kernel, dim3(static_cast<unsigned>((max_len + 255) / 256), bh),
-                     dim3(256), 0, st, c, counts, Ti, G, cap, flags, w);
+  e = launch_chained(
+      kv8_weights_kernel,
+      dim3(static_cast<unsigned>((max_len + KV8_WEIGHTS_KEYS - 1) / KV8_WEIGHTS_KEYS), bh),
+      dim3(128), 0, st, c, counts, Ti, G, cap, flags, w);
   return cuda_status(e, "kf_kv8_attention weights launch");
 }
