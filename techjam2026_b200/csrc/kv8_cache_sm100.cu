@@ -168,29 +168,36 @@ __global__ void __launch_bounds__(KV8_THREADS)
   const int g0 = blockIdx.x * (KV8_THREADS * KV8_READ_UNROLL) + threadIdx.x;
   uint32_t kw[KV8_READ_UNROLL][W], vw[KV8_READ_UNROLL][W];
   float2 s[KV8_READ_UNROLL];
+  bool live[KV8_READ_UNROLL];
 #pragma unroll
   for (int i = 0; i < KV8_READ_UNROLL; ++i) {
     const int g = g0 + i * KV8_THREADS;
     const int64_t pos = static_cast<int64_t>(from) + (g >> row_shift);
+    const bool held = g < total && pos < end;
+    bool ok = false;
+    const int page = end > 0 ? kv8_page_or0(c, b, held ? static_cast<int>(pos >> c.p_shift) : 0, &ok)
+                             : 0;
+    if (held && !ok) record_device_status(KF_DEV_BAD_KV_PAGE);
+    const int64_t block = static_cast<int64_t>(page) * c.H + h;
+    const int64_t at = (((block << c.p_shift) + (pos & (c.P - 1))) << c.d_shift) +
+                       N * (g & ((1 << row_shift) - 1));
     s[i] = make_float2(0.f, 0.f);
+    if (end > 0) {
+      const float2 f = __ldg(reinterpret_cast<const float2*>(c.scale + 2 * block));
+      if (held && ok) s[i] = f;
+    }
+    live[i] = held && ok;
 #pragma unroll
     for (int u = 0; u < W; ++u) kw[i][u] = vw[i][u] = 0u;
-    if (g < total && pos < end) {
-      const int page = kv8_page(c, b, static_cast<int>(pos >> c.p_shift));
-      if (page >= 0) {
-        const int64_t block = static_cast<int64_t>(page) * c.H + h;
-        const int64_t at = (((block << c.p_shift) + (pos & (c.P - 1))) << c.d_shift) +
-                           N * (g & ((1 << row_shift) - 1));
-        s[i] = __ldg(reinterpret_cast<const float2*>(c.scale + 2 * block));
-        if constexpr (W == 2) {
-          const uint2 a = __ldg(reinterpret_cast<const uint2*>(c.k + at));
-          const uint2 d = __ldg(reinterpret_cast<const uint2*>(c.v + at));
-          kw[i][0] = a.x; kw[i][W - 1] = a.y;
-          vw[i][0] = d.x; vw[i][W - 1] = d.y;
-        } else {
-          kw[i][0] = __ldg(reinterpret_cast<const uint32_t*>(c.k + at));
-          vw[i][0] = __ldg(reinterpret_cast<const uint32_t*>(c.v + at));
-        }
+    if (live[i]) {
+      if constexpr (W == 2) {
+        const uint2 a = __ldg(reinterpret_cast<const uint2*>(c.k + at));
+        const uint2 d = __ldg(reinterpret_cast<const uint2*>(c.v + at));
+        kw[i][0] = a.x; kw[i][W - 1] = a.y;
+        vw[i][0] = d.x; vw[i][W - 1] = d.y;
+      } else {
+        kw[i][0] = __ldg(reinterpret_cast<const uint32_t*>(c.k + at));
+        vw[i][0] = __ldg(reinterpret_cast<const uint32_t*>(c.v + at));
       }
     }
   }
@@ -266,17 +273,18 @@ __global__ void __launch_bounds__(KV8_SELECT_THREADS)
   for (int i = tid; i < recent; i += KV8_SELECT_THREADS) out[need + i] = cand + i;
   if (need == 0) return;
   auto load_key = [&](int pos) -> uint32_t {
-    const int page = kv8_page(c, b, pos >> c.p_shift);
-    if (page < 0) return 0u;
-    return weight_key(
-        c.weight[(static_cast<int64_t>(page) * c.H + h) * c.P + (pos & (c.P - 1))]);
+    bool ok;
+    const int page = kv8_page_or0(c, b, pos >> c.p_shift, &ok);
+    const float x = c.weight[(static_cast<int64_t>(page) * c.H + h) * c.P + (pos & (c.P - 1))];
+    if (!ok) record_device_status(KF_DEV_BAD_KV_PAGE);
+    return ok ? weight_key(x) : 0u;
   };
   for (int base = tid; base < cand && base < KV8_SELECT_KEYS; base += 8 * KV8_SELECT_THREADS) {
     uint32_t key[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int pos = base + i * KV8_SELECT_THREADS;
-      key[i] = pos < cand && pos < KV8_SELECT_KEYS ? load_key(pos) : 0u;
+      key[i] = load_key(pos < cand ? pos : 0);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -397,7 +405,7 @@ __device__ __forceinline__ void kv8_recode16(uint8_t* p, const uint4& v, float s
 // the same along it, so the largest value of a piece is its largest code
 // times that (rounding keeps the order): the codes are decoded once.
 template <int FMT, int NG>
-__global__ void __launch_bounds__(KV8_THREADS)
+__global__ void __launch_bounds__(KV8_THREADS, NG <= 2 ? 5 : 3)
     kv8_move_kernel(KV8 c, const int32_t* __restrict__ table_out, int64_t ld_out, int budget,
                     const int32_t* __restrict__ kept) {
   __shared__ uint2 red[KV8_THREADS / 32];

@@ -75,6 +75,14 @@ __device__ __forceinline__ int kv8_page(const KV8& c, int b, int j) {
   return kv8_page(c, c.table, c.ld_table, b, j);
 }
 
+// The same without a branch before the caller's next load, for several lookups
+// in flight: page 0 stands in for no page, and *ok tells.
+__device__ __forceinline__ int kv8_page_or0(const KV8& c, int b, int j, bool* ok) {
+  const int p = __ldg(c.table + b * c.ld_table + j);
+  *ok = p >= 0 && p < c.pages;
+  return *ok ? p : 0;
+}
+
 // ---------------------------------------------------------------- types
 
 __device__ __forceinline__ float kv8_load1(const void* p, int64_t i, int dtype) {

@@ -102,6 +102,27 @@ class KV8Cache:
         self.device = k.device
         self._work = {}              # workspace bytes by (type, T, heads, max_len, flags)
 
+    def with_table(self, table: torch.Tensor, lens: torch.Tensor) -> "KV8Cache":
+        """The same pool under another table [B, blocks] and other lengths [B]."""
+        new = object.__new__(KV8Cache)
+        for name in ("k", "v", "scale", "weight", "kv_heads", "block", "head_dim", "device"):
+            setattr(new, name, getattr(self, name))
+        if table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device \
+                or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError(f"KV8Cache: table must be an int32 tensor [B, blocks] on {self.device} "
+                             "with unit stride along its blocks")
+        if lens.dtype != torch.int32 or tuple(lens.shape) != (table.shape[0],) \
+                or lens.device != self.device or not lens.is_contiguous():
+            raise ValueError(f"KV8Cache: lens must be a contiguous int32 tensor "
+                             f"[{table.shape[0]}] on {self.device}")
+        new.table, new.lens, new.batch, new._work = table, lens, table.shape[0], {}
+        new.struct = _lib.KV8CacheStruct.from_buffer_copy(self.struct)
+        new.struct.table, new.struct.lens = table.data_ptr(), lens.data_ptr()
+        new.struct.ld_table = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+        new.struct.blocks, new.struct.batch = table.shape[1], table.shape[0]
+        new._ref = ctypes.byref(new.struct)
+        return new
+
     @classmethod
     def empty(cls, pages: int, kv_heads: int, block: int, head_dim: int, table: torch.Tensor,
               lens: torch.Tensor, dtype: torch.dtype = torch.int8, weight: bool = False):
@@ -280,8 +301,7 @@ def kv8_evict(cache: KV8Cache, table_out: torch.Tensor, budget: int, recent: int
         raise ValueError(f"{what}: the cache keeps no weight record")
     if budget <= 0 or not 0 <= recent <= budget:
         raise ValueError(f"{what}: needs budget > 0 and 0 <= recent <= budget")
-    new = KV8Cache(cache.k, cache.v, cache.scale, table_out, torch.empty_like(cache.lens),
-                   cache.weight)
+    new = cache.with_table(table_out, torch.empty_like(cache.lens))
     if new.batch != cache.batch or table_out.shape[1] * cache.block < budget:
         raise ValueError(f"{what}: table_out must be [{cache.batch}, at least "
                          f"{-(-budget // cache.block)}]")
