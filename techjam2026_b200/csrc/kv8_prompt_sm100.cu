@@ -208,21 +208,6 @@ __device__ __forceinline__ void kv8_expand(const uint8_t* raw, uint8_t* tile, in
   }
 }
 
-// Named barrier over `count` threads that tells all of them whether any came
-// with `flag` set.
-__device__ __forceinline__ bool named_bar_or(int id, int count, bool flag) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %3, 0;\n\t"
-      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(count), "r"(static_cast<uint32_t>(flag))
-      : "memory");
-  return r != 0;
-}
-
 // Untiled copy global -> shared, completion counted on an mbarrier; 16-byte
 // aligned addresses and size.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
@@ -253,7 +238,7 @@ struct PromptCfg {
   static constexpr int RAWK_OFF = V_OFF + ST * KV_BYTES;
   static constexpr int RAWV_OFF = RAWK_OFF + RS * RAW;
   static constexpr int BAR_OFF = RAWV_OFF + RS * RAW;
-  static constexpr int SC_OFF = BAR_OFF + 256;             // page scales of each step
+  static constexpr int SC_OFF = BAR_OFF + 320;             // page scales of each step
   // Four slots, each read by step j's softmax and rewritten for step j + 4: by
   // then every softmax warp has begun step j + 2.
   static constexpr int SLOTS = 4;
@@ -370,7 +355,9 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   uint64_t* rk_full = bars + 18;  // [RS] raw codes of K, of V: their bytes
   uint64_t* rv_full = bars + 20;  // [RS]
   uint64_t* s_free = bars + 22;   // [2] S read into registers (P apart), 4 warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  uint64_t* rk_empty = bars + 24; // [RS] raw codes expanded by the three warps
+  uint64_t* rv_empty = bars + 26; // [RS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_vmax = reinterpret_cast<float*>(tmem_slot + 2);  // [12]
   PromptScales* s_sc = reinterpret_cast<PromptScales*>(smem + Cfg::SC_OFF);
@@ -420,8 +407,10 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   if (tid == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&v_full[s], 1);
+      mbar_init(&k_full[s], 3);
+      mbar_init(&v_full[s], 3);
+      mbar_init(&rk_empty[s], 3);
+      mbar_init(&rv_empty[s], 3);
       mbar_init(&rk_full[s], 1);
       mbar_init(&rv_full[s], 1);
       mbar_init(&k_empty[s], 1 + 4 * NT);
@@ -602,28 +591,30 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
     }
   } else if (warp > 8) {
     // -------------------------------------------------- loaders (3 warps)
+    // The three expand a third of every tile each, without waiting for one
+    // another. Warp 9 also copies the raw K tiles, warp 10 the raw V tiles, and
+    // warp 11 stages the scales, each half a step after the slot was read.
     const int lt = tid - 9 * 32;
-    const float inv_vmax = vmax > 0.f ? 1.f / vmax : 0.f;
     uint8_t* rawk = smem + Cfg::RAWK_OFF;
     uint8_t* rawv = smem + Cfg::RAWV_OFF;
     const int segs = BN >> c.p_shift;              // pages of a tile (1 to 8)
     const uint32_t seg_bytes = static_cast<uint32_t>(c.P) * DH;
-    // Lane g < 8 of warp 9 keeps the pages of group g (16 keys) of the steps
-    // ahead: the table entry of step j + RS + 1 is loaded while step j runs, so
-    // no copy waits for it. pg[i]: step j + i, -1 where there is no key or the
-    // entry is no page (recorded).
+    // Lane g < 8 keeps the pages of group g (16 keys) of the steps ahead: the
+    // table entry of step j + RS + 1 is loaded while step j runs, so no copy
+    // waits for it. pg[i]: step j + i; -2 no key, -1 the entry is no page.
     int pg[Cfg::RS + 1];
-    int entry = -1;
+    int entry = -2;
     auto load_entry = [&](int j) {
       const int key = k0 + j * BN + lane * 16;
       entry = -2;
-      if (lane < Cfg::GROUPS && key < k1) entry = __ldg(c.table + b * c.ld_table + (key >> c.p_shift));
+      if (lane < Cfg::GROUPS && key < k1)
+        entry = __ldg(c.table + b * c.ld_table + (key >> c.p_shift));
     };
     auto take_entry = [&]() -> int {
-      if (entry == -2) return -2;                       // no key
+      if (entry == -2) return -2;
       if (entry >= 0 && entry < c.pages) return entry;
       record_device_status(KF_DEV_BAD_KV_PAGE);
-      return -1;                                        // a refused page
+      return -1;
     };
     // Copies the codes of the pages in lanes 0-7 into a raw slot. A page is
     // copied whole: its slots past the end exist, whatever they hold.
@@ -637,6 +628,37 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         bulk_load(raw + lane * seg_bytes, pool + (static_cast<int64_t>(page) * c.H + h) * seg_bytes,
                   seg_bytes, full);
     };
+#pragma unroll
+    for (int i = 0; i <= Cfg::RS; ++i) {
+      load_entry(i);
+      pg[i] = take_entry();
+    }
+    load_entry(Cfg::RS + 1);
+    int fetched = 0;                               // raw tiles asked for by this warp
+    if (warp < 11) {
+#pragma unroll
+      for (int i = 0; i < Cfg::RS; ++i)
+        if (i < n_steps) {
+          if (warp == 9)
+            fetch(c.k, rawk + i * Cfg::RAW, &rk_full[i], pg[i]);
+          else
+            fetch(c.v, rawv + i * Cfg::RAW, &rv_full[i], pg[i]);
+          ++fetched;
+        }
+    }
+    // The raw slot of step j is asked to hold step j + RS, once all three warps
+    // have expanded step j.
+    auto refill = [&](const uint8_t* pool, uint8_t* raw, uint64_t* full, uint64_t* empty, int j,
+                      int page8) -> bool {
+      if (fetched >= n_steps) return true;
+      const int slot = j % Cfg::RS;
+      if (!mbar_wait(&empty[slot], (j / Cfg::RS) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA))
+        return false;
+      fetch(pool, raw + slot * Cfg::RAW, &full[slot], page8);
+      ++fetched;
+      return true;
+    };
+    // scales of lane g's group: of the current step, loaded one step before
     float2 scale = make_float2(0.f, 0.f);
     auto load_scale = [&](int page8) {
       scale = make_float2(0.f, 0.f);
@@ -644,45 +666,24 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         scale = __ldg(reinterpret_cast<const float2*>(
             c.scale + 2 * (static_cast<int64_t>(page8) * c.H + h)));
     };
-    int fetched_k = 0, fetched_v = 0;
-    if (warp == 9) {
-#pragma unroll
-      for (int i = 0; i <= Cfg::RS; ++i) {
-        load_entry(i);
-        pg[i] = take_entry();
-      }
-      load_entry(Cfg::RS + 1);
-      load_scale(pg[0]);
-#pragma unroll
-      for (int i = 0; i < Cfg::RS; ++i)
-        if (i < n_steps) {
-          fetch(c.k, rawk + i * Cfg::RAW, &rk_full[i], pg[i]);
-          ++fetched_k;
-        }
-#pragma unroll
-      for (int i = 0; i < Cfg::RS; ++i)
-        if (i < n_steps) {
-          fetch(c.v, rawv + i * Cfg::RAW, &rv_full[i], pg[i]);
-          ++fetched_v;
-        }
-    }
+    if (warp == 11) load_scale(pg[0]);
+    const float inv_vmax = vmax > 0.f ? 1.f / vmax : 0.f;
     for (int j = 0; j < n_steps; ++j) {
       const int st = j & 1, slot = j % Cfg::RS;
       const uint32_t eph = ((j >> 1) & 1) ^ 1;  // phase of the release two steps back
       const uint32_t rph = (j / Cfg::RS) & 1;
-      bool ok = mbar_wait(&rk_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) &&
-                (j < 2 || mbar_wait(&k_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA));
-      if (ok) {
-        if (c.fmt == KF_KV8_INT8)
-          kv8_expand<DH, KF_KV8_INT8, false>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
-        else
-          kv8_expand<DH, KF_KV8_E4M3, false>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
-        fence_proxy_async_smem();
-      }
-      PromptScales& sc = s_sc[j & 3];
-      if (warp == 9 && ok) {
+      const uint32_t bad = __ballot_sync(0xffffffffu, lane < Cfg::GROUPS && pg[0] == -1);
+      if (!mbar_wait(&rk_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) ||
+          (j >= 2 && !mbar_wait(&k_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)))
+        break;
+      if (c.fmt == KF_KV8_INT8)
+        kv8_expand<DH, KF_KV8_INT8, false>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
+      else
+        kv8_expand<DH, KF_KV8_E4M3, false>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
+      fence_proxy_async_smem();
+      if (warp == 11) {
+        PromptScales& sc = s_sc[j & 3];
         const float sc_k = scale.x, sc_r = scale.y * inv_vmax;
-        const uint32_t bad = __ballot_sync(0xffffffffu, lane < Cfg::GROUPS && pg[0] == -1);
         const uint32_t spoiled_k = __ballot_sync(0xffffffffu, sc_k != sc_k);
         const uint32_t spoiled_v = __ballot_sync(0xffffffffu, sc_r != sc_r);
         if (lane < Cfg::GROUPS) {
@@ -694,22 +695,25 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
           sc.spoiled_k = spoiled_k;
           sc.spoiled_v = spoiled_v;
         }
-      }
-      if (named_bar_or(1, 96, !ok)) break;  // all three warps leave together
-      if (lt == 0) mbar_arrive(&k_full[st]);
-      if (warp == 9) {
-        if (fetched_k < n_steps) {
-          fetch(c.k, rawk + slot * Cfg::RAW, &rk_full[slot], pg[Cfg::RS]);
-          ++fetched_k;
-        }
         load_scale(pg[1]);
       }
-      ok = mbar_wait(&rv_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) &&
-           (j < 2 || mbar_wait(&v_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA));
-      if (ok) {
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&k_full[st]);
+        mbar_arrive(&rk_empty[slot]);
+      }
+      // Refills, where the slot was read half a step ago if there are two, and
+      // at once if there is one (its copy then has the rest of the step).
+      if (Cfg::RS == 1 && warp == 9 && !refill(c.k, rawk, rk_full, rk_empty, j, pg[Cfg::RS])) break;
+      if (Cfg::RS == 2 && warp == 10 && j >= 1 &&
+          !refill(c.v, rawv, rv_full, rv_empty, j - 1, pg[Cfg::RS - 1]))
+        break;
+      if (!mbar_wait(&rv_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) ||
+          (j >= 2 && !mbar_wait(&v_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)))
+        break;
+      {
         // An e4m3 NaN in a slot past the end must not meet a weight of 0.
         const int rows = k1 - (k0 + j * BN);
-        const uint32_t bad = sc.bad;
         const bool whole = rows >= BN && bad == 0;
         const uint8_t* raw = rawv + slot * Cfg::RAW;
         uint8_t* tile = sV + st * Cfg::KV_BYTES;
@@ -726,25 +730,23 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         }
         fence_proxy_async_smem();
       }
-      if (named_bar_or(1, 96, !ok)) break;
-      if (lt == 0) mbar_arrive(&v_full[st]);
-      if (warp == 9) {
-        if (fetched_v < n_steps) {
-          fetch(c.v, rawv + slot * Cfg::RAW, &rv_full[slot], pg[Cfg::RS]);
-          ++fetched_v;
-        }
-#pragma unroll
-        for (int i = 0; i < Cfg::RS; ++i) pg[i] = pg[i + 1];
-        pg[Cfg::RS] = take_entry();
-        load_entry(j + Cfg::RS + 2);
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&v_full[st]);
+        mbar_arrive(&rv_empty[slot]);
       }
+      if (Cfg::RS == 2 && warp == 9 && !refill(c.k, rawk, rk_full, rk_empty, j, pg[Cfg::RS])) break;
+      if (Cfg::RS == 1 && warp == 10 && !refill(c.v, rawv, rv_full, rv_empty, j, pg[Cfg::RS])) break;
+#pragma unroll
+      for (int i = 0; i < Cfg::RS; ++i) pg[i] = pg[i + 1];
+      pg[Cfg::RS] = take_entry();
+      load_entry(j + Cfg::RS + 2);
     }
-    if (warp == 9 && lane == 0) {
+    if (warp < 11 && lane == 0) {
       // no copy may be in flight when the CTA leaves
-      for (int j = fetched_k > Cfg::RS ? fetched_k - Cfg::RS : 0; j < fetched_k; ++j)
-        mbar_wait_drain(&rk_full[j % Cfg::RS], (j / Cfg::RS) & 1, KF_DEV_WAIT_TIMEOUT_TMA);
-      for (int j = fetched_v > Cfg::RS ? fetched_v - Cfg::RS : 0; j < fetched_v; ++j)
-        mbar_wait_drain(&rv_full[j % Cfg::RS], (j / Cfg::RS) & 1, KF_DEV_WAIT_TIMEOUT_TMA);
+      uint64_t* full = warp == 9 ? rk_full : rv_full;
+      for (int j = fetched > Cfg::RS ? fetched - Cfg::RS : 0; j < fetched; ++j)
+        mbar_wait_drain(&full[j % Cfg::RS], (j / Cfg::RS) & 1, KF_DEV_WAIT_TIMEOUT_TMA);
     }
   } else if (warp < 4 * NT) {
     // -------------------------------------------------- softmax
