@@ -132,7 +132,7 @@ struct KV8Call {
   int64_t q_sb, q_sh, q_st;
   void* out;
   int64_t o_sb, o_sh, o_st;
-  int dtype, q_vec, o_vec;
+  int dtype, q_vec, q_vec16, o_vec;  // alignment: runs of 4 of q, 16 bytes of q and of out
   const int32_t* counts;
   int T, G, max_len;
   float scale_log2;
@@ -197,10 +197,13 @@ static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
     return cuda_status(e, "kf_kv8_attention: set smem attribute");
   });
   if (rc) return rc;
-  cudaError_t e = launch_chained(kv8_prep_q_kernel<DH, PL>,
-                                 dim3(static_cast<unsigned>((w.rows + 63) / 64), bh), dim3(256), 0,
-                                 a.st, c, a.q, a.q_sb, a.q_sh, a.q_st, a.dtype, a.q_vec, a.counts,
-                                 a.T, a.G, a.scale_log2, w);
+  auto prep = a.dtype == KF_DT_F32    ? kv8_prep_q_kernel<KF_DT_F32>
+              : a.dtype == KF_DT_BF16 ? kv8_prep_q_kernel<KF_DT_BF16>
+                                      : kv8_prep_q_kernel<KF_DT_F16>;
+  const int rows_of_cta = 256 * (PL == 2 ? 4 : 8) / DH * KV8_PREP_UNROLL;
+  cudaError_t e = launch_chained(
+      prep, dim3(static_cast<unsigned>((w.rows + rows_of_cta - 1) / rows_of_cta), bh), dim3(256), 0,
+      a.st, c, a.q, a.q_sb, a.q_sh, a.q_st, a.q_vec16, a.counts, a.T, a.G, a.scale_log2, w);
   if (e == cudaSuccess)
     e = launch_chained(kern,
                        dim3(static_cast<unsigned>((w.rows + Cfg::ROWS - 1) / Cfg::ROWS),
@@ -266,7 +269,8 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
   const unsigned bh = static_cast<unsigned>(c.B * c.H);
   const int64_t per = 16 / es;
   const int o_vec = kv8_aligned(out, 16) && o_sb % per == 0 && o_sh % per == 0 && o_st % per == 0;
-  const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, o_vec, counts, Ti, G,
+  const int vec16 = kv8_aligned(q, 16) && q_sb % per == 0 && q_sh % per == 0 && q_st % per == 0;
+  const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, vec16, o_vec, counts, Ti, G,
                      cap, scale_log2, flags, lse, st};
   if (w.prompt) {
     const bool two = dtype == KF_DT_F32;

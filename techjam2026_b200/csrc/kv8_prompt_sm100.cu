@@ -57,59 +57,65 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
 
 // ---------------------------------------------------------------- q planes
 
-// q rows as fp16 planes [PL][B*H][rows][D] and their factors to log2 units.
-// Four lanes a row. Rows past a sequence's count get zeros.
-template <int DH, int PL>
+// q rows as fp16 planes [PL][B*H][rows][D] and their factors to log2 units. A
+// thread holds 16 bytes of each of four rows, neighbours the rest of the row.
+// Rows past a sequence's count get zeros. Bound by memory.
+constexpr int KV8_PREP_UNROLL = 4;
+
+template <int DT>
 __global__ void __launch_bounds__(256)
     kv8_prep_q_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh, int64_t q_st,
-                      int dtype, int vec, const int32_t* __restrict__ counts, int T, int G,
-                      float scale_log2, KV8Work w) {
-  const int rows = w.rows;
-  uint16_t* planes = w.planes;
-  float* qf = w.qf;
+                      int vec, const int32_t* __restrict__ counts, int T, int G, float scale_log2,
+                      KV8Work w) {
+  constexpr int N = KV8Type<DT>::N;
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int E = DH / 4;
-  const int row = blockIdx.x * 64 + (threadIdx.x >> 2);
-  const int t = threadIdx.x & 3;
+  const int l_shift = c.d_shift - (N == 8 ? 3 : 2);   // lanes of a row, as a power of two
+  const int l = threadIdx.x & ((1 << l_shift) - 1);
+  const int rows_of_pass = 256 >> l_shift;
+  const int row0 = blockIdx.x * rows_of_pass * KV8_PREP_UNROLL + (threadIdx.x >> l_shift);
   const int bh = blockIdx.y;
   const int b = bh / c.H, h = bh - b * c.H;
-  const int tok = row / G;
-  const bool real = row < rows && tok < kv8_count(counts, b, T);
-  float x[E];
-  float amax = 0.f;
+  const int real_rows = min(w.rows, kv8_count(counts, b, T) * G);
+  const int64_t base = b * q_sb + static_cast<int64_t>(h) * G * q_sh;
+  uint4 x[KV8_PREP_UNROLL];
 #pragma unroll
-  for (int e = 0; e < E; e += 4) {
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
-    if (real)
-      kv8_load4(q, b * q_sb + static_cast<int64_t>(h * G + row - tok * G) * q_sh + tok * q_st +
-                       t * E + e, dtype, vec != 0, y);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      x[e + u] = y[u];
-      amax = __uint_as_float(max(__float_as_uint(amax), __float_as_uint(fabsf(y[u]))));
+  for (int i = 0; i < KV8_PREP_UNROLL; ++i) {
+    const int row = row0 + i * rows_of_pass;
+    x[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < real_rows) {
+      const int tok = row / G;
+      x[i] = KV8Type<DT>::load(q, base + (row - tok * G) * q_sh + tok * q_st + l * N, vec != 0);
     }
   }
+  const int64_t plane = static_cast<int64_t>(c.B) * c.H * w.rows * c.D;
 #pragma unroll
-  for (int d = 1; d <= 2; d <<= 1)
-    amax = __uint_as_float(
-        max(__float_as_uint(amax), __shfl_xor_sync(0xffffffffu, __float_as_uint(amax), d)));
-  if (row >= rows) return;
-  float inv;
-  const float sc = kv8_row_scale(amax, &inv);
-  const int64_t at = (static_cast<int64_t>(bh) * rows + row) * DH + t * E;
-  const int64_t plane = static_cast<int64_t>(c.B) * c.H * rows * DH;
+  for (int i = 0; i < KV8_PREP_UNROLL; ++i) {
+    const int row = row0 + i * rows_of_pass;
+    uint32_t m = 0;
+    KV8Type<DT>::collect(x[i], m);
+    m = KV8Type<DT>::bits(m);
+    for (int d = 1; d < 1 << l_shift; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if (row >= w.rows) continue;
+    float inv, y[N];
+    const float sc = kv8_row_scale(__uint_as_float(m), &inv);
+    KV8Type<DT>::values(x[i], y);
+    uint32_t hi[N / 2];
 #pragma unroll
-  for (int e = 0; e < E; e += 4) {
-    const uint32_t h0 = pack_half2(x[e] * sc, x[e + 1] * sc);
-    const uint32_t h1 = pack_half2(x[e + 2] * sc, x[e + 3] * sc);
-    *reinterpret_cast<uint2*>(planes + at + e) = make_uint2(h0, h1);
-    if constexpr (PL == 2)
-      *reinterpret_cast<uint2*>(planes + plane + at + e) =
-          make_uint2(pack_half2_rest(x[e] * sc, x[e + 1] * sc, h0),
-                     pack_half2_rest(x[e + 2] * sc, x[e + 3] * sc, h1));
+    for (int u = 0; u < N; ++u) y[u] *= sc;
+#pragma unroll
+    for (int u = 0; u < N / 2; ++u) hi[u] = pack_half2(y[2 * u], y[2 * u + 1]);
+    uint16_t* at = w.planes + (static_cast<int64_t>(bh) * w.rows + row) * c.D + l * N;
+    if constexpr (N == 8) {
+      *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[N / 2 - 1]);
+    } else {
+      *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(at + plane) = make_uint2(pack_half2_rest(y[0], y[1], hi[0]),
+                                                         pack_half2_rest(y[2], y[3], hi[1]));
+    }
+    if (l == 0)
+      w.qf[static_cast<int64_t>(bh) * w.rows + row] = row < real_rows ? inv * scale_log2 : 0.f;
   }
-  if (t == 0) qf[static_cast<int64_t>(bh) * rows + row] = real ? inv * scale_log2 : 0.f;
 }
 
 // ---------------------------------------------------------------- tiles
