@@ -276,22 +276,33 @@ __global__ void __launch_bounds__(KV8_SELECT_THREADS)
     bool ok;
     const int page = kv8_page_or0(c, b, pos >> c.p_shift, &ok);
     const float x = c.weight[(static_cast<int64_t>(page) * c.H + h) * c.P + (pos & (c.P - 1))];
-    if (!ok) record_device_status(KF_DEV_BAD_KV_PAGE);
     return ok ? weight_key(x) : 0u;
   };
-  for (int base = tid; base < cand && base < KV8_SELECT_KEYS; base += 8 * KV8_SELECT_THREADS) {
-    uint32_t key[8];
+  // Eight keys a thread at a time: all table entries, then all weights (a
+  // refused page is recorded after them, or its branch would order the loads).
+  bool bad = false;
+  for (int base = tid; base < cand; base += 8 * KV8_SELECT_THREADS) {
+    int page[8];
+    float x[8];
+    bool ok[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int pos = base + i * KV8_SELECT_THREADS;
-      key[i] = load_key(pos < cand ? pos : 0);
+      page[i] = kv8_page_or0(c, b, (pos < cand ? pos : 0) >> c.p_shift, &ok[i]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int pos = base + i * KV8_SELECT_THREADS;
-      if (pos < cand && pos < KV8_SELECT_KEYS) s_key[pos] = key[i];
+      x[i] = c.weight[(static_cast<int64_t>(page[i]) * c.H + h) * c.P + (pos & (c.P - 1))];
+      bad = bad || !ok[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int pos = base + i * KV8_SELECT_THREADS;
+      if (pos < cand && pos < KV8_SELECT_KEYS) s_key[pos] = ok[i] ? weight_key(x[i]) : 0u;
     }
   }
+  if (bad) record_device_status(KF_DEV_BAD_KV_PAGE);
   auto key_at = [&](int pos) -> uint32_t {
     return pos < KV8_SELECT_KEYS ? s_key[pos] : load_key(pos);
   };

@@ -215,6 +215,76 @@ def test_chunks(T, group, dim, kind, dtype, track, causal):
     attend(cache, q, counts, causal=causal, track=track)
 
 
+@pytest.mark.parametrize("track", [True, False])
+@pytest.mark.parametrize("kind,dtype", [(F32, F8), (BF16, I8)])
+@pytest.mark.parametrize("T,group,dim,block", [(100, 1, 16, 16), (45, 2, 32, 128), (50, 1, 32, 64),
+                                               (31, 2, 16, 32), (11, 12, 128, 64)])
+def test_chunks_of_other_widths(T, group, dim, block, kind, dtype, track):
+    """Both kernels (up to and above 64 query rows of a kv head) at the small
+    head widths, and pages as wide as a step."""
+    lens = [3, 0, 140]
+    cache, _, g = make(lens, heads=1, dim=dim, block=block, dtype=dtype, weight=True, room=T)
+    cache.weight.zero_()
+    x = torch.randn(3, 1, T, dim, generator=g).cuda()
+    ops.kv8_append(cache, x, x)
+    q = torch.randn(3, group, T, dim, generator=g).to(kind).cuda()
+    attend(cache, q, None, track=track)
+
+
+@pytest.mark.parametrize("dtype", [I8, F8])
+@pytest.mark.parametrize("kind,T", [(F32, 80), (BF16, 80), (BF16, 20), (F32, 7)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_a_spoiled_page_reaches_the_rows_that_see_it(which, kind, T, dtype):
+    """A page whose scale is NaN: rows that see a token of it are NaN, the
+    others are as if it were not there (it shares a step with good pages)."""
+    cache, _, g = make([40 + 80 - T], heads=1, dim=64, block=16, dtype=dtype, room=96)
+    x = torch.randn(1, 1, T, 64, generator=g).cuda()
+    y = x.clone()
+    y[0, 0, T - 5, 3] = math.inf                     # position 115: page 7 (112 to 127)
+    ops.kv8_append(cache, y if which == "k" else x, y if which == "v" else x)
+    q = torch.randn(1, 2, T, 64, generator=g).to(kind).cuda()
+    out = ops.kv8_attention(q, cache).cpu()
+    plain = Plain(cache)
+    plain.weight = None
+    ref, tol, *_ = plain.attention(q, [T], True, 0.125, EPS_Q[kind], EPS_P[kind], EPS_OUT[kind])
+    # the first of the rows from position 112 on sees the page
+    seen = torch.arange(T) + 120 - T >= 112
+    assert out[:, :, seen].isnan().all() and ref[:, :, seen].isnan().all()
+    good = ~seen
+    assert ((out.double() - ref).abs()[:, :, good] <= tol[:, :, good]).all()
+    clean()
+
+
+@pytest.mark.parametrize("T", [80, 20])
+def test_a_refused_page_hides_its_tokens_from_a_chunk(T):
+    """A table entry outside the pool in the middle of a step: the rows attend
+    to the other tokens; the same with the hidden keys' weights."""
+    cache, _, g = make([60], heads=1, dim=64, block=16, room=96, weight=True)
+    cache.weight.zero_()
+    x = torch.randn(1, 1, T, 64, generator=g).cuda()
+    ops.kv8_append(cache, x, x)
+    q = torch.randn(1, 1, T, 64, generator=g).cuda()
+    keep = int(cache.table[0, 2])
+    cache.table[0, 2] = 1 << 20
+    out = ops.kv8_attention(q, cache, track=True).cpu()
+    assert _lib.lib().kf_device_status(1) == 6
+    weight = cache.weight.cpu()
+    cache.table[0, 2] = keep
+    plain = Plain(cache)
+    k = plain.values(0, 0, 0, 60 + T).double()
+    v = plain.values(1, 0, 0, 60 + T).double()
+    s = (q.cpu().double()[0, 0] @ k.T) / 8
+    pos = torch.arange(60 + T)
+    hidden = (pos >= 32) & (pos < 48)
+    s.masked_fill_(hidden[None] | (pos[None] > 60 + torch.arange(T)[:, None]), -math.inf)
+    p = torch.softmax(s, -1)
+    assert ((out[0, 0].double() - p @ v).abs() <= 1e-4).all()
+    got = torch.cat([weight[int(cache.table[0, i]), 0] for i in range(-(-(60 + T) // 16))])
+    want = p.sum(0)
+    assert ((got[:60 + T].double() - want).abs()[~hidden] <= 1e-4).all()
+    assert not weight[keep].any()
+
+
 @pytest.mark.parametrize("lens", [[4000], [1, 5000, 300]])
 def test_long_caches_are_split_and_joined(lens):
     cache, _, g = make(lens, heads=1, dim=64, block=64, dtype=I8, weight=True)
@@ -442,6 +512,20 @@ def test_evict_long_rows():
             order = torch.sort(row[:n - 100], descending=True, stable=True).indices[:1900]
             want = torch.cat([order.sort().values, torch.arange(n - 100, n)])
             assert torch.equal(kept[b, h].cpu().long(), want)
+    clean()
+
+
+def test_evict_rows_beyond_what_shared_memory_holds():
+    """More candidates than the selection keeps as keys on the chip."""
+    n = 56000
+    cache, spare, g = make([n], heads=1, dim=16, block=128, weight=True, spare=40)
+    w = torch.randint(0, 40, cache.weight.shape, generator=g).float()
+    cache.weight.copy_(w)
+    kept, _ = ops.kv8_evict(cache, spare.view(1, 40), 5000, 7)
+    row = torch.cat([w[int(p), 0] for p in cache.table[0]])[:n]
+    order = torch.sort(row[:n - 7], descending=True, stable=True).indices[:4993]
+    want = torch.cat([order.sort().values, torch.arange(n - 7, n)])
+    assert torch.equal(kept[0, 0].cpu().long(), want)
     clean()
 
 
