@@ -10,8 +10,10 @@ namespace kf {
 // load), takes max|x| of each as the largest bit pattern (so an infinity or a
 // NaN wins), fixes the scales, rescales the page's earlier codes if a scale
 // grew, and writes the new codes. Bound by memory, one read and one write of
-// the chunk, and by the loads in flight: K and V in CTAs of their own, held
-// as fp32, were 127 us for 400 MB of bf16 prompts and 52 for ragged fp32.
+// the chunk, and by the loads in flight. Measured: 16 prompts of 4096 tokens, 8
+// heads of 128, bf16: 69 us for 403 MB, 5.8 TB/s (K and V in CTAs of their own, held
+// as fp32: 127); ragged fp32 chunks of 64 sequences, 12 heads of 64: 45 us for
+// 195 MB (52), where half of the grid finds no token.
 
 constexpr int KV8_THREADS = 256;
 
@@ -146,7 +148,8 @@ __global__ void __launch_bounds__(KV8_THREADS)
 // ---------------------------------------------------------------- read
 
 // One thread per N codes of K and of V (16 bytes of output each), four rows
-// apart in flight. Bound by memory, mostly by what it writes.
+// apart in flight. Bound by memory, mostly by what it writes. Measured: 805 MB
+// (16 x 8 heads, 8192 tokens of 128, bf16) in 124 us, 6.5 TB/s.
 constexpr int KV8_READ_UNROLL = 4;
 
 template <int DT>
@@ -233,8 +236,10 @@ __global__ void __launch_bounds__(KV8_THREADS)
 // radix search, eleven bits a pass, for the need-th largest weight among the
 // tokens that are not protected, then a pass in order that lists the kept
 // positions. The weights are read from memory once and kept as sortable keys
-// in shared memory as far as they fit. The second moves one destination block
-// per CTA.
+// in shared memory as far as they fit: a latency chain per row (three searches,
+// two passes over its keys). The second moves one destination block per CTA; its
+// rows are gathered, 64 to 128 bytes each. Measured, 16 x 8 heads of 24k tokens
+// cut to 8192 of 128: selection 36 us, move 127 us for 537 MB (4.2 TB/s).
 
 constexpr int KV8_SELECT_THREADS = 1024;
 constexpr int KV8_SELECT_KEYS = 48 * 1024;  // keys that shared memory holds

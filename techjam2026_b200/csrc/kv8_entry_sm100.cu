@@ -5,11 +5,12 @@
 namespace kf {
 
 // Which kernel serves a call of `rows` query rows per kv head. Measured (us,
-// split / tensor-memory kernel; 8 x 8 heads of 128 over 8k tokens bf16, 16 x 12
-// heads of 64 over 1k fp32): 32 rows 94 / 137 and 38 / 81, 64 rows 140 / 146 and
-// 56 / 83, 128 rows 260 / 158 and 101 / 85. With weights the split kernel keeps every score for
-// the last pass; where that takes too much memory, 17 rows and more go to the
-// other kernel, which computes the scores again.
+// split / tensor-memory kernel): 8 x 8 heads of 128 over 8k tokens, bf16: 48
+// rows 106 / 134, 64 rows 145 / 137, 96 rows 194 / 142; 16 x 12 heads of 64 over 1k, fp32: 64 rows
+// 47 / 78, 128 rows 83 / 78; 8 heads of 64 over 16k, bf16: 64 rows 32 / 46, 128
+// rows 49 / 49. With weights the split kernel keeps every score for the last
+// pass; where that takes too much memory, 17 rows and more go to the other
+// kernel, which computes the scores again.
 static bool kv8_is_prompt(const KV8& c, int64_t rows, int64_t max_len, int flags) {
   if (rows > KV8_SPLIT_ROWS) return true;
   const int64_t scores = static_cast<int64_t>(c.B) * c.H * rows * max_len * 4;
@@ -165,7 +166,10 @@ static cudaError_t kv8_split_rows(const KV8& c, const KV8Call& a, const KV8Work&
 }
 template <int DH>
 static cudaError_t kv8_split_any(const KV8& c, const KV8Call& a, const KV8Work& w, bool half) {
-  const bool two = a.dtype == KF_DT_F32;
+  // fp16 q has the precision to show P's rounding (1.4 times the error of the
+  // output's own), and with at most 8 rows a second plane of P is all but free
+  // (42.2 against 41.3 us for a 65k sequence); bf16 does not show it.
+  const bool two = a.dtype == KF_DT_F32 || (a.dtype == KF_DT_F16 && half);
   if (c.fmt == KF_KV8_INT8)
     return two ? kv8_split_rows<DH, KF_KV8_INT8, 2>(c, a, w, half)
                : kv8_split_rows<DH, KF_KV8_INT8, 1>(c, a, w, half);

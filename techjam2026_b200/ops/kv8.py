@@ -66,6 +66,7 @@ class KV8Cache:
 
     __slots__ = ("k", "v", "scale", "table", "lens", "weight", "struct", "batch", "kv_heads",
                  "head_dim", "block", "device", "_ref", "_work")
+    _TENSORS = frozenset(("k", "v", "scale", "table", "lens", "weight"))
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, scale: torch.Tensor, table: torch.Tensor,
                  lens: torch.Tensor, weight: Optional[torch.Tensor] = None):
@@ -101,6 +102,14 @@ class KV8Cache:
         self.batch, self.kv_heads, self.block, self.head_dim = table.shape[0], heads, block, head_dim
         self.device = k.device
         self._work = {}              # workspace bytes by (type, T, heads, max_len, flags)
+
+    def __setattr__(self, name, value):
+        # The C side holds the tensors' addresses: `cache.lens += n` updates in
+        # place, but another tensor would go unseen.
+        if name in KV8Cache._TENSORS and getattr(self, "_ref", None) is not None \
+                and value is not getattr(self, name):
+            raise AttributeError(f"KV8Cache: {name} is fixed; update the tensor in place")
+        object.__setattr__(self, name, value)
 
     def with_table(self, table: torch.Tensor, lens: torch.Tensor) -> "KV8Cache":
         """The same pool under another table [B, blocks] and other lengths [B]."""
@@ -269,6 +278,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, counts: Optional[torch.Tenso
         need = L.kf_kv8_attention_workspace_bytes(cache._ref, *key)
         if need < 0:
             raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
+        if len(cache._work) >= 256:      # a max_len of its own every step
+            cache._work.clear()
         cache._work[key] = need
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     rc = L.kf_kv8_attention(

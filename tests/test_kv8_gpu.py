@@ -583,4 +583,7 @@ def test_refusals():
         ops.KV8Cache(cache.k, cache.v, cache.scale, cache.table.long(), cache.lens)
     with pytest.raises(TypeError):
         ops.KV8Cache(cache.k, cache.v, cache.scale, cache.table, cache.lens.long())
+    with pytest.raises(AttributeError):
+        cache.lens = cache.lens + 1                      # the C side would not see it
+    cache.lens += 0
     clean()
