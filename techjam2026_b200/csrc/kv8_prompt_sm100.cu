@@ -65,6 +65,12 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// What the lanes' bounded waits say, for the whole warp: its lanes leave a loop
+// together or not at all, since the code after a wait is warp-wide. (The softmax
+// warps, which wait in step as one instruction stream on the same barrier, flag and
+// clock, go without the vote: it cost 10 % at head_dim 64.)
+__device__ __forceinline__ bool warp_all(bool ok) { return __all_sync(0xffffffffu, ok); }
+
 // ---------------------------------------------------------------- q planes
 
 // q rows as fp16 planes [PL][B*H][rows][D] and their factors to log2 units. A
@@ -668,7 +674,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
                       int page8) -> bool {
       if (fetched >= n_steps) return true;
       const int slot = j % Cfg::RS;
-      if (!mbar_wait(&empty[slot], (j / Cfg::RS) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA))
+      if (!warp_all(
+              mbar_wait(&empty[slot], (j / Cfg::RS) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)))
         return false;
       fetch(pool, raw + slot * Cfg::RAW, &full[slot], page8);
       ++fetched;
@@ -689,8 +696,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       const uint32_t eph = ((j >> 1) & 1) ^ 1;  // phase of the release two steps back
       const uint32_t rph = (j / Cfg::RS) & 1;
       const uint32_t bad = __ballot_sync(0xffffffffu, lane < Cfg::GROUPS && pg[0] == -1);
-      if (!mbar_wait(&rk_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) ||
-          (j >= 2 && !mbar_wait(&k_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)))
+      if (!warp_all(mbar_wait(&rk_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) &&
+                    (j < 2 || mbar_wait(&k_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA))))
         break;
       if (c.fmt == KF_KV8_INT8)
         kv8_expand<DH, KF_KV8_INT8, false>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
@@ -724,8 +731,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       if (Cfg::RS == 2 && warp == 10 && j >= 1 &&
           !refill(c.v, rawv, rv_full, rv_empty, j - 1, pg[Cfg::RS - 1]))
         break;
-      if (!mbar_wait(&rv_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) ||
-          (j >= 2 && !mbar_wait(&v_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)))
+      if (!warp_all(mbar_wait(&rv_full[slot], rph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) &&
+                    (j < 2 || mbar_wait(&v_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA))))
         break;
       {
         // An e4m3 NaN in a slot past the end must not meet a weight of 0.
@@ -910,7 +917,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[buf]);
     }
-    if (ok && mbar_wait(&o_final[t], 0, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX)) {
+    if (ok && warp_all(mbar_wait(&o_final[t], 0, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX))) {
       tc_fence_after();
       const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
       const int hq = h * G + row - tok * G;
@@ -1074,8 +1081,8 @@ __global__ void __launch_bounds__(WeighCfg<DH, PL>::THREADS)
     for (int j = 0; j < n_steps; ++j) {
       const int st = j & 1;
       const uint32_t eph = ((j >> 1) & 1) ^ 1;
-      if (j >= 2 && (!mbar_wait(&q_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) ||
-                     !mbar_wait(&s_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)))
+      if (j >= 2 && !warp_all(mbar_wait(&q_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA) &&
+                              mbar_wait(&s_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA)))
         break;
       const int row0 = (r_begin + j) * BR;
       if (lane == 0) {
@@ -1147,8 +1154,8 @@ __global__ void __launch_bounds__(WeighCfg<DH, PL>::THREADS)
     float sum = 0.f;
     for (int j = half; j < n_steps; j += 2) {
       const uint32_t ph = (j >> 1) & 1;
-      if (!mbar_wait(&r_full[half], ph, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX) ||
-          !mbar_wait(&s_full[half], ph, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX))
+      if (!warp_all(mbar_wait(&r_full[half], ph, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX) &&
+                    mbar_wait(&s_full[half], ph, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX)))
         break;
       tc_fence_after();
       const float* fr = s_row + half * 2 * BR;

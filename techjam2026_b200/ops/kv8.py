@@ -153,14 +153,14 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
 
 def _check_call(what: str, cache: KV8Cache, counts: Optional[torch.Tensor], *tensors) -> int:
     """Checks that a call's tensors are where the cache is; its stream."""
-    device = cache.device
+    index = cache.device.index
     for t in tensors:
-        if t.device != device:
-            raise ValueError(f"{what}: tensors must be on the cache's device {device}, "
+        if t.get_device() != index:
+            raise ValueError(f"{what}: tensors must be on the cache's device {cache.device}, "
                              f"got {t.device}")
-    index = device.index
     if index != torch.cuda.current_device():
-        raise RuntimeError(f"{what}: the cache is on {device}, which is not the current device")
+        raise RuntimeError(f"{what}: the cache is on {cache.device}, which is not the current "
+                           "device")
     if counts is not None:
         _check_index(what, "counts", counts, cache)
     return torch._C._cuda_getCurrentRawStream(index)
@@ -168,7 +168,7 @@ def _check_call(what: str, cache: KV8Cache, counts: Optional[torch.Tensor], *ten
 
 def _check_index(what: str, name: str, t: torch.Tensor, cache: KV8Cache) -> None:
     if t.dtype is not torch.int32 or t.shape != cache.lens.shape or not t.is_contiguous() \
-            or t.device != cache.device:
+            or t.get_device() != cache.device.index:
         raise ValueError(f"{what}: {name} must be a contiguous int32 tensor [{cache.batch}] on "
                          f"{cache.device}")
 
