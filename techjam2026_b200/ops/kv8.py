@@ -113,23 +113,29 @@ class KV8Cache:
 
     def with_table(self, table: torch.Tensor, lens: torch.Tensor) -> "KV8Cache":
         """The same pool under another table [B, blocks] and other lengths [B]."""
-        new = object.__new__(KV8Cache)
-        for name in ("k", "v", "scale", "weight", "kv_heads", "block", "head_dim", "device"):
-            setattr(new, name, getattr(self, name))
         if table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device \
                 or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError(f"KV8Cache: table must be an int32 tensor [B, blocks] on {self.device} "
                              "with unit stride along its blocks")
-        if lens.dtype != torch.int32 or tuple(lens.shape) != (table.shape[0],) \
+        batch, blocks = table.shape
+        if lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) \
                 or lens.device != self.device or not lens.is_contiguous():
-            raise ValueError(f"KV8Cache: lens must be a contiguous int32 tensor "
-                             f"[{table.shape[0]}] on {self.device}")
-        new.table, new.lens, new.batch, new._work = table, lens, table.shape[0], {}
-        new.struct = _lib.KV8CacheStruct.from_buffer_copy(self.struct)
-        new.struct.table, new.struct.lens = table.data_ptr(), lens.data_ptr()
-        new.struct.ld_table = table.stride(0) if table.shape[0] > 1 else table.shape[1]
-        new.struct.blocks, new.struct.batch = table.shape[1], table.shape[0]
-        new._ref = ctypes.byref(new.struct)
+            raise ValueError(f"KV8Cache: lens must be a contiguous int32 tensor [{batch}] on "
+                             f"{self.device}")
+        struct = _lib.KV8CacheStruct.from_buffer_copy(self.struct)
+        struct.table, struct.lens = table.data_ptr(), lens.data_ptr()
+        struct.ld_table = table.stride(0) if batch > 1 else blocks
+        struct.blocks, struct.batch = blocks, batch
+        new = object.__new__(KV8Cache)
+        put = object.__setattr__
+        for name in ("k", "v", "scale", "weight", "kv_heads", "block", "head_dim", "device"):
+            put(new, name, getattr(self, name))
+        put(new, "table", table)
+        put(new, "lens", lens)
+        put(new, "batch", batch)
+        put(new, "_work", {})
+        put(new, "struct", struct)
+        put(new, "_ref", ctypes.byref(struct))
         return new
 
     @classmethod
