@@ -402,7 +402,9 @@ int kf_kv8_read(const kf_kv8_cache* cache, const int32_t* start, const int32_t* 
  * head h reads kv head h / (q_heads / kv_heads).
  *     out = softmax(sm_scale * q K^T) V,  lse = log of the softmax's sum
  * Scores, sums, maxima and the accumulators are fp32. q and the weights enter
- * the products as fp16 for 16-bit q, as two fp16 planes (22 bits) for fp32.
+ * the products as fp16 for 16-bit q (the weights as two planes for fp16 q with
+ * at most 8 query rows a kv head), as two fp16 planes (22 bits) for fp32.
+ * sm_scale must be finite and not negative.
  * out has q's type; rows without a visible key, and rows i >= counts[b], are 0
  * (lse -inf). lse (may be null) is fp32 [batch, q_heads, T]. With KF_KV8_TRACK
  * cache->weight[key] += the key's weight summed over the queries and the query
@@ -425,7 +427,7 @@ int64_t kf_kv8_attention_workspace_bytes(const kf_kv8_cache* cache, int dtype, i
  * are requantised by blocks (s' = max|code * s| * fl(1/Qmax)) into the pages
  * of table_out [batch, ld_out] (ceil(budget / block) columns; pages of the
  * same pool that no sequence of `cache` uses), their weights moved along;
- * lens_out[b] = n. kept (may not be null) is int32 [batch, kv_heads, budget]:
+ * lens_out[b] = n (lens_out is not cache->lens). kept (may not be null) is int32 [batch, kv_heads, budget]:
  * the kept positions in order, then -1. 0 <= recent <= budget, budget > 0. */
 int kf_kv8_evict(const kf_kv8_cache* cache, const int32_t* table_out, int64_t ld_out,
                  int64_t budget, int64_t recent, int32_t* kept, int32_t* lens_out, void* stream);

@@ -250,7 +250,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, counts: Optional[torch.Tenso
     counts    int32 [B], how many of the T queries are real (default all); the
               sequence's keys are the positions below lens[b] + counts[b]
     causal    query i sees positions up to its own; otherwise all keys
-    sm_scale  default head_dim ** -0.5
+    sm_scale  default head_dim ** -0.5; finite, not negative
     track     add to cache.weight each key's weight, summed over the queries
               and over the heads that read it
     max_len   an upper bound of lens + counts known to the caller (0: what the

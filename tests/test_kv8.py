@@ -29,8 +29,9 @@ def append(lib, c, k=FAKE, dtype=0, T=1):
     return lib.kf_kv8_append(c, k, 1, 1, 1, FAKE, 1, 1, 1, dtype, None, T, None)
 
 
-def attention(lib, c, q=FAKE, dtype=0, T=1, heads=2, flags=0, work=None, size=0, max_len=0):
-    return lib.kf_kv8_attention(c, q, 1, 1, 1, FAKE, 1, 1, 1, dtype, None, T, heads, max_len, 1.0,
+def attention(lib, c, q=FAKE, dtype=0, T=1, heads=2, flags=0, work=None, size=0, max_len=0,
+              scale=1.0):
+    return lib.kf_kv8_attention(c, q, 1, 1, 1, FAKE, 1, 1, 1, dtype, None, T, heads, max_len, scale,
                                 flags, None, work, size, None)
 
 
@@ -65,6 +66,9 @@ def test_bad_arguments_are_refused(lib):
     assert attention(lib, cache(), heads=0) == bad
     assert attention(lib, cache(), flags=4) == bad
     assert attention(lib, cache(), max_len=-1) == bad
+    for scale in (-0.125, float("nan"), float("inf")):
+        assert attention(lib, cache(), scale=scale) == bad
+        assert b"sm_scale" in lib.kf_last_error()
     assert attention(lib, cache(weight=None), flags=_lib.KF_KV8_TRACK) == bad
     assert attention(lib, cache(), flags=_lib.KF_KV8_TRACK) == bad        # no workspace
     assert b"workspace" in lib.kf_last_error()
