@@ -474,12 +474,14 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
         if constexpr (PL == 2)
           (RH == 1 ? hi[2 * n + 1] : lo[2 * n + r]) = pack_half2_rest(p[0], p[1], hi[2 * n + r]);
       }
-    // Slots past the end hold whatever was there (an e4m3 NaN among it): as
-    // zeros they cannot reach the product.
-    if (key + 16 > end) {
+    // Slots past the end, and page 0 where it stands in for a refused page, hold
+    // whatever was there (an e4m3 NaN among it): as zeros they cannot reach the
+    // product.
+    const int stop = min(end, bad);
+    if (key + 16 > stop) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (key + (i >> 1) * 8 + 2 * t + (i & 1) >= end) {
+        if (key + (i >> 1) * 8 + 2 * t + (i & 1) >= stop) {
 #pragma unroll
           for (int u = 0; u < VBytes<DH>::W; ++u) vb.w[i][u] = 0u;
         }

@@ -285,6 +285,37 @@ def test_a_refused_page_hides_its_tokens_from_a_chunk(T):
     assert not weight[keep].any()
 
 
+@pytest.mark.parametrize("dtype", [I8, F8])
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("T,group", [(1, 1), (1, 12), (20, 1), (31, 2), (80, 1)])
+def test_a_refused_page_is_as_if_its_tokens_were_not_there(T, group, kind, dtype):
+    """The same when every page that is not in the table holds codes and scales
+    that are no numbers (0x7F and 0xFF are e4m3 NaN): nothing of them may enter.
+    Without the block of the refused page, queries and keys stand 16 earlier."""
+    blocks = -(-(60 + T) // 16)
+    table = torch.arange(2, 2 + 2 * blocks, dtype=torch.int32, device="cuda").view(2, blocks)
+    lens = torch.tensor([60, 52], dtype=torch.int32, device="cuda")
+    cache = ops.KV8Cache.empty(2 * blocks + 4, 2, 16, 64, table, torch.zeros_like(lens), dtype)
+    cache.k.view(torch.uint8).fill_(0xFF)
+    cache.v.view(torch.uint8).fill_(0x7F)
+    cache.scale.fill_(math.nan)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(2, 2, 2, 60 + T, 64, generator=g).cuda()
+    ops.kv8_append(cache, x[0], x[1], counts=lens + T)
+    cache.lens.copy_(lens)
+    q = torch.randn(2, 2 * group, T, 64, generator=g).to(kind).cuda()
+    plain = Plain(cache)
+    plain.weight = None
+    plain.table = torch.cat([plain.table[:, :2], plain.table[:, 3:]], 1)
+    plain.lens = plain.lens - 16
+    ref, tol, *_ = plain.attention(q, [T, T], True, 0.125, EPS_Q[kind], EPS_P[kind], EPS_OUT[kind])
+    for wrong in (-1, 2 * blocks + 4, 1 << 30):
+        cache.table[:, 2] = wrong
+        out = ops.kv8_attention(q, cache).cpu().double()
+        assert _lib.lib().kf_device_status(1) == 6
+        assert ((out - ref).abs() <= tol).all(), (out - ref).abs().max()
+
+
 @pytest.mark.parametrize("lens", [[4000], [1, 5000, 300]])
 def test_long_caches_are_split_and_joined(lens):
     cache, _, g = make(lens, heads=1, dim=64, block=64, dtype=I8, weight=True)
