@@ -355,7 +355,8 @@ int kf_flash_fwd_tf32_keep_noalloc(const float* q, int64_t q_sb, int64_t q_sh, i
  * reference recomputes the whole sequence, kernelforge/optimized.py:397-458).
  * head_dim 16, 32, 64 or 128; block 16, 32, 64 or 128. All pointers are
  * device pointers owned by the caller. A sequence's pages must not be shared
- * with a sequence that is appended to. */
+ * with a sequence that is appended to. A sequence of a negative length holds no
+ * token and takes none. */
 typedef struct kf_kv8_cache {
   void* k;
   void* v;

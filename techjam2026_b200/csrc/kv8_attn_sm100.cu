@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
   const int bh = blockIdx.z;
   const int b = bh / c.H, h = bh - b * c.H;
   const int len = kv8_len(c, b);
-  const int count = kv8_count(counts, b, T);
+  const int count = kv8_count(c, counts, b, T);
   int end = kv8_end(c, len, count);
   if (end > max_len) {
     if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(128)
   const int bh = blockIdx.y;
   const int b = bh / c.H, h = bh - b * c.H;
   const int len = kv8_len(c, b);
-  const int count = kv8_count(counts, b, T);
+  const int count = kv8_count(c, counts, b, T);
   const int end = min(kv8_end(c, len, count), max_len);
   if (static_cast<int>(blockIdx.x) * KV8_WEIGHTS_KEYS >= end) return;
   if (threadIdx.x < w.rows)

@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(KV8_THREADS)
   const int h = blockIdx.y;
   const int b = blockIdx.z;
   const int len = kv8_len(c, b);
-  const int end = kv8_end(c, len, kv8_count(counts, b, T));
+  const int end = kv8_end(c, len, kv8_count(c, counts, b, T));
   const int j = (len >> c.p_shift) + static_cast<int>(blockIdx.x);
   const int p0 = j << c.p_shift;                    // the page's first position
   const int lo = p0 > len ? p0 : len;               // its new tokens are [lo, hi)
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(KV8_THREADS)
   const int h = blockIdx.y;
   const int b = blockIdx.z;
   const int len = kv8_len(c, b);
-  const int end = counts ? kv8_end(c, len, max(__ldg(counts + b), 0)) : len;
+  const int end = counts ? kv8_end(c, len, kv8_count(c, counts, b, INT32_MAX)) : len;
   const int from = start ? max(__ldg(start + b), 0) : 0;
   const int64_t out0 = (static_cast<int64_t>(b) * c.H + h) * n * c.D;
   const int total = n << row_shift;

@@ -47,11 +47,13 @@ __device__ __forceinline__ int kv8_len(const KV8& c, int b) {
   }
   return n;
 }
-// End of the tokens of sequence b with its counted new ones (counts null: T).
-__device__ __forceinline__ int kv8_count(const int32_t* counts, int b, int T) {
+// Tokens that a call adds to sequence b (counts null: T). None where its length
+// is negative: at position 0 they would fall on tokens that it may hold.
+__device__ __forceinline__ int kv8_count(const KV8& c, const int32_t* counts, int b, int T) {
   const int n = counts ? __ldg(counts + b) : T;
-  return n < 0 ? 0 : (n > T ? T : n);
+  return n < 0 || __ldg(c.lens + b) < 0 ? 0 : (n > T ? T : n);
 }
+// End of the tokens of sequence b with its counted new ones.
 __device__ __forceinline__ int kv8_end(const KV8& c, int len, int count) {
   const int64_t reach = static_cast<int64_t>(c.blocks) << c.p_shift;
   if (len + static_cast<int64_t>(count) > reach) {

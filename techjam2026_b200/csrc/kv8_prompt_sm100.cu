@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256)
   const int row0 = blockIdx.x * rows_of_pass * KV8_PREP_UNROLL + (threadIdx.x >> l_shift);
   const int bh = blockIdx.y;
   const int b = bh / c.H, h = bh - b * c.H;
-  const int real_rows = min(w.rows, kv8_count(counts, b, T) * G);
+  const int real_rows = min(w.rows, kv8_count(c, counts, b, T) * G);
   const int64_t base = b * q_sb + static_cast<int64_t>(h) * G * q_sh;
   uint4 x[KV8_PREP_UNROLL];
 #pragma unroll
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
   const int chunk = blockIdx.y;
   const int row0 = static_cast<int>(gridDim.x - 1 - blockIdx.x) * Cfg::ROWS;  // heaviest first
   const int len = kv8_len(c, b);
-  const int count = kv8_count(counts, b, T);
+  const int count = kv8_count(c, counts, b, T);
   int end = kv8_end(c, len, count);
   if (end > max_len) {
     if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
@@ -1021,7 +1021,7 @@ __global__ void __launch_bounds__(WeighCfg<DH, PL>::THREADS)
   const int bh = blockIdx.y;
   const int b = bh / c.H, h = bh - b * c.H;
   const int len = kv8_len(c, b);
-  const int count = kv8_count(counts, b, T);
+  const int count = kv8_count(c, counts, b, T);
   const int end = min(kv8_end(c, len, count), max_len);
   const int key0 = blockIdx.x * Cfg::BK;
   if (key0 >= end) return;

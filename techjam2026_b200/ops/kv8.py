@@ -23,7 +23,8 @@ Calls are stream-ordered on the current stream, launch a fixed number of
 kernels for given shapes and read lengths on the device, so a step may be
 captured in a CUDA graph. A length beyond the table or a page number outside
 the pool is never used as an index: it is recorded in the device status word
-(code 6) and the tokens count as absent.
+(code 6) and the tokens count as absent. A sequence of a negative length holds
+no token and takes none.
 """
 from __future__ import annotations
 

@@ -418,6 +418,37 @@ def test_bad_pages_and_lengths_are_refused_on_the_device():
     clean()
 
 
+@pytest.mark.parametrize("T", [1, 5, 80])
+def test_a_negative_length_holds_nothing_and_takes_nothing(T):
+    """Its new tokens are not written (they would fall on tokens that are valid
+    once the length is), its queries see no key, an eviction keeps none."""
+    cache, spare, g = make([40, 7], heads=2, dim=64, block=16, room=96, weight=True, spare=4)
+    cache.weight.zero_()
+    held = [t.clone() for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8),
+                                cache.scale, cache.weight)]
+    x = (torch.randn(2, 2, T, 64, generator=g) * 9).cuda()
+    q = torch.randn(2, 4, T, 64, generator=g).cuda()
+    cache.lens[1] = -5
+    for counts in (None, torch.full((2,), T, dtype=torch.int32, device="cuda")):
+        cache.lens[0] = 40
+        ops.kv8_append(cache, x, x, counts=counts)
+        assert _lib.lib().kf_device_status(1) == 6
+        own = cache.table[1].long()
+        for was, t in zip(held, (cache.k.view(torch.uint8), cache.v.view(torch.uint8),
+                                 cache.scale, cache.weight)):
+            assert torch.equal(t[own].nan_to_num(-1), was[own].nan_to_num(-1))
+        out, lse = ops.kv8_attention(q, cache, counts=counts, track=True, return_lse=True)
+        assert _lib.lib().kf_device_status(1) == 6
+        assert not out[1].any() and torch.isinf(lse[1]).all() and out[0].any()
+        assert not cache.weight[own].any()
+        k, v = ops.kv8_read(cache, 64, counts=counts)
+        assert _lib.lib().kf_device_status(1) == 6
+        assert not k[1].any() and not v[1].any() and k[0].any()
+        kept, new = ops.kv8_evict(cache, spare.view(2, 2), 20, 3)
+        assert _lib.lib().kf_device_status(1) == 6
+        assert (kept[1] == -1).all() and new.lens.tolist() == [20, 0]
+
+
 def test_nothing_to_do():
     cache, _, _ = make([0, 0], heads=2, dim=64, block=16)
     q = torch.randn(2, 2, 0, 64, device="cuda")
