@@ -326,6 +326,39 @@ def test_long_caches_are_split_and_joined(lens):
     attend(cache, q, None, track=True)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, I8), (128, F8)])
+@pytest.mark.parametrize("batch,heads,group,T", [(16, 20, 1, 1), (16, 20, 12, 1), (16, 10, 2, 20),
+                                                 (4, 4, 1, 200)])
+@pytest.mark.parametrize("mean", [0.0, 1.0])
+def test_fp32_keeps_its_precision_over_thousands_of_keys(mean, batch, heads, group, T, dim, dtype):
+    """Heads enough that a CTA takes 4096 keys in one part, and V with and
+    without a mean (its sums then grow key by key). The relative error has
+    2e-7 from q (22 bits), 4e-7 from the scores (8 products of 16, each with
+    its last place lost), 1.5e-7 from P and 4e-7 from the sums of 256 products
+    in fp32: 1.2e-6. A lost second plane of q or P would be 1e-4."""
+    L = 4090 - T
+    cache, _, g = make([0] * batch, heads=heads, dim=dim, block=64, dtype=dtype, room=4090)
+    x = torch.randn(2, batch, heads, 4090, dim, generator=torch.Generator("cuda").manual_seed(7),
+                    device="cuda")
+    x[1] += mean
+    ops.kv8_append(cache, x[0] * 1.5, x[1])
+    cache.lens += L
+    q = torch.randn(batch, heads * group, T, dim, generator=g).cuda()
+    out = ops.kv8_attention(q, cache)
+    count = torch.full((batch,), T, dtype=torch.int32, device="cuda")
+    k, v = ops.kv8_read(cache, 4090, counts=count)
+    off = size = 0.0
+    hidden = torch.arange(4090, device="cuda") > L + torch.arange(T, device="cuda")[:, None]
+    for b in range(batch):
+        s = q[b].double().view(heads, group, T, dim) @ k[b].double().transpose(1, 2)[:, None]
+        p = torch.softmax((s * dim ** -0.5).masked_fill(hidden, -math.inf), -1)
+        want = (p @ v[b].double()[:, None]).view(heads * group, T, dim)
+        off += float((out[b].double() - want).square().sum())
+        size += float(want.square().sum())
+    assert math.sqrt(off / size) <= 1.2e-6
+    clean()
+
+
 def test_scores_that_grow_along_the_cache():
     """Each page's scores exceed the last one's by far, then fall: the running
     reference moves often, and early weights vanish against late ones."""
