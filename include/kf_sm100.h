@@ -402,9 +402,9 @@ int kf_kv8_read(const kf_kv8_cache* cache, const int32_t* start, const int32_t* 
  * KF_KV8_CAUSAL: up to its own). q_heads is a multiple of kv_heads; query
  * head h reads kv head h / (q_heads / kv_heads).
  *     out = softmax(sm_scale * q K^T) V,  lse = log of the softmax's sum
- * Scores, sums, maxima and the accumulators are fp32. q and the weights enter
- * the products as fp16 for 16-bit q (the weights as two planes for fp16 q with
- * at most 8 query rows a kv head), as two fp16 planes (22 bits) for fp32.
+ * Scores, sums, maxima and the accumulators are fp32. q enters the products as
+ * fp16 for 16-bit q and as two fp16 planes (22 bits) for fp32; the weights as
+ * fp16 for bf16 q and as two planes for fp16 and fp32 q.
  * sm_scale must be finite and not negative.
  * out has q's type; rows without a visible key, and rows i >= counts[b], are 0
  * (lse -inf). lse (may be null) is fp32 [batch, q_heads, T]. With KF_KV8_TRACK

@@ -16,8 +16,8 @@
 // four V rows; the 16-byte pieces of the ring are placed so that those reads
 // touch all banks. 16 rows fill the m16 tile; the 128-row tensor-memory
 // products would waste 7/8 of theirs here. RH = 1 serves at most 8 rows and
-// skips the softmax of the upper half of the tile; with two planes (fp32 q) the
-// second plane then takes that half, so one product does both.
+// skips the softmax of the upper half of the tile; a second plane of q or of P
+// then takes that half, so one product does both.
 // Measured: 16 sequences of 16k to 32k tokens, 8 kv heads of 128, four query
 // heads each: 145 us for 805 MB, 5.6 TB/s (0.85 of the copy rate); a 65k
 // sequence of 16 heads of 64: 36 us for 134 MB, 3.7 TB/s, bound by
@@ -31,8 +31,9 @@
 // [2^14, 2^15) before it becomes one fp16 plane (16-bit q: nothing is lost
 // until 2^-28 of the row's largest) or two (fp32 q: 22 bits). P is relative to
 // a reference 2^9 below the running maximum, so it uses fp16 up to 2^15 and
-// loses precision only below 2^-23 of the largest weight; for fp32 output it
-// is two planes as well. The V scale of a page is folded into P as the ratio
+// loses precision only below 2^-23 of the largest weight. One plane of P is off
+// by 2.0e-4 of the output, which bf16's own rounding (1.65e-3) hides and fp16's
+// (2.07e-4) does not: fp16 and fp32 q have two. The V scale of a page is folded into P as the ratio
 // to the chunk's largest (<= 1, so P stays in range). The sum l adds the
 // unrounded fp32 weights.
 #include "kv8_common.cuh"
@@ -53,7 +54,7 @@ struct KV8Work {
   float* part;    // [B*H][rows][chunks][D]
   float* lse;     // [B*H][rows]: log2 of the softmax's sum
   float* score;   // [B*H][rows][ld_score] (few rows and track), in log2 units
-  uint16_t* planes;  // many rows: q as fp16 planes [PL][B*H][rows][D]
+  uint16_t* planes;  // many rows: q as fp16 planes [QP][B*H][rows][D]
   float* qf;         // and their factors [B*H][rows]
   int64_t ld_score;
   int rows;       // T * G
@@ -133,13 +134,13 @@ __device__ __forceinline__ float kv8_row_scale(float amax, float* inverse) {
 
 // The q fragments of 16 rows: lane (g, t) holds rows g and g + 8, the K bytes
 // it owns (see above). qf[r]: factor from the products to log2 units.
-template <int DH, int PL, int RH>
+template <int DH, int QP, int RH>
 struct QFrag {
   static constexpr int EPT = DH / 4 < 16 ? DH / 4 : 16;  // consecutive elements of a piece
   static constexpr int NPC = DH / 4 / EPT;               // pieces (64 elements apart)
   static constexpr int KS = DH / 16;                     // k-steps
   // RH = 1: rows g + 8 are zeros, or with two planes the second plane.
-  static constexpr int NP = RH == 1 ? 1 : PL;            // products per k-step
+  static constexpr int NP = RH == 1 ? 1 : QP;            // products per k-step
   uint32_t a[NP][KS][4];
   float qf[RH];
 
@@ -147,7 +148,7 @@ struct QFrag {
                                        int64_t q_st, int dtype, bool vec, int b, int h, int G,
                                        int row0, int rows, float scale_log2) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    if constexpr (RH == 1 && PL == 1) {
+    if constexpr (RH == 1 && QP == 1) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) a[0][s][1] = a[0][s][3] = 0u;
     }
@@ -190,7 +191,7 @@ struct QFrag {
         for (int u = 0; u < 4; ++u) y[u] = x[4 * s + u] * sc;
         a[0][s][r] = pack_half2(y[0], y[1]);
         a[0][s][2 + r] = pack_half2(y[2], y[3]);
-        if constexpr (PL == 2) {
+        if constexpr (QP == 2) {
           a[NP - 1][s][RH == 1 ? 1 : r] = pack_half2_rest(y[0], y[1], a[0][s][r]);
           a[NP - 1][s][RH == 1 ? 3 : 2 + r] = pack_half2_rest(y[2], y[3], a[0][s][2 + r]);
         }
@@ -261,8 +262,8 @@ struct SplitCfg {
 };
 
 // Products of 16 q rows with 16 keys: d[n][.] in the m16n8 accumulator layout.
-template <int DH, int FMT, int PL, int RH>
-__device__ __forceinline__ void score_tile(const QFrag<DH, PL, RH>& q, const KBytes<DH>& kb,
+template <int DH, int FMT, int QP, int RH>
+__device__ __forceinline__ void score_tile(const QFrag<DH, QP, RH>& q, const KBytes<DH>& kb,
                                            float (&d)[2][4]) {
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -271,19 +272,20 @@ __device__ __forceinline__ void score_tile(const QFrag<DH, PL, RH>& q, const KBy
     for (int s = 0; s < DH / 16; ++s) {
       uint32_t b0, b1;
       kv8_cvt4<FMT>(kb.w[n][s], b0, b1);
-      if constexpr (PL == 2 && RH == 2)
+      if constexpr (QP == 2 && RH == 2)
         mma_f16_16816(d[n], q.a[1][s][0], q.a[1][s][1], q.a[1][s][2], q.a[1][s][3], b0, b1);
       mma_f16_16816(d[n], q.a[0][s][0], q.a[0][s][1], q.a[0][s][2], q.a[0][s][3], b0, b1);
     }
-    if constexpr (PL == 2 && RH == 1) {
+    if constexpr (QP == 2 && RH == 1) {
       d[n][0] += d[n][2];
       d[n][1] += d[n][3];
     }
   }
 }
 
-template <int DH, int FMT, int PL, int RH>
-__global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
+// QP, PP: fp16 planes of q and of P.
+template <int DH, int FMT, int QP, int PP, int RH>
+__global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     kv8_split_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh, int64_t q_st,
                      void* __restrict__ out, int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype,
                      int vec, const int32_t* __restrict__ counts, int T, int G, int max_len,
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
     s_vs[j - j0] = s.y;
     vmax = fmaxf(vmax, s.y);
   }
-  QFrag<DH, PL, RH> qa;
+  QFrag<DH, QP, RH> qa;
   qa.load(c, q, q_sb, q_sh, q_st, dtype, vec != 0, b, h, G, row0, w.rows, scale_log2);
 #pragma unroll
   for (int d = 16; d; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
@@ -357,11 +359,11 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
   vmax = fmaxf(fmaxf(s_vmax[0], s_vmax[1]), fmaxf(s_vmax[2], s_vmax[3]));
   const float inv_vmax = vmax > 0.f ? 1.f / vmax : 0.f;
 
-  // With two planes O collects the products of 16 keys by fp32 additions: the
+  // With two planes of P, O collects the products of 16 keys by fp32 additions: the
   // tensor core's own accumulation drops what lies below the running sum (with
   // 1024 keys a warp 1.4e-6 to 2.9e-6 against float64; so 4e-7 to 8e-7, in the
   // same time).
-  constexpr int OW = PL == 2 ? 2 * RH : 4;  // of a tile's columns, held by a lane
+  constexpr int OW = PP == 2 ? 2 * RH : 4;  // of a tile's columns, held by a lane
   float o[NT][OW];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
     const int bad = s_page[pj] < 0 ? 0 : 0x7fffffff;  // a refused page has no visible key
 
     float f[2][4];
-    score_tile<DH, FMT, PL, RH>(qa, kb, f);
+    score_tile<DH, FMT, QP, RH>(qa, kb, f);
     float top = -INFINITY;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -485,7 +487,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
           p[u] = x == -INFINITY ? 0.f : e * ratio;
         }
         hi[2 * n + r] = pack_half2(p[0], p[1]);
-        if constexpr (PL == 2)
+        if constexpr (PP == 2)
           (RH == 1 ? hi[2 * n + 1] : lo[2 * n + r]) = pack_half2_rest(p[0], p[1], hi[2 * n + r]);
       }
     // Slots past the end, and page 0 where it stands in for a refused page, hold
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(PL))
         kv8_cvt4<FMT>(__byte_perm(vb.w[0][u], vb.w[1][u], sel), b00, b01);
         kv8_cvt4<FMT>(__byte_perm(vb.w[2][u], vb.w[3][u], sel), b10, b11);
         const int n = 4 * u + 2 * half;
-        if constexpr (PL == 1) {
+        if constexpr (PP == 1) {
           mma_f16_16816(o[n], hi[0], hi[1], hi[2], hi[3], b00, b10);
           mma_f16_16816(o[n + 1], hi[0], hi[1], hi[2], hi[3], b01, b11);
         } else {

@@ -142,9 +142,9 @@ struct KV8Call {
   cudaStream_t st;
 };
 
-template <int DH, int FMT, int PL, int RH>
+template <int DH, int FMT, int QP, int PP, int RH>
 static cudaError_t kv8_split(const KV8& c, const KV8Call& a, const KV8Work& w) {
-  auto kern = kv8_split_kernel<DH, FMT, PL, RH>;
+  auto kern = kv8_split_kernel<DH, FMT, QP, PP, RH>;
   constexpr int smem = SplitCfg<DH>::SMEM;
   static DeviceOnce once;
   cudaError_t attr = cudaSuccess;
@@ -160,38 +160,42 @@ static cudaError_t kv8_split(const KV8& c, const KV8Call& a, const KV8Work& w) {
                         a.o_sb, a.o_sh, a.o_st, a.dtype, a.q_vec, a.counts, a.T, a.G, a.max_len,
                         a.scale_log2, a.flags, a.lse, w);
 }
-template <int DH, int FMT, int PL>
+template <int DH, int FMT, int QP, int PP>
 static cudaError_t kv8_split_rows(const KV8& c, const KV8Call& a, const KV8Work& w, bool half) {
-  return half ? kv8_split<DH, FMT, PL, 1>(c, a, w) : kv8_split<DH, FMT, PL, 2>(c, a, w);
+  return half ? kv8_split<DH, FMT, QP, PP, 1>(c, a, w) : kv8_split<DH, FMT, QP, PP, 2>(c, a, w);
+}
+// fp16 outputs show one plane's rounding of P (1.4 times their own error), bf16
+// ones do not. The second plane costs (us, one / two): a token of 4 rows a kv
+// head, 24k tokens of 128, 147 / 148; of 12 rows 168 / 205; a chunk of 1024 over
+// 8k tokens of 64 246 / 436 (P then takes the place of S), prompts of 2048 tokens of
+// 128 288 / 380.
+template <int DH, int FMT>
+static cudaError_t kv8_split_type(const KV8& c, const KV8Call& a, const KV8Work& w, bool half) {
+  if (a.dtype == KF_DT_F32) return kv8_split_rows<DH, FMT, 2, 2>(c, a, w, half);
+  if (a.dtype == KF_DT_F16) return kv8_split_rows<DH, FMT, 1, 2>(c, a, w, half);
+  return kv8_split_rows<DH, FMT, 1, 1>(c, a, w, half);
 }
 template <int DH>
 static cudaError_t kv8_split_any(const KV8& c, const KV8Call& a, const KV8Work& w, bool half) {
-  // fp16 q has the precision to show P's rounding (1.4 times the error of the
-  // output's own), and with at most 8 rows a second plane of P is all but free
-  // (42.2 against 41.3 us for a 65k sequence); bf16 does not show it.
-  const bool two = a.dtype == KF_DT_F32 || (a.dtype == KF_DT_F16 && half);
-  if (c.fmt == KF_KV8_INT8)
-    return two ? kv8_split_rows<DH, KF_KV8_INT8, 2>(c, a, w, half)
-               : kv8_split_rows<DH, KF_KV8_INT8, 1>(c, a, w, half);
-  return two ? kv8_split_rows<DH, KF_KV8_E4M3, 2>(c, a, w, half)
-             : kv8_split_rows<DH, KF_KV8_E4M3, 1>(c, a, w, half);
+  return c.fmt == KF_KV8_INT8 ? kv8_split_type<DH, KF_KV8_INT8>(c, a, w, half)
+                              : kv8_split_type<DH, KF_KV8_E4M3>(c, a, w, half);
 }
 
-template <int DH, int PL>
+template <int DH, int QP, int PP>
 static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
-  using Cfg = PromptCfg<DH, PL>;
-  using Wei = WeighCfg<DH, PL>;
+  using Cfg = PromptCfg<DH, QP, PP>;
+  using Wei = WeighCfg<DH, QP>;
   const unsigned bh = static_cast<unsigned>(c.B * c.H);
   const bool track = (a.flags & KF_KV8_TRACK) != 0;
   CUtensorMap map;
-  const uint64_t dims[3] = {DH, static_cast<uint64_t>(w.rows), static_cast<uint64_t>(PL) * bh};
+  const uint64_t dims[3] = {DH, static_cast<uint64_t>(w.rows), static_cast<uint64_t>(QP) * bh};
   const uint64_t strides[2] = {DH * 2, static_cast<uint64_t>(w.rows) * DH * 2};
   const uint32_t box[3] = {64, 128, 1};
   int rc = encode_tensor_map(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, w.planes, dims, strides, box,
                              CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  auto kern = kv8_prompt_kernel<DH, PL>;
-  auto kern_w = kv8_prompt_weights_kernel<DH, PL>;
+  auto kern = kv8_prompt_kernel<DH, QP, PP>;
+  auto kern_w = kv8_prompt_weights_kernel<DH, QP>;
   static DeviceOnce once;
   rc = once.run("kf_kv8_attention", nullptr, [&](int) {
     cudaError_t e =
@@ -204,7 +208,7 @@ static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
   auto prep = a.dtype == KF_DT_F32    ? kv8_prep_q_kernel<KF_DT_F32>
               : a.dtype == KF_DT_BF16 ? kv8_prep_q_kernel<KF_DT_BF16>
                                       : kv8_prep_q_kernel<KF_DT_F16>;
-  const int rows_of_cta = 256 * (PL == 2 ? 4 : 8) / DH * KV8_PREP_UNROLL;
+  const int rows_of_cta = 256 * (QP == 2 ? 4 : 8) / DH * KV8_PREP_UNROLL;
   cudaError_t e = launch_chained(
       prep, dim3(static_cast<unsigned>((w.rows + rows_of_cta - 1) / rows_of_cta), bh), dim3(256), 0,
       a.st, c, a.q, a.q_sb, a.q_sh, a.q_st, a.q_vec16, a.counts, a.T, a.G, a.scale_log2, w);
@@ -222,6 +226,13 @@ static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
                        dim3(Wei::THREADS), Wei::SMEM, a.st, map, c, a.counts, a.T, a.G, a.max_len,
                        a.flags, w);
   return cuda_status(e, "kf_kv8_attention launch");
+}
+
+template <int DH>
+static int kv8_prompt_type(const KV8& c, const KV8Call& a, const KV8Work& w) {
+  if (a.dtype == KF_DT_F32) return kv8_prompt<DH, 2, 2>(c, a, w);
+  if (a.dtype == KF_DT_F16) return kv8_prompt<DH, 1, 2>(c, a, w);
+  return kv8_prompt<DH, 1, 1>(c, a, w);
 }
 
 }  // namespace kf
@@ -277,12 +288,11 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
   const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, vec16, o_vec, counts, Ti, G,
                      cap, scale_log2, flags, lse, st};
   if (w.prompt) {
-    const bool two = dtype == KF_DT_F32;
     switch (c.D) {
-      case 16: return two ? kv8_prompt<16, 2>(c, a, w) : kv8_prompt<16, 1>(c, a, w);
-      case 32: return two ? kv8_prompt<32, 2>(c, a, w) : kv8_prompt<32, 1>(c, a, w);
-      case 64: return two ? kv8_prompt<64, 2>(c, a, w) : kv8_prompt<64, 1>(c, a, w);
-      default: return two ? kv8_prompt<128, 2>(c, a, w) : kv8_prompt<128, 1>(c, a, w);
+      case 16: return kv8_prompt_type<16>(c, a, w);
+      case 32: return kv8_prompt_type<32>(c, a, w);
+      case 64: return kv8_prompt_type<64>(c, a, w);
+      default: return kv8_prompt_type<128>(c, a, w);
     }
   }
   cudaError_t e = cudaSuccess;

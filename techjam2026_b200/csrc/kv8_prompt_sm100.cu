@@ -16,7 +16,7 @@
 //                   bytes: rows are keys); they also stage the scales. (Codes
 //                   fetched through registers with a page lookup per piece held
 //                   the whole kernel at 6000 clocks a step.)
-// TMEM: S0 | S1 (128 columns each), O0 | O1, and P. At head_dim <= 64 with 16-bit
+// TMEM: S0 | S1 (128 columns each), O0 | O1, and P. At head_dim <= 64 with bf16
 // q, P has 64 columns of its own per tile, and S(j + 1) is issued as soon as
 // step j's scores are in registers, so it is there when their softmax ends.
 // Elsewhere P overwrites S and each tile's order is P V(j), then S(j + 1): the
@@ -36,8 +36,9 @@
 // (every product twice, one tile a CTA).
 //
 // Numbers as in the split kernel: q rows scaled by powers of two and P relative
-// to a lazily moved reference, one fp16 plane for 16-bit q and two for fp32 q
-// (then both products run twice); page scales enter S exactly and P as the
+// to a lazily moved reference. bf16 q: one fp16 plane of each. fp16 q: two of P
+// (P V runs twice; with one, outputs were 1.4 times as far off float64 as fp16's own
+// rounding). fp32 q: two of both (both products run twice); page scales enter S exactly and P as the
 // ratio to the range's largest V scale.
 //
 // kv8_prompt_weights_kernel: one CTA = 128 keys against all rows that see
@@ -73,7 +74,7 @@ __device__ __forceinline__ bool warp_all(bool ok) { return __all_sync(0xffffffff
 
 // ---------------------------------------------------------------- q planes
 
-// q rows as fp16 planes [PL][B*H][rows][D] and their factors to log2 units. A
+// q rows as fp16 planes [QP][B*H][rows][D] and their factors to log2 units. A
 // thread holds 16 bytes of each of four rows, neighbours the rest of the row.
 // Rows past a sequence's count get zeros. Bound by memory.
 constexpr int KV8_PREP_UNROLL = 4;
@@ -241,16 +242,17 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-template <int DH, int PL>
+// QP, PP: fp16 planes of q (two for fp32) and of P (two for fp32 and fp16).
+template <int DH, int QP, int PP>
 struct PromptCfg {
   // Tiles of 128 query rows. fp32 at head_dim 128 takes one: its Q planes fill
   // shared memory and its second accumulator TMEM.
-  static constexpr int NT = (DH == 128 && PL == 2) ? 1 : 2;
+  static constexpr int NT = (DH == 128 && QP == 2) ? 1 : 2;
   static constexpr int BM = 128;
   static constexpr int BN = 128;                           // keys of a step
   static constexpr int CH = DH > 64 ? 2 : 1;               // 64-column halves of a row
   static constexpr int Q_PLANE = BM * 128 * CH;            // bytes of one tile's plane
-  static constexpr int Q_BYTES = NT * PL * Q_PLANE;
+  static constexpr int Q_BYTES = NT * QP * Q_PLANE;
   static constexpr int KV_BYTES = BN * 128 * CH;
   static constexpr int ST = 2;                             // stages of K and of V
   static constexpr int RAW = BN * DH;                      // bytes of a tile's codes
@@ -278,14 +280,14 @@ struct PromptCfg {
   static constexpr int M_COL = O_COL + NT * O_STRIDE;
   // With room in TMEM P has columns of its own, and S of the next step is
   // computed while this step's softmax runs; otherwise P overwrites S.
-  static constexpr bool SEP = NT == 2 && PL == 1 && DH <= 64;
+  static constexpr bool SEP = NT == 2 && PP == 1 && DH <= 64;
   static constexpr int P_COL = O_COL + NT * O_STRIDE;
   static constexpr int ROWS = NT * BM;
   // Twelve warps leave 168 registers a thread: a softmax row's 128 scores and
   // what goes with them.
   static constexpr int THREADS = 12 * 32;
   static_assert(SMEM <= 232448, "smem");
-  static_assert((PL == 2 ? M_COL : O_COL) + NT * O_STRIDE <= 512, "TMEM");
+  static_assert((QP == 2 ? M_COL : O_COL) + NT * O_STRIDE <= 512, "TMEM");
   static_assert(!SEP || P_COL + 128 <= 512, "TMEM");
 };
 
@@ -349,13 +351,13 @@ __device__ __forceinline__ float max16(const float* s) {
   return fmax3(fmaxf(m, n), s[14], s[15]);
 }
 
-template <int DH, int PL>
-__global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
+template <int DH, int QP, int PP>
+__global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
     kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, KV8 c, void* __restrict__ out,
                       int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype, int o_vec,
                       const int32_t* __restrict__ counts, int T, int G, int max_len, int flags,
                       float* __restrict__ lse_out, KV8Work w) {
-  using Cfg = PromptCfg<DH, PL>;
+  using Cfg = PromptCfg<DH, QP, PP>;
   constexpr int BM = Cfg::BM, BN = Cfg::BN, NT = Cfg::NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -478,9 +480,9 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       // ------------------------------------------------ Q, products
       mbar_arrive_expect_tx(q_full, Cfg::Q_BYTES);
       for (int t = 0; t < NT; ++t)
-        for (int pl = 0; pl < PL; ++pl)
+        for (int pl = 0; pl < QP; ++pl)
           for (int ch = 0; ch < Cfg::CH; ++ch)
-            tma_load_3d(sQ + (t * PL + pl) * Cfg::Q_PLANE + ch * BM * 128, &tmQ, q_full, ch * 64,
+            tma_load_3d(sQ + (t * QP + pl) * Cfg::Q_PLANE + ch * BM * 128, &tmQ, q_full, ch * 64,
                         row0 + t * BM, pl * c.B * c.H + bh);
       constexpr uint32_t idesc_s = make_idesc_f16(BM, BN, 0);
       constexpr uint32_t idesc_o = make_idesc_f16(BM, DH, 1);
@@ -488,16 +490,16 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       // S of tile t and the K tile of `stage` into S buffer `buf`.
       auto issue_s = [&](int t, int buf, int stage) {
 #pragma unroll
-        for (int pl = PL - 1; pl >= 0; --pl)  // the small plane first
+        for (int pl = QP - 1; pl >= 0; --pl)  // the small plane first
 #pragma unroll
           for (int kk = 0; kk < DH / 16; ++kk) {
-            const uint64_t ad = make_smem_desc(sQa + (t * PL + pl) * Cfg::Q_PLANE +
+            const uint64_t ad = make_smem_desc(sQa + (t * QP + pl) * Cfg::Q_PLANE +
                                                    (kk >> 2) * BM * 128 + (kk & 3) * 32,
                                                16, 1024, KF_SWIZZLE_128B);
             const uint64_t bd =
                 make_smem_desc(sKa + stage * Cfg::KV_BYTES + (kk >> 2) * BN * 128 + (kk & 3) * 32,
                                16, 1024, KF_SWIZZLE_128B);
-            mma_bf16_ss(tmem_base + buf * 128, ad, bd, idesc_s, (pl < PL - 1 || kk > 0) ? 1u : 0u);
+            mma_bf16_ss(tmem_base + buf * 128, ad, bd, idesc_s, (pl < QP - 1 || kk > 0) ? 1u : 0u);
           }
         mma_commit(&s_full[buf]);
       };
@@ -505,14 +507,14 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       auto issue_o = [&](int t, int buf, int stage, bool fresh) {
         const uint32_t p_base = tmem_base + (Cfg::SEP ? Cfg::P_COL + t * 64 : buf * 128);
 #pragma unroll
-        for (int pl = PL - 1; pl >= 0; --pl)
+        for (int pl = PP - 1; pl >= 0; --pl)
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk) {
             const uint64_t bd = make_smem_desc(sVa + stage * Cfg::KV_BYTES + kk * 16 * 128, BN * 128,
                                                1024, KF_SWIZZLE_128B);
             mma_f16_ts(tmem_base + Cfg::O_COL + t * Cfg::O_STRIDE,
                        p_base + (Cfg::SEP ? kk * 8 : (kk >> 2) * 64 + pl * 32 + (kk & 3) * 8), bd, idesc_o,
-                       (!fresh || pl < PL - 1 || kk > 0) ? 1u : 0u);
+                       (!fresh || pl < PP - 1 || kk > 0) ? 1u : 0u);
           }
       };
       bool ok = mbar_wait(q_full, 0, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA) &&
@@ -565,7 +567,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       for (int j = 0; j < n_steps && ok && !Cfg::SEP; ++j) {
         const int st = j & 1, nx = st ^ 1;
         const uint32_t ph = (j >> 1) & 1, nph = ((j + 1) >> 1) & 1;
-        const bool fresh = PL == 2 ? j % Cfg::FLUSH == 0 : j == 0;
+        const bool fresh = QP == 2 ? j % Cfg::FLUSH == 0 : j == 0;
         const bool more = j + 1 < n_steps;
         if (NT == 1) {
           // S runs one step ahead of the softmax, in the other buffer: the P
@@ -816,8 +818,8 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
         tc_fence_after();
         return ok;
       };
-      const bool flush = PL == 2 && j > 0 && j % Cfg::FLUSH == 0;
-      const bool have_m = PL == 2 && j >= Cfg::FLUSH;  // M holds something
+      const bool flush = QP == 2 && j > 0 && j % Cfg::FLUSH == 0;
+      const bool have_m = QP == 2 && j >= Cfg::FLUSH;  // M holds something
       if (flush) {
         if (!at_rest()) break;
 #pragma unroll
@@ -901,12 +903,12 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
           const float r = sc.ratio[k >> 4];
           f2_unpack(f2_mul(f2_pack(x, y), f2_pack(r, r)), x, y);
           hi[u] = pack_half2(x, y);
-          if constexpr (PL == 2) lo[u] = pack_half2_rest(x, y, hi[u]);
+          if constexpr (PP == 2) lo[u] = pack_half2_rest(x, y, hi[u]);
         }
         const uint32_t at = Cfg::SEP ? t_row + Cfg::P_COL + t * 64 + part * 16
                                      : t_s + (part >> 1) * 64 + (part & 1) * 16;
         tmem_st16(at, hi);
-        if constexpr (PL == 2) tmem_st16(at + 32, lo);
+        if constexpr (PP == 2) tmem_st16(at + 32, lo);
       }
       float x0, x1, x2, x3;
       f2_unpack(acc[0], x0, x1);
@@ -925,7 +927,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
       if (nan_k) sum = nan;
       float f = alone ? vmax / sum : vmax;  // not used where sum is 0
       if (nan_v) f = nan;
-      const bool have_m = PL == 2 && n_steps > Cfg::FLUSH;
+      const bool have_m = QP == 2 && n_steps > Cfg::FLUSH;
 #pragma unroll
       for (int cc = 0; cc < (DH + 31) / 32; ++cc) {
         float o[32];
@@ -973,14 +975,14 @@ __global__ void __launch_bounds__(PromptCfg<DH, PL>::THREADS, 1)
 
 // ---------------------------------------------------------------- weights
 
-template <int DH, int PL>
+template <int DH, int QP>
 struct WeighCfg {
   static constexpr int BK = 128;                   // keys of a CTA (TMEM lanes)
   static constexpr int BR = 128;                   // query rows of a step
   static constexpr int CH = DH > 64 ? 2 : 1;
   static constexpr int K_BYTES = BK * 128 * CH;
   static constexpr int Q_PLANE = BR * 128 * CH;
-  static constexpr int Q_STAGE = PL * Q_PLANE;
+  static constexpr int Q_STAGE = QP * Q_PLANE;
   static constexpr int ST = 2;
   static constexpr int Q_OFF = K_BYTES;
   static constexpr int ROW_OFF = Q_OFF + ST * Q_STAGE;   // factors and lse of a stage's rows
@@ -992,12 +994,12 @@ struct WeighCfg {
   static_assert(SMEM <= 232448, "smem");
 };
 
-template <int DH, int PL>
-__global__ void __launch_bounds__(WeighCfg<DH, PL>::THREADS)
+template <int DH, int QP>
+__global__ void __launch_bounds__(WeighCfg<DH, QP>::THREADS)
     kv8_prompt_weights_kernel(const __grid_constant__ CUtensorMap tmQ, KV8 c,
                               const int32_t* __restrict__ counts, int T, int G, int max_len,
                               int flags, KV8Work w) {
-  using Cfg = WeighCfg<DH, PL>;
+  using Cfg = WeighCfg<DH, QP>;
   constexpr int BR = Cfg::BR;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -1087,7 +1089,7 @@ __global__ void __launch_bounds__(WeighCfg<DH, PL>::THREADS)
       const int row0 = (r_begin + j) * BR;
       if (lane == 0) {
         mbar_arrive_expect_tx(&q_full[st], Cfg::Q_STAGE);
-        for (int pl = 0; pl < PL; ++pl)
+        for (int pl = 0; pl < QP; ++pl)
           for (int ch = 0; ch < Cfg::CH; ++ch)
             tma_load_3d(sQ + st * Cfg::Q_STAGE + pl * Cfg::Q_PLANE + ch * BR * 128, &tmQ,
                         &q_full[st], ch * 64, row0, pl * c.B * c.H + bh);
@@ -1121,7 +1123,7 @@ __global__ void __launch_bounds__(WeighCfg<DH, PL>::THREADS)
         if (j >= 2 && !mbar_wait(&s_empty[st], ph ^ 1, abort_flag, KF_DEV_WAIT_TIMEOUT_MMA)) break;
         tc_fence_after();
 #pragma unroll
-        for (int pl = PL - 1; pl >= 0; --pl)
+        for (int pl = QP - 1; pl >= 0; --pl)
 #pragma unroll
           for (int kk = 0; kk < DH / 16; ++kk) {
             const uint64_t ad = make_smem_desc(sKa + (kk >> 2) * Cfg::BK * 128 + (kk & 3) * 32, 16,
@@ -1129,7 +1131,7 @@ __global__ void __launch_bounds__(WeighCfg<DH, PL>::THREADS)
             const uint64_t bd = make_smem_desc(sQa + st * Cfg::Q_STAGE + pl * Cfg::Q_PLANE +
                                                    (kk >> 2) * BR * 128 + (kk & 3) * 32,
                                                16, 1024, KF_SWIZZLE_128B);
-            mma_bf16_ss(tmem_base + st * 128, ad, bd, idesc, (pl < PL - 1 || kk > 0) ? 1u : 0u);
+            mma_bf16_ss(tmem_base + st * 128, ad, bd, idesc, (pl < QP - 1 || kk > 0) ? 1u : 0u);
           }
         mma_commit(&s_full[st]);
         mma_commit(&q_empty[st]);

@@ -359,6 +359,34 @@ def test_fp32_keeps_its_precision_over_thousands_of_keys(mean, batch, heads, gro
     clean()
 
 
+@pytest.mark.parametrize("dim,dtype", [(32, I8), (64, F8), (128, I8)])
+@pytest.mark.parametrize("group,T", [(1, 1), (12, 1), (1, 20), (3, 20), (1, 300)])
+@pytest.mark.parametrize("kind", [F16, BF16])
+def test_16_bit_outputs_are_as_near_as_their_own_rounding(kind, group, T, dim, dtype):
+    """Against float64, relative to the error of rounding the float64 result to
+    the type. fp16 (2.1e-4): q and two planes of P leave less than 2e-6, which
+    does not show. bf16 (1.65e-3): P rounded to fp16 is off by at most 2.9e-4
+    (2^-11 of a value over the square root of 3), which adds in squares: 1.016."""
+    cache, _, g = make([2000, 1500], heads=3, dim=dim, block=32, dtype=dtype, room=T)
+    x = torch.randn(2, 2, 3, T, dim, generator=g).cuda()
+    ops.kv8_append(cache, x[0], x[1])
+    q = torch.randn(2, 3 * group, T, dim, generator=g).to(kind).cuda()
+    out = ops.kv8_attention(q, cache)
+    count = torch.full((2,), T, dtype=torch.int32, device="cuda")
+    k, v = ops.kv8_read(cache, 2000 + T, counts=count)
+    off = own = 0.0
+    for b, have in enumerate((2000, 1500)):
+        pos = torch.arange(2000 + T, device="cuda")
+        hidden = pos > have + torch.arange(T, device="cuda")[:, None]
+        s = q[b].double().view(3, group, T, dim) @ k[b].double().transpose(1, 2)[:, None]
+        p = torch.softmax((s * dim ** -0.5).masked_fill(hidden, -math.inf), -1)
+        want = (p @ v[b].double()[:, None]).view(3 * group, T, dim)
+        off += float((out[b].double() - want).square().sum())
+        own += float((want.to(kind).double() - want).square().sum())
+    assert math.sqrt(off / own) <= 1.03
+    clean()
+
+
 def test_scores_that_grow_along_the_cache():
     """Each page's scores exceed the last one's by far, then fall: the running
     reference moves often, and early weights vanish against late ones."""
