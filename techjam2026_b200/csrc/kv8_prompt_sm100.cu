@@ -68,8 +68,9 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
 
 // What the lanes' bounded waits say, for the whole warp: its lanes leave a loop
 // together or not at all, since the code after a wait is warp-wide. (The softmax
-// warps, which wait in step as one instruction stream on the same barrier, flag and
-// clock, go without the vote: it cost 10 % at head_dim 64.)
+// warps go without the vote, which cost 10 % at head_dim 64: a lane whose wait has
+// failed stays in the loop to its last step, without further waits or arrivals, and
+// writes nothing, which costs 1 to 2 %.)
 __device__ __forceinline__ bool warp_all(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 // ---------------------------------------------------------------- q planes
@@ -786,6 +787,9 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
     const uint32_t t_m = t_row + Cfg::M_COL + t * Cfg::O_STRIDE;
     float ref = -INFINITY, sum = 0.f;
     bool ok = true, nan_k = false, nan_v = false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (ok) ok = mbar_wait(bar, parity, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX);
+    };
     auto scale_cols = [&](uint32_t at, float alpha) {
 #pragma unroll 1
       for (int cc = 0; cc < Cfg::O_STRIDE / 16; ++cc) {
@@ -803,25 +807,23 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
       const int buf = NT == 1 ? st : t;
       const uint32_t t_s = t_row + buf * 128;
       const uint32_t sph = NT == 1 ? (j >> 1) & 1 : j & 1;
-      if (!mbar_wait(&k_full[st], (j >> 1) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX) ||
-          !mbar_wait(&s_full[buf], sph, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX)) {
-        ok = false;
-        break;
-      }
+      wait(&k_full[st], (j >> 1) & 1);
+      wait(&s_full[buf], sph);
+      __syncwarp();
       tc_fence_after();
-      if (lane == 0) mbar_arrive(&k_empty[st]);
+      if (lane == 0 && ok) mbar_arrive(&k_empty[st]);
       // In place with two tiles, S of this step was issued after P V of the last
       // one, so O is at rest. Otherwise S runs ahead: wait for that product.
-      auto at_rest = [&]() -> bool {
-        if (NT == 2 && !Cfg::SEP) return true;
-        ok = mbar_wait(&o_done[t], (j - 1) & 1, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX);
+      auto at_rest = [&]() {
+        if (NT == 2 && !Cfg::SEP) return;
+        wait(&o_done[t], (j - 1) & 1);
+        __syncwarp();
         tc_fence_after();
-        return ok;
       };
       const bool flush = QP == 2 && j > 0 && j % Cfg::FLUSH == 0;
       const bool have_m = QP == 2 && j >= Cfg::FLUSH;  // M holds something
       if (flush) {
-        if (!at_rest()) break;
+        at_rest();
 #pragma unroll
         for (int cc = 0; cc < Cfg::O_STRIDE / 16; ++cc) {
           uint32_t o[16], m[16];
@@ -841,7 +843,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
       if (Cfg::SEP) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t]);
+        if (lane == 0 && ok) mbar_arrive(&s_free[t]);
       }
       const PromptScales& sc = s_sc[j & 3];
       const int lim = min(limit, k1) - (k0 + j * BN);
@@ -879,8 +881,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
         sum *= alpha;
       }
       const bool rescale = j > 0 && __any_sync(0xffffffffu, move);
-      if (Cfg::SEP ? j > 0 : rescale)
-        if (!at_rest()) break;       // (P apart: its columns are free then, too)
+      if (Cfg::SEP ? j > 0 : rescale) at_rest();  // (P apart: its columns are free then, too)
       if (rescale) {
         if (!flush) scale_cols(t_o, alpha);
         if (have_m) scale_cols(t_m, alpha);
@@ -917,9 +918,10 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[buf]);
+      if (lane == 0 && ok) mbar_arrive(&p_full[buf]);
     }
-    if (ok && warp_all(mbar_wait(&o_final[t], 0, abort_flag, KF_DEV_WAIT_TIMEOUT_SOFTMAX))) {
+    wait(&o_final[t], 0);
+    if (__any_sync(0xffffffffu, ok)) {
       tc_fence_after();
       const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
       const int hq = h * G + row - tok * G;
@@ -938,7 +940,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
 #pragma unroll
           for (int u = 0; u < 32; ++u) o[u] += m[u];
         }
-        if (row >= w.rows) continue;
+        if (row >= w.rows || !ok) continue;
 #pragma unroll
         for (int u = 0; u < 32; ++u) o[u] = sum == 0.f ? 0.f : o[u] * f;
         constexpr int NC = DH < 32 ? DH : 32;
@@ -951,7 +953,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
             p[u >> 2] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
         }
       }
-      if (row < w.rows) {
+      if (row < w.rows && ok) {
         if (alone) {
           const float l2 = sum == 0.f ? -INFINITY : ref + log2f(sum);
           if (lse_out)

@@ -583,6 +583,41 @@ def test_a_step_in_a_graph_and_on_another_stream():
     assert torch.equal(a.weight.nan_to_num(-1), b.weight.nan_to_num(-1))
 
 
+@pytest.mark.parametrize("track", [False])
+@pytest.mark.parametrize("kind,dim", [(BF16, 64), (BF16, 32), (F16, 64), (BF16, 128), (F32, 64),
+                                      (F32, 128)])
+def test_waits_that_run_out_end_the_call_and_the_next_is_right(kind, dim, track):
+    """Under a limit of one cycle the waits of the prompt kernels give up where
+    what they wait for is not there at once (which at head_dim <= 64 and bf16
+    it never is: products are issued as their inputs come). Every role leaves,
+    the call returns, the status word tells, the next call is as before."""
+    L = _lib.lib()
+    cache, _, g = make([700, 90], heads=2, dim=dim, block=32, dtype=F8, weight=True, room=200)
+    x = torch.randn(2, 2, 200, dim, generator=g).cuda()
+    ops.kv8_append(cache, x, x)
+    q = torch.randn(2, 4, 200, dim, generator=g).to(kind).cuda()
+    cache.weight.zero_()
+    good = ops.kv8_attention(q, cache, track=track)
+    weight = cache.weight.clone()
+    clean()
+    _lib.check(L.kf_set_wait_limit(1), "kf_set_wait_limit")
+    try:
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        ops.kv8_attention(q, cache, track=track)
+        end.record()
+        torch.cuda.synchronize()
+        status = L.kf_device_status(1)
+    finally:
+        L.kf_set_wait_limit(0)
+    assert begin.elapsed_time(end) < 1000
+    assert status in ((1, 2, 4) if kind == BF16 and dim <= 64 else (0, 1, 2, 4))
+    cache.weight.zero_()
+    assert torch.equal(ops.kv8_attention(q, cache, track=track), good)
+    assert torch.equal(cache.weight, weight)
+    clean()
+
+
 # ---------------------------------------------------------------- evict
 
 
