@@ -1111,7 +1111,8 @@ __global__ void __launch_bounds__(WeighCfg<DH, QP>::THREADS)
       }
       mbar_arrive(&r_full[st]);
     }
-    if (lane == 0 && *abort_flag)
+    // No copy may be in flight when the CTA leaves, whatever role gives up later.
+    if (lane == 0)
       for (int j = issued > 2 ? issued - 2 : 0; j < issued; ++j)
         mbar_wait_drain(&q_full[j & 1], (j >> 1) & 1, KF_DEV_WAIT_TIMEOUT_TMA);
   } else if (warp == 8) {

@@ -583,7 +583,7 @@ def test_a_step_in_a_graph_and_on_another_stream():
     assert torch.equal(a.weight.nan_to_num(-1), b.weight.nan_to_num(-1))
 
 
-@pytest.mark.parametrize("track", [False])
+@pytest.mark.parametrize("track", [False, True])
 @pytest.mark.parametrize("kind,dim", [(BF16, 64), (BF16, 32), (F16, 64), (BF16, 128), (F32, 64),
                                       (F32, 128)])
 def test_waits_that_run_out_end_the_call_and_the_next_is_right(kind, dim, track):
