@@ -19,6 +19,7 @@ reference recomputes the sequence (kernelforge/optimized.py:397-458).
 """
 from __future__ import annotations
 
+import itertools
 from typing import List, Optional, Sequence
 
 import torch
@@ -46,17 +47,16 @@ class PagePool:
         return [self.free.pop() for _ in range(n)]
 
     def reserve(self, tokens: Sequence[int]) -> None:
-        """Pages for sequences of these lengths."""
+        """Pages for sequences of these lengths: for all of them, or an error
+        and nothing changed."""
         if max(tokens) > self.table.shape[1] * self.block:
             raise RuntimeError(f"PagePool: a sequence of {max(tokens)} tokens does not fit "
                                f"{self.table.shape[1]} pages of {self.block}")
-        grown = False
-        for row, n in zip(self.rows, tokens):
-            more = -(-n // self.block) - len(row)
-            if more > 0:
-                row.extend(self.take(more))
-                grown = True
-        if grown:
+        more = [max(0, -(-n // self.block) - len(row)) for row, n in zip(self.rows, tokens)]
+        if any(more):
+            pages = iter(self.take(sum(more)))
+            for row, n in zip(self.rows, more):
+                row.extend(itertools.islice(pages, n))
             self._upload()
 
     def replace(self, rows: List[List[int]]) -> None:

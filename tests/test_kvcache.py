@@ -28,3 +28,19 @@ def test_a_full_pool_and_a_long_sequence_are_refused():
         pool.reserve([0, 49])
     with pytest.raises(RuntimeError):
         pool.reserve([33, 17])
+
+
+def test_a_refused_reservation_changes_nothing():
+    """The first sequence's pages are there, the second one's are not: neither
+    gets any, and a later reservation that fits is on the table."""
+    pool = PagePool(pages=3, batch=2, blocks=3, block=16, device="cpu")
+    pool.table.fill_(-1)
+    with pytest.raises(RuntimeError):
+        pool.reserve([33, 17])
+    assert pool.rows == [[], []] and len(pool.free) == 3
+    pool.reserve([33, 0])
+    assert sorted(pool.rows[0]) == [0, 1, 2] and pool.rows[1] == []
+    assert pool.table[0].tolist() == pool.rows[0]
+    with pytest.raises(RuntimeError):
+        pool.reserve([33, 1])
+    assert pool.rows[1] == [] and pool.table[0].tolist() == pool.rows[0]
