@@ -5,8 +5,8 @@ every earlier token. `CachedStack` keeps each layer's K and V in an 8-bit cache
 (`ops.KV8Cache`) and runs only the new tokens: a prompt in chunks of any
 length, then one token at a time, each sequence of the batch at its own length.
 With a `budget` it records the attention weight every cached token receives
-and, when a sequence outgrows the budget, cuts every head to its most recent
-and its heaviest tokens.
+and, when a sequence outgrows the budget, cuts its heads to their most recent
+and their heaviest tokens.
 
     model = CachedStack(stack, batch=8, max_tokens=2048)
     out = model(prompt, counts=lengths)      # [B, T, d], ragged prompts
@@ -59,11 +59,12 @@ class PagePool:
                 row.extend(itertools.islice(pages, n))
             self._upload()
 
-    def replace(self, rows: List[List[int]]) -> None:
-        """New pages for every sequence; the old ones are free."""
-        for old in self.rows:
-            self.free.extend(old)
-        self.rows = rows
+    def replace(self, rows: List[List[int]], which: Optional[Sequence[int]] = None) -> None:
+        """New pages for every sequence, or for those in `which`; the old ones
+        are free."""
+        for i, row in zip(range(len(self.rows)) if which is None else which, rows):
+            self.free.extend(self.rows[i])
+            self.rows[i] = row
         self._upload()
 
     def _upload(self) -> None:
@@ -79,24 +80,36 @@ class CachedStack:
     max_tokens  longest sequence a cache row holds
     code        torch.int8 or torch.float8_e4m3fn
     block       tokens that share a scale (a page)
-    budget      None, or the tokens each head keeps once a sequence exceeds it
-                (by at most one chunk); `recent` of them are the latest"""
+    budget      None, or the most tokens a sequence holds between calls. One
+                that has outgrown it is cut to budget - slack tokens, of which
+                `recent` (or all, if that is more) are the latest
+    slack       how far below the budget a cut goes, so that a sequence that is
+                generated token by token is cut once in so many tokens: default
+                a page, at most a quarter of the budget. A cut rounds the kept
+                tokens again under the scales of their new pages: over 256
+                tokens past a budget of 256, K and V went from 0.8 to 1.1 %
+                off what was appended (int8), from 2.6 to 3.1 % (e4m3)"""
 
     def __init__(self, model: LayerStack, batch: int, max_tokens: int,
                  code: torch.dtype = torch.int8, block: int = 64, budget: Optional[int] = None,
-                 recent: int = 0, device="cuda"):
+                 recent: int = 0, device="cuda", slack: Optional[int] = None):
         cfg = model.config
         if not cfg.causal:
             raise ValueError("CachedStack: only a causal stack can be extended token by token")
         if budget is not None and not (0 < budget <= max_tokens and 0 <= recent <= budget):
             raise ValueError("CachedStack: needs 0 <= recent <= budget <= max_tokens, budget > 0")
+        if slack is not None and (budget is None or not 0 <= slack < budget):
+            raise ValueError("CachedStack: needs a budget and 0 <= slack < budget")
         self.heads, self.head_dim = cfg.num_heads, cfg.d_model // cfg.num_heads
-        self.budget, self.recent = budget, recent
+        self.budget = budget
+        if budget is not None:
+            self.keep = budget - (min(block, budget // 4) if slack is None else slack)
+            self.recent = min(recent, self.keep)
         device = torch.device(device, torch.cuda.current_device()) \
             if torch.device(device).index is None else torch.device(device)
         blocks = -(-max_tokens // block)
         # an eviction writes the kept tokens before the old pages are free
-        spare = -(-budget // block) if budget is not None else 0
+        spare = -(-self.keep // block) if budget is not None else 0
         pages = batch * (blocks + spare)
         self.pool = PagePool(pages, batch, blocks, block, device)
         self.held = [0] * batch
@@ -153,23 +166,26 @@ class CachedStack:
         _, out = add_mask_layernorm(res, y, keep, *self.final, mask_out=True)
         self.lens += new
         self.held = [a + n for a, n in zip(self.held, counts)]
-        if self.budget is not None and max(self.held) > self.budget:
-            self._evict()
+        if self.budget is not None:
+            self._evict([i for i, n in enumerate(self.held) if n > self.budget])
         return out.view(B, T, d)
 
-    def _evict(self) -> None:
-        held = [min(n, self.budget) for n in self.held]
-        block = self.pool.block
-        rows = [self.pool.take(-(-n // block)) for n in held]
-        table = torch.zeros((len(held), -(-self.budget // block)), dtype=torch.int32)
-        for i, row in enumerate(rows):
-            table[i, :len(row)] = torch.tensor(row, dtype=torch.int32)
-        table = table.to(self.lens.device)
+    def _evict(self, which: List[int]) -> None:
+        """Cuts the sequences in `which`; the others stay where they are."""
+        if not which:
+            return
+        n = -(-self.keep // self.pool.block)
+        pages = self.pool.take(n * len(which))
+        rows = [pages[i * n:(i + 1) * n] for i in range(len(which))]
+        table = torch.tensor(rows, dtype=torch.int32, device=self.lens.device)
+        at = torch.tensor(which, device=self.lens.device)
+        old, lens = self.pool.table[at], self.lens[at]
         for cache in self.caches:
-            _, new = kv8_evict(cache, table, self.budget, self.recent)
-        self.lens.copy_(new.lens)
-        self.held = held
-        self.pool.replace(rows)
+            _, new = kv8_evict(cache.with_table(old, lens), table, self.keep, self.recent)
+        self.lens.index_copy_(0, at, new.lens)
+        for i in which:
+            self.held[i] = self.keep
+        self.pool.replace(rows, which)
 
 
 def main() -> None:

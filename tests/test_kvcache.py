@@ -44,3 +44,15 @@ def test_a_refused_reservation_changes_nothing():
     with pytest.raises(RuntimeError):
         pool.reserve([33, 1])
     assert pool.rows[1] == [] and pool.table[0].tolist() == pool.rows[0]
+
+
+def test_pages_of_some_sequences_are_replaced():
+    pool = PagePool(pages=9, batch=3, blocks=3, block=16, device="cpu")
+    pool.reserve([40, 20, 33])
+    before = [list(r) for r in pool.rows]
+    rows = [pool.take(1)]
+    pool.replace(rows, [1])
+    assert pool.rows == [before[0], rows[0], before[2]]
+    assert sorted(pool.free) == sorted(before[1])
+    assert pool.table[0].tolist() == before[0] and pool.table[2].tolist() == before[2]
+    assert pool.table[1, 0] == rows[0][0]

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import oracle
+from techjam2026_b200 import ops
 from techjam2026_b200.configs import TransformerConfig, make_state_dict
 from techjam2026_b200.kvcache import CachedStack
 from techjam2026_b200.model import LayerStack
@@ -75,6 +76,56 @@ def test_a_budget_bounds_the_cache_and_keeps_the_outputs_near():
     assert rel(got, want) < 0.15 and torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("code,step", [(torch.int8, 0.011), (torch.float8_e4m3fn, 0.035)])
+def test_tokens_past_a_budget_are_evicted_by_the_page_and_keep_their_values(code, step, monkeypatch):
+    """200 tokens one by one past a budget of 96 in pages of 16: a sequence is
+    cut once a page, only it is moved, and what it still holds is near what was
+    appended. A cut rounds anew, independently of the rounding before at worst:
+    relative errors of one rounding (`step`) add in squares."""
+    from techjam2026_b200 import kvcache
+    stack, x, _ = setup(296, 128, 2, layers=1, B=2)
+    model = CachedStack(stack, 2, 128, code, block=16, budget=96, recent=16)
+    put, cut = kvcache.kv8_append, kvcache.kv8_evict
+    told = [[[], []] for _ in range(2)]          # K and V rows of each sequence, by position
+    cuts = []
+
+    def append(cache, k, v, counts):
+        for b, n in enumerate(counts.tolist()):
+            for i in range(n):
+                told[b][0].append(k[b, :, i].clone())
+                told[b][1].append(v[b, :, i].clone())
+        put(cache, k, v, counts=counts)
+
+    def evict(cache, table, budget, recent):
+        kept, new = cut(cache, table, budget, recent)
+        assert kept.shape[0] == 1                # the other sequence is within its budget
+        for which in (0, 1):
+            rows = torch.stack(told[0][which], 1)                     # [H, L, D]
+            at = kept[0].long()[..., None].expand(-1, -1, rows.shape[2])
+            told[0][which] = list(torch.gather(rows, 1, at).unbind(1))
+        cuts.append(budget)
+        return kept, new
+
+    monkeypatch.setattr(kvcache, "kv8_append", append)
+    monkeypatch.setattr(kvcache, "kv8_evict", evict)
+    model(x[:, :96].cuda(), counts=[96, 40])
+    other = list(model.pool.rows[1])
+    for i in range(96, 296):
+        model(x[:, i:i + 1].cuda(), counts=[1, 0])
+        assert max(model.held) <= 96 and model.lens.tolist() == model.held
+    assert cuts == [80] * 12                     # at 97, then every 17 tokens
+    assert model.pool.rows[1] == other and model.held[1] == 40
+    used = [p for r in model.pool.rows for p in r]
+    assert len(used) == len(set(used)) and not set(used) & set(model.pool.free)
+    k, v = ops.kv8_read(model.caches[0], 96)
+    for b, n in enumerate(model.held):
+        for which, got in ((0, k), (1, v)):
+            want = torch.stack(told[b][which], 1)
+            assert want.shape[1] == n
+            bound = step * (1 + (len(cuts) if b == 0 else 0)) ** 0.5
+            assert rel(got[b, :, :n], want.cpu()) < bound, (b, which)
+
+
 def test_refusals():
     stack, x, _ = setup(16, 64, 4, layers=1)
     with pytest.raises(ValueError):
@@ -90,3 +141,12 @@ def test_refusals():
     cfg = TransformerConfig(1, 8, 64, 4, 64, 1, False)
     with pytest.raises(ValueError):
         CachedStack(LayerStack(cfg), 1, 8)
+
+
+def test_a_slack_needs_a_budget_above_it():
+    stack, _, _ = setup(16, 64, 4, layers=1)
+    for slack, budget in ((4, None), (-1, 16), (16, 16)):
+        with pytest.raises(ValueError):
+            CachedStack(stack, 3, 16, budget=budget, slack=slack)
+    assert CachedStack(stack, 3, 64, block=16, budget=32, recent=32).keep == 24
+    assert CachedStack(stack, 3, 64, block=16, budget=32, slack=0).keep == 32
