@@ -108,6 +108,8 @@ class CachedStack:
         device = torch.device(device, torch.cuda.current_device()) \
             if torch.device(device).index is None else torch.device(device)
         blocks = -(-max_tokens // block)
+        if budget is not None and self.keep >= blocks * block:
+            raise ValueError("CachedStack: a budget that fills the rows needs a slack")
         # an eviction writes the kept tokens before the old pages are free
         spare = -(-self.keep // block) if budget is not None else 0
         pages = batch * (blocks + spare)
@@ -145,6 +147,12 @@ class CachedStack:
             raise ValueError(f"CachedStack: counts must be {B} numbers from 0 to {T}")
         if T == 0:
             return x
+        if self.budget is not None:
+            # a full row makes room first, if that is enough for every sequence
+            reach = self.pool.table.shape[1] * self.pool.block
+            full = [i for i, n in enumerate(counts) if self.held[i] + n > reach]
+            if all(min(self.held[i], self.keep) + counts[i] <= reach for i in full):
+                self._evict(full)
         self.pool.reserve([a + n for a, n in zip(self.held, counts)])
         new = torch.tensor(counts, dtype=torch.int32, device=x.device)
         keep = None

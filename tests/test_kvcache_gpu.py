@@ -150,3 +150,23 @@ def test_a_slack_needs_a_budget_above_it():
             CachedStack(stack, 3, 16, budget=budget, slack=slack)
     assert CachedStack(stack, 3, 64, block=16, budget=32, recent=32).keep == 24
     assert CachedStack(stack, 3, 64, block=16, budget=32, slack=0).keep == 32
+
+
+@pytest.mark.parametrize("recent", [8, 32])
+def test_a_budget_that_fills_the_rows_is_served_past(recent):
+    """budget == max_tokens, a multiple of the page: the token that finds no
+    room cuts its sequence first. A chunk that fits in no case is refused and
+    cuts nothing."""
+    stack, x, _ = setup(80, 64, 4, layers=2, B=2)
+    model = CachedStack(stack, 2, 32, block=16, budget=32, recent=recent)
+    model(x[:, :32].cuda(), counts=[32, 5])
+    for i in range(32, 80):
+        out = model(x[:, i:i + 1].cuda(), counts=[1, 0])
+        assert torch.isfinite(out).all() and out[0].any()
+        assert model.lens.tolist() == model.held and max(model.held) <= 32 and model.held[1] == 5
+    held = list(model.held)
+    with pytest.raises(RuntimeError):
+        model(x[:, :30].cuda(), counts=[30, 0])
+    assert model.held == held and model.lens.tolist() == held
+    with pytest.raises(ValueError):
+        CachedStack(stack, 2, 32, block=16, budget=32, slack=0)
