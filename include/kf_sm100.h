@@ -413,7 +413,11 @@ int kf_kv8_read(const kf_kv8_cache* cache, const int32_t* start, const int32_t* 
  * counts[b] known to the caller (0: the table's reach); longer sequences are
  * cut there and recorded in the device status. `workspace`: at least
  * kf_kv8_attention_workspace_bytes of the same arguments, 256-byte aligned;
- * calls that overlap on the GPU must not share it. */
+ * calls that overlap on the GPU must not share it. With KF_KV8_TRACK and up to
+ * 64 query rows a kv head it holds their scores, 4 * batch * q_heads * T *
+ * max_len bytes (up to 4 GB; beyond, and from 17 rows on beyond 512 MB, the
+ * scores are computed twice): pass max_len where the table reaches far beyond
+ * the sequences. */
 int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_t q_sb, int64_t q_sh,
                      int64_t q_st, void* out, int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype,
                      const int32_t* counts, int64_t T, int64_t q_heads, int64_t max_len,

@@ -9,12 +9,16 @@ namespace kf {
 // rows 106 / 134, 64 rows 145 / 137, 96 rows 194 / 142; 16 x 12 heads of 64 over 1k, fp32: 64 rows
 // 47 / 78, 128 rows 83 / 78; 8 heads of 64 over 16k, bf16: 64 rows 32 / 46, 128
 // rows 49 / 49. With weights the split kernel keeps every score for the last
-// pass; where that takes too much memory, 17 rows and more go to the other
-// kernel, which computes the scores again.
+// pass; where that takes too much memory (512 MB for 17 rows and more, 4 GB for
+// fewer), the call goes to the other kernel, which computes the scores again.
+// Few rows gain from the scores as long as they can: one token of 64 sequences of
+// 4096, 8 kv heads of 128, 8 rows each, takes 331 us with 2.1 GB of scores (a
+// table that reaches 131k tokens), 3625 without, and 165 us, either way, when
+// max_len tells the sequences' length.
 static bool kv8_is_prompt(const KV8& c, int64_t rows, int64_t max_len, int flags) {
   if (rows > KV8_SPLIT_ROWS) return true;
   const int64_t scores = static_cast<int64_t>(c.B) * c.H * rows * max_len * 4;
-  return (flags & KF_KV8_TRACK) && rows > KV8_ROWS && scores > (512LL << 20);
+  return (flags & KF_KV8_TRACK) && scores > (rows > KV8_ROWS ? 512LL << 20 : 4LL << 30);
 }
 
 // How a call is cut: chunks of keys so that there are a few CTAs per SM, each

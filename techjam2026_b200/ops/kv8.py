@@ -255,7 +255,9 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, counts: Optional[torch.Tenso
     track     add to cache.weight each key's weight, summed over the queries
               and over the heads that read it
     max_len   an upper bound of lens + counts known to the caller (0: what the
-              table can hold); a smaller one saves work
+              table can hold); a smaller one saves work and, with track,
+              workspace (4 * B * heads * T * max_len bytes up to 64 query rows
+              of a kv head, at most 4 GB)
 
     Returns out [B, heads, T, head_dim] of q's type (with return_lse also the
     float32 log of each softmax's sum [B, heads, T]). Rows that see no key, and

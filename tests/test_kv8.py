@@ -104,6 +104,19 @@ def test_workspace_grows_with_the_work(lib):
     assert size(long, flags=_lib.KF_KV8_TRACK) > size(long)
 
 
+@pytest.mark.parametrize("T,heads", [(1, 8), (1, 64), (2, 64), (4, 64), (8, 64), (64, 64)])
+@pytest.mark.parametrize("blocks", [128, 2048, 16384])
+def test_recorded_weights_take_a_bounded_workspace(lib, blocks, T, heads):
+    """A table may reach far beyond what its sequences hold: 64 sequences, 8 kv
+    heads of 128, up to a million tokens a row. Scores that are kept for the last
+    pass stay within 4 GiB; parts and planes are under half a gigabyte."""
+    c = cache(blocks=blocks, ld_table=blocks, block=64, batch=64, kv_heads=8, head_dim=128,
+              pages=1 << 20)
+    for dtype in (0, 1):
+        need = lib.kf_kv8_attention_workspace_bytes(c, dtype, T, heads, 0, _lib.KF_KV8_TRACK)
+        assert 0 <= need <= 9 << 29
+
+
 def test_python_refuses_what_is_no_cache():
     k = torch.zeros(3, 2, 16, 64, dtype=torch.int8)
     scale, lens = torch.zeros(3, 2, 2), torch.zeros(1, dtype=torch.int32)

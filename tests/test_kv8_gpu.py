@@ -438,6 +438,23 @@ def test_strided_views_offsets_and_out():
             assert got.data_ptr() == out.data_ptr()
 
 
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_few_rows_under_a_table_of_a_million_tokens(kind):
+    """16 rows of a kv head with weights recorded: kept scores would take 8 GB,
+    so the kernel for many rows serves the call; with max_len the other one."""
+    table = torch.zeros(16, 1 << 14, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(1, 17, device="cuda")
+    g = torch.Generator().manual_seed(2)
+    lens = torch.randint(0, 40, (16,), generator=g).int().cuda()
+    cache = ops.KV8Cache.empty(17, 8, 64, 64, table, torch.zeros_like(lens), I8, weight=True)
+    x = torch.randn(2, 16, 8, 40, 64, generator=g).cuda()
+    ops.kv8_append(cache, x[0], x[1], counts=lens + 1)
+    cache.lens.copy_(lens)
+    q = torch.randn(16, 128, 1, 64, generator=g).to(kind).cuda()
+    attend(cache, q, None, track=True)
+    attend(cache, q, None, track=True, max_len=64)
+
+
 def test_max_len_cuts_the_work_not_the_result():
     cache, _, g = make([100, 37], heads=2, dim=64, block=16, room=4000)
     x = torch.randn(2, 2, 1, 64, generator=g).cuda()
