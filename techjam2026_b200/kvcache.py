@@ -26,6 +26,7 @@ import torch
 
 from .model import LayerStack
 from .ops import (KV8Cache, add_mask_layernorm, kv8_append, kv8_attention, kv8_evict, linear)
+from .ops.kv8 import HEAD_DIMS
 
 
 class PagePool:
@@ -196,18 +197,23 @@ class CachedStack:
         self.pool.replace(rows, which)
 
 
-def main() -> None:
+def main(argv: Optional[Sequence[str]] = None) -> None:
     import argparse
 
     from .configs import WORKLOADS, init_params_
     from .fused import FusedTransformer
 
     ap = argparse.ArgumentParser(description="prompt, then single tokens, over an 8-bit cache")
-    ap.add_argument("--config", default="c2", choices=sorted(WORKLOADS))
+    ap.add_argument("--config", default="c2", choices=sorted(
+        name for name, w in WORKLOADS.items()
+        if w.cfg.causal and w.cfg.d_model // w.cfg.num_heads in HEAD_DIMS))
     ap.add_argument("--tokens", type=int, default=16, help="single tokens after the prompt")
     ap.add_argument("--code", default="int8", choices=("int8", "float8_e4m3fn"))
-    a = ap.parse_args()
+    a = ap.parse_args(argv)
     cfg = WORKLOADS[a.config].cfg
+    if not 0 < a.tokens < cfg.seq_len:
+        ap.error(f"--tokens must be from 1 to {cfg.seq_len - 1}")
+    warm = min(2, a.tokens - 1)      # single tokens before the timed ones
     stack = init_params_(LayerStack(cfg), 0)
     x = torch.randn(cfg.batch_size, cfg.seq_len, cfg.d_model,
                     generator=torch.Generator().manual_seed(1)).cuda()
@@ -218,17 +224,15 @@ def main() -> None:
     n = cfg.seq_len - a.tokens
     begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
     outs = [model(x[:, :n])]
-    timed = 0
     for i in range(n, cfg.seq_len):
-        if i == n + 2:
+        if i == n + warm:
             begin.record()
         outs.append(model(x[:, i:i + 1]))
-        timed += i >= n + 2
     end.record()
     got = torch.cat(outs, 1)
     torch.cuda.synchronize()
     rel = float((got - want).norm() / want.norm())
-    ms = begin.elapsed_time(end) / max(1, timed)
+    ms = begin.elapsed_time(end) / (a.tokens - warm)
     print(f"{a.config}: {n} prompt tokens and {a.tokens} single ones of {cfg.batch_size} sequences, "
           f"{a.code} cache: relative difference from the whole-sequence forward {rel:.2e}, "
           f"{ms:.3f} ms a token")

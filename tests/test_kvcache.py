@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import pytest
 
-from techjam2026_b200.kvcache import PagePool
+from techjam2026_b200.kvcache import PagePool, main
 
 
 def test_pages_are_handed_out_once_and_come_back():
@@ -56,3 +56,15 @@ def test_pages_of_some_sequences_are_replaced():
     assert sorted(pool.free) == sorted(before[1])
     assert pool.table[0].tolist() == before[0] and pool.table[2].tolist() == before[2]
     assert pool.table[1, 0] == rows[0][0]
+
+
+@pytest.mark.parametrize("argv", [["--config", "c3a"], ["--config", "c3b"], ["--tokens", "0"],
+                                  ["--config", "c1", "--tokens", "64"]])
+def test_the_example_refuses_what_it_cannot_run(argv, capsys):
+    """Heads of 8 and 256, no single token, no prompt: a usage error, not a
+    traceback from inside the cache."""
+    with pytest.raises(SystemExit) as told:
+        main(argv)
+    assert told.value.code == 2
+    said = capsys.readouterr().err
+    assert argv[-2] in said and "usage" in said

@@ -10,7 +10,7 @@ import torch
 import oracle
 from techjam2026_b200 import ops
 from techjam2026_b200.configs import TransformerConfig, make_state_dict
-from techjam2026_b200.kvcache import CachedStack
+from techjam2026_b200.kvcache import CachedStack, main
 from techjam2026_b200.model import LayerStack
 
 pytestmark = pytest.mark.gpu
@@ -170,3 +170,11 @@ def test_a_budget_that_fills_the_rows_is_served_past(recent):
     assert model.held == held and model.lens.tolist() == held
     with pytest.raises(ValueError):
         CachedStack(stack, 2, 32, block=16, budget=32, slack=0)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 5])
+def test_the_example_runs(tokens, capsys):
+    main(["--config", "c1", "--tokens", str(tokens)])
+    said = capsys.readouterr().out
+    assert f"{tokens} single ones" in said and "ms a token" in said
+    assert float(said.split("forward ")[1].split(",")[0]) < 0.02
