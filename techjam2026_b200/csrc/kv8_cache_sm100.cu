@@ -503,8 +503,10 @@ static int log2_exact(int x) {
 
 // Checks a cache description; fills the device view.
 static int kv8_view(const char* what, const kf_kv8_cache* c, KV8* out) {
-  if (!c || !c->k || !c->v || !c->scale || !c->table || !c->lens || c->pages < 0 ||
-      c->batch < 0 || c->kv_heads <= 0 || c->blocks < 0 || c->ld_table < c->blocks) {
+  // (tensors without elements have no address)
+  if (!c || (c->pages && (!c->k || !c->v || !c->scale)) ||
+      (c->batch && ((c->blocks && !c->table) || !c->lens)) || c->pages < 0 || c->batch < 0 ||
+      c->kv_heads <= 0 || c->blocks < 0 || c->ld_table < c->blocks) {
     set_last_error("%s: invalid cache (null pointer, negative size or ld_table < blocks)", what);
     return KF_E_INVALID;
   }
@@ -647,18 +649,18 @@ extern "C" int kf_kv8_evict(const kf_kv8_cache* cache, const int32_t* table_out,
   KV8 c;
   int rc = kv8_view("kf_kv8_evict", cache, &c);
   if (rc) return rc;
-  if (!table_out || !kept || !lens_out || budget <= 0 || recent < 0 || recent > budget ||
+  if ((c.B && (!table_out || !kept || !lens_out)) || budget <= 0 || recent < 0 || recent > budget ||
       budget > INT32_MAX / 2 || ld_out * c.P < budget) {
     set_last_error("kf_kv8_evict: needs 0 <= recent <= budget, budget > 0 and a table_out that "
                    "holds budget tokens (budget %lld, recent %lld)",
                    (long long)budget, (long long)recent);
     return KF_E_INVALID;
   }
-  if (lens_out == c.lens) {
+  if (c.B && lens_out == c.lens) {
     set_last_error("kf_kv8_evict: lens_out must not be the cache's lens");
     return KF_E_INVALID;
   }
-  if (!c.weight) {
+  if (c.pages && !c.weight) {
     set_last_error("kf_kv8_evict: the cache keeps no weight record");
     return KF_E_INVALID;
   }

@@ -117,7 +117,7 @@ static int kv8_attention_check(const char* what, const kf_kv8_cache* cache, int 
     set_last_error("%s: needs T >= 0, q_heads a multiple of kv_heads and known flags", what);
     return KF_E_INVALID;
   }
-  if ((flags & KF_KV8_TRACK) && !c->weight) {
+  if ((flags & KF_KV8_TRACK) && c->pages && !c->weight) {
     set_last_error("%s: KF_KV8_TRACK needs a cache with a weight record", what);
     return KF_E_INVALID;
   }

@@ -92,6 +92,21 @@ def test_empty_calls_are_no_ops(lib):
     assert lib.kf_kv8_read(cache(), None, None, 0, FAKE, FAKE, 0, None) == 0
 
 
+def test_empty_tensors_have_no_address(lib):
+    """A batch, a table or a pool of size 0 comes with null pointers."""
+    none = cache(batch=0, table=None, lens=None)
+    assert append(lib, none, k=None) == 0
+    assert attention(lib, none, q=None) == 0
+    assert lib.kf_kv8_read(none, None, None, 1, None, None, 0, None) == 0
+    assert lib.kf_kv8_evict(none, None, 4, 8, 0, None, None, None) == 0
+    assert lib.kf_kv8_evict(none, None, 4, 8, 9, None, None, None) == _lib.KF_E_INVALID
+    pool = dict(pages=0, k=None, v=None, scale=None, weight=None)
+    for c in (cache(**pool), cache(blocks=0, ld_table=0, table=None)):
+        assert lib.kf_kv8_attention_workspace_bytes(c, 0, 1, 2, 0, 0) == 0
+        assert append(lib, c, T=0) == 0
+        assert append(lib, c, k=None) == _lib.KF_E_INVALID
+
+
 def test_workspace_grows_with_the_work(lib):
     size = lambda c, **kw: lib.kf_kv8_attention_workspace_bytes(   # noqa: E731
         c, 0, kw.get("T", 1), kw.get("heads", 2), kw.get("max_len", 0), kw.get("flags", 0))

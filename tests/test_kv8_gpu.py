@@ -541,6 +541,29 @@ def test_nothing_to_do():
     clean()
 
 
+@pytest.mark.parametrize("T", [1, 70])
+@pytest.mark.parametrize("batch,blocks,pages", [(0, 4, 8), (2, 0, 8), (2, 4, 0), (0, 0, 0)])
+def test_no_sequence_no_page_no_table(batch, blocks, pages, T):
+    table = torch.zeros(batch, blocks, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    cache = ops.KV8Cache.empty(pages, 2, 16, 64, table, lens, weight=True)
+    held = cache.k.clone()
+    x = torch.randn(batch, 2, T, 64, device="cuda")
+    none = torch.zeros_like(lens)
+    ops.kv8_append(cache, x, x, counts=none)
+    out, lse = ops.kv8_attention(x, cache, counts=none, track=True, return_lse=True)
+    assert out.shape == x.shape and not out.any() and torch.isinf(lse).all()
+    k, v = ops.kv8_read(cache, 5)
+    assert k.shape == (batch, 2, 5, 64) and not k.any() and not v.any()
+    kept, new = ops.kv8_evict(cache, torch.zeros(batch, 2, dtype=torch.int32, device="cuda"), 20)
+    assert kept.shape == (batch, 2, 20) and (kept == -1).all() and not new.lens.any()
+    clean()
+    ops.kv8_append(cache, x, x)                       # no place: recorded where there is a batch
+    ops.kv8_attention(x, cache)
+    assert _lib.lib().kf_device_status(1) == (6 if batch and not (blocks and pages) else 0)
+    assert torch.equal(cache.k, held)
+
+
 def test_repeated_calls_give_the_same_bits():
     cache, _, g = make([3000, 900], heads=2, dim=64, block=64, weight=True)
     for T in (1, 60):
