@@ -405,7 +405,11 @@ int kf_kv8_read(const kf_kv8_cache* cache, const int32_t* start, const int32_t* 
  * Scores, sums, maxima and the accumulators are fp32. q enters the products as
  * fp16 for 16-bit q and as two fp16 planes (22 bits) for fp32; the weights as
  * fp16 for bf16 q and as two planes for fp16 and fp32 q.
- * sm_scale must be finite and not negative.
+ * The weights enter relative to the largest V scale among the keys that a CTA
+ * takes (up to 4096, or a part of the sequence): an error of up to 2^-33 of the
+ * largest |V| among them remains, so a page whose V is below 2^-11 (fp32), 2^-22
+ * (fp16) of another's keeps fewer bits than its type. sm_scale must be finite and
+ * not negative.
  * out has q's type; rows without a visible key, and rows i >= counts[b], are 0
  * (lse -inf). lse (may be null) is fp32 [batch, q_heads, T]. With KF_KV8_TRACK
  * cache->weight[key] += the key's weight summed over the queries and the query

@@ -18,11 +18,13 @@
 // products would waste 7/8 of theirs here. RH = 1 serves at most 8 rows and
 // skips the softmax of the upper half of the tile; a second plane of q or of P
 // then takes that half, so one product does both.
-// Measured: 16 sequences of 16k to 32k tokens, 8 kv heads of 128, four query
-// heads each: 145 us for 805 MB, 5.6 TB/s (0.85 of the copy rate); a 65k
-// sequence of 16 heads of 64: 36 us for 134 MB, 3.7 TB/s, bound by
-// instructions (62 % of the issue slots: a head width of 64 converts, and pays
-// per 16 keys, as much for half the bytes). Rings of 4 slots and 5 or 6 CTAs an
+// Measured: 16 sequences of 24k tokens, 8 kv heads of 128, four query heads each,
+// bf16: 146 us for 787 MB with the join, 5.4 TB/s (0.82 of the copy rate; fp16 151,
+// fp32 157); a 65k sequence of 16 heads of 64, fp16: 36 us for 134 MB, 3.7 TB/s, and 6
+// to 9 for the join. There the schedulers issue in 65 % of the cycles from 3.5 warps
+// each; the stalls after that are fixed latencies and the math pipes, not loads: a
+// head width of 64 converts, and pays per 16 keys, as much for half the bytes.
+// Rings of 4 slots and 5 or 6 CTAs an
 // SM at head_dim 64 were 10 to 25 % slower: the registers they take away cost
 // more than their warps hide. (Codes loaded straight into registers, one group
 // ahead, left 8 warps an SM and 2.5 TB/s on the first case.)
@@ -34,8 +36,9 @@
 // loses precision only below 2^-23 of the largest weight. One plane of P is off
 // by 2.0e-4 of the output, which bf16's own rounding (1.65e-3) hides and fp16's
 // (2.07e-4) does not: fp16 and fp32 q have two. The V scale of a page is folded into P as the ratio
-// to the chunk's largest (<= 1, so P stays in range). The sum l adds the
-// unrounded fp32 weights.
+// to the chunk's largest (<= 1, so P stays in range; what is lost is below 2^-33 of
+// the chunk's largest value, whether or not the row sees it). The sum l adds
+// the unrounded fp32 weights.
 #include "kv8_common.cuh"
 
 namespace kf {

@@ -5,10 +5,13 @@
 namespace kf {
 
 // Which kernel serves a call of `rows` query rows per kv head. Measured (us,
-// split / tensor-memory kernel): 8 x 8 heads of 128 over 8k tokens, bf16: 48
-// rows 106 / 134, 64 rows 145 / 137, 96 rows 194 / 142; 16 x 12 heads of 64 over 1k, fp32: 64 rows
-// 47 / 78, 128 rows 83 / 78; 8 heads of 64 over 16k, bf16: 64 rows 32 / 46, 128
-// rows 49 / 49. With weights the split kernel keeps every score for the last
+// split / tensor-memory kernel, at 48, 64, 96 and 128 rows): 8 x 8 heads of 128 over
+// 8k tokens, bf16 107 / 138, 147 / 141, 196 / 146, 262 / 152, fp16 140 / 170, 176 / 173,
+// 236 / 178, 316 / 179, fp32 133 / 162, 190 / 163, 256 / 170, 354 / 161; 16 x 12 heads of
+// 64 over 1k, bf16 52 / 56, 41 / 56, 54 / 57, 72 / 56, fp32 60 / 81, 50 / 82, 65 / 83, 88 /
+// 82; 8 heads of 64 over 16k, bf16 27 / 47, 33 / 47, 42 / 50, 51 / 51. The two cross
+// between 48 and 64 rows at head_dim 128 and between 96 and 128 at 64; one
+// threshold serves both, so 65 to about 110 rows at 64 lose up to a fifth. With weights the split kernel keeps every score for the last
 // pass; where that takes too much memory (512 MB for 17 rows and more, 4 GB for
 // fewer), the call goes to the other kernel, which computes the scores again.
 // Few rows gain from the scores as long as they can: one token of 64 sequences of

@@ -27,13 +27,14 @@
 // tiles against 128 keys (the products 1024 at head_dim 64, 2048 at 128). A step
 // takes about 3600 clocks at head_dim 64: each softmax warp is busy for 3300 of
 // them, 1800 in its exponentials, where 128 scores of 168 registers leave one
-// warp little to overlap them with, and about 1000 in reading the row and its
-// maximum. At 128, P V and S of a tile run between its softmax passes.
+// warp little to overlap them with (40 to 80 bytes a thread spill), and about 1000
+// in reading the row and its maximum. The schedulers issue in 48 % of the cycles
+// there and in 31 % at 128, where P V and S of a tile run between its softmax passes.
 // Measured: a chunk of 1024 over 16k tokens, 2 sequences, 16 heads of 64, bf16:
-// 276 us for the whole call, 142 GFLOP (513 TFLOP/s); 4 prompts of 2048, 32 heads of
-// 128 on 8 kv heads: 273 us, 138 GFLOP (504 TFLOP/s, short rows: 8 steps a CTA);
-// fp32 q, a chunk of 700 over 3000, 3 x 16 heads of 128: 215 us for 58 GFLOP
-// (every product twice, one tile a CTA).
+// 274 us for the whole call, 139 GFLOP (505 TFLOP/s); fp16 500, fp32 498: P in the place
+// of S, and the second planes' products and conversions between the softmax
+// passes. 4 prompts of 2048, 32 heads of 128 on 8 kv heads: bf16 280 us, 138 GFLOP
+// (492 TFLOP/s, short rows: 8 steps a CTA), fp16 365, fp32 619 (one tile a CTA).
 //
 // Numbers as in the split kernel: q rows scaled by powers of two and P relative
 // to a lazily moved reference. bf16 q: one fp16 plane of each. fp16 q: two of P
@@ -44,7 +45,7 @@
 // kv8_prompt_weights_kernel: one CTA = 128 keys against all rows that see
 // them: S^T = K Q^T puts a key in each TMEM lane, so a thread adds its key's
 // weights in a register over every row, in a fixed order and without atomics.
-// Measured: 3 x 4 kv heads of 128, 2800 rows, 3000 tokens, fp32: 125 us.
+// Measured: 3 x 4 kv heads of 128, 2800 rows, 3700 tokens, fp32: 115 us, bf16 87.
 #include "kv8_common.cuh"
 
 namespace kf {
