@@ -261,7 +261,7 @@ struct SplitCfg {
   static constexpr int JOIN = 4 * KV8_ROWS * DH * 4;
   static constexpr int SMEM = RING > JOIN ? RING : JOIN;
   // CTAs an SM is to hold: what the rings (and, at 128, the registers) allow.
-  static constexpr int min_blocks(int planes) { return DH == 128 ? (planes == 1 ? 3 : 2) : 4; }
+  static constexpr int min_blocks(int q_planes) { return DH == 128 ? (q_planes == 1 ? 3 : 2) : 4; }
 };
 
 // Products of 16 q rows with 16 keys: d[n][.] in the m16n8 accumulator layout.
