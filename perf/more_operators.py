@@ -264,8 +264,8 @@ def run(state):
             return _held(state)
         return ops.kv8_attention_shared(
             state["q"], state["cache"], state["starts"], state["shared"], counts=state["counts"],
-            causal=case["causal"], max_len=case["shared_max"] + case["own_max"] + case["new"],
-            max_shared=case["shared_max"], return_lse=True)
+            causal=case["causal"], max_shared=case["shared_max"],
+            max_own=case["own_max"] + case["new"], return_lse=True)
     if case["kind"] == "copy":
         return _copy(state)
     return _attend(state) if case["kind"] == "attend" else _select(state)
