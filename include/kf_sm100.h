@@ -48,8 +48,9 @@ const char* kf_last_error(void);
  * of the first failure: 1-4 a bounded wait gave up (1 TMA producer, 2 MMA
  * issuer, 3 GEMM epilogue, 4 attention softmax), 5 an ordered attention
  * call got a batch_order entry outside [0, B), 6 an 8-bit cache call found a
- * length beyond its table or a page number outside its pool. `reset` != 0
- * clears it. */
+ * length beyond its table or a page number outside its pool (or was asked to
+ * copy into a page that another copy of the call names), 7 groups of sequences
+ * out of order. `reset` != 0 clears it. */
 int kf_device_status(int reset);
 
 /* The same status word copied into host_dst (pinned host memory, one int32)
@@ -440,6 +441,69 @@ int64_t kf_kv8_attention_workspace_bytes(const kf_kv8_cache* cache, int dtype, i
  * the kept positions in order, then -1. 0 <= recent <= budget, budget > 0. */
 int kf_kv8_evict(const kf_kv8_cache* cache, const int32_t* table_out, int64_t ld_out,
                  int64_t budget, int64_t recent, int32_t* kept, int32_t* lens_out, void* stream);
+
+/* kf_kv8_attention for a batch whose groups of consecutive sequences share
+ * their leading pages (samples of one prompt, beams, questions about one
+ * document): group n is the sequences starts[n] .. starts[n + 1] - 1 (n_groups
+ * + 1 ascending entries; a sequence in no group shares nothing), and the first
+ * shared[n] tokens of its sequences lie on pages that their table rows name
+ * alike (the first sequence's row is read). What counts is shared[n] cut to
+ * whole pages, to max_shared and to the shortest of the group's lens. Those
+ * tokens are read once for all rows of the group; the result is that of
+ * kf_kv8_attention, but for rounding. max_shared, max_own: upper bounds, known
+ * to the caller, of shared[n] and of the tokens that a sequence has besides
+ * (lens[b] + counts[b] less what counts of shared[n]); 0: the table's reach. A
+ * sequence that has more of its own is cut there and recorded in the device
+ * status. KF_KV8_TRACK is refused. n_groups = 0: kf_kv8_attention with
+ * max_len = max_own. At most 32767 groups. Other arguments as
+ * kf_kv8_attention. */
+int kf_kv8_attention_shared(const kf_kv8_cache* cache, const void* q, int64_t q_sb, int64_t q_sh,
+                            int64_t q_st, void* out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+                            int dtype, const int32_t* counts, int64_t T, int64_t q_heads,
+                            const int32_t* starts, const int32_t* shared, int64_t n_groups,
+                            int64_t max_shared, int64_t max_own, float sm_scale, int flags,
+                            float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t kf_kv8_attention_shared_workspace_bytes(const kf_kv8_cache* cache, int dtype, int64_t T,
+                                                int64_t q_heads, int64_t n_groups,
+                                                int64_t max_shared, int64_t max_own, int flags);
+
+/* Copies pages of a pool: page dst[i] of `into` (may be `from`) becomes page
+ * src[i] of `from`, i < n, for all kv heads: codes, scales and, where both keep
+ * one, the weight record. tokens (null: whole pages): only the first tokens[i]
+ * slots are copied, with the scales; the others stay as they are (tokens[i] <=
+ * 0: nothing is copied). `layers` caches of one geometry are copied in one
+ * call: from and into are arrays of that many. A pair src[i] == dst[i] within one
+ * pool is no copy. A pair is not done, and is recorded in the device status, if
+ * an entry is no page of its pool, or if its dst[i] is the dst of another pair
+ * or, within one pool, the src of another one (pairs that copy nothing do not
+ * count). `workspace`: kf_kv8_copy_workspace_bytes(...) bytes, 16-byte aligned (0
+ * for few pairs). Table and lens of the caches are not used. layers <= 256. */
+int kf_kv8_copy(const kf_kv8_cache* const* from, const kf_kv8_cache* const* into, int64_t layers,
+                const int32_t* src, const int32_t* dst, const int32_t* tokens, int64_t n,
+                void* workspace, int64_t workspace_bytes, void* stream);
+int64_t kf_kv8_copy_workspace_bytes(const kf_kv8_cache* from, const kf_kv8_cache* into, int64_t n);
+
+/* ----------------------------------------------------------- beam search */
+
+/* The best continuations of beams. Beam k of batch row b has the score
+ * scores[b, k] (fp32, its log probability so far) and logits[b, k, :] (fp32, bf16
+ * or fp16; strides in elements, unit stride along the vocabulary). Candidate
+ * (k, v) is
+ *     scores[b, k] + logits[b, k, v] - log(sum_w exp(logits[b, k, w]))
+ * with the logarithm's sum in fp32 and the rest in fp64. A beam with
+ * ended[b, k] != 0 (uint8, may be null) has one candidate: (k, pad) with its
+ * score unchanged. Per row the n largest candidates, largest first (of equal
+ * ones the lowest k * V + v): out_score fp32, out_beam and out_token int32
+ * [batch, n]. Candidates that are -inf or NaN are none (a logit of +inf or NaN
+ * makes its beam's candidates NaN); entries without a candidate get -inf, -1, -1. 1 <= n <= 128, beams <=
+ * 1024, vocab < 2^31. `workspace`: at least kf_beam_select_workspace_bytes bytes,
+ * 16-byte aligned; calls that overlap on the GPU must not share it. No
+ * reference counterpart. */
+int kf_beam_select(const void* logits, int64_t l_sb, int64_t l_sk, int dtype, const float* scores,
+                   int64_t s_sb, const uint8_t* ended, int64_t e_sb, int64_t batch, int64_t beams,
+                   int64_t vocab, int64_t n, int32_t pad, float* out_score, int32_t* out_beam,
+                   int32_t* out_token, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t kf_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t n);
 
 /* ----------------------------------------------------------- utilities */
 

@@ -29,6 +29,7 @@ class KV8CacheStruct(ctypes.Structure):
 
 
 _c_cache = ctypes.POINTER(KV8CacheStruct)
+_c_caches = ctypes.POINTER(_c_cache)
 
 # name -> (restype, argtypes); must mirror include/kf_sm100.h exactly.
 SIGNATURES = {
@@ -95,6 +96,19 @@ SIGNATURES = {
     "kf_kv8_attention_workspace_bytes": (_c_i64, [_c_cache, _c_int, _c_i64, _c_i64, _c_i64,
                                                   _c_int]),
     "kf_kv8_evict": (_c_int, [_c_cache, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr]),
+    "kf_kv8_attention_shared": (_c_int, [_c_cache, _c_ptr, _c_i64, _c_i64, _c_i64,
+                                         _c_ptr, _c_i64, _c_i64, _c_i64, _c_int, _c_ptr, _c_i64,
+                                         _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_float,
+                                         _c_int, _c_ptr, _c_ptr, _c_i64, _c_ptr]),
+    "kf_kv8_attention_shared_workspace_bytes": (_c_i64, [_c_cache, _c_int, _c_i64, _c_i64, _c_i64,
+                                                         _c_i64, _c_i64, _c_int]),
+    "kf_kv8_copy": (_c_int, [_c_caches, _c_caches, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr,
+                             _c_i64, _c_ptr]),
+    "kf_kv8_copy_workspace_bytes": (_c_i64, [_c_cache, _c_cache, _c_i64]),
+    "kf_beam_select": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_int, _c_ptr, _c_i64, _c_ptr, _c_i64,
+                                _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int32, _c_ptr, _c_ptr,
+                                _c_ptr, _c_ptr, _c_i64, _c_ptr]),
+    "kf_beam_select_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64]),
 }
 
 # C-ABI constants (include/kf_sm100.h)

@@ -10,3 +10,5 @@
 #include "kv8_attn_sm100.cu"
 #include "kv8_prompt_sm100.cu"
 #include "kv8_entry_sm100.cu"
+#include "kv8_copy_sm100.cu"
+#include "beam_sm100.cu"

@@ -66,6 +66,85 @@ struct KV8Work {
   bool prompt;    // the tensor-memory kernel runs
 };
 
+// Groups of sequences that share leading pages (kf_kv8_attention_shared). The
+// rows of a call are cut twice: the rows of a whole group against the tokens
+// that it shares, and the rows of each sequence against its other tokens.
+struct KV8Groups {
+  const int32_t* starts;  // [N + 1]: group n is the sequences starts[n] .. starts[n + 1] - 1
+  const int32_t* shared;  // [N]: tokens its table rows have in common
+  int N;
+  int max_shared;         // whole pages
+  int max_own;
+  int tiles;              // row tiles of all groups, at most
+  int chunks, chunk;      // parts of the shared tokens; KV8Work has those of the others
+  int own_tiles;          // row tiles of a sequence
+};
+
+// The sequences of group n; none (recorded) where starts is out of order.
+__device__ __forceinline__ int2 kv8_group(const KV8Groups& gr, int B, int n) {
+  const int a = __ldg(gr.starts + n), z = __ldg(gr.starts + n + 1);
+  if (a < 0 || z < a || z > B) {
+    record_device_status(KF_DEV_BAD_GROUPS);
+    return make_int2(0, 0);
+  }
+  return make_int2(a, z);
+}
+// Tokens that group n shares, of whole pages that all of its sequences hold. All
+// lanes of a warp call this together.
+__device__ __forceinline__ int kv8_group_tokens(const KV8& c, const KV8Groups& gr, int n, int2 seq) {
+  int s = __ldg(gr.shared + n);
+  s = s < 0 ? 0 : min(s, gr.max_shared);
+  for (int b = seq.x + (threadIdx.x & 31); b < seq.y; b += 32) s = min(s, kv8_len(c, b));
+  s = __reduce_min_sync(0xffffffffu, s);
+  return s & ~(c.P - 1);
+}
+// Group and tile of the index-th tile of `tile` rows, `per` rows a sequence;
+// n < 0: there are fewer. All lanes of a warp call this together.
+struct KV8GroupTile {
+  int n, tile;
+  int2 seq;
+};
+__device__ __forceinline__ KV8GroupTile kv8_group_tile(const KV8Groups& gr, int B, int per,
+                                                       int tile, int index) {
+  const int lane = threadIdx.x & 31;
+  for (int base = 0; base < gr.N; base += 32) {
+    const int2 seq = base + lane < gr.N ? kv8_group(gr, B, base + lane) : make_int2(0, 0);
+    const int tiles = ((seq.y - seq.x) * per + tile - 1) / tile;
+    int sum = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, sum > index);
+    if (past) {
+      const int l = __ffs(static_cast<int>(past)) - 1;
+      KV8GroupTile t;
+      t.n = base + l;
+      t.tile = index - __shfl_sync(0xffffffffu, sum - tiles, l);
+      t.seq.x = __shfl_sync(0xffffffffu, seq.x, l);
+      t.seq.y = __shfl_sync(0xffffffffu, seq.y, l);
+      return t;
+    }
+    index -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return KV8GroupTile{-1, 0, make_int2(0, 0)};
+}
+// Tokens that sequence b shares with its group (0: it is in none).
+__device__ __forceinline__ int kv8_shared_of(const KV8& c, const KV8Groups& gr, int b) {
+  const int lane = threadIdx.x & 31;
+  for (int base = 0; base < gr.N; base += 32) {
+    const int2 seq = base + lane < gr.N ? kv8_group(gr, c.B, base + lane) : make_int2(0, 0);
+    const uint32_t in = __ballot_sync(0xffffffffu, b >= seq.x && b < seq.y);
+    if (in) {
+      const int l = __ffs(static_cast<int>(in)) - 1;
+      return kv8_group_tokens(c, gr, base + l, make_int2(__shfl_sync(0xffffffffu, seq.x, l),
+                                                         __shfl_sync(0xffffffffu, seq.y, l)));
+    }
+  }
+  return 0;
+}
+
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                               uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -147,9 +226,10 @@ struct QFrag {
   uint32_t a[NP][KS][4];
   float qf[RH];
 
-  __device__ __forceinline__ void load(const KV8& c, const void* q, int64_t q_sb, int64_t q_sh,
-                                       int64_t q_st, int dtype, bool vec, int b, int h, int G,
-                                       int row0, int rows, float scale_log2) {
+  // at(row): the element where a row of q begins.
+  template <class At>
+  __device__ __forceinline__ void load(const void* q, At&& at, int dtype, bool vec, int row0,
+                                       int rows, float scale_log2) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if constexpr (RH == 1 && QP == 1) {
 #pragma unroll
@@ -161,9 +241,7 @@ struct QFrag {
       float x[NPC * EPT];
       float amax = 0.f;
       if (row < rows) {
-        const int tok = row / G;
-        const int64_t base = b * q_sb + static_cast<int64_t>(h * G + row - tok * G) * q_sh +
-                             tok * q_st;
+        const int64_t base = at(row);
 #pragma unroll
         for (int p = 0; p < NPC; ++p)
 #pragma unroll
@@ -286,13 +364,16 @@ __device__ __forceinline__ void score_tile(const QFrag<DH, QP, RH>& q, const KBy
   }
 }
 
-// QP, PP: fp16 planes of q and of P.
-template <int DH, int FMT, int QP, int PP, int RH>
+// QP, PP: fp16 planes of q and of P. SH: the call has groups; the CTAs (x) are then
+// [row tile of a group][part of its shared tokens], then [sequence][row tile]
+// [part of its own tokens], and y is the kv head.
+template <int DH, int FMT, int QP, int PP, int RH, bool SH>
 __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     kv8_split_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh, int64_t q_st,
                      void* __restrict__ out, int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype,
                      int vec, const int32_t* __restrict__ counts, int T, int G, int max_len,
-                     float scale_log2, int flags, float* __restrict__ lse_out, KV8Work w) {
+                     float scale_log2, int flags, float* __restrict__ lse_out, KV8Work w,
+                     KV8Groups gr) {
   constexpr int NT = DH / 8;  // n8 tiles of the output
   __shared__ int s_page[KV8_CHUNK_MAX / 16];
   __shared__ float s_ks[KV8_CHUNK_MAX / 16];
@@ -303,40 +384,115 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int chunk = blockIdx.x;
-  const int row0 = blockIdx.y * KV8_ROWS;
-  const int bh = blockIdx.z;
-  const int b = bh / c.H, h = bh - b * c.H;
-  const int len = kv8_len(c, b);
-  const int count = kv8_count(c, counts, b, T);
-  int end = kv8_end(c, len, count);
-  if (end > max_len) {
-    if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
-    end = max_len;
-  }
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
-  // Last key that any row of this tile sees, and the rows' own limits.
-  int limit[RH];
-  int reach = 0;
+  int chunk, row0, h, b;    // b: whose table row has the pages (the group's first sequence)
+  int rows;                 // rows that the tile is cut from
+  int end;                  // no key is at or past it
+  int limit[RH];            // the rows' own limits
+  int k0, k1;               // the CTA's keys
+  if constexpr (!SH) {
+    chunk = blockIdx.x;
+    row0 = blockIdx.y * KV8_ROWS;
+    const int bh = blockIdx.z;
+    b = bh / c.H;
+    h = bh - b * c.H;
+    rows = w.rows;
+    const int len = kv8_len(c, b);
+    const int count = kv8_count(c, counts, b, T);
+    end = kv8_end(c, len, count);
+    if (end > max_len) {
+      if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
+      end = max_len;
+    }
+    // Last key that any row of this tile sees.
+    int reach = 0;
 #pragma unroll
-  for (int r = 0; r < RH; ++r) {
-    const int row = row0 + g + 8 * r;
-    const int tok = row / G;
-    limit[r] = (row < w.rows && tok < count) ? (causal ? min(len + tok + 1, end) : end) : 0;
+    for (int r = 0; r < RH; ++r) {
+      const int row = row0 + g + 8 * r;
+      const int tok = row / G;
+      limit[r] = (row < w.rows && tok < count) ? (causal ? min(len + tok + 1, end) : end) : 0;
+    }
+    {
+      const int last_row = min(row0 + KV8_ROWS, w.rows) - 1;
+      const int last_tok = min(last_row / G, count - 1);
+      reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
+    }
+    k0 = chunk * w.chunk;
+    k1 = min(k0 + w.chunk, reach);
+  } else {
+    h = blockIdx.y;
+    int i = blockIdx.x;
+    if (i < gr.tiles * gr.chunks) {
+      chunk = i % gr.chunks;
+      const KV8GroupTile t = kv8_group_tile(gr, c.B, w.rows, KV8_ROWS, i / gr.chunks);
+      if (t.n < 0) return;
+      b = t.seq.x;
+      row0 = t.tile * KV8_ROWS;
+      rows = (t.seq.y - t.seq.x) * w.rows;
+      // every row of a sequence that takes its token sees all that is shared
+      end = kv8_group_tokens(c, gr, t.n, t.seq);
+      if (end == 0) return;  // the sequences' own CTAs leave the empty parts
+#pragma unroll
+      for (int r = 0; r < RH; ++r) {
+        const int row = row0 + g + 8 * r;
+        const int m = row / w.rows;
+        limit[r] =
+            row < rows && (row - m * w.rows) / G < kv8_count(c, counts, b + m, T) ? end : 0;
+      }
+      k0 = chunk * gr.chunk;
+      k1 = min(k0 + gr.chunk, end);
+    } else {
+      i -= gr.tiles * gr.chunks;
+      const int own = w.chunks - gr.chunks;
+      chunk = i % own;
+      i /= own;
+      b = i / gr.own_tiles;
+      row0 = (i - b * gr.own_tiles) * KV8_ROWS;
+      rows = w.rows;
+      const int shared = kv8_shared_of(c, gr, b);
+      const int len = kv8_len(c, b);
+      const int count = kv8_count(c, counts, b, T);
+      end = kv8_end(c, len, count);
+      if (end - shared > gr.max_own) {
+        if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
+        end = shared + gr.max_own;
+      }
+#pragma unroll
+      for (int r = 0; r < RH; ++r) {
+        const int row = row0 + g + 8 * r;
+        const int tok = row / G;
+        limit[r] = (row < rows && tok < count) ? (causal ? min(len + tok + 1, end) : end) : 0;
+      }
+      const int last_row = min(row0 + KV8_ROWS, rows) - 1;
+      const int last_tok = min(last_row / G, count - 1);
+      const int reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
+      k0 = shared + chunk * w.chunk;
+      k1 = min(k0 + w.chunk, reach);
+      if (shared == 0 && chunk == 0) {
+        for (int u = tid; u < KV8_ROWS * gr.chunks; u += 128) {
+          const int row = row0 + u / gr.chunks;
+          if (row >= rows) break;
+          const int64_t at =
+              (static_cast<int64_t>(b * c.H + h) * w.rows + row) * w.chunks + u % gr.chunks;
+          w.ref[at] = -INFINITY;
+          w.sum[at] = 0.f;
+        }
+      }
+      chunk += gr.chunks;
+    }
   }
-  {
-    const int last_row = min(row0 + KV8_ROWS, w.rows) - 1;
-    const int last_tok = min(last_row / G, count - 1);
-    reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
-  }
-  const int k0 = chunk * w.chunk;
-  const int k1 = min(k0 + w.chunk, reach);
+  // Where a row's numbers are: [B * H][rows of a sequence]
+  auto spot = [&](int row) -> int64_t {
+    if constexpr (!SH) return static_cast<int64_t>(blockIdx.z) * w.rows + row;
+    const int m = row / w.rows;
+    return static_cast<int64_t>((b + m) * c.H + h) * w.rows + (row - m * w.rows);
+  };
   const bool alone = w.chunks == 1;
   if (k0 >= k1 && !alone) {
     // nothing here: the join reads this chunk's sums all the same
     for (int r = tid; r < KV8_ROWS; r += 128)
-      if (row0 + r < w.rows) {
-        const int64_t at = (static_cast<int64_t>(bh) * w.rows + row0 + r) * w.chunks + chunk;
+      if (row0 + r < rows) {
+        const int64_t at = spot(row0 + r) * w.chunks + chunk;
         w.ref[at] = -INFINITY;
         w.sum[at] = 0.f;
       }
@@ -354,7 +510,12 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     vmax = fmaxf(vmax, s.y);
   }
   QFrag<DH, QP, RH> qa;
-  qa.load(c, q, q_sb, q_sh, q_st, dtype, vec != 0, b, h, G, row0, w.rows, scale_log2);
+  qa.load(q, [&](int row) {
+    const int m = SH ? row / w.rows : 0;
+    if constexpr (SH) row -= m * w.rows;
+    const int tok = row / G;
+    return (b + m) * q_sb + static_cast<int64_t>(h * G + row - tok * G) * q_sh + tok * q_st;
+  }, dtype, vec != 0, row0, rows, scale_log2);
 #pragma unroll
   for (int d = 16; d; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
   if (lane == 0) s_vmax[warp] = vmax;
@@ -433,12 +594,11 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
         const float x = f[n][e] * (qa.qf[e >> 1] * ks);
         f[n][e] = kk < min(limit[e >> 1], bad) ? x : -INFINITY;
       }
-    if (w.score) {
+    if (!SH && w.score) {
 #pragma unroll
       for (int r = 0; r < RH; ++r)
         if (row0 + g + 8 * r < w.rows) {
-          float* sp = w.score + (static_cast<int64_t>(bh) * w.rows + row0 + g + 8 * r) * w.ld_score +
-                      key + 2 * t;
+          float* sp = w.score + spot(row0 + g + 8 * r) * w.ld_score + key + 2 * t;
           *reinterpret_cast<float2*>(sp) = make_float2(f[0][2 * r], f[0][2 * r + 1]);
           *reinterpret_cast<float2*>(sp + 8) = make_float2(f[1][2 * r], f[1][2 * r + 1]);
         }
@@ -566,7 +726,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
   for (int i = tid; i < KV8_ROWS * DH; i += 128) {
     const int r = i / DH, d = i - r * DH;
     const int row = row0 + r;
-    if (row >= w.rows) break;
+    if (row >= rows) break;
     float top = s_ref[0][r];
 #pragma unroll
     for (int u = 1; u < 4; ++u) top = fmaxf(top, s_ref[u][r]);
@@ -578,8 +738,8 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
       x += a * s_o[(u * KV8_ROWS + r) * DH + d];
     }
     x *= vmax;
-    const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
-    if (alone) {
+    const int64_t at = spot(row);
+    if (!SH && alone) {
       const int tok = row / G;
       const int hq = h * G + row - tok * G;
       kv8_store1(out, b * o_sb + hq * o_sh + tok * o_st + d, dtype, l == 0.f ? 0.f : x / l);

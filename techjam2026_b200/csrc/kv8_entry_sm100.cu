@@ -147,11 +147,12 @@ struct KV8Call {
   int flags;
   float* lse;
   cudaStream_t st;
+  KV8Groups gr;                      // N = 0: no groups
 };
 
-template <int DH, int FMT, int QP, int PP, int RH>
+template <int DH, int FMT, int QP, int PP, int RH, bool SH>
 static cudaError_t kv8_split(const KV8& c, const KV8Call& a, const KV8Work& w) {
-  auto kern = kv8_split_kernel<DH, FMT, QP, PP, RH>;
+  auto kern = kv8_split_kernel<DH, FMT, QP, PP, RH, SH>;
   constexpr int smem = SplitCfg<DH>::SMEM;
   static DeviceOnce once;
   cudaError_t attr = cudaSuccess;
@@ -160,16 +161,24 @@ static cudaError_t kv8_split(const KV8& c, const KV8Call& a, const KV8Work& w) {
     return attr == cudaSuccess ? KF_OK : KF_E_CUDA;
   });
   if (attr != cudaSuccess) return attr;
-  const dim3 grid(static_cast<unsigned>(w.chunks),
-                  static_cast<unsigned>((w.rows + KV8_ROWS - 1) / KV8_ROWS),
-                  static_cast<unsigned>(c.B * c.H));
+  dim3 grid(static_cast<unsigned>(w.chunks),
+            static_cast<unsigned>((w.rows + KV8_ROWS - 1) / KV8_ROWS),
+            static_cast<unsigned>(c.B * c.H));
+  if constexpr (SH)
+    grid = dim3(static_cast<unsigned>(a.gr.tiles * a.gr.chunks +
+                                      c.B * a.gr.own_tiles * (w.chunks - a.gr.chunks)),
+                static_cast<unsigned>(c.H));
   return launch_chained(kern, grid, dim3(128), smem, a.st, c, a.q, a.q_sb, a.q_sh, a.q_st, a.out,
                         a.o_sb, a.o_sh, a.o_st, a.dtype, a.q_vec, a.counts, a.T, a.G, a.max_len,
-                        a.scale_log2, a.flags, a.lse, w);
+                        a.scale_log2, a.flags, a.lse, w, a.gr);
 }
 template <int DH, int FMT, int QP, int PP>
 static cudaError_t kv8_split_rows(const KV8& c, const KV8Call& a, const KV8Work& w, bool half) {
-  return half ? kv8_split<DH, FMT, QP, PP, 1>(c, a, w) : kv8_split<DH, FMT, QP, PP, 2>(c, a, w);
+  if (a.gr.N > 0)
+    return half ? kv8_split<DH, FMT, QP, PP, 1, true>(c, a, w)
+                : kv8_split<DH, FMT, QP, PP, 2, true>(c, a, w);
+  return half ? kv8_split<DH, FMT, QP, PP, 1, false>(c, a, w)
+              : kv8_split<DH, FMT, QP, PP, 2, false>(c, a, w);
 }
 // fp16 outputs show one plane's rounding of P (1.4 times their own error), bf16
 // ones do not. The second plane costs (us, one / two): a token of 4 rows a kv
@@ -293,7 +302,7 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
   const int o_vec = kv8_aligned(out, 16) && o_sb % per == 0 && o_sh % per == 0 && o_st % per == 0;
   const int vec16 = kv8_aligned(q, 16) && q_sb % per == 0 && q_sh % per == 0 && q_st % per == 0;
   const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, vec16, o_vec, counts, Ti, G,
-                     cap, scale_log2, flags, lse, st};
+                     cap, scale_log2, flags, lse, st, {}};
   if (w.prompt) {
     switch (c.D) {
       case 16: return kv8_prompt_type<16>(c, a, w);
@@ -322,4 +331,142 @@ extern "C" int kf_kv8_attention(const kf_kv8_cache* cache, const void* q, int64_
       dim3(static_cast<unsigned>((max_len + KV8_WEIGHTS_KEYS - 1) / KV8_WEIGHTS_KEYS), bh),
       dim3(128), 0, st, c, counts, Ti, G, cap, flags, w);
   return cuda_status(e, "kf_kv8_attention weights launch");
+}
+
+// ---------------------------------------------------------------- shared pages
+
+namespace kf {
+
+// Rows, parts and workspace of a call with groups. A part is a CTA's keys; all
+// parts of a row, shared and own, meet in the join.
+static int kv8_shared_plan(const char* what, const KV8& c, int dtype, int64_t T, int64_t q_heads,
+                           int64_t n_groups, int64_t max_shared, int64_t max_own, KV8Groups* gr,
+                           KV8Work* w) {
+  const int64_t reach = static_cast<int64_t>(c.blocks) * c.P;
+  if (n_groups < 0 || n_groups > 32767 || max_shared < 0 || max_own < 0) {
+    set_last_error("%s: needs 0 <= n_groups <= 32767 and bounds that are not negative", what);
+    return KF_E_INVALID;
+  }
+  if (max_shared == 0 || max_shared > reach) max_shared = reach;
+  if (max_own == 0 || max_own > reach) max_own = reach;
+  max_shared &= ~static_cast<int64_t>(c.P - 1);
+  const int64_t per = T * (q_heads / c.H);
+  if (c.B * per > (1LL << 30)) {
+    set_last_error("%s: needs batch * T * q_heads / kv_heads <= 2^30", what);
+    return KF_E_UNSUPPORTED;
+  }
+  gr->N = static_cast<int>(n_groups);
+  gr->max_shared = static_cast<int>(max_shared);
+  gr->max_own = static_cast<int>(max_own);
+  const int64_t most = n_groups < c.B ? n_groups : c.B;  // groups that hold a sequence
+  const int64_t tiles = (c.B * per + most * (KV8_ROWS - 1)) / KV8_ROWS;
+  gr->own_tiles = static_cast<int>((per + KV8_ROWS - 1) / KV8_ROWS);
+  const int64_t want =
+      static_cast<int64_t>(sm_count()) *
+      (c.D == 128 ? SplitCfg<128>::min_blocks(dtype == KF_DT_F32 ? 2 : 1) : SplitCfg<64>::min_blocks(1));
+  // Parts of `keys` keys for `items` tiles, as in kv8_plan.
+  auto cut = [&](int64_t keys, int64_t items, int* chunks, int* chunk) {
+    int64_t n = (want + items - 1) / items;
+    const int64_t least = (keys + KV8_CHUNK_MAX - 1) / KV8_CHUNK_MAX;
+    if (n > (keys + 127) / 128) n = (keys + 127) / 128;
+    if (n < least) n = least;
+    if (n < 1) n = 1;
+    int64_t m = ((keys + n - 1) / n + 127) / 128 * 128;
+    if (m < 128) m = 128;
+    *chunk = static_cast<int>(m);
+    *chunks = static_cast<int>((keys + m - 1) / m);
+    if (*chunks < 1) *chunks = 1;
+  };
+  int own_chunks;
+  cut(max_shared, tiles * c.H, &gr->chunks, &gr->chunk);
+  cut(max_own, static_cast<int64_t>(c.B) * gr->own_tiles * c.H, &own_chunks, &w->chunk);
+  gr->tiles = static_cast<int>(tiles);
+  w->chunks = gr->chunks + own_chunks;
+  w->rows = static_cast<int>(per);
+  w->ld_score = 0;
+  w->prompt = false;
+  if (tiles * gr->chunks + static_cast<int64_t>(c.B) * gr->own_tiles * own_chunks > INT32_MAX) {
+    set_last_error("%s: too many rows and keys for one call", what);
+    return KF_E_UNSUPPORTED;
+  }
+  return KF_OK;
+}
+
+}  // namespace kf
+
+extern "C" int64_t kf_kv8_attention_shared_workspace_bytes(const kf_kv8_cache* cache, int dtype,
+                                                           int64_t T, int64_t q_heads,
+                                                           int64_t n_groups, int64_t max_shared,
+                                                           int64_t max_own, int flags) {
+  const char* what = "kf_kv8_attention_shared_workspace_bytes";
+  KV8 c;
+  KV8Groups gr;
+  KV8Work w;
+  int64_t max_len = 0;
+  if (kv8_attention_check(what, cache, dtype, T, q_heads, &max_len, 1.f, flags, &c)) return -1;
+  if (T == 0 || c.B == 0) return 0;
+  if (n_groups == 0)
+    return kf_kv8_attention_workspace_bytes(cache, dtype, T, q_heads, max_own, flags);
+  if (kv8_shared_plan(what, c, dtype, T, q_heads, n_groups, max_shared, max_own, &gr, &w)) return -1;
+  return kv8_carve(c, dtype, flags, nullptr, &w);
+}
+
+extern "C" int kf_kv8_attention_shared(const kf_kv8_cache* cache, const void* q, int64_t q_sb,
+                                       int64_t q_sh, int64_t q_st, void* out, int64_t o_sb,
+                                       int64_t o_sh, int64_t o_st, int dtype,
+                                       const int32_t* counts, int64_t T, int64_t q_heads,
+                                       const int32_t* starts, const int32_t* shared,
+                                       int64_t n_groups, int64_t max_shared, int64_t max_own,
+                                       float sm_scale, int flags, float* lse, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
+  const char* what = "kf_kv8_attention_shared";
+  if (n_groups == 0)
+    return kf_kv8_attention(cache, q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, counts, T,
+                            q_heads, max_own, sm_scale, flags, lse, workspace, workspace_bytes,
+                            stream);
+  KV8 c;
+  int64_t max_len = 0;
+  int rc = kv8_attention_check(what, cache, dtype, T, q_heads, &max_len, sm_scale, flags, &c);
+  if (rc) return rc;
+  if (flags & KF_KV8_TRACK) {
+    set_last_error("%s: sequences that share pages have no weight record of their own", what);
+    return KF_E_UNSUPPORTED;
+  }
+  if (T == 0 || c.B == 0) return KF_OK;
+  if (!q || !out || !starts || !shared) {
+    set_last_error("%s: q, out, starts and shared must not be null", what);
+    return KF_E_INVALID;
+  }
+  KV8Groups gr;
+  KV8Work w;
+  rc = kv8_shared_plan(what, c, dtype, T, q_heads, n_groups, max_shared, max_own, &gr, &w);
+  if (rc) return rc;
+  gr.starts = starts;
+  gr.shared = shared;
+  const int64_t need = kv8_carve(c, dtype, flags, static_cast<uint8_t*>(workspace), &w);
+  if (!workspace || workspace_bytes < need || !kv8_aligned(workspace, 256)) {
+    set_last_error("%s: needs a 256-byte aligned workspace of %lld bytes", what, (long long)need);
+    return KF_E_INVALID;
+  }
+  const int64_t es = dtype_size(dtype), per = 16 / es;
+  const int G = static_cast<int>(q_heads / c.H), Ti = static_cast<int>(T);
+  const int vec = kv8_aligned(q, 4 * es) && q_sb % 4 == 0 && q_sh % 4 == 0 && q_st % 4 == 0;
+  const int o_vec = kv8_aligned(out, 16) && o_sb % per == 0 && o_sh % per == 0 && o_st % per == 0;
+  const int vec16 = kv8_aligned(q, 16) && q_sb % per == 0 && q_sh % per == 0 && q_st % per == 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const KV8Call a = {q, q_sb, q_sh, q_st, out, o_sb, o_sh, o_st, dtype, vec, vec16, o_vec, counts,
+                     Ti, G, 0, sm_scale * 1.4426950408889634f, flags, lse, st, gr};
+  const bool half = static_cast<int64_t>(c.B) * w.rows <= 8;
+  cudaError_t e;
+  switch (c.D) {
+    case 16: e = kv8_split_any<16>(c, a, w, half); break;
+    case 32: e = kv8_split_any<32>(c, a, w, half); break;
+    case 64: e = kv8_split_any<64>(c, a, w, half); break;
+    default: e = kv8_split_any<128>(c, a, w, half); break;
+  }
+  if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention_shared launch");
+  e = launch_chained(kv8_join_kernel,
+                     dim3(static_cast<unsigned>(w.rows), static_cast<unsigned>(c.B * c.H)),
+                     dim3(KV8_JOIN_THREADS), 0, st, c, out, o_sb, o_sh, o_st, dtype, Ti, G, lse, w);
+  return cuda_status(e, "kf_kv8_attention_shared join launch");
 }

@@ -11,13 +11,16 @@ table, so sequences grow and shrink without copies.
                  every cached token received;
   kv8_evict      cuts each head's tokens to a budget: the most recent and, of
                  the others, the ones with the most recorded weight;
-  kv8_read       values of a range of tokens.
+  kv8_read       values of a range of tokens;
+  kv8_attention_shared  kv8_attention for sequences that share leading pages,
+                 which are read once for all of them;
+  kv8_copy       copies of pages, of all layers at once.
 
 A step over one layer: `kv8_append(cache, k, v)`, `kv8_attention(q, cache)`;
 after the last layer, `cache.lens += T` (all layers of a model may share one
 `lens` and one `table`). `techjam2026_b200.kvcache` does this for the layer
 stack. Runs csrc/kv8_cache_sm100.cu, csrc/kv8_attn_sm100.cu and
-csrc/kv8_prompt_sm100.cu. The reference has no cache: it recomputes the whole
+csrc/kv8_prompt_sm100.cu, and csrc/kv8_copy_sm100.cu. The reference has no cache: it recomputes the whole
 sequence (kernelforge/optimized.py:397-458).
 
 Calls are stream-ordered on the current stream, launch a fixed number of
@@ -25,12 +28,12 @@ kernels for given shapes and read lengths on the device, so a step may be
 captured in a CUDA graph. A length beyond the table or a page number outside
 the pool is never used as an index: it is recorded in the device status word
 (code 6) and the tokens count as absent. A sequence of a negative length holds
-no token and takes none.
+no token and takes none. Groups of sequences out of order are recorded as code 7.
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -335,3 +338,131 @@ def kv8_evict(cache: KV8Cache, table_out: torch.Tensor, budget: int, recent: int
                                  recent, kept.data_ptr(), new.lens.data_ptr(), stream)
     _lib.check(rc, "kf_kv8_evict")
     return kept, new
+
+
+def kv8_attention_shared(q: torch.Tensor, cache: KV8Cache, starts: torch.Tensor,
+                         shared: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                         causal: bool = True, sm_scale: Optional[float] = None,
+                         max_shared: int = 0, max_own: int = 0,
+                         out: Optional[torch.Tensor] = None, return_lse: bool = False
+                         ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """kv8_attention for a batch whose groups share their leading pages: samples
+    or beams of one prompt, questions about one document. What a group shares is
+    read once for all of its rows; the result is kv8_attention's, but for
+    rounding.
+
+    starts      int32 [N + 1], ascending: group n is the sequences starts[n] to
+                starts[n + 1] - 1. A sequence in no group shares nothing
+    shared      int32 [N]: how many leading tokens of its sequences lie on pages
+                that their table rows name alike. Cut to whole pages, and to the
+                shortest of the group's lens (new tokens are not shared)
+    max_shared  an upper bound of shared known to the caller (0: what the table
+                can hold); what is beyond it is read sequence by sequence
+    max_own     an upper bound of the tokens of a sequence, new ones among them,
+                besides those (0: what the table can hold). A sequence with more
+                is cut there and recorded in the device status word
+
+    The other arguments, what is returned and which rows are 0 as for
+    kv8_attention. There is no weight record to add to: it belongs to the pages,
+    which here are several sequences'."""
+    what = "kv8_attention_shared"
+    B, Hq, T, D = q.shape
+    if B != cache.batch or D != cache.head_dim or Hq % cache.kv_heads:
+        raise ValueError(f"{what}: q must be [{cache.batch}, a multiple of {cache.kv_heads}, T, "
+                         f"{cache.head_dim}], got {tuple(q.shape)}")
+    code = _dtype_code(q, f"{what}: q")
+    if q.stride(3) != 1:
+        raise ValueError(f"{what}: q needs unit stride along head_dim")
+    if out is None:
+        out = torch.empty((B, Hq, T, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+        raise ValueError(f"{what}: out must have q's shape and type and unit stride along "
+                         "head_dim")
+    stream = _check_call(what, cache, counts, q, out)
+    for t, name in ((starts, "starts"), (shared, "shared")):
+        if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() \
+                or t.get_device() != cache.device.index:
+            raise ValueError(f"{what}: {name} must be a contiguous int32 tensor on {cache.device}")
+    groups = shared.shape[0]
+    if starts.shape[0] != groups + 1:
+        raise ValueError(f"{what}: starts must have one entry more than shared, got "
+                         f"{starts.shape[0]} and {groups}")
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
+    flags = _lib.KF_KV8_CAUSAL if causal else 0
+    L = _lib.lib()
+    key = (code, T, Hq, groups, max_shared, max_own, flags)
+    need = cache._work.get(key)
+    if need is None:
+        need = L.kf_kv8_attention_shared_workspace_bytes(cache._ref, *key)
+        if need < 0:
+            raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
+        if len(cache._work) >= 256:      # bounds of its own every step
+            cache._work.clear()
+        cache._work[key] = need
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    rc = L.kf_kv8_attention_shared(
+        cache._ref, q.data_ptr(), *q.stride()[:3], out.data_ptr(), *out.stride()[:3], code,
+        counts.data_ptr() if counts is not None else None, T, Hq, starts.data_ptr(),
+        shared.data_ptr(), groups, max_shared, max_own,
+        float(sm_scale) if sm_scale is not None else D ** -0.5, flags,
+        lse.data_ptr() if lse is not None else None,
+        work.data_ptr() if work is not None else None, need, stream)
+    _lib.check(rc, "kf_kv8_attention_shared")
+    return (out, lse) if return_lse else out
+
+
+Caches = Union[KV8Cache, Sequence[KV8Cache]]
+
+
+def _refs(caches: Sequence[KV8Cache]):
+    return (ctypes.POINTER(_lib.KV8CacheStruct) * len(caches))(
+        *(ctypes.pointer(c.struct) for c in caches))
+
+
+def kv8_copy(cache: Caches, src: torch.Tensor, dst: torch.Tensor,
+             tokens: Optional[torch.Tensor] = None, into: Optional[Caches] = None) -> None:
+    """Copy pages: page dst[i] becomes page src[i], for all kv heads, codes and
+    scales, and the weight record where both caches keep one.
+
+    cache     the cache, or the layers' caches (of one geometry), copied in one
+              call
+    src, dst  int32 [n]; a pair of the same page is no copy
+    tokens    int32 [n] (default whole pages): only the first tokens[i] slots
+              are copied, with the scales; the others stay as they are
+    into      the caches whose pages dst are (default: the same ones); another
+              pool, of any number of pages
+
+    A pair is not done, and recorded in the device status word (code 6), if an
+    entry is no page of its pool, or if another pair writes the same page or,
+    within one pool, reads it. The caches' tables and lens are not used."""
+    what = "kv8_copy"
+    caches = [cache] if isinstance(cache, KV8Cache) else list(cache)
+    to = caches if into is None else [into] if isinstance(into, KV8Cache) else list(into)
+    if not caches:
+        return
+    if len(to) != len(caches):
+        raise ValueError(f"{what}: {len(caches)} caches into {len(to)}")
+    first = caches[0]
+    for c in caches + to:
+        if c.device != first.device:
+            raise ValueError(f"{what}: all caches must be on one device")
+        if c.k.dtype != first.k.dtype or c.k.shape[1:] != first.k.shape[1:]:
+            raise ValueError(f"{what}: all caches must have the codes, heads, block and head_dim of "
+                             "the first")
+    stream = _check_call(what, first, None)
+    n = src.shape[0] if src.dim() == 1 else -1
+    for t, name in ((src, "src"), (dst, "dst"), (tokens, "tokens")):
+        if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n
+                              or not t.is_contiguous() or t.get_device() != first.device.index):
+            raise ValueError(f"{what}: src, dst and tokens must be contiguous int32 tensors [n] on "
+                             f"{first.device}; {name} is {t.dtype} {tuple(t.shape)} on {t.device}")
+    L = _lib.lib()
+    need = L.kf_kv8_copy_workspace_bytes(first._ref, to[0]._ref, n)
+    if need < 0:
+        raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
+    work = torch.empty(need, dtype=torch.uint8, device=first.device) if need else None
+    refs = _refs(caches)
+    rc = L.kf_kv8_copy(refs, refs if into is None else _refs(to), len(caches), src.data_ptr(),
+                       dst.data_ptr(), tokens.data_ptr() if tokens is not None else None, n,
+                       work.data_ptr() if work is not None else None, need, stream)
+    _lib.check(rc, "kf_kv8_copy")
