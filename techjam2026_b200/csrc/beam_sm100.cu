@@ -69,15 +69,106 @@ __device__ void beam_sort(Key* list, int count) {
     }
 }
 
+// The n best of the first `count` keys of a list in shared memory, best first, by
+// put(place, key): every key counts those before it, which for a few hundred keys
+// is far shorter than a sort's chain of barriers. All threads of the CTA; `list` is
+// read only after a barrier of the caller's. Many keys are sorted.
+constexpr int BEAM_COUNTED = 512;
+template <class Key, class Put>
+__device__ __forceinline__ void beam_best(Key* list, int count, int n, Put&& put) {
+  if (count > BEAM_COUNTED) {
+    beam_sort(list, count);
+    for (int i = threadIdx.x; i < min(n, count); i += BEAM_THREADS) put(i, list[i]);
+    return;
+  }
+  for (int i = threadIdx.x; i < count; i += BEAM_THREADS) {
+    const Key mine = list[i];
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) place += beam_before(list[j], mine) ? 1 : 0;
+    if (place < n) put(place, mine);
+  }
+}
+
 // ---------------------------------------------------------------- one pass over the logits
+//
+// One CTA = a slice of a beam's vocabulary, 4 x 16 bytes of logits a thread in
+// flight. The first round (up to 4096 or 8192 tokens) gives the threads' largest
+// logits; the n-th largest of those is a bound that at least n tokens reach, so what
+// is below it is passed over with one comparison for each 16 bytes, and the list
+// of the others stays short without any barrier in the loop. Where it does not
+// (many equal logits, or logits that grow along the slice), the slice is read
+// again in small rounds that cut the list as it fills.
+// Bound by memory, and by the exponentials for 16-bit logits (16 a clock and SM).
 
 template <int DT>
-__global__ void __launch_bounds__(BEAM_THREADS)
+__device__ __forceinline__ void beam_load(const void* logits, int64_t base, int64_t i, int64_t last,
+                                          bool vec, uint4& v) {
+  constexpr int N = KV8Type<DT>::N;
+  if (i + N <= last) {
+    v = KV8Type<DT>::load(logits, base + i, vec);
+    return;
+  }
+  // the end: what is not there is -inf
+  uint32_t w[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if constexpr (DT == KF_DT_F32) {
+      w[u] = i + u < last ? static_cast<const uint32_t*>(logits)[base + i + u] : 0xff800000u;
+    } else {
+      constexpr uint32_t none = DT == KF_DT_BF16 ? 0xff80u : 0xfc00u;
+      const uint16_t* q = static_cast<const uint16_t*>(logits) + base;
+      const int64_t j = i + 2 * u;
+      w[u] = (j < last ? q[j] : none) | ((j + 1 < last ? q[j + 1] : none) << 16);
+    }
+  }
+  v = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Keys of the n best tokens of a slice, at the front of the list; how many.
+template <int DT>
+__device__ __noinline__ int beam_careful(uint64_t* list, int* s_count, const void* logits,
+                                         int64_t base, int64_t first, int64_t last, bool vec, int n) {
+  constexpr int N = KV8Type<DT>::N;
+  uint64_t cut = 0;   // keys up to it are out: n better ones are known
+  __syncthreads();
+  if (threadIdx.x == 0) *s_count = 0;
+  __syncthreads();
+  for (int64_t at = first; at < last; at += N * BEAM_THREADS) {
+    const int64_t i = at + threadIdx.x * N;
+    uint4 v;
+    float x[N];
+    beam_load<DT>(logits, base, i, last, vec, v);
+    KV8Type<DT>::values(v, x);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      if (!(x[u] > -INFINITY)) continue;   // NaN among them
+      const uint64_t key = static_cast<uint64_t>(beam_order(x[u])) << 32 |
+                           (0xffffffffu - static_cast<uint32_t>(i + u));
+      if (key > cut) list[atomicAdd(s_count, 1)] = key;
+    }
+    __syncthreads();
+    const int count = *s_count;
+    if (count > BEAM_CAP - N * BEAM_THREADS) {
+      beam_sort(list, count);
+      cut = list[n - 1];
+      if (threadIdx.x == 0) *s_count = n;
+    }
+    __syncthreads();
+  }
+  return *s_count;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(BEAM_THREADS, 4)
     beam_scan_kernel(const void* __restrict__ logits, int64_t l_sb, int64_t l_sk, int vec,
                      const uint8_t* __restrict__ ended, int64_t e_sb, int beams, int64_t vocab,
                      int n, BeamWork w) {
-  constexpr int N = KV8Type<DT>::N;
+  constexpr int N = KV8Type<DT>::N, U = 4;
+  constexpr float LOG2E = 1.4426950408889634f;
   __shared__ uint64_t list[BEAM_CAP];
+  __shared__ __align__(16) uint32_t s_max[BEAM_THREADS];
+  __shared__ uint32_t s_cut;
   __shared__ int s_count;
   __shared__ float s_top[BEAM_THREADS / 32];
   __shared__ double s_sum[BEAM_THREADS / 32];
@@ -92,54 +183,74 @@ __global__ void __launch_bounds__(BEAM_THREADS)
   const int64_t last = first + w.slice < vocab ? first + w.slice : vocab;
   const int64_t base = b * l_sb + k * l_sk;
   float top = -INFINITY, sum = 0.f;
-  uint64_t cut = 0;   // keys up to it are out: n better ones are known
-  if (tid == 0) s_count = 0;
-  __syncthreads();
-  for (int64_t at = first; at < last; at += N * BEAM_THREADS) {
-    const int64_t i = at + tid * N;
-    float x[N];
-    if (i + N <= last) {
-      KV8Type<DT>::values(KV8Type<DT>::load(logits, base + i, vec != 0), x);
-    } else {
+  float cut = -INFINITY;   // logits below it are out, and those equal to it after the first round
+  if (tid == 0) {
+    s_count = 0;
+    s_cut = 0;
+  }
+  for (int64_t at = first; at < last; at += U * N * BEAM_THREADS) {
+    uint4 v[U];
 #pragma unroll
-      for (int u = 0; u < N; ++u) x[u] = i + u < last ? kv8_load1(logits, base + i + u, DT) : -INFINITY;
+    for (int r = 0; r < U; ++r)
+      beam_load<DT>(logits, base, at + (r * BEAM_THREADS + tid) * N, last, vec != 0, v[r]);
+    float m[U];
+#pragma unroll
+    for (int r = 0; r < U; ++r) {
+      float x[N];
+      KV8Type<DT>::values(v[r], x);
+      m[r] = x[0];
+#pragma unroll
+      for (int u = 1; u < N; ++u) m[r] = fmaxf(m[r], x[u]);
     }
-    float m = x[0];
+    float most = m[0];
 #pragma unroll
-    for (int u = 1; u < N; ++u) m = fmaxf(m, x[u]);
-    if (m > top) {
-      sum *= fast_exp2((top - m) * 1.4426950408889634f);
-      top = m;
+    for (int r = 1; r < U; ++r) most = fmaxf(most, m[r]);
+    if (at == first) {
+      // (a thread without a number has 0, below every number's order)
+      const uint32_t mine = most > -INFINITY ? beam_order(most) : 0u;
+      s_max[tid] = mine;
+      __syncthreads();
+      int before = 0;
+#pragma unroll 8
+      for (int j = 0; j < BEAM_THREADS; j += 4) {
+        const uint4 o = *reinterpret_cast<const uint4*>(s_max + j);
+        before += (o.x > mine || (o.x == mine && j < tid)) + (o.y > mine || (o.y == mine && j + 1 < tid)) +
+                  (o.z > mine || (o.z == mine && j + 2 < tid)) + (o.w > mine || (o.w == mine && j + 3 < tid));
+      }
+      if (before == n - 1) s_cut = mine;
+      __syncthreads();
+      if (s_cut) cut = beam_value(s_cut);
+    }
+    if (most > top) {
+      sum *= fast_exp2((top - most) * LOG2E);
+      top = most;
     }
     const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int u = 0; u < N; ++u) sum += fast_exp2((x[u] - ref) * 1.4426950408889634f);
-    if (at == first) {
-      // The n-th largest of the threads' largest: at least n tokens are not below it.
-      list[tid] = m > -INFINITY ? static_cast<uint64_t>(beam_order(m)) << 32 | (255 - tid) : 0;
-      beam_sort(list, BEAM_THREADS);
-      const uint64_t t = list[n - 1];
-      __syncthreads();
-      cut = t >> 32 << 32;   // (a real key with this value is above it)
-    }
+    for (int r = 0; r < U; ++r) {
+      float x[N];
+      KV8Type<DT>::values(v[r], x);
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      if (!(x[u] > -INFINITY)) continue;   // NaN among them
-      const uint64_t key = static_cast<uint64_t>(beam_order(x[u])) << 32 |
-                           (0xffffffffu - static_cast<uint32_t>(i + u));
-      if (key > cut) list[atomicAdd(&s_count, 1)] = key;
-    }
-    __syncthreads();
-    if (s_count > BEAM_CAP - N * BEAM_THREADS) {
-      beam_sort(list, s_count);
-      cut = list[n - 1];
-      if (tid == 0) s_count = n;
-      __syncthreads();
+      for (int u = 0; u < N; ++u) sum += fast_exp2((x[u] - ref) * LOG2E);
+      if (at == first ? m[r] >= cut : m[r] > cut) {
+        const uint32_t i = static_cast<uint32_t>(at + (r * BEAM_THREADS + tid) * N);
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+          if (x[u] > -INFINITY && (at == first ? x[u] >= cut : x[u] > cut)) {
+            const int to = atomicAdd(&s_count, 1);
+            if (to < BEAM_CAP)
+              list[to] = static_cast<uint64_t>(beam_order(x[u])) << 32 | (0xffffffffu - (i + u));
+          }
+      }
     }
   }
-  const int count = s_count;
-  beam_sort(list, count);
-  for (int i = tid; i < n; i += BEAM_THREADS) w.key[spot * n + i] = i < count ? list[i] : 0;
+  __syncthreads();
+  int count = s_count;
+  if (count > BEAM_CAP)
+    count = beam_careful<DT>(list, &s_count, logits, base, first, last, vec != 0, n);
+  uint64_t* out = w.key + spot * n;
+  beam_best(list, count, n, [&](int place, uint64_t key) { out[place] = key; });
+  for (int i = count + tid; i < n; i += BEAM_THREADS) out[i] = 0;
   // the slice's sum
   float m = top;
 #pragma unroll
@@ -149,8 +260,7 @@ __global__ void __launch_bounds__(BEAM_THREADS)
 #pragma unroll
   for (int u = 0; u < BEAM_THREADS / 32; ++u) m = fmaxf(m, s_top[u]);
   // (a thread that saw no number has a sum of 0, or NaN)
-  double s = static_cast<double>(
-      top == -INFINITY ? sum : sum * fast_exp2((top - m) * 1.4426950408889634f));
+  double s = static_cast<double>(top == -INFINITY ? sum : sum * fast_exp2((top - m) * LOG2E));
 #pragma unroll
   for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   if (lane == 0) s_sum[warp] = s;
@@ -163,6 +273,10 @@ __global__ void __launch_bounds__(BEAM_THREADS)
 }
 
 // ---------------------------------------------------------------- the best of all beams
+//
+// One CTA a batch row: the beams' sums, a warp each, then their keys as candidates.
+// Latency is what it costs. The slices' lists are in order, so the n-th best of
+// their first entries bounds the answer, and few candidates are left to compare.
 
 __global__ void __launch_bounds__(BEAM_THREADS)
     beam_join_kernel(const float* __restrict__ scores, int64_t s_sb,
@@ -170,67 +284,101 @@ __global__ void __launch_bounds__(BEAM_THREADS)
                      float* __restrict__ out_score, int32_t* __restrict__ out_beam,
                      int32_t* __restrict__ out_token, BeamWork w) {
   __shared__ BeamKey list[BEAM_JOIN_CAP];
-  __shared__ double s_lse[1024];
+  __shared__ BeamKey s_cut;
+  __shared__ double s_lse[1024];   // of a beam; of an ended one not used
+  __shared__ float s_score[1024];
+  __shared__ uint8_t s_ended[1024];
   __shared__ int s_count;
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x;
-  for (int k = tid; k < beams; k += BEAM_THREADS) {
+  for (int k = warp; k < beams; k += BEAM_THREADS / 32) {
     const int64_t spot = (static_cast<int64_t>(b) * beams + k) * w.slices;
-    if (ended && ended[b * e_sb + k]) continue;
+    const bool end = ended && ended[b * e_sb + k];
+    if (lane == 0) {
+      s_ended[k] = end;
+      s_score[k] = scores[b * s_sb + k];
+    }
+    if (end) continue;
     float m = -INFINITY;
-    for (int i = 0; i < w.slices; ++i) m = fmaxf(m, w.top[spot + i]);
+    for (int i = lane; i < w.slices; i += 32) m = fmaxf(m, w.top[spot + i]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     double s = 0.0;
-    for (int i = 0; i < w.slices; ++i) {
+    for (int i = lane; i < w.slices; i += 32) {
       const double part = w.sum[spot + i];
       if (part != 0.0) s += part * exp(static_cast<double>(w.top[spot + i]) - m);
     }
-    s_lse[k] = m + log(s);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (lane == 0) s_lse[k] = m + log(s);
   }
-  if (tid == 0) s_count = 0;
+  if (tid == 0) {
+    s_count = 0;
+    beam_none(s_cut);
+  }
   __syncthreads();
-  BeamKey cut;
-  beam_none(cut);
   const int64_t per = static_cast<int64_t>(w.slices) * n;
   const int64_t all = beams * per;
-  for (int64_t at = 0; at < all; at += BEAM_THREADS) {
-    const int64_t i = at + tid;
-    if (i < all) {
-      const int k = static_cast<int>(i / per);
-      const float score = scores[b * s_sb + k];
+  // Entry i of the row's lists as a candidate; false: it is none.
+  auto candidate = [&](int64_t i, BeamKey& c) -> bool {
+    const int k = static_cast<int>(i / per);
+    if (s_ended[k]) {
+      if (i != k * per) return false;
+      c.c = s_score[k];
+      c.at = static_cast<uint64_t>(k) << 32 | static_cast<uint32_t>(pad);
+    } else {
+      const uint64_t key = w.key[static_cast<int64_t>(b) * all + i];
+      if (!key) return false;
+      c.c = (static_cast<double>(beam_value(static_cast<uint32_t>(key >> 32))) - s_lse[k]) +
+            s_score[k];
+      c.at = static_cast<uint64_t>(k) << 32 | (0xffffffffu - static_cast<uint32_t>(key));
+    }
+    return c.c > -INFINITY;
+  };
+  const int64_t heads = static_cast<int64_t>(beams) * w.slices;
+  if (all > BEAM_COUNTED && heads >= n && heads <= BEAM_COUNTED) {
+    for (int64_t i = tid; i < heads; i += BEAM_THREADS) {
       BeamKey c;
-      beam_none(c);
-      if (ended && ended[b * e_sb + k]) {
-        if (i == k * per) {
-          c.c = score;
-          c.at = static_cast<uint64_t>(k) << 32 | static_cast<uint32_t>(pad);
-        }
-      } else {
-        const uint64_t key = w.key[static_cast<int64_t>(b) * all + i];
-        if (key) {
-          c.c = (static_cast<double>(beam_value(static_cast<uint32_t>(key >> 32))) - s_lse[k]) + score;
-          c.at = static_cast<uint64_t>(k) << 32 | (0xffffffffu - static_cast<uint32_t>(key));
-        }
-      }
-      if (c.c > -INFINITY && beam_before(c, cut)) list[atomicAdd(&s_count, 1)] = c;
+      if (candidate(i * n, c)) list[atomicAdd(&s_count, 1)] = c;
     }
     __syncthreads();
-    if (s_count > BEAM_JOIN_CAP - BEAM_THREADS) {
-      beam_sort(list, s_count);
+    const int count = s_count;
+    beam_best(list, count, n, [&](int place, const BeamKey& c) {
+      if (place == n - 1) s_cut = c;
+    });
+    __syncthreads();
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+  }
+  BeamKey cut = s_cut;   // candidates after it are out
+  for (int64_t at = 0; at < all; at += BEAM_THREADS) {
+    const int64_t i = at + tid;
+    BeamKey c;
+    if (i < all && candidate(i, c) && !beam_before(cut, c)) list[atomicAdd(&s_count, 1)] = c;
+    if (all <= BEAM_JOIN_CAP) continue;
+    __syncthreads();
+    const int count = s_count;
+    if (count > BEAM_JOIN_CAP - BEAM_THREADS) {
+      beam_sort(list, count);
       cut = list[n - 1];
       if (tid == 0) s_count = n;
-      __syncthreads();
     }
+    __syncthreads();
   }
+  __syncthreads();
   const int count = s_count;
-  beam_sort(list, count);
-  for (int i = tid; i < n; i += BEAM_THREADS) {
-    const int64_t o = static_cast<int64_t>(b) * n + i;
-    const bool some = i < count;
-    out_score[o] = some ? static_cast<float>(list[i].c) : -INFINITY;
-    out_beam[o] = some ? static_cast<int32_t>(list[i].at >> 32) : -1;
-    out_token[o] = some ? static_cast<int32_t>(static_cast<uint32_t>(list[i].at)) : -1;
+  const int64_t o = static_cast<int64_t>(b) * n;
+  beam_best(list, count, n, [&](int place, const BeamKey& c) {
+    out_score[o + place] = static_cast<float>(c.c);
+    out_beam[o + place] = static_cast<int32_t>(c.at >> 32);
+    out_token[o + place] = static_cast<int32_t>(static_cast<uint32_t>(c.at));
+  });
+  for (int i = count + tid; i < n; i += BEAM_THREADS) {
+    out_score[o + i] = -INFINITY;
+    out_beam[o + i] = -1;
+    out_token[o + i] = -1;
   }
 }
 
@@ -252,9 +400,11 @@ static int beam_check(const char* what, int64_t batch, int64_t beams, int64_t vo
 static int64_t beam_carve(int64_t batch, int64_t beams, int64_t vocab, int64_t n, uint8_t* base,
                           BeamWork* w) {
   const int64_t rows = batch * beams;
-  int64_t slices = rows ? (sm_count() * 4 + rows - 1) / rows : 1;
-  const int64_t most = (vocab + 2047) / 2048;
+  // One wave of four CTAs an SM; slices of at least a round of 4096 tokens.
+  int64_t slices = rows ? sm_count() * 4 / rows : 1;
+  const int64_t most = (vocab + 4095) / 4096;
   if (slices > most) slices = most;
+  if (slices < 1) slices = 1;
   w->slice = ((vocab + slices - 1) / slices + 7) / 8 * 8;
   w->slices = static_cast<int>((vocab + w->slice - 1) / w->slice);
   int64_t at = 0;

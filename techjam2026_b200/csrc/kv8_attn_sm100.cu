@@ -72,12 +72,22 @@ struct KV8Work {
 struct KV8Groups {
   const int32_t* starts;  // [N + 1]: group n is the sequences starts[n] .. starts[n + 1] - 1
   const int32_t* shared;  // [N]: tokens its table rows have in common
+  const int32_t* live;    // [B + 1]: new tokens of the sequences before; null: T of each
   int N;
   int max_shared;         // whole pages
   int max_own;
   int tiles;              // row tiles of all groups, at most
   int chunks, chunk;      // parts of the shared tokens; KV8Work has those of the others
   int own_tiles;          // row tiles of a sequence
+  // Of kv8_groups_kernel, for the tensor-memory kernel (null otherwise):
+  const int4* group;      // [N]: shared tokens, rows, first sequence, one past the last
+  const int64_t* work;    // [N + 1]: steps of the groups before; then a CTA's steps
+  const int4* record;     // [ctas][2]: where a CTA begins: the group's entry, and {item,
+                          // step, steps of an item, part}; item = row tile * H + head
+  const int32_t* of_seq;  // [B]: tokens that a sequence shares
+  int32_t* used;          // [B * H][rows]: parts of the shared tokens that a row has
+  int least;              // steps of a part, at least
+  bool paired;            // the kernel of the own tokens follows that of the shared ones
 };
 
 // The sequences of group n; none (recorded) where starts is out of order.
@@ -98,18 +108,42 @@ __device__ __forceinline__ int kv8_group_tokens(const KV8& c, const KV8Groups& g
   s = __reduce_min_sync(0xffffffffu, s);
   return s & ~(c.P - 1);
 }
-// Group and tile of the index-th tile of `tile` rows, `per` rows a sequence;
-// n < 0: there are fewer. All lanes of a warp call this together.
+// Query rows of a group's sequences: the rows of their new tokens one after
+// another, or where `live` is null `per` rows of each (with tokens past counts).
+__device__ __forceinline__ int kv8_group_rows(const KV8Groups& gr, int2 seq, int per, int G) {
+  return gr.live ? (__ldg(gr.live + seq.y) - __ldg(gr.live + seq.x)) * G : (seq.y - seq.x) * per;
+}
+// Sequence (x, counted from the group's first) and row within it (y) of a row.
+__device__ __forceinline__ int2 kv8_group_row(const KV8Groups& gr, int2 seq, int per, int G,
+                                              int row) {
+  if (!gr.live) {
+    const int m = row / per;
+    return make_int2(m, row - m * per);
+  }
+  const int first = __ldg(gr.live + seq.x), tok = row / G;
+  int lo = seq.x, hi = seq.y;       // the last sequence that begins at or before tok
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(gr.live + mid) - first <= tok)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return make_int2(lo - seq.x, row - (__ldg(gr.live + lo) - first) * G);
+}
+// Group and tile of the index-th tile of `tile` rows; n < 0: there are fewer. All
+// lanes of a warp call this together.
 struct KV8GroupTile {
-  int n, tile;
+  int n, tile, rows;
   int2 seq;
 };
-__device__ __forceinline__ KV8GroupTile kv8_group_tile(const KV8Groups& gr, int B, int per,
+__device__ __forceinline__ KV8GroupTile kv8_group_tile(const KV8Groups& gr, int B, int per, int G,
                                                        int tile, int index) {
   const int lane = threadIdx.x & 31;
   for (int base = 0; base < gr.N; base += 32) {
     const int2 seq = base + lane < gr.N ? kv8_group(gr, B, base + lane) : make_int2(0, 0);
-    const int tiles = ((seq.y - seq.x) * per + tile - 1) / tile;
+    const int rows = kv8_group_rows(gr, seq, per, G);
+    const int tiles = (rows + tile - 1) / tile;
     int sum = tiles;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -122,16 +156,18 @@ __device__ __forceinline__ KV8GroupTile kv8_group_tile(const KV8Groups& gr, int 
       KV8GroupTile t;
       t.n = base + l;
       t.tile = index - __shfl_sync(0xffffffffu, sum - tiles, l);
+      t.rows = __shfl_sync(0xffffffffu, rows, l);
       t.seq.x = __shfl_sync(0xffffffffu, seq.x, l);
       t.seq.y = __shfl_sync(0xffffffffu, seq.y, l);
       return t;
     }
     index -= __shfl_sync(0xffffffffu, sum, 31);
   }
-  return KV8GroupTile{-1, 0, make_int2(0, 0)};
+  return KV8GroupTile{-1, 0, 0, make_int2(0, 0)};
 }
 // Tokens that sequence b shares with its group (0: it is in none).
 __device__ __forceinline__ int kv8_shared_of(const KV8& c, const KV8Groups& gr, int b) {
+  if (gr.of_seq) return __ldg(gr.of_seq + b);
   const int lane = threadIdx.x & 31;
   for (int base = 0; base < gr.N; base += 32) {
     const int2 seq = base + lane < gr.N ? kv8_group(gr, c.B, base + lane) : make_int2(0, 0);
@@ -143,6 +179,32 @@ __device__ __forceinline__ int kv8_shared_of(const KV8& c, const KV8Groups& gr, 
     }
   }
   return 0;
+}
+
+// The kernel of the own tokens starts without waiting for that of the shared
+// ones, which waited for everything earlier before it let it start. It ends
+// after it, so that the join has to wait for one kernel.
+__device__ __forceinline__ void kv8_end_of_pair(const KV8Groups& gr) {
+  if (gr.tiles == 0 && gr.paired) pdl_wait();
+}
+// Empty parts in the places of the shared tokens, or none, for rows that share
+// nothing.
+__device__ __forceinline__ void kv8_no_shared_parts(const KV8& c, const KV8Groups& gr,
+                                                    const KV8Work& w, int b, int h, int row0,
+                                                    int tile, int threads) {
+  if (gr.used) {
+    for (int u = threadIdx.x; u < tile && row0 + u < w.rows; u += threads)
+      gr.used[static_cast<int64_t>(b * c.H + h) * w.rows + row0 + u] = 0;
+    return;
+  }
+  for (int u = threadIdx.x; u < tile * gr.chunks; u += threads) {
+    const int row = row0 + u / gr.chunks;
+    if (row >= w.rows) break;
+    const int64_t at =
+        (static_cast<int64_t>(b * c.H + h) * w.rows + row) * w.chunks + u % gr.chunks;
+    w.ref[at] = -INFINITY;
+    w.sum[at] = 0.f;
+  }
 }
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -364,9 +426,9 @@ __device__ __forceinline__ void score_tile(const QFrag<DH, QP, RH>& q, const KBy
   }
 }
 
-// QP, PP: fp16 planes of q and of P. SH: the call has groups; the CTAs (x) are then
-// [row tile of a group][part of its shared tokens], then [sequence][row tile]
-// [part of its own tokens], and y is the kv head.
+// QP, PP: fp16 planes of q and of P. SH: the call has groups; y is then the kv head,
+// and the CTAs (x) are [row tile of a group][part of its shared tokens] (none if
+// gr.tiles is 0), then [sequence][row tile][part of its own tokens].
 template <int DH, int FMT, int QP, int PP, int RH, bool SH>
 __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     kv8_split_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh, int64_t q_st,
@@ -381,8 +443,16 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
   __shared__ float s_vmax[4];
   extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ float s_ref[4][KV8_ROWS], s_sum[4][KV8_ROWS];
-  pdl_launch_dependents();
-  pdl_wait();
+  __shared__ int2 s_row[SH ? KV8_ROWS : 1];
+  // The kernel of the own tokens alone runs beside that of the shared ones
+  // (kv8_end_of_pair).
+  if constexpr (!SH) {
+    pdl_launch_dependents();
+    pdl_wait();
+  } else {
+    if (gr.tiles > 0 || !gr.paired) pdl_wait();
+    pdl_launch_dependents();
+  }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
   int chunk, row0, h, b;    // b: whose table row has the pages (the group's first sequence)
@@ -424,23 +494,27 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     int i = blockIdx.x;
     if (i < gr.tiles * gr.chunks) {
       chunk = i % gr.chunks;
-      const KV8GroupTile t = kv8_group_tile(gr, c.B, w.rows, KV8_ROWS, i / gr.chunks);
-      if (t.n < 0) return;
-      b = t.seq.x;
-      row0 = t.tile * KV8_ROWS;
-      rows = (t.seq.y - t.seq.x) * w.rows;
+      const KV8GroupTile tl = kv8_group_tile(gr, c.B, w.rows, G, KV8_ROWS, i / gr.chunks);
+      if (tl.n < 0) return;
+      b = tl.seq.x;
+      row0 = tl.tile * KV8_ROWS;
+      rows = tl.rows;
       // every row of a sequence that takes its token sees all that is shared
-      end = kv8_group_tokens(c, gr, t.n, t.seq);
-      if (end == 0) return;  // the sequences' own CTAs leave the empty parts
-#pragma unroll
-      for (int r = 0; r < RH; ++r) {
-        const int row = row0 + g + 8 * r;
-        const int m = row / w.rows;
-        limit[r] =
-            row < rows && (row - m * w.rows) / G < kv8_count(c, counts, b + m, T) ? end : 0;
-      }
+      end = kv8_group_tokens(c, gr, tl.n, tl.seq);
       k0 = chunk * gr.chunk;
       k1 = min(k0 + gr.chunk, end);
+      if (end == 0) return;  // the sequences' own CTAs leave the empty parts
+      if (tid < KV8_ROWS && row0 + tid < rows)
+        s_row[tid] = kv8_group_row(gr, tl.seq, w.rows, G, row0 + tid);
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < RH; ++r) {
+        limit[r] = 0;
+        if (row0 + g + 8 * r < rows) {
+          const int2 at = s_row[g + 8 * r];
+          if (at.y / G < kv8_count(c, counts, b + at.x, T)) limit[r] = end;
+        }
+      }
     } else {
       i -= gr.tiles * gr.chunks;
       const int own = w.chunks - gr.chunks;
@@ -463,29 +537,22 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
         const int tok = row / G;
         limit[r] = (row < rows && tok < count) ? (causal ? min(len + tok + 1, end) : end) : 0;
       }
+      if (tid < KV8_ROWS) s_row[tid] = make_int2(0, row0 + tid);
+      __syncthreads();
       const int last_row = min(row0 + KV8_ROWS, rows) - 1;
       const int last_tok = min(last_row / G, count - 1);
       const int reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
       k0 = shared + chunk * w.chunk;
       k1 = min(k0 + w.chunk, reach);
-      if (shared == 0 && chunk == 0) {
-        for (int u = tid; u < KV8_ROWS * gr.chunks; u += 128) {
-          const int row = row0 + u / gr.chunks;
-          if (row >= rows) break;
-          const int64_t at =
-              (static_cast<int64_t>(b * c.H + h) * w.rows + row) * w.chunks + u % gr.chunks;
-          w.ref[at] = -INFINITY;
-          w.sum[at] = 0.f;
-        }
-      }
+      if (shared == 0 && chunk == 0) kv8_no_shared_parts(c, gr, w, b, h, row0, KV8_ROWS, 128);
       chunk += gr.chunks;
     }
   }
   // Where a row's numbers are: [B * H][rows of a sequence]
   auto spot = [&](int row) -> int64_t {
     if constexpr (!SH) return static_cast<int64_t>(blockIdx.z) * w.rows + row;
-    const int m = row / w.rows;
-    return static_cast<int64_t>((b + m) * c.H + h) * w.rows + (row - m * w.rows);
+    const int2 at = s_row[SH ? row - row0 : 0];
+    return static_cast<int64_t>((b + at.x) * c.H + h) * w.rows + at.y;
   };
   const bool alone = w.chunks == 1;
   if (k0 >= k1 && !alone) {
@@ -496,6 +563,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
         w.ref[at] = -INFINITY;
         w.sum[at] = 0.f;
       }
+    if constexpr (SH) kv8_end_of_pair(gr);
     return;
   }
   const int j0 = k0 >> c.p_shift;
@@ -511,8 +579,12 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
   }
   QFrag<DH, QP, RH> qa;
   qa.load(q, [&](int row) {
-    const int m = SH ? row / w.rows : 0;
-    if constexpr (SH) row -= m * w.rows;
+    int m = 0;
+    if constexpr (SH) {
+      const int2 at = s_row[row - row0];
+      m = at.x;
+      row = at.y;
+    }
     const int tok = row / G;
     return (b + m) * q_sb + static_cast<int64_t>(h * G + row - tok * G) * q_sh + tok * q_st;
   }, dtype, vec != 0, row0, rows, scale_log2);
@@ -757,6 +829,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
       }
     }
   }
+  if constexpr (SH) kv8_end_of_pair(gr);
 }
 
 // ---------------------------------------------------------------- join
@@ -826,6 +899,216 @@ __global__ void __launch_bounds__(KV8_JOIN_THREADS)
         lse_out[(static_cast<int64_t>(b) * c.H * G + hq) * T + tok] = l2 * 0.6931471805599453f;
       if (w.lse) w.lse[static_cast<int64_t>(bh) * w.rows + row] = l2;
     }
+  }
+}
+
+// The parts of calls with groups: D / 4 lanes a row, so that many rows join at
+// once (a CTA a row took 68 us for 30720 rows of 64, 17 for 2048 rows of 17 parts).
+// Rows of tokens past counts are zeros.
+__global__ void __launch_bounds__(KV8_JOIN_THREADS)
+    kv8_join_rows_kernel(KV8 c, void* __restrict__ out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+                         int dtype, int vec, const int32_t* __restrict__ counts, int T, int G,
+                         float* __restrict__ lse_out, KV8Work w, KV8Groups gr) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int shift = c.d_shift - 2;                  // lanes of a row, as a power of two
+  const int l = threadIdx.x & ((1 << shift) - 1);
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * KV8_JOIN_THREADS + threadIdx.x) >> shift;
+  const int64_t all = static_cast<int64_t>(c.B) * c.H * w.rows;
+  if (at >= all) return;                            // (whole rows leave together)
+  const int bh = static_cast<int>(at / w.rows), row = static_cast<int>(at - static_cast<int64_t>(bh) * w.rows);
+  const int b = bh / c.H, h = bh - b * c.H;
+  const int tok = row / G, hq = h * G + row - tok * G;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f, top = -INFINITY;
+  if (tok < kv8_count(c, counts, b, T)) {
+    const float* ref = w.ref + at * w.chunks;
+    const float* part_sum = w.sum + at * w.chunks;
+    const float* part = w.part + at * w.chunks * c.D + 4 * l;
+    // (within its room, whatever a kernel that gave up has left)
+    const int used = gr.used ? min(max(gr.used[at], 0), gr.chunks) : gr.chunks;
+    // then the parts of the own tokens
+    const int n = used + w.chunks - gr.chunks, skip = gr.chunks - used;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) top = fmaxf(top, ref[i < used ? i : i + skip]);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const int i = j < used ? j : j + skip;
+      const float r = ref[i], s = part_sum[i];
+      const float a = top == -INFINITY ? 1.f : fast_exp2(r - top);
+      sum += a * s;
+      // an empty part was not written (its sum is 0; a NaN sum has a part)
+      if (!(r == -INFINITY && s == 0.f)) {
+        const float4 y = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(i) * c.D);
+        x[0] += a * y.x;
+        x[1] += a * y.y;
+        x[2] += a * y.z;
+        x[3] += a * y.w;
+      }
+    }
+  }
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) x[u] = sum == 0.f ? 0.f : x[u] * f;
+  const int64_t o = b * o_sb + hq * o_sh + tok * o_st + 4 * l;
+  if (!vec) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) kv8_store1(out, o + u, dtype, x[u]);
+  } else if (dtype == KF_DT_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + o) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    uint2 y;
+    if (dtype == KF_DT_BF16) {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(x[0], x[1]), q = __floats2bfloat162_rn(x[2], x[3]);
+      y = make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+    } else {
+      y = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o) = y;
+  }
+  if (l == 0 && lse_out)
+    lse_out[(static_cast<int64_t>(b) * c.H * G + hq) * T + tok] =
+        sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+// What the tensor-memory kernel goes by: each group's shared tokens, rows and
+// steps (128 keys of a tile of `tile` rows and a kv head), what each sequence
+// shares, (live) the rows of new tokens, and where its CTAs begin. One CTA, a warp a
+// group at a time; latency is all it costs, so the groups stay in shared memory.
+constexpr int KV8_GROUPS_MAX = 1024;
+constexpr int KV8_GROUPS_THREADS = 256;
+
+__global__ void __launch_bounds__(KV8_GROUPS_THREADS)
+    kv8_groups_kernel(KV8 c, const int32_t* __restrict__ counts, int T, int G, int per, int tile,
+                      KV8Groups gr, int4* __restrict__ group, int64_t* __restrict__ work,
+                      int4* __restrict__ record, int ctas, int32_t* __restrict__ of_seq,
+                      int32_t* __restrict__ live) {
+  constexpr int WARPS = KV8_GROUPS_THREADS / 32;
+  __shared__ int4 s_g[KV8_GROUPS_MAX];
+  __shared__ int64_t s_work[KV8_GROUPS_MAX + 1];
+  __shared__ int s_sum[WARPS], s_share, s_whole;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int before = 0;
+  for (int base = 0; base < c.B; base += KV8_GROUPS_THREADS) {
+    const int b = base + tid;
+    if (b < c.B) of_seq[b] = 0;
+    if (!live) continue;
+    int sum = b < c.B ? kv8_count(c, counts, b, T) : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = sum;
+    __syncthreads();
+    int all = 0;
+    for (int u = 0; u < WARPS; ++u) {
+      if (u < warp) sum += s_sum[u];
+      all += s_sum[u];
+    }
+    if (b < c.B) live[b + 1] = before + sum;
+    before += all;
+  }
+  if (live && tid == 0) live[0] = 0;
+  __syncthreads();
+  for (int n = warp; n < gr.N; n += WARPS) {
+    const int2 seq = kv8_group(gr, c.B, n);
+    const int shared = seq.x < seq.y ? kv8_group_tokens(c, gr, n, seq) : 0;
+    const int rows = live ? (live[seq.y] - live[seq.x]) * G : (seq.y - seq.x) * per;
+    if (lane == 0) group[n] = s_g[n] = make_int4(shared, rows, seq.x, seq.y);
+    if (shared)
+      for (int b = seq.x + lane; b < seq.y; b += 32) of_seq[b] = shared;
+  }
+  __syncthreads();
+  auto items_of = [&](const int4& g) -> int {
+    return g.x ? (g.y + tile - 1) / tile * c.H : 0;
+  };
+  auto steps_of = [&](const int4& g) -> int { return (g.x + 127) / 128; };
+  if (warp == 0) {
+    int64_t total = 0;
+    int items = 0;
+    for (int n = lane; n < gr.N; n += 32) {
+      const int64_t i = items_of(s_g[n]);
+      total += i * steps_of(s_g[n]);
+      items += static_cast<int>(min(i, static_cast<int64_t>(ctas) + 1));
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    items = __reduce_add_sync(0xffffffffu, items);
+    // A CTA's steps: an equal share of all of them, which may end one tile and begin
+    // the next; or, where that costs less (a stretch's start and end take about five
+    // steps), one stretch each: the shortest that needs no more CTAs than there are.
+    const int64_t even = max(static_cast<int64_t>(gr.least), (total + ctas - 1) / ctas);
+    int64_t share = even;
+    bool whole = false;
+    if (items <= ctas) {
+      int lo = static_cast<int>(even), hi = max(lo, (gr.max_shared + 127) / 128);
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        int need = 0;
+        for (int n = lane; n < gr.N; n += 32)
+          need += items_of(s_g[n]) * ((steps_of(s_g[n]) + mid - 1) / mid);
+        need = __reduce_add_sync(0xffffffffu, need);
+        if (need <= ctas)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      whole = lo <= even + 5;
+      if (whole) share = lo;
+    }
+    // Steps of the groups before; with one stretch a CTA, those of an item made full.
+    int64_t sum = 0;
+    for (int base = 0; base < gr.N; base += 32) {
+      int64_t x = 0;
+      if (base + lane < gr.N) {
+        const int4 g = s_g[base + lane];
+        const int64_t steps = steps_of(g);
+        x = items_of(g) * (whole ? (steps + share - 1) / share * share : steps);
+      }
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += o;
+      }
+      if (base + lane < gr.N) s_work[base + lane + 1] = work[base + lane + 1] = sum + x;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) {
+      s_work[0] = work[0] = 0;
+      work[gr.N + 1] = whole ? -share : share;
+      // (a share is at most a tile's steps, or an even one; both fit)
+      s_share = static_cast<int>(min(share, static_cast<int64_t>(INT32_MAX)));
+      s_whole = whole;
+    }
+  }
+  __syncthreads();
+  const int share = s_share;
+  for (int i = tid; i < ctas; i += KV8_GROUPS_THREADS) {
+    const int64_t at = static_cast<int64_t>(i) * share;
+    int4 g = make_int4(0, 0, 0, 0), r = make_int4(0, 0, 1, 0);
+    if (at < s_work[gr.N]) {
+      int lo = 0, hi = gr.N;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_work[mid] <= at)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      g = s_g[lo];
+      const int64_t off = at - s_work[lo];
+      r.z = steps_of(g);
+      if (s_whole) r.z = (r.z + share - 1) / share * share;
+      r.x = static_cast<int>(off / r.z);
+      r.y = static_cast<int>(off - static_cast<int64_t>(r.x) * r.z);
+      r.w = static_cast<int>(i - (at - r.y) / share);
+    }
+    record[2 * i] = g;
+    record[2 * i + 1] = r;
   }
 }
 

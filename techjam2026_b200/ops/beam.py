@@ -58,33 +58,33 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
                          f"{MAX_TAKE}, got {K}, {V} and {n}")
     if not 0 <= pad < 2 ** 31:
         raise ValueError(f"{what}: pad must be a token, got {pad}")
-    for t, name in ((scores, "scores"), (ended, "ended")):
-        if t is None:
-            continue
-        if t.shape != (B, K) or (K > 1 and t.stride(1) != 1):
-            raise ValueError(f"{what}: {name} must be [{B}, {K}] with unit stride along the beams")
-        if t.device != logits.device:
-            raise ValueError(f"{what}: {name} must be on {logits.device}, got {t.device}")
+    index = logits.get_device()
+    for t in (scores,) if ended is None else (scores, ended):
+        if t.shape != (B, K) or (K > 1 and t.stride(1) != 1) or t.get_device() != index:
+            raise ValueError(f"{what}: scores and ended must be [{B}, {K}] with unit stride along the "
+                             f"beams, on {logits.device}; got {tuple(t.shape)}, strides {t.stride()}, "
+                             f"on {t.device}")
     if V > 1 and logits.stride(2) != 1:
         raise ValueError(f"{what}: logits need unit stride along the vocabulary")
     if ended is not None and ended.dtype is not torch.bool:
         raise TypeError(f"{what}: ended must be bool, got {ended.dtype}")
-    index = logits.get_device()
     if index != torch.cuda.current_device():
         raise RuntimeError(f"{what}: logits are on {logits.device}, which is not the current device")
     dev = logits.device
-    out_score = torch.empty((B, n), dtype=torch.float32, device=dev)
-    out = torch.empty((2, B, n), dtype=torch.int32, device=dev)
+    score = torch.empty((B, n), dtype=torch.float32, device=dev)
+    beam = torch.empty((B, n), dtype=torch.int32, device=dev)
+    token = torch.empty((B, n), dtype=torch.int32, device=dev)
     L = _lib.lib()
     need = L.kf_beam_select_workspace_bytes(B, K, V, n)
     if need < 0:
         raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    sb, sk, _ = logits.stride()
     rc = L.kf_beam_select(
-        logits.data_ptr(), logits.stride(0), logits.stride(1), code, scores.data_ptr(),
-        scores.stride(0), ended.data_ptr() if ended is not None else None,
-        ended.stride(0) if ended is not None else 0, B, K, V, n, pad, out_score.data_ptr(),
-        out[0].data_ptr(), out[1].data_ptr(), work.data_ptr() if work is not None else None, need,
+        logits.data_ptr(), sb, sk, code, scores.data_ptr(), scores.stride(0),
+        ended.data_ptr() if ended is not None else None,
+        ended.stride(0) if ended is not None else 0, B, K, V, n, pad, score.data_ptr(),
+        beam.data_ptr(), token.data_ptr(), work.data_ptr() if work is not None else None, need,
         torch._C._cuda_getCurrentRawStream(index))
     _lib.check(rc, "kf_beam_select")
-    return out_score, out[0], out[1]
+    return score, beam, token

@@ -70,7 +70,7 @@ class KV8Cache:
     """
 
     __slots__ = ("k", "v", "scale", "table", "lens", "weight", "struct", "batch", "kv_heads",
-                 "head_dim", "block", "device", "_ref", "_work")
+                 "head_dim", "block", "device", "_ref", "_ptr", "_kind", "_work")
     _TENSORS = frozenset(("k", "v", "scale", "table", "lens", "weight"))
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, scale: torch.Tensor, table: torch.Tensor,
@@ -104,6 +104,8 @@ class KV8Cache:
             pages, table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1],
             table.shape[0], heads, head_dim, block, CODE_DTYPES[k.dtype])
         self._ref = ctypes.byref(self.struct)
+        self._ptr = ctypes.pointer(self.struct)
+        self._kind = (k.dtype, heads, block, head_dim, k.get_device())
         self.batch, self.kv_heads, self.block, self.head_dim = table.shape[0], heads, block, head_dim
         self.device = k.device
         self._work = {}              # workspace bytes by (type, T, heads, max_len, flags)
@@ -133,7 +135,8 @@ class KV8Cache:
         struct.blocks, struct.batch = blocks, batch
         new = object.__new__(KV8Cache)
         put = object.__setattr__
-        for name in ("k", "v", "scale", "weight", "kv_heads", "block", "head_dim", "device"):
+        for name in ("k", "v", "scale", "weight", "kv_heads", "block", "head_dim", "device",
+                     "_kind"):
             put(new, name, getattr(self, name))
         put(new, "table", table)
         put(new, "lens", lens)
@@ -141,6 +144,7 @@ class KV8Cache:
         put(new, "_work", {})
         put(new, "struct", struct)
         put(new, "_ref", ctypes.byref(struct))
+        put(new, "_ptr", ctypes.pointer(struct))
         return new
 
     @classmethod
@@ -379,14 +383,16 @@ def kv8_attention_shared(q: torch.Tensor, cache: KV8Cache, starts: torch.Tensor,
         raise ValueError(f"{what}: out must have q's shape and type and unit stride along "
                          "head_dim")
     stream = _check_call(what, cache, counts, q, out)
-    for t, name in ((starts, "starts"), (shared, "shared")):
-        if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() \
-                or t.get_device() != cache.device.index:
-            raise ValueError(f"{what}: {name} must be a contiguous int32 tensor on {cache.device}")
-    groups = shared.shape[0]
-    if starts.shape[0] != groups + 1:
-        raise ValueError(f"{what}: starts must have one entry more than shared, got "
-                         f"{starts.shape[0]} and {groups}")
+    groups = shared.shape[0] if shared.dim() == 1 else -1
+    index = q.get_device()
+    if starts.dtype is not torch.int32 or shared.dtype is not torch.int32 \
+            or starts.shape != (groups + 1,) or not starts.is_contiguous() \
+            or not shared.is_contiguous() or starts.get_device() != index \
+            or shared.get_device() != index:
+        raise ValueError(f"{what}: starts and shared must be contiguous int32 tensors [N + 1] and [N] "
+                         f"on {cache.device}, got {starts.dtype} {tuple(starts.shape)} on "
+                         f"{starts.device} and {shared.dtype} {tuple(shared.shape)} on "
+                         f"{shared.device}")
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
     flags = _lib.KF_KV8_CAUSAL if causal else 0
     L = _lib.lib()
@@ -415,8 +421,7 @@ Caches = Union[KV8Cache, Sequence[KV8Cache]]
 
 
 def _refs(caches: Sequence[KV8Cache]):
-    return (ctypes.POINTER(_lib.KV8CacheStruct) * len(caches))(
-        *(ctypes.pointer(c.struct) for c in caches))
+    return (ctypes.POINTER(_lib.KV8CacheStruct) * len(caches))(*[c._ptr for c in caches])
 
 
 def kv8_copy(cache: Caches, src: torch.Tensor, dst: torch.Tensor,
@@ -443,23 +448,25 @@ def kv8_copy(cache: Caches, src: torch.Tensor, dst: torch.Tensor,
     if len(to) != len(caches):
         raise ValueError(f"{what}: {len(caches)} caches into {len(to)}")
     first = caches[0]
-    for c in caches + to:
-        if c.device != first.device:
-            raise ValueError(f"{what}: all caches must be on one device")
-        if c.k.dtype != first.k.dtype or c.k.shape[1:] != first.k.shape[1:]:
-            raise ValueError(f"{what}: all caches must have the codes, heads, block and head_dim of "
-                             "the first")
+    kind, index = first._kind, first._kind[4]
+    for c in caches if into is None else caches + to:
+        if c._kind != kind:
+            raise ValueError(f"{what}: all caches must have the codes, heads, block, head_dim and "
+                             "device of the first")
     stream = _check_call(what, first, None)
-    n = src.shape[0] if src.dim() == 1 else -1
-    for t, name in ((src, "src"), (dst, "dst"), (tokens, "tokens")):
-        if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n
-                              or not t.is_contiguous() or t.get_device() != first.device.index):
+    shape = src.shape
+    for t in (src, dst) if tokens is None else (src, dst, tokens):
+        if t.dtype is not torch.int32 or t.shape != shape or len(shape) != 1 \
+                or not t.is_contiguous() or t.get_device() != index:
             raise ValueError(f"{what}: src, dst and tokens must be contiguous int32 tensors [n] on "
-                             f"{first.device}; {name} is {t.dtype} {tuple(t.shape)} on {t.device}")
+                             f"{first.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    n = shape[0]
     L = _lib.lib()
-    need = L.kf_kv8_copy_workspace_bytes(first._ref, to[0]._ref, n)
-    if need < 0:
-        raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
+    need = 0
+    if n > 256:                  # few pairs need no workspace
+        need = L.kf_kv8_copy_workspace_bytes(first._ref, to[0]._ref, n)
+        if need < 0:
+            raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
     work = torch.empty(need, dtype=torch.uint8, device=first.device) if need else None
     refs = _refs(caches)
     rc = L.kf_kv8_copy(refs, refs if into is None else _refs(to), len(caches), src.data_ptr(),
