@@ -13,6 +13,7 @@ constexpr int BEAM_THREADS = 256;
 constexpr int BEAM_MAX = 128;    // candidates of a call
 constexpr int BEAM_CAP = 4096;   // keys that the first kernel's list holds
 constexpr int BEAM_JOIN_CAP = 2048;
+constexpr float BEAM_LOG2E = 1.4426950408889634f;
 
 struct BeamWork {
   uint64_t* key;   // [rows][slices][n]: a logit in order, then the complement of its index; 0: none
@@ -31,20 +32,25 @@ __device__ __forceinline__ float beam_value(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 
-// A candidate of the second kernel.
+// A candidate of the second kernel: its fp64 value as an integer in the same order,
+// then the complements of beam and token. 0: none.
 struct alignas(16) BeamKey {
-  double c;
-  uint64_t at;     // beam << 32 | token
+  uint64_t c;
+  uint64_t at;
 };
+__device__ __forceinline__ uint64_t beam_order(double x) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x + 0.0));  // (-0 and +0 are one)
+  return (u >> 63) ? ~u : (u | (1ull << 63));
+}
+__device__ __forceinline__ double beam_value(uint64_t o) {
+  return __longlong_as_double(static_cast<long long>((o >> 63) ? (o ^ (1ull << 63)) : ~o));
+}
 __device__ __forceinline__ bool beam_before(const BeamKey& a, const BeamKey& b) {
-  return a.c > b.c || (a.c == b.c && a.at < b.at);
+  return a.c > b.c || (a.c == b.c && a.at > b.at);
 }
 __device__ __forceinline__ bool beam_before(uint64_t a, uint64_t b) { return a > b; }
 __device__ __forceinline__ void beam_none(uint64_t& k) { k = 0; }
-__device__ __forceinline__ void beam_none(BeamKey& k) {
-  k.c = -INFINITY;
-  k.at = ~0ull;
-}
+__device__ __forceinline__ void beam_none(BeamKey& k) { k.c = k.at = 0; }
 
 // Sorts the first `count` of a list in shared memory, best first. The list has
 // room up to the next power of two. All threads of the CTA.
@@ -125,6 +131,33 @@ __device__ __forceinline__ void beam_load(const void* logits, int64_t base, int6
   v = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The largest number of a 16-byte run (NaN if it has none), and its u-th one.
+template <int DT>
+struct BeamMax {
+  __device__ __forceinline__ static float of(const uint4& v) {
+    if constexpr (DT == KF_DT_F32) {
+      return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                   fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    } else if constexpr (DT == KF_DT_BF16) {
+      auto h = [](const uint32_t& w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+      const __nv_bfloat162 m = __hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w)));
+      return fmaxf(__low2float(m), __high2float(m));
+    } else {
+      auto h = [](const uint32_t& w) { return *reinterpret_cast<const __half2*>(&w); };
+      const __half2 m = __hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w)));
+      return fmaxf(__low2float(m), __high2float(m));
+    }
+  }
+  __device__ __forceinline__ static float at(const uint4& v, int u) {
+    const int i = DT == KF_DT_F32 ? u : u >> 1;
+    const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+    if constexpr (DT == KF_DT_F32) return __uint_as_float(w);
+    const uint32_t h = (u & 1) ? w >> 16 : w & 0xffffu;
+    if constexpr (DT == KF_DT_BF16) return __uint_as_float(h << 16);
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(h)));
+  }
+};
+
 // Keys of the n best tokens of a slice, at the front of the list; how many.
 template <int DT>
 __device__ __noinline__ int beam_careful(uint64_t* list, int* s_count, const void* logits,
@@ -165,7 +198,6 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
                      const uint8_t* __restrict__ ended, int64_t e_sb, int beams, int64_t vocab,
                      int n, BeamWork w) {
   constexpr int N = KV8Type<DT>::N, U = 4;
-  constexpr float LOG2E = 1.4426950408889634f;
   __shared__ uint64_t list[BEAM_CAP];
   __shared__ __align__(16) uint32_t s_max[BEAM_THREADS];
   __shared__ uint32_t s_cut;
@@ -182,74 +214,116 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
   const int64_t first = blockIdx.x * w.slice;
   const int64_t last = first + w.slice < vocab ? first + w.slice : vocab;
   const int64_t base = b * l_sb + k * l_sk;
-  float top = -INFINITY, sum = 0.f;
+  float top = -INFINITY;
+  uint64_t sum = f2_pack(0.f, 0.f);  // two sums
   float cut = -INFINITY;   // logits below it are out, and those equal to it after the first round
-  if (tid == 0) {
-    s_count = 0;
-    s_cut = 0;
-  }
-  for (int64_t at = first; at < last; at += U * N * BEAM_THREADS) {
-    uint4 v[U];
-#pragma unroll
-    for (int r = 0; r < U; ++r)
-      beam_load<DT>(logits, base, at + (r * BEAM_THREADS + tid) * N, last, vec != 0, v[r]);
+  if (tid == 0) s_count = 0;   // (a barrier comes before it is used)
+  // The n-th largest of the threads' numbers: at least n logits are not below it.
+  // -inf if there are fewer.
+  auto bound = [&](float most) -> float {
+    const uint32_t mine = most > -INFINITY ? beam_order(most) : 0u;
+    s_max[tid] = mine;
+    if (tid == 0) s_cut = 0xffffffffu;
+    __syncthreads();
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < BEAM_THREADS; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(s_max + j);
+      above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+    }
+    if (above < n) atomicMin(&s_cut, mine);
+    __syncthreads();
+    return s_cut ? beam_value(s_cut) : -INFINITY;
+  };
+  float best = -INFINITY;  // this thread's largest logit
+  auto round = [&](const uint4 (&v)[U], int64_t at, bool begin) {
     float m[U];
 #pragma unroll
-    for (int r = 0; r < U; ++r) {
-      float x[N];
-      KV8Type<DT>::values(v[r], x);
-      m[r] = x[0];
-#pragma unroll
-      for (int u = 1; u < N; ++u) m[r] = fmaxf(m[r], x[u]);
-    }
+    for (int r = 0; r < U; ++r) m[r] = BeamMax<DT>::of(v[r]);
     float most = m[0];
 #pragma unroll
     for (int r = 1; r < U; ++r) most = fmaxf(most, m[r]);
-    if (at == first) {
-      // (a thread without a number has 0, below every number's order)
-      const uint32_t mine = most > -INFINITY ? beam_order(most) : 0u;
-      s_max[tid] = mine;
-      __syncthreads();
-      int before = 0;
-#pragma unroll 8
-      for (int j = 0; j < BEAM_THREADS; j += 4) {
-        const uint4 o = *reinterpret_cast<const uint4*>(s_max + j);
-        before += (o.x > mine || (o.x == mine && j < tid)) + (o.y > mine || (o.y == mine && j + 1 < tid)) +
-                  (o.z > mine || (o.z == mine && j + 2 < tid)) + (o.w > mine || (o.w == mine && j + 3 < tid));
-      }
-      if (before == n - 1) s_cut = mine;
-      __syncthreads();
-      if (s_cut) cut = beam_value(s_cut);
-    }
+    if (begin) cut = bound(most);
+    best = fmaxf(best, most);
     if (most > top) {
-      sum *= fast_exp2((top - most) * LOG2E);
+      const float a = fast_exp2((top - most) * BEAM_LOG2E);
+      sum = f2_mul(sum, f2_pack(a, a));
       top = most;
     }
-    const float ref = top == -INFINITY ? 0.f : top;
+    // (x - top first: the fused x log2 e - top log2 e would leave the rounding of the
+    // second product in the exponent, which at logits of 10^4 is 2^-10)
+    const float ref = top == -INFINITY ? 0.f : -top;
 #pragma unroll
     for (int r = 0; r < U; ++r) {
       float x[N];
       KV8Type<DT>::values(v[r], x);
 #pragma unroll
-      for (int u = 0; u < N; ++u) sum += fast_exp2((x[u] - ref) * LOG2E);
-      if (at == first ? m[r] >= cut : m[r] > cut) {
+      for (int u = 0; u < N; u += 2) {
+        float e, f;
+        f2_unpack(f2_mul(f2_add(f2_pack(x[u], x[u + 1]), f2_pack(ref, ref)),
+                         f2_pack(BEAM_LOG2E, BEAM_LOG2E)), e, f);
+        sum = f2_add(sum, f2_pack(fast_exp2(e), fast_exp2(f)));
+      }
+      if (begin ? m[r] >= cut : m[r] > cut) {
         const uint32_t i = static_cast<uint32_t>(at + (r * BEAM_THREADS + tid) * N);
 #pragma unroll
         for (int u = 0; u < N; ++u)
-          if (x[u] > -INFINITY && (at == first ? x[u] >= cut : x[u] > cut)) {
+          if (x[u] > -INFINITY && (begin ? x[u] >= cut : x[u] > cut)) {
             const int to = atomicAdd(&s_count, 1);
             if (to < BEAM_CAP)
               list[to] = static_cast<uint64_t>(beam_order(x[u])) << 32 | (0xffffffffu - (i + u));
           }
       }
+      __syncwarp();   // (lanes that went that way would go on alone: five of 32 active)
     }
+  };
+  constexpr int64_t ROUND = U * N * BEAM_THREADS;
+#pragma unroll 1
+  for (int64_t at = first; at < last; at += ROUND) {
+    uint4 v[U];
+    if (vec && at + ROUND <= last) {
+      const uint4* p = reinterpret_cast<const uint4*>(
+          static_cast<const uint8_t*>(logits) + (base + at) * (DT == KF_DT_F32 ? 4 : 2)) + tid;
+#pragma unroll
+      for (int r = 0; r < U; ++r) v[r] = __ldg(p + r * BEAM_THREADS);
+    } else {
+#pragma unroll 1
+      for (int r = 0; r < U; ++r) {
+        uint4 one;
+        beam_load<DT>(logits, base, at + (r * BEAM_THREADS + tid) * N, last, vec != 0, one);
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+          if (q == r) v[q] = one;
+      }
+    }
+    round(v, at, at == first);
   }
   __syncthreads();
   int count = s_count;
-  if (count > BEAM_CAP)
+  uint64_t* from = list;
+  if (count > BEAM_CAP) {
     count = beam_careful<DT>(list, &s_count, logits, base, first, last, vec != 0, n);
+  } else if (count > 2 * n) {
+    // By now a better bound is known: what reaches it moves behind the list.
+    const float last_cut = bound(best);
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    const uint64_t least = static_cast<uint64_t>(beam_order(last_cut)) << 32;
+    const int room = min(BEAM_CAP - count, BEAM_COUNTED);   // (what is sorted needs more)
+    from = list + count;
+    for (int i = tid; i < count; i += BEAM_THREADS)
+      if (list[i] >= least) {
+        const int to = atomicAdd(&s_count, 1);
+        if (to < room) from[to] = list[i];
+      }
+    __syncthreads();
+    if (s_count <= room)
+      count = s_count;
+    else
+      from = list;       // too many to move: all of them, then
+  }
   uint64_t* out = w.key + spot * n;
-  beam_best(list, count, n, [&](int place, uint64_t key) { out[place] = key; });
+  beam_best(from, count, n, [&](int place, uint64_t key) { out[place] = key; });
   for (int i = count + tid; i < n; i += BEAM_THREADS) out[i] = 0;
   // the slice's sum
   float m = top;
@@ -260,7 +334,10 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
 #pragma unroll
   for (int u = 0; u < BEAM_THREADS / 32; ++u) m = fmaxf(m, s_top[u]);
   // (a thread that saw no number has a sum of 0, or NaN)
-  double s = static_cast<double>(top == -INFINITY ? sum : sum * fast_exp2((top - m) * LOG2E));
+  float s0, s1;
+  f2_unpack(sum, s0, s1);
+  double s = static_cast<double>(s0) + static_cast<double>(s1);
+  if (top != -INFINITY) s *= fast_exp2((top - m) * BEAM_LOG2E);
 #pragma unroll
   for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   if (lane == 0) s_sum[warp] = s;
@@ -276,7 +353,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
 //
 // One CTA a batch row: the beams' sums, a warp each, then their keys as candidates.
 // Latency is what it costs. The slices' lists are in order, so the n-th best of
-// their first entries bounds the answer, and few candidates are left to compare.
+// their first ones bounds the answer, and few candidates are left to compare.
 
 __global__ void __launch_bounds__(BEAM_THREADS)
     beam_join_kernel(const float* __restrict__ scores, int64_t s_sb,
@@ -324,24 +401,28 @@ __global__ void __launch_bounds__(BEAM_THREADS)
   // Entry i of the row's lists as a candidate; false: it is none.
   auto candidate = [&](int64_t i, BeamKey& c) -> bool {
     const int k = static_cast<int>(i / per);
+    double x;
     if (s_ended[k]) {
       if (i != k * per) return false;
-      c.c = s_score[k];
-      c.at = static_cast<uint64_t>(k) << 32 | static_cast<uint32_t>(pad);
+      x = s_score[k];
+      c.at = ~(static_cast<uint64_t>(k) << 32 | static_cast<uint32_t>(pad));
     } else {
       const uint64_t key = w.key[static_cast<int64_t>(b) * all + i];
       if (!key) return false;
-      c.c = (static_cast<double>(beam_value(static_cast<uint32_t>(key >> 32))) - s_lse[k]) +
-            s_score[k];
-      c.at = static_cast<uint64_t>(k) << 32 | (0xffffffffu - static_cast<uint32_t>(key));
+      x = (static_cast<double>(beam_value(static_cast<uint32_t>(key >> 32))) - s_lse[k]) + s_score[k];
+      c.at = ~(static_cast<uint64_t>(k) << 32 | (0xffffffffu - static_cast<uint32_t>(key)));
     }
-    return c.c > -INFINITY;
+    if (!(x > -INFINITY)) return false;
+    c.c = beam_order(x);
+    return true;
   };
-  const int64_t heads = static_cast<int64_t>(beams) * w.slices;
-  if (all > BEAM_COUNTED && heads >= n && heads <= BEAM_COUNTED) {
-    for (int64_t i = tid; i < heads; i += BEAM_THREADS) {
+  const int lists = beams * w.slices;
+  const int depth = (n + lists - 1) / lists;   // first entries of every list: at least n
+  if (all > 2 * BEAM_MAX && lists * depth <= BEAM_COUNTED) {
+    for (int i = tid; i < lists * depth; i += BEAM_THREADS) {
       BeamKey c;
-      if (candidate(i * n, c)) list[atomicAdd(&s_count, 1)] = c;
+      if (candidate(static_cast<int64_t>(i / depth) * n + i % depth, c))
+        list[atomicAdd(&s_count, 1)] = c;
     }
     __syncthreads();
     const int count = s_count;
@@ -371,9 +452,9 @@ __global__ void __launch_bounds__(BEAM_THREADS)
   const int count = s_count;
   const int64_t o = static_cast<int64_t>(b) * n;
   beam_best(list, count, n, [&](int place, const BeamKey& c) {
-    out_score[o + place] = static_cast<float>(c.c);
-    out_beam[o + place] = static_cast<int32_t>(c.at >> 32);
-    out_token[o + place] = static_cast<int32_t>(static_cast<uint32_t>(c.at));
+    out_score[o + place] = static_cast<float>(beam_value(c.c));
+    out_beam[o + place] = static_cast<int32_t>(~c.at >> 32);
+    out_token[o + place] = static_cast<int32_t>(static_cast<uint32_t>(~c.at));
   });
   for (int i = count + tid; i < n; i += BEAM_THREADS) {
     out_score[o + i] = -INFINITY;

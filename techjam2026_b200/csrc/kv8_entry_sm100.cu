@@ -585,12 +585,18 @@ extern "C" int kf_kv8_attention_shared(const kf_kv8_cache* cache, const void* q,
                        const_cast<int32_t*>(p.gr.live));
     if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention_shared groups launch");
   }
-  // Two kernels that run at once; where both are the split kernel, one. (64 samples of
-  // a prompt of 1800 tokens, 12 heads of 64: 28.3 us, as two 31.)
-  e = kv8_shared_part(c, a, w, p.tc_shared, p.tiles, static_cast<int64_t>(c.B) * w.rows);
+  // Two kernels that run at once. One does for both where they are the split kernel
+  // and have the same rows in a tile; otherwise the own tokens of up to 8 rows would
+  // pay for 16 (us, one / two kernels: 61 sequences in 8 groups, 4 rows of 128 a
+  // sequence, 102 / 94; 4 beams, 20.5 / 24, where launches count).
+  const int64_t rows = static_cast<int64_t>(c.B) * w.rows;
+  const bool two = p.tc_shared || (w.rows <= 8 && rows > 8);
+  if (two) a.gr.own_tiles = 0;
+  e = kv8_shared_part(c, a, w, p.tc_shared, p.tiles, rows);
   if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention_shared launch");
-  if (p.tc_shared) {
+  if (two) {
     a.gr.tiles = 0;
+    a.gr.own_tiles = p.gr.own_tiles;
     e = kv8_shared_part(c, a, w, p.tc_own, p.own_tiles, w.rows);
     if (e != cudaSuccess) return cuda_status(e, "kf_kv8_attention_shared launch");
   }
