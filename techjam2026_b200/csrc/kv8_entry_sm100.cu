@@ -420,10 +420,10 @@ static int kv8_shared_plan(const char* what, const KV8& c, int dtype, int64_t T,
   gr->least = 1;
   if (p->tc_shared) {
     // Parts of at least `least` steps: four, or what keeps the parts' room within
-    // 256 MB. A tile of n steps is cut into at most n / least + 2.
+    // 256 MB (or four parts). A tile of n steps is cut into at most n / least + 2.
     const int64_t steps = (max_shared + 127) / 128;
     const int64_t room = (256LL << 20) / (total * c.H * c.D * 4);
-    const int64_t parts = room > 8 ? room : 8;
+    const int64_t parts = room > 4 ? room : 4;
     gr->least = static_cast<int>(steps / (parts - 2) + 1);
     if (gr->least < 4) gr->least = 4;
     gr->chunk = 128 * gr->least;

@@ -371,62 +371,75 @@ struct PromptQ {
 
 // 32 rows of q, one a lane (at element `base`; < 0: zeros), as one fp16 plane (two)
 // in rows r0.. of a tile; returns the lane's factor from the products to log2
-// units. A row is loaded by as many lanes as it has 16-byte runs of type DT, eight
-// runs in flight (a thread a row, run after run, took 12000 clocks).
-template <int DH, int DT, int QP, int BM, bool VEC>
-__device__ __forceinline__ float prompt_put_q(const PromptQ& q, int64_t base, uint8_t* tile,
-                                              int plane, int r0) {
-  constexpr int N = KV8Type<DT>::N, LPR = DH / N, RPI = 32 / LPR, U = LPR < 8 ? LPR : 8;
-  const int lane = threadIdx.x & 31, l = lane & (LPR - 1), rr = lane / LPR;
-  float mine = 0.f;
-#pragma unroll 1
-  for (int it = 0; it < LPR; it += U) {
-    uint4 x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t from = __shfl_sync(0xffffffffu, base, (it + u) * RPI + rr);
-      x[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (from >= 0) x[u] = KV8Type<DT>::load(q.q, from + l * N, VEC);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int row = (it + u) * RPI + rr;
-      uint32_t m = 0;
-      KV8Type<DT>::collect(x[u], m);
-      m = KV8Type<DT>::bits(m);
-#pragma unroll
-      for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-      float inv, y[N];
-      const float sc = kv8_row_scale(__uint_as_float(m), &inv);
-      KV8Type<DT>::values(x[u], y);
-      uint32_t hi[N / 2], lo[N / 2];
-#pragma unroll
-      for (int v = 0; v < N / 2; ++v) {
-        const float a = y[2 * v] * sc, z = y[2 * v + 1] * sc;
-        hi[v] = pack_half2(a, z);
-        lo[v] = QP == 2 ? pack_half2_rest(a, z, hi[v]) : 0u;
-      }
-      const int piece = N == 8 ? l : l >> 1;          // of 16 bytes of the plane's row
-      uint8_t* at = tile + (piece >> 3) * BM * 128 + (r0 + row) * 128 +
-                    (((piece & 7) ^ (row & 7)) << 4);
-      if constexpr (N == 8) {
-        *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[N / 2 - 1]);
-      } else {
-        at += (l & 1) * 8;
-        *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-        if constexpr (QP == 2) *reinterpret_cast<uint2*>(at + plane) = make_uint2(lo[0], lo[1]);
-      }
-      const float f = __shfl_sync(0xffffffffu, inv, (lane & (RPI - 1)) * LPR);
-      if (lane / RPI == it + u) mine = f;
-    }
-  }
-  return mine * q.scale_log2;
-}
+// units. A row is taken by as many lanes as it has 16-byte runs of type DT: copied as
+// it is to the places of its planes, all rows in flight, then converted there, in a
+// loop that is not unrolled. (Code that runs once a CTA costs its fetch, about 200
+// clocks for eight instructions: eight runs at a time in registers took 14000 clocks, a
+// thread a row as long.)
 template <int DH, int DT, int QP, int BM>
 __device__ __forceinline__ float prompt_put_q(const PromptQ& q, int64_t base, uint8_t* tile,
                                               int plane, int r0) {
-  return q.vec ? prompt_put_q<DH, DT, QP, BM, true>(q, base, tile, plane, r0)
-               : prompt_put_q<DH, DT, QP, BM, false>(q, base, tile, plane, r0);
+  constexpr int N = KV8Type<DT>::N, LPR = DH / N, RPI = 32 / LPR;
+  const int lane = threadIdx.x & 31, l = lane & (LPR - 1), rr = lane / LPR;
+  const int piece = N == 8 ? l : l >> 1;          // of 16 bytes of the plane's row
+  auto place = [&](int row) -> uint8_t* {
+    return tile + (piece >> 3) * BM * 128 + (r0 + row) * 128 + (((piece & 7) ^ (row & 7)) << 4);
+  };
+  // fp32: the first run of a piece waits in the first plane, the second in the other
+  const int wait_at = N == 4 ? (l & 1) * plane : 0;
+#pragma unroll 1
+  for (int it = 0; it < LPR; ++it) {
+    const int row = it * RPI + rr;
+    const int64_t from = __shfl_sync(0xffffffffu, base, row);
+    uint8_t* to = place(row) + wait_at;
+    if (q.vec) {
+      const int64_t at = from < 0 ? 0 : from + l * N;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)),
+                   "l"(static_cast<const uint8_t*>(q.q) + at * (DT == KF_DT_F32 ? 4 : 2)),
+                   "r"(from < 0 ? 0 : 16)
+                   : "memory");
+    } else {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (from >= 0) x = KV8Type<DT>::load(q.q, from + l * N, false);
+      *reinterpret_cast<uint4*>(to) = x;
+    }
+  }
+  copy_commit();
+  copy_wait<0>();
+  __syncwarp();
+  float mine = 0.f;
+#pragma unroll 1
+  for (int it = 0; it < LPR; ++it) {
+    const int row = it * RPI + rr;
+    uint8_t* at = place(row);
+    const uint4 x = *reinterpret_cast<const uint4*>(at + wait_at);
+    uint32_t m = 0;
+    KV8Type<DT>::collect(x, m);
+    m = KV8Type<DT>::bits(m);
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    float inv, y[N];
+    const float sc = kv8_row_scale(__uint_as_float(m), &inv);
+    KV8Type<DT>::values(x, y);
+    uint32_t hi[N / 2], lo[N / 2];
+#pragma unroll
+    for (int v = 0; v < N / 2; ++v) {
+      const float a = y[2 * v] * sc, z = y[2 * v + 1] * sc;
+      hi[v] = pack_half2(a, z);
+      lo[v] = QP == 2 ? pack_half2_rest(a, z, hi[v]) : 0u;
+    }
+    if constexpr (N == 8) {
+      *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[N / 2 - 1]);
+    } else {
+      __syncwarp();   // (the shuffles before it have all lanes' reads behind them, too)
+      at += (l & 1) * 8;
+      *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+      if constexpr (QP == 2) *reinterpret_cast<uint2*>(at + plane) = make_uint2(lo[0], lo[1]);
+    }
+    const float f = __shfl_sync(0xffffffffu, inv, (lane & (RPI - 1)) * LPR);
+    if (lane / RPI == it) mine = f;
+  }
+  return mine * q.scale_log2;
 }
 
 // SH: the call has groups, and Q comes without a tensor map. gr.tiles > 0: the shared

@@ -103,6 +103,59 @@ def test_long_shared_prefixes_are_split_and_joined(members, T, group, kind):
     check(cache, starts, shared, queries(cache, group, T, kind) * 3)
 
 
+@pytest.mark.parametrize("kind,dim,dtype", [(F32, 32, I8), (BF16, 64, F8), (F16, 128, I8),
+                                            (F32, 128, F8), (BF16, 16, F8)])
+@pytest.mark.parametrize("T", [1, 9])
+def test_more_tiles_than_processors(T, kind, dim, dtype):
+    """Many tiles of unequal lengths: a CTA ends one and begins others, and some
+    groups share nothing or have one sequence."""
+    sizes = [70, 1, 40, 0, 55, 64]
+    cache, starts, shared = make_groups(sizes, [640, 576, 64, 128, 0, 1280],
+                                        [b % 19 for b in range(sum(sizes) + 1)], dim=dim, block=64,
+                                        dtype=dtype, heads=16, room=T, rest=1)
+    counts = None if T == 1 else ints([b % (T + 1) for b in range(sum(sizes) + 1)])
+    append(cache, T, counts)
+    check(cache, starts, shared, queries(cache, 8 if T == 1 else 2, T, kind), counts)
+
+
+@pytest.mark.parametrize("T,group", [(1, 1), (70, 1)])
+def test_more_groups_than_one_list_holds(T, group):
+    cache, starts, shared = make_groups([1] * 1100, [16 * (n % 4) for n in range(1100)],
+                                        [n % 3 for n in range(1100)], dim=16, block=16, heads=1,
+                                        room=T)
+    append(cache, T)
+    check(cache, starts, shared, queries(cache, group, T, BF16))
+
+
+@pytest.mark.parametrize("kind,dim", [(BF16, 64), (BF16, 32), (F16, 64), (BF16, 128), (F32, 64),
+                                      (F32, 128)])
+@pytest.mark.parametrize("members,T", [(40, 1), (90, 1), (6, 100)])
+def test_waits_that_run_out_end_the_call_and_the_next_is_right(members, T, kind, dim):
+    """Under a limit of one cycle the waits of the tensor-memory kernel give up where
+    what they wait for is not there at once. Every role leaves, the call returns, the
+    next one is as before."""
+    L = _lib.lib()
+    cache, starts, shared = make_groups([members, 3], [1216, 640], [20] * (members + 3), dim=dim,
+                                        block=32, dtype=F8, heads=3, room=T)
+    append(cache, T)
+    q = queries(cache, 2, T, kind)
+    good = check(cache, starts, shared, q)
+    _lib.check(L.kf_set_wait_limit(1), "kf_set_wait_limit")
+    try:
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        ops.kv8_attention_shared(q, cache, starts, shared)
+        end.record()
+        torch.cuda.synchronize()
+        got = status()
+    finally:
+        L.kf_set_wait_limit(0)
+    assert begin.elapsed_time(end) < 1000
+    assert got in (0, 1, 2, 4)
+    assert torch.equal(ops.kv8_attention_shared(q, cache, starts, shared), good)
+    assert status() == 0
+
+
 def test_what_counts_as_shared_is_cut():
     """shared is cut to whole pages, to the shortest of the group's lens and to
     max_shared; the result is that of kv8_attention whatever it says."""
