@@ -105,7 +105,11 @@ __device__ __forceinline__ void beam_best(Key* list, int count, int n, Put&& put
 // of the others stays short without any barrier in the loop. Where it does not
 // (many equal logits, or logits that grow along the slice), the slice is read
 // again in small rounds that cut the list as it fills.
-// Bound by memory, and by the exponentials for 16-bit logits (16 a clock and SM).
+// What bounds it: issue. A logit takes four instructions of the sum (and an
+// exponential, 16 a clock and SM); as many more go to 16-byte runs that hold a token above
+// the bound, 2 % of them, which is every second run of a warp. Measured: 64 x 8 rows
+// of 128000 bf16 logits, 62 us for 124 MB (floor 19; with a barrier and a list of all
+// candidates in every round 138); 24 x 8 rows of 50021 fp32 logits, 35 MB, about 20 us.
 
 template <int DT>
 __device__ __forceinline__ void beam_load(const void* logits, int64_t base, int64_t i, int64_t last,
@@ -236,7 +240,8 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
     return s_cut ? beam_value(s_cut) : -INFINITY;
   };
   float best = -INFINITY;  // this thread's largest logit
-  auto round = [&](const uint4 (&v)[U], int64_t at, bool begin) {
+  // `apart`: the thread's logits are BEAM_THREADS tokens apart, not runs of N.
+  auto round = [&](const uint4 (&v)[U], int64_t at, bool begin, bool apart) {
     float m[U];
 #pragma unroll
     for (int r = 0; r < U; ++r) m[r] = BeamMax<DT>::of(v[r]);
@@ -265,13 +270,14 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
         sum = f2_add(sum, f2_pack(fast_exp2(e), fast_exp2(f)));
       }
       if (begin ? m[r] >= cut : m[r] > cut) {
-        const uint32_t i = static_cast<uint32_t>(at + (r * BEAM_THREADS + tid) * N);
+        const uint32_t i = static_cast<uint32_t>(at + r * BEAM_THREADS * N + (apart ? tid : tid * N));
+        const uint32_t next = apart ? BEAM_THREADS : 1;
 #pragma unroll
         for (int u = 0; u < N; ++u)
           if (x[u] > -INFINITY && (begin ? x[u] >= cut : x[u] > cut)) {
             const int to = atomicAdd(&s_count, 1);
             if (to < BEAM_CAP)
-              list[to] = static_cast<uint64_t>(beam_order(x[u])) << 32 | (0xffffffffu - (i + u));
+              list[to] = static_cast<uint64_t>(beam_order(x[u])) << 32 | (0xffffffffu - (i + u * next));
           }
       }
       __syncwarp();   // (lanes that went that way would go on alone: five of 32 active)
@@ -281,7 +287,26 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
 #pragma unroll 1
   for (int64_t at = first; at < last; at += ROUND) {
     uint4 v[U];
-    if (vec && at + ROUND <= last) {
+    const bool apart = !vec && at + ROUND <= last;
+    if (apart) {
+      // Rows that are not aligned (an odd vocabulary): neighbours load neighbours.
+      constexpr int SIZE = DT == KF_DT_F32 ? 4 : 2;
+      const uint8_t* p = static_cast<const uint8_t*>(logits) + (base + at + tid) * SIZE;
+#pragma unroll
+      for (int r = 0; r < U; ++r) {
+        uint32_t x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if constexpr (DT == KF_DT_F32) {
+            x[u] = __ldg(reinterpret_cast<const uint32_t*>(p) + (r * N + u) * BEAM_THREADS);
+          } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + (r * N + 2 * u) * BEAM_THREADS;
+            x[u] = __ldg(h) | (static_cast<uint32_t>(__ldg(h + BEAM_THREADS)) << 16);
+          }
+        }
+        v[r] = make_uint4(x[0], x[1], x[2], x[3]);
+      }
+    } else if (vec && at + ROUND <= last) {
       const uint4* p = reinterpret_cast<const uint4*>(
           static_cast<const uint8_t*>(logits) + (base + at) * (DT == KF_DT_F32 ? 4 : 2)) + tid;
 #pragma unroll
@@ -296,7 +321,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
           if (q == r) v[q] = one;
       }
     }
-    round(v, at, at == first);
+    round(v, at, at == first, apart);
   }
   __syncthreads();
   int count = s_count;
@@ -352,8 +377,9 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4)
 // ---------------------------------------------------------------- the best of all beams
 //
 // One CTA a batch row: the beams' sums, a warp each, then their keys as candidates.
-// Latency is what it costs. The slices' lists are in order, so the n-th best of
-// their first ones bounds the answer, and few candidates are left to compare.
+// Latency is what it costs, 10 to 16 us when its code is fetched for the first time.
+// The slices' lists are in order, so the n-th best of their first ones bounds the
+// answer, and few candidates are left to compare.
 
 __global__ void __launch_bounds__(BEAM_THREADS)
     beam_join_kernel(const float* __restrict__ scores, int64_t s_sb,
@@ -385,7 +411,7 @@ __global__ void __launch_bounds__(BEAM_THREADS)
     double s = 0.0;
     for (int i = lane; i < w.slices; i += 32) {
       const double part = w.sum[spot + i];
-      if (part != 0.0) s += part * exp(static_cast<double>(w.top[spot + i]) - m);
+      if (part != 0.0) s += part * fast_exp2((w.top[spot + i] - m) * BEAM_LOG2E);
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);

@@ -199,7 +199,7 @@ static cudaError_t kv8_split_any(const KV8& c, const KV8Call& a, const KV8Work& 
 
 template <int DH, int QP, int PP>
 static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
-  using Cfg = PromptCfg<DH, QP, PP, prompt_tiles(DH, QP), false>;
+  using Cfg = PromptCfg<DH, QP, PP>;
   using Wei = WeighCfg<DH, QP>;
   const unsigned bh = static_cast<unsigned>(c.B * c.H);
   const bool track = (a.flags & KF_KV8_TRACK) != 0;
@@ -210,7 +210,7 @@ static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
   int rc = encode_tensor_map(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, w.planes, dims, strides, box,
                              CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  auto kern = kv8_prompt_kernel<DH, QP, PP, prompt_tiles(DH, QP), false>;
+  auto kern = kv8_prompt_kernel<DH, QP, PP>;
   auto kern_w = kv8_prompt_weights_kernel<DH, QP>;
   static DeviceOnce once;
   rc = once.run("kf_kv8_attention", nullptr, [&](int) {
@@ -233,8 +233,7 @@ static int kv8_prompt(const KV8& c, const KV8Call& a, const KV8Work& w) {
                        dim3(static_cast<unsigned>((w.rows + Cfg::ROWS - 1) / Cfg::ROWS),
                             static_cast<unsigned>(w.chunks), bh),
                        dim3(Cfg::THREADS), Cfg::SMEM, a.st, map, c, a.out, a.o_sb, a.o_sh, a.o_st,
-                       a.dtype, a.o_vec, a.counts, a.T, a.G, a.max_len, a.flags, a.lse, w,
-                       PromptQ{}, KV8Groups{});
+                       a.dtype, a.o_vec, a.counts, a.T, a.G, a.max_len, a.flags, a.lse, w);
   if (e == cudaSuccess && w.chunks > 1)
     e = launch_chained(kv8_join_kernel, dim3(static_cast<unsigned>(w.rows), bh), dim3(KV8_JOIN_THREADS), 0, a.st,
                        c, a.out, a.o_sb, a.o_sh, a.o_st, a.dtype, a.T, a.G, a.lse, w);
@@ -377,7 +376,7 @@ static int kv8_shared_plan(const char* what, const KV8& c, int dtype, int64_t T,
   p->tc_own = per > KV8_SPLIT_ROWS && p->tc_shared;
   p->packed = T > 1 && counts && p->tc_shared;
   // Two tiles share the expansion of the codes, one pays for no empty second one.
-  const int two = prompt_tiles(c.D, dtype == KF_DT_F32 ? 2 : 1);
+  const int two = group_tiles(c.D, dtype == KF_DT_F32 ? 2 : 1);
   p->tiles = mean > 128 ? two : 1;
   p->own_tiles = per > 128 ? two : 1;
   const int64_t tile = p->tc_shared ? 128 * p->tiles : KV8_ROWS;
@@ -448,8 +447,8 @@ static int kv8_shared_plan(const char* what, const KV8& c, int dtype, int64_t T,
 
 template <int DH, int QP, int PP, int TILES>
 static cudaError_t kv8_shared_tc(const KV8& c, const KV8Call& a, const KV8Work& w) {
-  using Cfg = PromptCfg<DH, QP, PP, TILES, true>;
-  auto kern = kv8_prompt_kernel<DH, QP, PP, TILES, true>;
+  using Cfg = GroupCfg<DH, QP, PP, TILES>;
+  auto kern = kv8_group_kernel<DH, QP, PP, TILES>;
   static DeviceOnce once;
   cudaError_t attr = cudaSuccess;
   once.run("kf_kv8_attention_shared", nullptr, [&](int) {
@@ -460,14 +459,13 @@ static cudaError_t kv8_shared_tc(const KV8& c, const KV8Call& a, const KV8Work& 
   dim3 grid(static_cast<unsigned>(c.B * a.gr.own_tiles * (w.chunks - a.gr.chunks)),
             static_cast<unsigned>(c.H));
   if (a.gr.tiles > 0) grid = dim3(static_cast<unsigned>(sm_count()));
-  const PromptQ q = {a.q, a.q_sb, a.q_sh, a.q_st, a.q_vec16, a.scale_log2};
-  return launch_chained(kern, grid,
-                        dim3(Cfg::THREADS), Cfg::SMEM, a.st, CUtensorMap{}, c, a.out, a.o_sb, a.o_sh,
-                        a.o_st, a.dtype, a.o_vec, a.counts, a.T, a.G, 0, a.flags, a.lse, w, q, a.gr);
+  const GroupQ q = {a.q, a.q_sb, a.q_sh, a.q_st, a.q_vec16, a.scale_log2};
+  return launch_chained(kern, grid, dim3(Cfg::THREADS), Cfg::SMEM, a.st, c, a.dtype, a.counts, a.T, a.G,
+                        a.flags, w, q, a.gr);
 }
 template <int DH, int QP, int PP>
 static cudaError_t kv8_shared_tiles(const KV8& c, const KV8Call& a, const KV8Work& w, int tiles) {
-  if constexpr (prompt_tiles(DH, QP) == 2)
+  if constexpr (group_tiles(DH, QP) == 2)
     if (tiles == 2) return kv8_shared_tc<DH, QP, PP, 2>(c, a, w);
   return kv8_shared_tc<DH, QP, PP, 1>(c, a, w);
 }

@@ -244,18 +244,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-// QP, PP: fp16 planes of q (two for fp32) and of P (two for fp32 and fp16). TILES:
-// tiles of 128 query rows. (fp32 at head_dim 128 has room for one: its Q planes fill
-// shared memory and its second accumulator TMEM.)
-__host__ __device__ constexpr int prompt_tiles(int dim, int q_planes) {
-  return dim == 128 && q_planes == 2 ? 1 : 2;
-}
-template <int DH, int QP, int PP, int TILES, bool SH>
+// QP, PP: fp16 planes of q (two for fp32) and of P (two for fp32 and fp16).
+template <int DH, int QP, int PP>
 struct PromptCfg {
-  static constexpr int NT = TILES;
-  // Loading warps: 9 to 11, and with groups and one tile 4 to 7, whose rows there
-  // are none.
-  static constexpr int LW = SH && NT == 1 ? 7 : 3;
+  // Tiles of 128 query rows. fp32 at head_dim 128 takes one: its Q planes fill
+  // shared memory and its second accumulator TMEM.
+  static constexpr int NT = (DH == 128 && QP == 2) ? 1 : 2;
   static constexpr int BM = 128;
   static constexpr int BN = 128;                           // keys of a step
   static constexpr int CH = DH > 64 ? 2 : 1;               // 64-column halves of a row
@@ -264,9 +258,7 @@ struct PromptCfg {
   static constexpr int KV_BYTES = BN * 128 * CH;
   static constexpr int ST = 2;                             // stages of K and of V
   static constexpr int RAW = BN * DH;                      // bytes of a tile's codes
-  // Raw tiles of K and of V: two where shared memory holds them, so that a copy
-  // has a whole step's time.
-  static constexpr int RS = DH > 64 && !(SH && NT == 1 && QP == 1) ? 1 : 2;
+  static constexpr int RS = DH > 64 ? 1 : 2;               // raw tiles of K and of V
   static constexpr int K_OFF = Q_BYTES;
   static constexpr int V_OFF = K_OFF + ST * KV_BYTES;
   static constexpr int RAWK_OFF = V_OFF + ST * KV_BYTES;
@@ -361,102 +353,13 @@ __device__ __forceinline__ float max16(const float* s) {
   return fmax3(fmaxf(m, n), s[14], s[15]);
 }
 
-// q of a call with groups, which the softmax warps bring into shared memory.
-struct PromptQ {
-  const void* q;
-  int64_t sb, sh, st;
-  int vec;             // 16-byte aligned runs
-  float scale_log2;
-};
-
-// 32 rows of q, one a lane (at element `base`; < 0: zeros), as one fp16 plane (two)
-// in rows r0.. of a tile; returns the lane's factor from the products to log2
-// units. A row is taken by as many lanes as it has 16-byte runs of type DT: copied as
-// it is to the places of its planes, all rows in flight, then converted there, in a
-// loop that is not unrolled. (Code that runs once a CTA costs its fetch, about 200
-// clocks for eight instructions: eight runs at a time in registers took 14000 clocks, a
-// thread a row as long.)
-template <int DH, int DT, int QP, int BM>
-__device__ __forceinline__ float prompt_put_q(const PromptQ& q, int64_t base, uint8_t* tile,
-                                              int plane, int r0) {
-  constexpr int N = KV8Type<DT>::N, LPR = DH / N, RPI = 32 / LPR;
-  const int lane = threadIdx.x & 31, l = lane & (LPR - 1), rr = lane / LPR;
-  const int piece = N == 8 ? l : l >> 1;          // of 16 bytes of the plane's row
-  auto place = [&](int row) -> uint8_t* {
-    return tile + (piece >> 3) * BM * 128 + (r0 + row) * 128 + (((piece & 7) ^ (row & 7)) << 4);
-  };
-  // fp32: the first run of a piece waits in the first plane, the second in the other
-  const int wait_at = N == 4 ? (l & 1) * plane : 0;
-#pragma unroll 1
-  for (int it = 0; it < LPR; ++it) {
-    const int row = it * RPI + rr;
-    const int64_t from = __shfl_sync(0xffffffffu, base, row);
-    uint8_t* to = place(row) + wait_at;
-    if (q.vec) {
-      const int64_t at = from < 0 ? 0 : from + l * N;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)),
-                   "l"(static_cast<const uint8_t*>(q.q) + at * (DT == KF_DT_F32 ? 4 : 2)),
-                   "r"(from < 0 ? 0 : 16)
-                   : "memory");
-    } else {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (from >= 0) x = KV8Type<DT>::load(q.q, from + l * N, false);
-      *reinterpret_cast<uint4*>(to) = x;
-    }
-  }
-  copy_commit();
-  copy_wait<0>();
-  __syncwarp();
-  float mine = 0.f;
-#pragma unroll 1
-  for (int it = 0; it < LPR; ++it) {
-    const int row = it * RPI + rr;
-    uint8_t* at = place(row);
-    const uint4 x = *reinterpret_cast<const uint4*>(at + wait_at);
-    uint32_t m = 0;
-    KV8Type<DT>::collect(x, m);
-    m = KV8Type<DT>::bits(m);
-#pragma unroll
-    for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    float inv, y[N];
-    const float sc = kv8_row_scale(__uint_as_float(m), &inv);
-    KV8Type<DT>::values(x, y);
-    uint32_t hi[N / 2], lo[N / 2];
-#pragma unroll
-    for (int v = 0; v < N / 2; ++v) {
-      const float a = y[2 * v] * sc, z = y[2 * v + 1] * sc;
-      hi[v] = pack_half2(a, z);
-      lo[v] = QP == 2 ? pack_half2_rest(a, z, hi[v]) : 0u;
-    }
-    if constexpr (N == 8) {
-      *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[N / 2 - 1]);
-    } else {
-      __syncwarp();   // (the shuffles before it have all lanes' reads behind them, too)
-      at += (l & 1) * 8;
-      *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-      if constexpr (QP == 2) *reinterpret_cast<uint2*>(at + plane) = make_uint2(lo[0], lo[1]);
-    }
-    const float f = __shfl_sync(0xffffffffu, inv, (lane & (RPI - 1)) * LPR);
-    if (lane / RPI == it) mine = f;
-  }
-  return mine * q.scale_log2;
-}
-
-// SH: the call has groups, and Q comes without a tensor map. gr.tiles > 0: the shared
-// tokens. A CTA an SM takes an equal share of all steps ([group][row tiles][kv
-// head][128 keys]), one or more stretches of keys of row tiles; a row tile's
-// parts are the CTAs that had some of its steps. (Grids of parts of a fixed size
-// ended in a wave of few CTAs: ragged questions on two documents of 8k to 16k
-// tokens 234 us.) Otherwise the own tokens: y is the kv head and x [sequence][row
-// tiles][part].
-template <int DH, int QP, int PP, int TILES, bool SH>
-__global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
+template <int DH, int QP, int PP>
+__global__ void __launch_bounds__(PromptCfg<DH, QP, PP>::THREADS, 1)
     kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, KV8 c, void* __restrict__ out,
                       int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype, int o_vec,
                       const int32_t* __restrict__ counts, int T, int G, int max_len, int flags,
-                      float* __restrict__ lse_out, KV8Work w, PromptQ pq, KV8Groups gr) {
-  using Cfg = PromptCfg<DH, QP, PP, TILES, SH>;
-  constexpr int LW = Cfg::LW;
+                      float* __restrict__ lse_out, KV8Work w) {
+  using Cfg = PromptCfg<DH, QP, PP>;
   constexpr int BM = Cfg::BM, BN = Cfg::BN, NT = Cfg::NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -486,14 +389,54 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
   PromptScales* s_sc = reinterpret_cast<PromptScales*>(smem + Cfg::SC_OFF);
   static_assert(sizeof(PromptScales) <= 128, "scale ring");
 
+  pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto set_up_barriers = [&]() {
-    mbar_init(q_full, SH ? 4 * NT : 1);
+  const int bh = blockIdx.z;
+  const int b = bh / c.H, h = bh - b * c.H;
+  const int chunk = blockIdx.y;
+  const int row0 = static_cast<int>(gridDim.x - 1 - blockIdx.x) * Cfg::ROWS;  // heaviest first
+  const int len = kv8_len(c, b);
+  const int count = kv8_count(c, counts, b, T);
+  int end = kv8_end(c, len, count);
+  if (end > max_len) {
+    if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
+    end = max_len;
+  }
+  const bool causal = (flags & KF_KV8_CAUSAL) != 0;
+  const int last_row = min(row0 + Cfg::ROWS, w.rows) - 1;
+  const int last_tok = min(last_row / G, count - 1);
+  const int reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
+  const int k0 = chunk * w.chunk;
+  const int k1 = min(k0 + w.chunk, reach);
+  const bool alone = w.chunks == 1;
+  if (k0 >= k1) {
+    // No key: zeros, or an empty part for the join.
+    for (int i = tid; i < Cfg::ROWS; i += Cfg::THREADS) {
+      const int row = row0 + i;
+      if (row >= w.rows) break;
+      const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
+      if (!alone) {
+        w.ref[at * w.chunks + chunk] = -INFINITY;
+        w.sum[at * w.chunks + chunk] = 0.f;
+        continue;
+      }
+      const int tok = row / G, hq = h * G + row - tok * G;
+      for (int d = 0; d < DH; ++d)
+        kv8_store1(out, b * o_sb + hq * o_sh + tok * o_st + d, dtype, 0.f);
+      if (lse_out) lse_out[(static_cast<int64_t>(b) * c.H * G + hq) * T + tok] = -INFINITY;
+      if (w.lse) w.lse[at] = -INFINITY;
+    }
+    return;
+  }
+  const int n_steps = (k1 - k0 + BN - 1) / BN;
+
+  if (tid == 0) {
+    mbar_init(q_full, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], LW);
-      mbar_init(&v_full[s], LW);
-      mbar_init(&rk_empty[s], LW);
-      mbar_init(&rv_empty[s], LW);
+      mbar_init(&k_full[s], 3);
+      mbar_init(&v_full[s], 3);
+      mbar_init(&rk_empty[s], 3);
+      mbar_init(&rv_empty[s], 3);
       mbar_init(&rk_full[s], 1);
       mbar_init(&rv_full[s], 1);
       mbar_init(&k_empty[s], 1 + 4 * NT);
@@ -507,165 +450,15 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
-  };
-  if constexpr (SH) {
-    // While the kernel before ends: barriers and TMEM.
-    if (tid == 0) set_up_barriers();
-    if (warp == 8) {
-      tmem_alloc(tmem_slot, 512);
-      tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (gr.tiles > 0 || !gr.paired) pdl_wait();
-    pdl_launch_dependents();  // every CTA that runs holds its TMEM by now
-  } else {
-    pdl_wait();
+    tma_prefetch_desc(&tmQ);
   }
-  const bool causal = (flags & KF_KV8_CAUSAL) != 0;
-  const bool alone = !SH && w.chunks == 1;
-  int64_t at = 0, stop = 1, share = 1;   // this CTA's steps of the shared tokens
-  bool whole = false;                    // one stretch of keys a CTA
-  int stretch = 0;                       // stretches of keys done
-  int4 begin_g = make_int4(0, 0, 0, 0), begin = begin_g;
-  if (SH && gr.tiles > 0) {
-    begin_g = __ldg(gr.record + 2 * blockIdx.x);
-    begin = __ldg(gr.record + 2 * blockIdx.x + 1);
-    const int64_t all = __ldg(gr.work + gr.N);
-    share = __ldg(gr.work + gr.N + 1);
-    whole = share < 0;
-    if (whole) share = -share;
-    at = blockIdx.x * share;
-    stop = min(at + share, all);
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
   }
-  bool more = !SH || gr.tiles == 0 || at < stop;
-  while (more) {
-  int b, h, chunk, row0, rows;   // b: whose table row has the pages (the group's first sequence)
-  int end, k0, k1;
-  int2 seq = make_int2(0, 0);    // the group's sequences
-  bool last_part = false;        // no CTA has later keys of this tile
-  if constexpr (!SH) {
-    more = false;
-    const int bh = blockIdx.z;
-    b = bh / c.H;
-    h = bh - b * c.H;
-    chunk = blockIdx.y;
-    row0 = static_cast<int>(gridDim.x - 1 - blockIdx.x) * Cfg::ROWS;  // heaviest first
-    rows = w.rows;
-    const int len = kv8_len(c, b);
-    const int count = kv8_count(c, counts, b, T);
-    end = kv8_end(c, len, count);
-    if (end > max_len) {
-      if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
-      end = max_len;
-    }
-    const int last_row = min(row0 + Cfg::ROWS, w.rows) - 1;
-    const int last_tok = min(last_row / G, count - 1);
-    const int reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
-    k0 = chunk * w.chunk;
-    k1 = min(k0 + w.chunk, reach);
-  } else {
-    if (gr.tiles > 0) {
-      int4 g = begin_g;
-      int item = begin.x, step = begin.y, steps = begin.z;
-      chunk = begin.w;
-      if (stretch) {
-        // The group that holds step `at` of all of them, and its item.
-        int lo = 0, hi = gr.N;
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (__ldg(gr.work + mid) <= at)
-            lo = mid;
-          else
-            hi = mid;
-        }
-        g = __ldg(gr.group + lo);
-        steps = (g.x + 127) / 128;
-        item = static_cast<int>((at - __ldg(gr.work + lo)) / steps);
-        step = 0;
-        chunk = 0;
-      }
-      const int take = static_cast<int>(min(static_cast<int64_t>(steps - step), stop - at));
-      h = item % c.H;
-      row0 = item / c.H * Cfg::ROWS;
-      seq = make_int2(g.z, g.w);
-      b = g.z;
-      rows = g.y;
-      end = g.x;
-      k0 = step * BN;
-      k1 = min(k0 + take * BN, end);
-      last_part = (step + take) * BN >= end;
-      at += take;
-      more = at < stop;
-    } else {
-      h = blockIdx.y;
-      int i = blockIdx.x;
-      const int own = w.chunks - gr.chunks;
-      more = false;
-      chunk = i % own;
-      i /= own;
-      b = i / gr.own_tiles;
-      row0 = (i - b * gr.own_tiles) * Cfg::ROWS;
-      rows = w.rows;
-      const int shared = kv8_shared_of(c, gr, b);
-      const int len = kv8_len(c, b);
-      const int count = kv8_count(c, counts, b, T);
-      end = kv8_end(c, len, count);
-      if (end - shared > gr.max_own) {
-        if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
-        end = shared + gr.max_own;
-      }
-      const int last_row = min(row0 + Cfg::ROWS, rows) - 1;
-      const int last_tok = min(last_row / G, count - 1);
-      const int reach = last_tok < row0 / G ? 0 : (causal ? min(len + last_tok + 1, end) : end);
-      k0 = shared + chunk * w.chunk;
-      k1 = min(k0 + w.chunk, reach);
-      if (shared == 0 && chunk == 0)
-        kv8_no_shared_parts(c, gr, w, b, h, row0, Cfg::ROWS, Cfg::THREADS);
-      chunk += gr.chunks;
-    }
-  }
-  // Sequence (from b on) and row within it of a row, and where its numbers are:
-  // [B * H][rows of a sequence].
-  auto row_of = [&](int row) -> int2 {
-    return SH && gr.tiles > 0 ? kv8_group_row(gr, seq, w.rows, G, row) : make_int2(0, row);
-  };
-  auto spot_of = [&](int2 at) -> int64_t {
-    return static_cast<int64_t>((b + at.x) * c.H + h) * w.rows + at.y;
-  };
-  if (k0 >= k1) {
-    // No key: zeros, or an empty part for the join.
-    for (int i = tid; i < Cfg::ROWS; i += Cfg::THREADS) {
-      const int row = row0 + i;
-      if (row >= rows) break;
-      const int64_t at = spot_of(row_of(row));
-      if (!alone) {
-        w.ref[at * w.chunks + chunk] = -INFINITY;
-        w.sum[at * w.chunks + chunk] = 0.f;
-        continue;
-      }
-      const int tok = row / G, hq = h * G + row - tok * G;
-      for (int d = 0; d < DH; ++d)
-        kv8_store1(out, b * o_sb + hq * o_sh + tok * o_st + d, dtype, 0.f);
-      if (lse_out) lse_out[(static_cast<int64_t>(b) * c.H * G + hq) * T + tok] = -INFINITY;
-      if (w.lse) w.lse[at] = -INFINITY;
-    }
-    if constexpr (SH) break;
-    return;
-  }
-  const int n_steps = (k1 - k0 + BN - 1) / BN;
-
-  float vmax = 0.f;  // the largest V scale of the range
-  if constexpr (!SH) {
-    if (tid == 0) {
-      set_up_barriers();
-      tma_prefetch_desc(&tmQ);
-    }
-    if (warp == 8) {
-      tmem_alloc(tmem_slot, 512);
-      tmem_relinquish();
-    }
+  // The largest V scale of the range.
+  {
+    float vmax = 0.f;
     for (int j = (k0 >> c.p_shift) + tid; (j << c.p_shift) < k1; j += Cfg::THREADS) {
       const int page = kv8_page(c, b, j);
       if (page >= 0)
@@ -674,30 +467,25 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
 #pragma unroll
     for (int d = 16; d; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
     if (lane == 0) s_vmax[warp] = vmax;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    pdl_launch_dependents();  // every CTA that runs holds its TMEM by now
-    vmax = s_vmax[0];
-#pragma unroll
-    for (int i = 1; i < 12; ++i) vmax = fmaxf(vmax, s_vmax[i]);
-  } else if (stretch) {
-    if (tid == 0) set_up_barriers();
-    __syncthreads();
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_launch_dependents();  // every CTA that runs holds its TMEM by now
+  float vmax = s_vmax[0];
+#pragma unroll
+  for (int i = 1; i < 12; ++i) vmax = fmaxf(vmax, s_vmax[i]);
 
   if (warp == 8) {
     if (lane == 0) {
       // ------------------------------------------------ Q, products
-      if constexpr (!SH) {
-        mbar_arrive_expect_tx(q_full, Cfg::Q_BYTES);
-        for (int t = 0; t < NT; ++t)
-          for (int pl = 0; pl < QP; ++pl)
-            for (int ch = 0; ch < Cfg::CH; ++ch)
-              tma_load_3d(sQ + (t * QP + pl) * Cfg::Q_PLANE + ch * BM * 128, &tmQ, q_full, ch * 64,
-                          row0 + t * BM, pl * c.B * c.H + static_cast<int>(blockIdx.z));
-      }
+      mbar_arrive_expect_tx(q_full, Cfg::Q_BYTES);
+      for (int t = 0; t < NT; ++t)
+        for (int pl = 0; pl < QP; ++pl)
+          for (int ch = 0; ch < Cfg::CH; ++ch)
+            tma_load_3d(sQ + (t * QP + pl) * Cfg::Q_PLANE + ch * BM * 128, &tmQ, q_full, ch * 64,
+                        row0 + t * BM, pl * c.B * c.H + bh);
       constexpr uint32_t idesc_s = make_idesc_f16(BM, BN, 0);
       constexpr uint32_t idesc_o = make_idesc_f16(BM, DH, 1);
       const uint32_t sQa = smem_u32(sQ), sKa = smem_u32(sK), sVa = smem_u32(sV);
@@ -825,14 +613,14 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
       }
       mma_commit(drain);
       mbar_wait_drain(drain, 0, KF_DEV_WAIT_TIMEOUT_MMA);
-      if (!SH) mbar_wait_drain(q_full, 0, KF_DEV_WAIT_TIMEOUT_MMA);
+      mbar_wait_drain(q_full, 0, KF_DEV_WAIT_TIMEOUT_MMA);
     }
-  } else if (warp > 8 || (LW == 7 && warp >= 4)) {
-    // -------------------------------------------------- loaders (3 or 7 warps)
-    // They expand a share of every tile each, without waiting for one
+  } else if (warp > 8) {
+    // -------------------------------------------------- loaders (3 warps)
+    // The three expand a third of every tile each, without waiting for one
     // another. Warp 9 also copies the raw K tiles, warp 10 the raw V tiles, and
     // warp 11 stages the scales, each half a step after the slot was read.
-    const int lt = tid - 9 * 32 + (warp < 8 ? 8 * 32 : 0);
+    const int lt = tid - 9 * 32;
     uint8_t* rawk = smem + Cfg::RAWK_OFF;
     uint8_t* rawv = smem + Cfg::RAWV_OFF;
     const int segs = BN >> c.p_shift;              // pages of a tile (1 to 8)
@@ -873,7 +661,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
     }
     load_entry(Cfg::RS + 1);
     int fetched = 0;                               // raw tiles asked for by this warp
-    if (warp == 9 || warp == 10) {
+    if (warp < 11) {
 #pragma unroll
       for (int i = 0; i < Cfg::RS; ++i)
         if (i < n_steps) {
@@ -884,7 +672,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
           ++fetched;
         }
     }
-    // The raw slot of step j is asked to hold step j + RS, once all loading warps
+    // The raw slot of step j is asked to hold step j + RS, once all three warps
     // have expanded step j.
     auto refill = [&](const uint8_t* pool, uint8_t* raw, uint64_t* full, uint64_t* empty, int j,
                       int page8) -> bool {
@@ -906,23 +694,6 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
             c.scale + 2 * (static_cast<int64_t>(page8) * c.H + h)));
     };
     if (warp == 11) load_scale(pg[0]);
-    if constexpr (SH) {
-      // the largest V scale, by the loading warps while the first copies come
-      for (int j = (k0 >> c.p_shift) + lt; (j << c.p_shift) < k1; j += 32 * LW) {
-        const int page = kv8_page(c, b, j);
-        if (page >= 0)
-          vmax = fmaxf(vmax, __ldg(c.scale + 2 * (static_cast<int64_t>(page) * c.H + h) + 1));
-      }
-#pragma unroll
-      for (int d = 16; d; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
-      if (lane == 0) s_vmax[warp] = vmax;
-      named_bar_sync(1, 32 * LW);
-      if (warp == 11) {
-#pragma unroll
-        for (int i = 12 - LW - (LW > 3 ? 1 : 0); i < 12; ++i)
-          if (i != 8) vmax = fmaxf(vmax, s_vmax[i]);
-      }
-    }
     const float inv_vmax = vmax > 0.f ? 1.f / vmax : 0.f;
     for (int j = 0; j < n_steps; ++j) {
       const int st = j & 1, slot = j % Cfg::RS;
@@ -933,9 +704,9 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
                     (j < 2 || mbar_wait(&k_empty[st], eph, abort_flag, KF_DEV_WAIT_TIMEOUT_TMA))))
         break;
       if (c.fmt == KF_KV8_INT8)
-        kv8_expand<DH, KF_KV8_INT8, false, 32 * LW>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
+        kv8_expand<DH, KF_KV8_INT8, false, 96>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
       else
-        kv8_expand<DH, KF_KV8_E4M3, false, 32 * LW>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
+        kv8_expand<DH, KF_KV8_E4M3, false, 96>(rawk + slot * Cfg::RAW, sK + st * Cfg::KV_BYTES, lt, 0, 0);
       fence_proxy_async_smem();
       if (warp == 11) {
         PromptScales& sc = s_sc[j & 3];
@@ -975,14 +746,14 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
         uint8_t* tile = sV + st * Cfg::KV_BYTES;
         if (c.fmt == KF_KV8_INT8) {
           if (whole)
-            kv8_expand<DH, KF_KV8_INT8, false, 32 * LW>(raw, tile, lt, 0, 0);
+            kv8_expand<DH, KF_KV8_INT8, false, 96>(raw, tile, lt, 0, 0);
           else
-            kv8_expand<DH, KF_KV8_INT8, true, 32 * LW>(raw, tile, lt, rows, bad);
+            kv8_expand<DH, KF_KV8_INT8, true, 96>(raw, tile, lt, rows, bad);
         } else {
           if (whole)
-            kv8_expand<DH, KF_KV8_E4M3, false, 32 * LW>(raw, tile, lt, 0, 0);
+            kv8_expand<DH, KF_KV8_E4M3, false, 96>(raw, tile, lt, 0, 0);
           else
-            kv8_expand<DH, KF_KV8_E4M3, true, 32 * LW>(raw, tile, lt, rows, bad);
+            kv8_expand<DH, KF_KV8_E4M3, true, 96>(raw, tile, lt, rows, bad);
         }
         fence_proxy_async_smem();
       }
@@ -998,7 +769,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
       pg[Cfg::RS] = take_entry();
       load_entry(j + Cfg::RS + 2);
     }
-    if ((warp == 9 || warp == 10) && lane == 0) {
+    if (warp < 11 && lane == 0) {
       // no copy may be in flight when the CTA leaves
       uint64_t* full = warp == 9 ? rk_full : rv_full;
       for (int j = fetched > Cfg::RS ? fetched - Cfg::RS : 0; j < fetched; ++j)
@@ -1009,48 +780,12 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
     const int t = warp >> 2;
     const int quarter = warp & 3;
     const int row = row0 + t * BM + quarter * 32 + lane;
-    int2 my_seq = make_int2(0, row);     // sequence (from b on) and row in it
-    bool live = false;                   // the row sees a key
-    int limit = 0;
-    float qf = 0.f;
-    if constexpr (!SH) {
-      const int len = kv8_len(c, b);
-      const int tok = row / G;
-      if (row < w.rows && tok < kv8_count(c, counts, b, T)) limit = causal ? min(len + tok + 1, end) : end;
-      qf = row < w.rows ? __ldg(w.qf + static_cast<int64_t>(blockIdx.z) * w.rows + row) : 0.f;
-    } else {
-      if (row < rows) {
-        my_seq = row_of(row);
-        live = my_seq.y / G < kv8_count(c, counts, b + my_seq.x, T);
-      }
-      const int tok = my_seq.y / G;
-      // Rows that are not there take all keys of a group like the others (their q is
-      // 0): masks cost a third of a step, and nothing of them is written.
-      if (gr.tiles > 0)
-        limit = end;
-      else if (live)
-        limit = causal ? min(kv8_len(c, b) + tok + 1, end) : end;
-      const int64_t base = !live ? -1
-                                 : (b + my_seq.x) * pq.sb +
-                                       static_cast<int64_t>(h * G + my_seq.y - tok * G) * pq.sh +
-                                       tok * pq.st;
-      uint8_t* tile = sQ + t * QP * Cfg::Q_PLANE;
-      if constexpr (QP == 2)
-        qf = prompt_put_q<DH, KF_DT_F32, QP, BM>(pq, base, tile, Cfg::Q_PLANE, quarter * 32);
-      else if (dtype == KF_DT_BF16)
-        qf = prompt_put_q<DH, KF_DT_BF16, QP, BM>(pq, base, tile, Cfg::Q_PLANE, quarter * 32);
-      else
-        qf = prompt_put_q<DH, KF_DT_F16, QP, BM>(pq, base, tile, Cfg::Q_PLANE, quarter * 32);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    }
-    const int tok = my_seq.y / G;
-    // A warp without a row that sees a key leaves P as it is: no other row reads it.
-    const bool idle = SH && !__any_sync(0xffffffffu, live);
-    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t t_o = t_lane + Cfg::O_COL + t * Cfg::O_STRIDE;
-    const uint32_t t_m = t_lane + Cfg::M_COL + t * Cfg::O_STRIDE;
+    const int tok = row / G;
+    const int limit = (row < w.rows && tok < count) ? (causal ? min(len + tok + 1, end) : end) : 0;
+    const float qf = row < w.rows ? __ldg(w.qf + static_cast<int64_t>(bh) * w.rows + row) : 0.f;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t t_o = t_row + Cfg::O_COL + t * Cfg::O_STRIDE;
+    const uint32_t t_m = t_row + Cfg::M_COL + t * Cfg::O_STRIDE;
     float ref = -INFINITY, sum = 0.f;
     bool ok = true, nan_k = false, nan_v = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -1071,20 +806,13 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
     for (int j = 0; j < n_steps; ++j) {
       const int st = j & 1;
       const int buf = NT == 1 ? st : t;
-      const uint32_t t_s = t_lane + buf * 128;
+      const uint32_t t_s = t_row + buf * 128;
       const uint32_t sph = NT == 1 ? (j >> 1) & 1 : j & 1;
       wait(&k_full[st], (j >> 1) & 1);
       wait(&s_full[buf], sph);
       __syncwarp();
       tc_fence_after();
       if (lane == 0 && ok) mbar_arrive(&k_empty[st]);
-      if (idle) {
-        if (Cfg::SEP && lane == 0 && ok) mbar_arrive(&s_free[t]);
-        if (Cfg::SEP && j > 0) wait(&o_done[t], (j - 1) & 1);
-        __syncwarp();
-        if (lane == 0 && ok) mbar_arrive(&p_full[buf]);
-        continue;
-      }
       // In place with two tiles, S of this step was issued after P V of the last
       // one, so O is at rest. Otherwise S runs ahead: wait for that product.
       auto at_rest = [&]() {
@@ -1179,7 +907,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
           hi[u] = pack_half2(x, y);
           if constexpr (PP == 2) lo[u] = pack_half2_rest(x, y, hi[u]);
         }
-        const uint32_t at = Cfg::SEP ? t_lane + Cfg::P_COL + t * 64 + part * 16
+        const uint32_t at = Cfg::SEP ? t_row + Cfg::P_COL + t * 64 + part * 16
                                      : t_s + (part >> 1) * 64 + (part & 1) * 16;
         tmem_st16(at, hi);
         if constexpr (PP == 2) tmem_st16(at + 32, lo);
@@ -1196,13 +924,7 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
     wait(&o_final[t], 0);
     if (__any_sync(0xffffffffu, ok)) {
       tc_fence_after();
-      if (SH && !live) sum = 0.f, ref = -INFINITY, nan_k = nan_v = false;
-      if constexpr (SH) {
-#pragma unroll
-        for (int i = 12 - LW - (LW > 3 ? 1 : 0); i < 12; ++i)
-          if (i != 8) vmax = fmaxf(vmax, s_vmax[i]);
-      }
-      const int64_t spot = spot_of(my_seq);
+      const int64_t at = static_cast<int64_t>(bh) * w.rows + row;
       const int hq = h * G + row - tok * G;
       const float nan = __uint_as_float(0x7fc00000u);
       if (nan_k) sum = nan;
@@ -1219,53 +941,28 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
 #pragma unroll
           for (int u = 0; u < 32; ++u) o[u] += m[u];
         }
-        constexpr int NC = DH < 32 ? DH : 32;
-        if constexpr (SH) {
-          // Through this warp's quarter of the tile's Q, which no product reads any
-          // more, so that eight lanes write 128 bytes of a row. (A row a lane: 15000
-          // clocks for 256 rows of 128.)
-          uint8_t* stage = sQ + t * QP * Cfg::Q_PLANE + quarter * 4096;
-#pragma unroll
-          for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<float4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-                sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                           : make_float4(o[4 * u] * f, o[4 * u + 1] * f, o[4 * u + 2] * f,
-                                         o[4 * u + 3] * f);
-          __syncwarp();
-          const int64_t mine = row < rows && ok ? spot : -1;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + (lane >> 3), piece = lane & 7;
-            const int64_t to = __shfl_sync(0xffffffffu, mine, r);
-            if (to >= 0 && 4 * piece < NC)
-              *reinterpret_cast<float4*>(w.part + (to * w.chunks + chunk) * DH + cc * 32 + 4 * piece) =
-                  *reinterpret_cast<const float4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
-          }
-          __syncwarp();
-          continue;
-        }
-        if (row >= rows || !ok) continue;
+        if (row >= w.rows || !ok) continue;
 #pragma unroll
         for (int u = 0; u < 32; ++u) o[u] = sum == 0.f ? 0.f : o[u] * f;
+        constexpr int NC = DH < 32 ? DH : 32;
         if (alone) {
           kv8_store_run<NC>(out, b * o_sb + hq * o_sh + tok * o_st + cc * 32, dtype, o_vec != 0, o);
         } else {
-          float4* p = reinterpret_cast<float4*>(w.part + (spot * w.chunks + chunk) * DH + cc * 32);
+          float4* p = reinterpret_cast<float4*>(w.part + (at * w.chunks + chunk) * DH + cc * 32);
 #pragma unroll
           for (int u = 0; u < NC; u += 4)
             p[u >> 2] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
         }
       }
-      if (row < rows && ok) {
+      if (row < w.rows && ok) {
         if (alone) {
           const float l2 = sum == 0.f ? -INFINITY : ref + log2f(sum);
           if (lse_out)
             lse_out[(static_cast<int64_t>(b) * c.H * G + hq) * T + tok] = l2 * 0.6931471805599453f;
-          if (w.lse) w.lse[spot] = l2;
+          if (w.lse) w.lse[at] = l2;
         } else {
-          w.ref[spot * w.chunks + chunk] = ref;
-          w.sum[spot * w.chunks + chunk] = sum;
-          if (SH && last_part) gr.used[spot] = chunk + 1;
+          w.ref[at * w.chunks + chunk] = ref;
+          w.sum[at * w.chunks + chunk] = sum;
         }
       }
     }
@@ -1273,19 +970,10 @@ __global__ void __launch_bounds__(PromptCfg<DH, QP, PP, TILES, SH>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if constexpr (SH) {
-    if (!more || *abort_flag) break;
-    __syncthreads();   // (the flag has been read)
-    if (tid == 0)
-      for (int i = 0; i < 28; ++i) mbar_inval(bars + i);
-    ++stretch;
-  }
-  }
   if (warp == 8) {
     __syncwarp();
-    tmem_dealloc(*tmem_slot, 512);
+    tmem_dealloc(tmem_base, 512);
   }
-  if constexpr (SH) kv8_end_of_pair(gr);
 }
 
 // ---------------------------------------------------------------- weights

@@ -70,15 +70,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
         raise TypeError(f"{what}: ended must be bool, got {ended.dtype}")
     if index != torch.cuda.current_device():
         raise RuntimeError(f"{what}: logits are on {logits.device}, which is not the current device")
-    dev = logits.device
-    score = torch.empty((B, n), dtype=torch.float32, device=dev)
-    beam = torch.empty((B, n), dtype=torch.int32, device=dev)
-    token = torch.empty((B, n), dtype=torch.int32, device=dev)
+    score = scores.new_empty((B, n))
+    beam = scores.new_empty((B, n), dtype=torch.int32)
+    token = torch.empty_like(beam)
     L = _lib.lib()
     need = L.kf_beam_select_workspace_bytes(B, K, V, n)
     if need < 0:
         raise _lib.KernelError(f"{what}: {L.kf_last_error().decode(errors='replace')}")
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    work = scores.new_empty(need, dtype=torch.uint8) if need else None
     sb, sk, _ = logits.stride()
     rc = L.kf_beam_select(
         logits.data_ptr(), sb, sk, code, scores.data_ptr(), scores.stride(0),
