@@ -447,14 +447,15 @@ int kf_kv8_evict(const kf_kv8_cache* cache, const int32_t* table_out, int64_t ld
  * document): group n is the sequences starts[n] .. starts[n + 1] - 1 (n_groups
  * + 1 ascending entries; a sequence in no group shares nothing), and the first
  * shared[n] tokens of its sequences lie on pages that their table rows name
- * alike (the first sequence's row is read). What counts is shared[n] cut to
- * whole pages, to max_shared and to the shortest of the group's lens. Those
- * tokens are read once for all rows of the group; the result is that of
- * kf_kv8_attention, but for rounding. max_shared, max_own: upper bounds, known
- * to the caller, of shared[n] and of the tokens that a sequence has besides
- * (lens[b] + counts[b] less what counts of shared[n]); 0: the table's reach. A
- * sequence that has more of its own is cut there and recorded in the device
- * status. KF_KV8_TRACK is refused. n_groups = 0: kf_kv8_attention with
+ * alike (the row of its first sequence with a new token is read). What counts is
+ * shared[n] cut to whole pages, to max_shared and to the shortest of the lens of the
+ * group's sequences with a new token; a sequence without one (counts[b] <= 0, a
+ * negative length) may hold anything. Those tokens are read once for all rows
+ * of the group; the result is that of kf_kv8_attention, but for rounding.
+ * max_shared, max_own: upper bounds, known to the caller, of shared[n] and of the
+ * tokens that a sequence with a new one has besides (lens[b] + counts[b] less what
+ * counts of shared[n]); 0: the table's reach. A sequence that has more of its own is
+ * cut there and recorded in the device status. KF_KV8_TRACK is refused. n_groups = 0: kf_kv8_attention with
  * max_len = max_own. At most 32767 groups. Other arguments as
  * kf_kv8_attention. */
 int kf_kv8_attention_shared(const kf_kv8_cache* cache, const void* q, int64_t q_sb, int64_t q_sh,

@@ -99,14 +99,25 @@ __device__ __forceinline__ int2 kv8_group(const KV8Groups& gr, int B, int n) {
   }
   return make_int2(a, z);
 }
-// Tokens that group n shares, of whole pages that all of its sequences hold. All
-// lanes of a warp call this together.
-__device__ __forceinline__ int kv8_group_tokens(const KV8& c, const KV8Groups& gr, int n, int2 seq) {
+// Tokens that group n shares (x), of whole pages that all of its sequences with a new
+// token hold, and the first such sequence (y), whose table row names the pages. (One
+// without a new token reads nothing: its length, 0 or negative in an idle place,
+// would leave the others without what they share.) All lanes of a warp call this
+// together.
+__device__ __forceinline__ int2 kv8_group_tokens(const KV8& c, const KV8Groups& gr,
+                                                 const int32_t* counts, int T, int n, int2 seq) {
   int s = __ldg(gr.shared + n);
   s = s < 0 ? 0 : min(s, gr.max_shared);
-  for (int b = seq.x + (threadIdx.x & 31); b < seq.y; b += 32) s = min(s, kv8_len(c, b));
+  int first = INT32_MAX;
+  for (int b = seq.x + (threadIdx.x & 31); b < seq.y; b += 32)
+    if (kv8_count(c, counts, b, T) > 0) {
+      s = min(s, kv8_len(c, b));
+      first = min(first, b);
+    }
   s = __reduce_min_sync(0xffffffffu, s);
-  return s & ~(c.P - 1);
+  first = __reduce_min_sync(0xffffffffu, first);
+  if (first == INT32_MAX) return make_int2(0, seq.x);
+  return make_int2(s & ~(c.P - 1), first);
 }
 // Query rows of a group's sequences: the rows of their new tokens one after
 // another, or where `live` is null `per` rows of each (with tokens past counts).
@@ -166,7 +177,8 @@ __device__ __forceinline__ KV8GroupTile kv8_group_tile(const KV8Groups& gr, int 
   return KV8GroupTile{-1, 0, 0, make_int2(0, 0)};
 }
 // Tokens that sequence b shares with its group (0: it is in none).
-__device__ __forceinline__ int kv8_shared_of(const KV8& c, const KV8Groups& gr, int b) {
+__device__ __forceinline__ int kv8_shared_of(const KV8& c, const KV8Groups& gr,
+                                             const int32_t* counts, int T, int b) {
   if (gr.of_seq) return __ldg(gr.of_seq + b);
   const int lane = threadIdx.x & 31;
   for (int base = 0; base < gr.N; base += 32) {
@@ -174,8 +186,9 @@ __device__ __forceinline__ int kv8_shared_of(const KV8& c, const KV8Groups& gr, 
     const uint32_t in = __ballot_sync(0xffffffffu, b >= seq.x && b < seq.y);
     if (in) {
       const int l = __ffs(static_cast<int>(in)) - 1;
-      return kv8_group_tokens(c, gr, base + l, make_int2(__shfl_sync(0xffffffffu, seq.x, l),
-                                                         __shfl_sync(0xffffffffu, seq.y, l)));
+      return kv8_group_tokens(c, gr, counts, T, base + l,
+                              make_int2(__shfl_sync(0xffffffffu, seq.x, l),
+                                        __shfl_sync(0xffffffffu, seq.y, l))).x;
     }
   }
   return 0;
@@ -455,7 +468,8 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
-  int chunk, row0, h, b;    // b: whose table row has the pages (the group's first sequence)
+  int chunk, row0, h, b;    // b: the sequence, or the group's first one
+  int pages_of;             // whose table row has the pages
   int rows;                 // rows that the tile is cut from
   int end;                  // no key is at or past it
   int limit[RH];            // the rows' own limits
@@ -466,6 +480,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     const int bh = blockIdx.z;
     b = bh / c.H;
     h = bh - b * c.H;
+    pages_of = b;
     rows = w.rows;
     const int len = kv8_len(c, b);
     const int count = kv8_count(c, counts, b, T);
@@ -500,7 +515,9 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
       row0 = tl.tile * KV8_ROWS;
       rows = tl.rows;
       // every row of a sequence that takes its token sees all that is shared
-      end = kv8_group_tokens(c, gr, tl.n, tl.seq);
+      const int2 common = kv8_group_tokens(c, gr, counts, T, tl.n, tl.seq);
+      end = common.x;
+      pages_of = common.y;
       k0 = chunk * gr.chunk;
       k1 = min(k0 + gr.chunk, end);
       if (end == 0) return;  // the sequences' own CTAs leave the empty parts
@@ -521,13 +538,14 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
       chunk = i % own;
       i /= own;
       b = i / gr.own_tiles;
+      pages_of = b;
       row0 = (i - b * gr.own_tiles) * KV8_ROWS;
       rows = w.rows;
-      const int shared = kv8_shared_of(c, gr, b);
+      const int shared = kv8_shared_of(c, gr, counts, T, b);
       const int len = kv8_len(c, b);
       const int count = kv8_count(c, counts, b, T);
       end = kv8_end(c, len, count);
-      if (end - shared > gr.max_own) {
+      if (count > 0 && end - shared > gr.max_own) {
         if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
         end = shared + gr.max_own;
       }
@@ -569,7 +587,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
   const int j0 = k0 >> c.p_shift;
   float vmax = 0.f;
   for (int j = j0 + tid; (j << c.p_shift) < k1; j += 128) {
-    const int page = kv8_page(c, b, j);
+    const int page = kv8_page(c, pages_of, j);
     s_page[j - j0] = page;
     float2 s = make_float2(0.f, 0.f);
     if (page >= 0) s = *reinterpret_cast<const float2*>(c.scale + 2 * (static_cast<int64_t>(page) * c.H + h));
@@ -1015,8 +1033,13 @@ __global__ void __launch_bounds__(KV8_GROUPS_THREADS)
   if (live && tid == 0) live[0] = 0;
   __syncthreads();
   for (int n = warp; n < gr.N; n += WARPS) {
-    const int2 seq = kv8_group(gr, c.B, n);
-    const int shared = seq.x < seq.y ? kv8_group_tokens(c, gr, n, seq) : 0;
+    int2 seq = kv8_group(gr, c.B, n);
+    int shared = 0;
+    if (seq.x < seq.y) {
+      const int2 common = kv8_group_tokens(c, gr, counts, T, n, seq);
+      shared = common.x;
+      seq.x = common.y;    // (sequences before it have no row that is joined)
+    }
     const int rows = live ? (live[seq.y] - live[seq.x]) * G : (seq.y - seq.x) * per;
     if (lane == 0) group[n] = s_g[n] = make_int4(shared, rows, seq.x, seq.y);
     if (shared)

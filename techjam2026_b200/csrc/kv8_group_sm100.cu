@@ -237,9 +237,9 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
   }
   bool more = gr.tiles == 0 || at < stop;
   while (more) {
-  int b, h, chunk, row0, rows;   // b: whose table row has the pages (the group's first sequence)
+  int b, h, chunk, row0, rows;   // b: whose table row has the pages (the group's first with a new token)
   int end, k0, k1;
-  int2 seq = make_int2(0, 0);    // the group's sequences
+  int2 seq = make_int2(0, 0);    // the group's sequences from b on
   bool last_part = false;        // no CTA has later keys of this tile
   if (gr.tiles > 0) {
     int4 g = begin_g;
@@ -283,11 +283,11 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
     b = i / gr.own_tiles;
     row0 = (i - b * gr.own_tiles) * Cfg::ROWS;
     rows = w.rows;
-    const int shared = kv8_shared_of(c, gr, b);
+    const int shared = kv8_shared_of(c, gr, counts, T, b);
     const int len = kv8_len(c, b);
     const int count = kv8_count(c, counts, b, T);
     end = kv8_end(c, len, count);
-    if (end - shared > gr.max_own) {
+    if (count > 0 && end - shared > gr.max_own) {
       if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
       end = shared + gr.max_own;
     }

@@ -360,12 +360,14 @@ def kv8_attention_shared(q: torch.Tensor, cache: KV8Cache, starts: torch.Tensor,
                 starts[n + 1] - 1. A sequence in no group shares nothing
     shared      int32 [N]: how many leading tokens of its sequences lie on pages
                 that their table rows name alike. Cut to whole pages, and to the
-                shortest of the group's lens (new tokens are not shared)
+                shortest of the group's lens (new tokens are not shared). A
+                sequence without a new token does not count: it may hold anything
     max_shared  an upper bound of shared known to the caller (0: what the table
                 can hold); what is beyond it is read sequence by sequence
-    max_own     an upper bound of the tokens of a sequence, new ones among them,
-                besides those (0: what the table can hold). A sequence with more
-                is cut there and recorded in the device status word
+    max_own     an upper bound of the tokens of a sequence that has a new one, new
+                ones among them, besides those (0: what the table can hold). A
+                sequence with more is cut there and recorded in the device status
+                word
 
     The other arguments, what is returned and which rows are 0 as for
     kv8_attention. There is no weight record to add to: it belongs to the pages,

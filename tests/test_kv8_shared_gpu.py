@@ -244,6 +244,42 @@ def test_a_sequence_of_a_negative_length_holds_nothing():
     assert ((out.double() - want).abs() <= tol)[[0, 1, 2, 4]].all()
 
 
+@pytest.mark.parametrize("kind,dim", [(F32, 32), (BF16, 64), (F16, 128)])
+@pytest.mark.parametrize("members,T", [(5, 1), (40, 1), (6, 9), (12, 9), (4, 100)])
+@pytest.mark.parametrize("idle", [[0], [2], [0, 1, 3]])
+def test_members_without_a_new_token_take_nothing_from_the_others(idle, members, T, kind, dim):
+    """Idle members of a group: of length 0, of a negative one, with more tokens of
+    their own than the bound and a table row that names no page. The others have what
+    they share, under bounds that just hold."""
+    own = [(7 * b) % 20 for b in range(members + 3)]
+    for i in idle:
+        own[i] = 90
+    cache, starts, shared = make_groups([members, 3], [320, 64], own, dim=dim, block=16, room=T)
+    counts = [1 + (5 * b) % T for b in range(members + 3)]
+    for i in idle:
+        counts[i] = 0
+    counts = ints(counts)
+    append(cache, T, counts)
+    bounds = dict(max_shared=320, max_own=19 + T)
+    q = queries(cache, 4, T, kind)
+    check(cache, starts, shared, q, counts, **bounds)
+    cache.table[idle] = -1
+    check(cache, starts, shared, q, counts, **bounds)
+    cache.lens[idle] = 0
+    want = check(cache, starts, shared, q, counts, **bounds)
+    cache.lens[idle] = -3
+    out = ops.kv8_attention_shared(q, cache, starts, shared, counts=counts, **bounds)
+    assert status() == 6
+    assert torch.equal(out, want) and not out[idle].any()
+
+
+def test_a_group_of_idle_members_only():
+    cache, starts, shared = make_groups([3, 2], [160, 64], [200, 100, 3, 4, 5], block=16)
+    counts = ints([0, 0, 0, 1, 1])
+    append(cache, 1, counts)
+    check(cache, starts, shared, queries(cache, 2, 1), counts, max_shared=160, max_own=6)
+
+
 def test_strided_views_and_out():
     cache, starts, shared = make_groups([3], [80], [3, 0, 30], heads=2, dim=32, block=16, room=9)
     append(cache, 7)
