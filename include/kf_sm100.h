@@ -473,8 +473,10 @@ int64_t kf_kv8_attention_shared_workspace_bytes(const kf_kv8_cache* cache, int d
  * one, the weight record. tokens (null: whole pages): only the first tokens[i]
  * slots are copied, with the scales; the others stay as they are (tokens[i] <=
  * 0: nothing is copied). `layers` caches of one geometry are copied in one
- * call: from and into are arrays of that many. A pair src[i] == dst[i] within one
- * pool is no copy. A pair is not done, and is recorded in the device status, if
+ * call: from and into are arrays of that many. They are one pool in every layer, or
+ * two in every layer; tensors that are written may have no memory in common with one
+ * another, whatever the layer, nor those of two pools with what is read
+ * (KF_E_INVALID). A pair src[i] == dst[i] within one pool is no copy. A pair is not done, and is recorded in the device status, if
  * an entry is no page of its pool, or if its dst[i] is the dst of another pair
  * or, within one pool, the src of another one (pairs that copy nothing do not
  * count). `workspace`: kf_kv8_copy_workspace_bytes(...) bytes, 16-byte aligned (0

@@ -13,9 +13,12 @@
 // us for 2.1 GB, 6.2 TB/s (0.95); 8 half full pages of 6 layers, 5 us of a call of 19.
 #include "kv8_common.cuh"
 
+#include <algorithm>
+
 namespace kf {
 
 constexpr int KV8_COPY_THREADS = 256;
+constexpr int KV8_COPY_MOST = 256;       // layers of a call
 constexpr int KV8_COPY_LAYERS = 32;      // layers of a launch
 constexpr int KV8_COPY_SCAN = 512;       // pairs that every CTA looks through
 
@@ -128,6 +131,46 @@ static bool kv8_alike(const KV8& a, const KV8& b) {
   return a.H == b.H && a.D == b.D && a.P == b.P && a.fmt == b.fmt;
 }
 
+// Whether a tensor that the call writes has memory in common with another one that
+// it writes, or with one that it reads (within one pool: but for the same tensor of
+// the same layer). The pairs are checked for clashes within a tensor only, so the
+// result would depend on the order of CTAs.
+struct KV8Range {
+  uintptr_t at, end;
+  bool written;
+};
+static bool kv8_copy_overlaps(const KV8CopyLayers* at, int64_t layers, bool same, const KV8& from,
+                              const KV8& into) {
+  KV8Range all[8 * KV8_COPY_MOST];
+  int64_t n = 0;
+  auto add = [&](const void* p, int64_t bytes, bool written) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    if (bytes > 0) all[n++] = {a, a + static_cast<uintptr_t>(bytes), written};
+  };
+  const int64_t codes = static_cast<int64_t>(from.H) * from.P * from.D;
+  auto pool = [&](const void* k, const void* v, const void* scale, const void* weight, int64_t pages,
+                  bool written) {
+    add(k, pages * codes, written);
+    add(v, pages * codes, written);
+    add(scale, pages * from.H * 8, written);
+    if (weight) add(weight, pages * from.H * from.P * 4, written);
+  };
+  for (int64_t i = 0; i < layers; ++i) {
+    const KV8CopyLayer& l = at[i / KV8_COPY_LAYERS].at[i % KV8_COPY_LAYERS];
+    const bool record = l.weight && l.weight_to;
+    pool(l.k_to, l.v_to, l.scale_to, record ? l.weight_to : nullptr, into.pages, true);
+    if (!same) pool(l.k, l.v, l.scale, record ? l.weight : nullptr, from.pages, false);
+  }
+  std::sort(all, all + n, [](const KV8Range& a, const KV8Range& b) { return a.at < b.at; });
+  uintptr_t end = 0, end_written = 0;   // of what began earlier
+  for (int64_t i = 0; i < n; ++i) {
+    if (all[i].at < (all[i].written ? end : end_written)) return true;
+    end = std::max(end, all[i].end);
+    if (all[i].written) end_written = std::max(end_written, all[i].end);
+  }
+  return false;
+}
+
 }  // namespace kf
 
 using namespace kf;
@@ -146,13 +189,13 @@ extern "C" int kf_kv8_copy(const kf_kv8_cache* const* from, const kf_kv8_cache* 
                            const int32_t* tokens, int64_t n, void* workspace,
                            int64_t workspace_bytes, void* stream) {
   const char* what = "kf_kv8_copy";
-  if (layers < 0 || layers > 256 || n < 0 || n > (1LL << 29) || (layers && (!from || !into))) {
+  if (layers < 0 || layers > KV8_COPY_MOST || n < 0 || n > (1LL << 29) || (layers && (!from || !into))) {
     set_last_error("%s: needs 0 <= layers <= 256, their caches, and 0 <= n <= 2^29", what);
     return KF_E_INVALID;
   }
   if (layers == 0) return KF_OK;
   KV8 first, first_to;
-  KV8CopyLayers at[256 / KV8_COPY_LAYERS];
+  KV8CopyLayers at[KV8_COPY_MOST / KV8_COPY_LAYERS];
   bool same = false;
   for (int64_t i = 0; i < layers; ++i) {
     KV8 a, b;
@@ -185,6 +228,10 @@ extern "C" int kf_kv8_copy(const kf_kv8_cache* const* from, const kf_kv8_cache* 
   const int64_t need = n <= KV8_COPY_SCAN ? 0 : first_to.pages * 4;
   if (need && (!workspace || workspace_bytes < need || !kv8_aligned(workspace, 16))) {
     set_last_error("%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
+    return KF_E_INVALID;
+  }
+  if (kv8_copy_overlaps(at, layers, same, first, first_to)) {
+    set_last_error("%s: a tensor that is written occurs twice, or is read too", what);
     return KF_E_INVALID;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);

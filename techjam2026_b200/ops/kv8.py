@@ -438,7 +438,9 @@ def kv8_copy(cache: Caches, src: torch.Tensor, dst: torch.Tensor,
     tokens    int32 [n] (default whole pages): only the first tokens[i] slots
               are copied, with the scales; the others stay as they are
     into      the caches whose pages dst are (default: the same ones); another
-              pool, of any number of pages
+              pool, of any number of pages. A tensor that is written may not
+              occur twice in a call, nor be read by it (but for copies within a
+              pool)
 
     A pair is not done, and recorded in the device status word (code 6), if an
     entry is no page of its pool, or if another pair writes the same page or,

@@ -125,6 +125,41 @@ def test_copy_refuses_bad_arguments(lib):
     assert call([], []) == 0 and call([one], [one], n=0) == 0
 
 
+def test_copy_refuses_tensors_that_it_would_write_twice_or_read_as_well(lib):
+    """8 pages of 2 heads of 16 x 64 codes: 16384 bytes of K and of V, 128 of scales,
+    1024 of the record."""
+    kind = ctypes.POINTER(_lib.KV8CacheStruct)
+
+    def pool(n, **kw):
+        base = (n + 1) << 20
+        f = dict(k=base, v=base + 0x10000, scale=base + 0x20000, weight=base + 0x30000)
+        f.update(kw)
+        return struct(**f)
+
+    def refused(a, b):
+        x = (kind * len(a))(*map(ctypes.pointer, a))
+        y = (kind * len(b))(*map(ctypes.pointer, b))
+        rc = lib.kf_kv8_copy(x, y, len(a), FAKE, FAKE, None, 1, None, 0, None)
+        return rc == _lib.KF_E_INVALID
+
+    p = [pool(n) for n in range(4)]
+    assert refused([p[0], p[1]], [p[1], p[0]])                   # layers the other way round
+    assert refused([p[0], p[1]], [p[1], p[2]])                   # read by another layer
+    assert refused([p[0], p[1]], [p[2], p[2]])                   # written twice
+    assert refused([p[0], p[0]], [p[0], p[0]])
+    far = [pool(n) for n in range(40)]
+    assert refused(far[:20] + [p[0]], far[20:] + [far[39]])      # (the list may be long)
+    for name, size in (("k", 16384), ("v", 16384), ("scale", 128), ("weight", 1024)):
+        at = getattr(p[0], name)
+        # one tensor in common, or the end of one and the beginning of another
+        for where in (at, at + size - 16, at - size + 16):
+            assert refused([p[0]], [pool(3, **{name: where})]), name
+            assert refused([p[1], p[2]], [p[0], pool(3, **{name: where})]), name
+    # the record of one pool over the codes of the other
+    assert refused([p[0]], [pool(3, weight=p[0].k)])
+    assert refused([pool(3, weight=p[0].k)], [p[0]])
+
+
 def test_beam_select_refuses_bad_arguments(lib):
     def call(logits=FAKE, dtype=0, scores=FAKE, batch=1, beams=2, vocab=10, n=2, pad=0, out=FAKE,
              work=FAKE, size=1 << 20):

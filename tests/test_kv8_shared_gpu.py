@@ -525,6 +525,32 @@ def test_copies_of_nothing_and_refusals():
         ops.kv8_copy(from_[0], ints([0]), ints([1]), into=half)
 
 
+def test_pools_that_lie_side_by_side_or_are_read_twice():
+    """Views of one allocation, one cache read for two layers, and a record that only
+    one side keeps: nothing that is written is written or read elsewhere."""
+    whole = pools(1, 30, 2, 16, 32, I8, True)[0]
+
+    def part(a, z, weight=True):
+        return ops.KV8Cache(whole.k[a:z], whole.v[a:z], whole.scale[a:z], whole.table, whole.lens,
+                            whole.weight[a:z] if weight else None)
+
+    check_copy([part(0, 10)], [part(10, 20)], [3, 4], [0, 9])
+    check_copy([part(0, 10), part(0, 10)], [part(10, 20), part(20, 30)], [1, 2], [5, 6], [16, 7])
+    one = ops.KV8Cache(whole.k[:10], whole.v[:10], whole.scale[:10], whole.table, whole.lens)
+    two = ops.KV8Cache(whole.k[10:20], whole.v[10:20], whole.scale[10:20], whole.table, whole.lens,
+                       whole.weight[:10])
+    record = whole.weight.clone()
+    ops.kv8_copy(one, ints([7]), ints([2]), into=two)
+    assert torch.equal(whole.k[12], whole.k[7]) and torch.equal(whole.weight, record)
+    assert status() == 0
+    for from_, into in (([part(0, 10)], [part(9, 19)]), ([part(0, 10)] * 2, [part(10, 20)] * 2),
+                        ([part(0, 10), part(10, 20)], [part(10, 20), part(0, 10)]),
+                        ([part(0, 10)] * 2, None)):
+        with pytest.raises(_lib.KernelError):
+            ops.kv8_copy(from_, ints([1]), ints([2]), into=into)
+    assert status() == 0
+
+
 def test_copies_in_a_graph_and_without_a_record():
     from_ = pools(3, 30, 2, 32, 32, I8, True)
     into = pools(3, 30, 2, 32, 32, I8, False, seed=4)
