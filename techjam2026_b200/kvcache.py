@@ -141,29 +141,49 @@ class PagePool:
                 self.free.append(p)
 
     def _group(self) -> None:
-        """Consecutive sequences that begin with the same page, and how many
-        leading tokens (of whole pages) each such group shares."""
+        """Groups of consecutive sequences that begin with the same pages, and how
+        many leading tokens (of whole pages) each group shares. A sequence that has
+        little in common with its neighbours does not join them: what a group shares
+        is what all of it does."""
         self.groups = None
         if max(self.uses, default=0) < 2:
             return
-        starts, shared, of = [0], [], []
-        for i, row in enumerate(self.rows):
-            one = i and row and self.rows[i - 1] and row[0] == self.rows[i - 1][0]
-            if i and not one:
-                starts.append(i)
-            of.append(len(starts) - 1)
+        starts, common, run = [], [], []
+        for i in range(1, len(self.rows) + 1):
+            both = self._common(i, run[-1] if run else 0) if i < len(self.rows) else 0
+            if both:
+                run.append(both)
+                continue
+            at = i - 1 - len(run)         # sequences that begin with one page: from here on
+            for m, n in _cut(run):
+                starts.append(at)
+                common.append(n)
+                at += m
+            run = []
         starts.append(len(self.rows))
-        for a, z in zip(starts, starts[1:]):
-            n = 0
-            if z - a > 1:
-                n = sum(1 for _ in itertools.takewhile(lambda pages: len(set(pages)) == 1,
-                                                       zip(*self.rows[a:z])))
-            shared.append(n * self.block)
+        shared = [n * self.block for n in common]
+        of = [n for n, (a, z) in enumerate(zip(starts, starts[1:])) for _ in range(z - a)]
         if not any(shared):
             return
         dev = self.table.device
         self.groups = (torch.tensor(starts, dtype=torch.int32).to(dev),
                        torch.tensor(shared, dtype=torch.int32).to(dev), [shared[n] for n in of])
+
+    def _common(self, i: int, guess: int) -> int:
+        """Leading pages that sequences i - 1 and i have in common."""
+        a, b = self.rows[i - 1], self.rows[i]
+        lo, hi = 0, min(len(a), len(b))
+        if guess < hi and a[guess] != b[guess]:
+            hi = guess                    # (siblings have what the pair before them has)
+        if a[:hi] == b[:hi]:
+            return hi
+        while hi - lo > 1:                # a[:lo] == b[:lo], a[:hi] != b[:hi]
+            mid = (lo + hi) // 2
+            if a[lo:mid] == b[lo:mid]:
+                lo = mid
+            else:
+                hi = mid
+        return lo
 
     def _upload(self) -> None:
         host = torch.zeros(self.table.shape, dtype=torch.int32)
@@ -171,6 +191,30 @@ class PagePool:
             host[i, :len(row)] = torch.tensor(row, dtype=torch.int32)
         self.table.copy_(host)
         self._group()
+
+
+def _cut(both: List[int]) -> List[Tuple[int, int]]:
+    """Groups (members, pages that all of them share) of consecutive sequences of
+    which neighbours have these numbers of leading pages in common. Reading them by
+    groups saves (members - 1) * pages reads. One group of all, or what a pass along
+    them finds better: a sequence joins the group before it, begins one, or takes
+    the sequence before it along into a new one, as saves most."""
+    if not both:
+        return [(1, 0)]
+    groups = [(2, both[0])]
+    for b in both[1:]:
+        m, n = groups[-1]
+        join = m * min(n, b) if m > 1 else b
+        along = (m - 2) * n + b if m > 1 else 0
+        if join >= max((m - 1) * n, along):
+            groups[-1] = (m + 1, min(n, b) if m > 1 else b)
+        elif along > (m - 1) * n:
+            groups[-1:] = [(m - 1, n if m > 2 else 0), (2, b)]
+        else:
+            groups.append((1, 0))
+    if sum((m - 1) * n for m, n in groups) > len(both) * min(both):
+        return groups
+    return [(len(both) + 1, min(both))]
 
 
 class CachedStack:

@@ -127,6 +127,59 @@ def test_random_histories_keep_the_books():
                 assert all(each[i] == n <= held[i] for i in range(a, z))
 
 
+def rows_that_share(common, own=2, block=16):
+    """A pool in which row i has common[i] leading pages in common with row i - 1."""
+    B, blocks = len(common), max(common) + own + 1
+    pool = PagePool(pages=B * blocks, batch=B, blocks=blocks, block=block, device="cpu")
+    rows = [pool.take(blocks)]
+    for n in common[1:]:
+        rows.append(rows[-1][:n] + pool.take(blocks - n))
+    pool.replace(rows)
+    consistent(pool)
+    return pool
+
+
+@pytest.mark.parametrize("common,starts,shared", [
+    ([0, 10, 10, 1], [0, 3, 4], [10, 0]),           # the last one has only the beginning
+    ([0, 1, 10, 10], [0, 1, 4], [0, 10]),           # the first one
+    ([0, 10, 10, 1, 10, 10], [0, 3, 6], [10, 10]),  # two prompts behind one beginning
+    ([0, 10, 9, 10], [0, 4], [9]),                  # nearly the same: one group
+    ([0, 3, 0, 5], [0, 2, 4], [3, 5]),
+    ([0, 2, 2, 2, 9], [0, 3, 5], [2, 9]),           # 4 * 2 or 2 * 2 + 9 reads saved
+    ([0, 5, 11, 6, 5], [0, 5], [5]),                # 4 * 5 or 11 and less
+    ([0, 0, 4], [0, 1, 3], [0, 4]),
+])
+def test_a_sequence_with_little_in_common_takes_nothing_from_a_group(common, starts, shared):
+    pool = rows_that_share(common)
+    assert pool.groups[0].tolist() == starts
+    assert pool.groups[1].tolist() == [16 * n for n in shared]
+    assert pool.groups[2] == [16 * n for (a, z), n in zip(zip(starts, starts[1:]), shared)
+                              for _ in range(z - a)]
+
+
+def test_groups_save_at_least_as_much_as_one_for_each_first_page():
+    """Against groups of all consecutive rows that begin with one page."""
+    rng = random.Random(1)
+    for _ in range(500):
+        common = [0] + [rng.choice([0, 1, 2, 3, 5, 6, 8, 11]) for _ in range(rng.randint(1, 9))]
+        pool = rows_that_share(common)
+        saved = 0
+        if pool.groups is not None:
+            starts, shared = pool.groups[0].tolist(), pool.groups[1].tolist()
+            for a, z, n in zip(starts, starts[1:], shared):
+                assert len({tuple(r[:n // 16]) for r in pool.rows[a:z]}) == 1
+                assert z - a > 1 or n == 0
+                saved += (z - a - 1) * n // 16
+        plain, run = 0, []
+        for n in common[1:] + [0]:
+            if n:
+                run.append(n)
+            else:
+                plain += len(run) * min(run, default=0)
+                run = []
+        assert saved >= plain
+
+
 @pytest.mark.parametrize("argv", [["--beams", "129"], ["--beams", "-1"],
                                   ["--beams", "2", "--vocab", "3"]])
 def test_the_example_refuses_beams_it_cannot_run(argv, capsys):
