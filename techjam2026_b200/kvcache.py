@@ -35,6 +35,7 @@ import torch
 from .model import LayerStack
 from .ops import (KV8Cache, add_mask_layernorm, beam_select, kv8_append, kv8_attention,
                   kv8_attention_shared, kv8_copy, kv8_evict, linear)
+from .ops.beam import MAX_TAKE
 from .ops.kv8 import HEAD_DIMS
 
 
@@ -409,12 +410,13 @@ def beam_search(model: CachedStack, prompts: torch.Tensor, lengths: Sequence[int
                 end: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The `beams` best continuations of each prompt that beam search finds.
 
-    model    a CachedStack of N * beams sequences that hold nothing, without a
-             budget; prompt n has the sequences n * beams and following
+    model    a CachedStack of N * beams sequences that hold nothing, beams at most
+             128, without a budget; prompt n has the sequences n * beams and following
     prompts  [N, T, d] float32 embeddings, prompt n of lengths[n] >= 1 tokens
     embed    [V, d] float32, the embedding of each token
     head     [V, d] float32, the output projection
-    steps    tokens to generate; a beam that takes the token `end` stays as it is
+    steps    tokens to generate, with the prompts at most what the model's sequences
+             hold and one; a beam that takes the token `end` stays as it is
 
     Returns (tokens [N, beams, steps] int32, scores [N, beams] float32: the sums of
     the tokens' log probabilities), best first. A beam that ended is filled with
@@ -426,6 +428,11 @@ def beam_search(model: CachedStack, prompts: torch.Tensor, lengths: Sequence[int
     if len(lengths) != N or steps < 1 or any(not 0 < n <= prompts.shape[1] for n in lengths):
         raise ValueError("beam_search: needs a length of at least 1 for each prompt, and steps")
     dev, V = prompts.device, head.shape[0]
+    reach = model.pool.table.shape[1] * model.pool.block
+    if not 0 < beams <= MAX_TAKE or max(lengths, default=0) + steps - 1 > reach \
+            or not (end is None or 0 <= end < V):
+        raise ValueError(f"beam_search: needs 1 to {MAX_TAKE} beams, prompts that leave room for "
+                         f"{steps} steps within {reach} tokens, and an end below {V}")
     first = [n * beams for n in range(N)]
     out = model(prompts, counts=lengths, rows=first)
     last = out[torch.arange(N, device=dev), torch.tensor(lengths, device=dev) - 1]

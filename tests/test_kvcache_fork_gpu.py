@@ -177,6 +177,24 @@ def test_refusals():
         beam_search(model, tokens(1, 4), [4], embed, embed, 2, 1)
 
 
+def test_a_search_that_cannot_be_done_is_refused_before_it_begins():
+    """Too many beams, no room for the tokens, an end outside the vocabulary: the
+    model holds nothing afterwards."""
+    stack = stack_of(layers=1)
+    embed = torch.randn(8, 128, generator=torch.Generator().manual_seed(0)).cuda()
+    many = CachedStack(stack, 129, 32, block=16)
+    with pytest.raises(ValueError):
+        beam_search(many, tokens(1, 4), [4], embed, embed, 129, 2)
+    model = CachedStack(stack, 2, 32, block=16)
+    for T, steps, end in ((32, 2, None), (20, 14, None), (4, 2, 8), (4, 2, -1)):
+        with pytest.raises(ValueError):
+            beam_search(model, tokens(1, T), [T], embed, embed, 2, steps, end)
+    for m in (many, model):
+        assert not any(m.held) and not m.lens.any() and not any(m.pool.uses)
+    out, _ = beam_search(model, tokens(1, 20), [20], embed, embed, 2, 13)    # just fits
+    assert out.shape == (1, 2, 13) and max(model.held) == 32
+
+
 def test_the_example_searches(capsys):
     main(["--config", "c1", "--beams", "3", "--tokens", "4", "--vocab", "100"])
     assert "3 beams" in capsys.readouterr().out
