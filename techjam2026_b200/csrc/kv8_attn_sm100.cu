@@ -109,11 +109,15 @@ __device__ __forceinline__ int2 kv8_group_tokens(const KV8& c, const KV8Groups& 
   int s = __ldg(gr.shared + n);
   s = s < 0 ? 0 : min(s, gr.max_shared);
   int first = INT32_MAX;
-  for (int b = seq.x + (threadIdx.x & 31); b < seq.y; b += 32)
-    if (kv8_count(c, counts, b, T) > 0) {
-      s = min(s, kv8_len(c, b));
+  for (int b = seq.x + (threadIdx.x & 31); b < seq.y; b += 32) {
+    // (a length beyond the table's reach, which max_shared is within, is recorded by
+    // the sequence's own tokens)
+    const int len = __ldg(c.lens + b), count = counts ? __ldg(counts + b) : T;
+    if (len >= 0 && count > 0) {
+      s = min(s, len);
       first = min(first, b);
     }
+  }
   s = __reduce_min_sync(0xffffffffu, s);
   first = __reduce_min_sync(0xffffffffu, first);
   if (first == INT32_MAX) return make_int2(0, seq.x);
@@ -545,8 +549,8 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
       const int len = kv8_len(c, b);
       const int count = kv8_count(c, counts, b, T);
       end = kv8_end(c, len, count);
-      if (count > 0 && end - shared > gr.max_own) {
-        if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
+      if (end - shared > gr.max_own) {
+        if (tid == 0 && count > 0) record_device_status(KF_DEV_BAD_KV_PAGE);
         end = shared + gr.max_own;
       }
 #pragma unroll

@@ -445,10 +445,10 @@ static int kv8_shared_plan(const char* what, const KV8& c, int dtype, int64_t T,
   return KF_OK;
 }
 
-template <int DH, int QP, int PP, int TILES>
+template <int DH, int QP, int PP, int TILES, bool OWN>
 static cudaError_t kv8_shared_tc(const KV8& c, const KV8Call& a, const KV8Work& w) {
   using Cfg = GroupCfg<DH, QP, PP, TILES>;
-  auto kern = kv8_group_kernel<DH, QP, PP, TILES>;
+  auto kern = kv8_group_kernel<DH, QP, PP, TILES, OWN>;
   static DeviceOnce once;
   cudaError_t attr = cudaSuccess;
   once.run("kf_kv8_attention_shared", nullptr, [&](int) {
@@ -456,18 +456,24 @@ static cudaError_t kv8_shared_tc(const KV8& c, const KV8Call& a, const KV8Work& 
     return attr == cudaSuccess ? KF_OK : KF_E_CUDA;
   });
   if (attr != cudaSuccess) return attr;
-  dim3 grid(static_cast<unsigned>(c.B * a.gr.own_tiles * (w.chunks - a.gr.chunks)),
-            static_cast<unsigned>(c.H));
-  if (a.gr.tiles > 0) grid = dim3(static_cast<unsigned>(sm_count()));
+  dim3 grid(static_cast<unsigned>(sm_count()));
+  if constexpr (OWN)
+    grid = dim3(static_cast<unsigned>(c.B * a.gr.own_tiles * (w.chunks - a.gr.chunks)),
+                static_cast<unsigned>(c.H));
   const GroupQ q = {a.q, a.q_sb, a.q_sh, a.q_st, a.q_vec16, a.scale_log2};
   return launch_chained(kern, grid, dim3(Cfg::THREADS), Cfg::SMEM, a.st, c, a.dtype, a.counts, a.T, a.G,
                         a.flags, w, q, a.gr);
 }
+template <int DH, int QP, int PP, int TILES>
+static cudaError_t kv8_shared_side(const KV8& c, const KV8Call& a, const KV8Work& w) {
+  return a.gr.tiles > 0 ? kv8_shared_tc<DH, QP, PP, TILES, false>(c, a, w)
+                        : kv8_shared_tc<DH, QP, PP, TILES, true>(c, a, w);
+}
 template <int DH, int QP, int PP>
 static cudaError_t kv8_shared_tiles(const KV8& c, const KV8Call& a, const KV8Work& w, int tiles) {
   if constexpr (group_tiles(DH, QP) == 2)
-    if (tiles == 2) return kv8_shared_tc<DH, QP, PP, 2>(c, a, w);
-  return kv8_shared_tc<DH, QP, PP, 1>(c, a, w);
+    if (tiles == 2) return kv8_shared_side<DH, QP, PP, 2>(c, a, w);
+  return kv8_shared_side<DH, QP, PP, 1>(c, a, w);
 }
 template <int DH>
 static cudaError_t kv8_shared_type(const KV8& c, const KV8Call& a, const KV8Work& w, int tiles) {

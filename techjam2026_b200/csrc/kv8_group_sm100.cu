@@ -145,16 +145,17 @@ __device__ __forceinline__ float group_put_q(const GroupQ& q, int64_t base, uint
   return mine * q.scale_log2;
 }
 
-// gr.tiles > 0: the shared tokens. A CTA an SM takes an equal share of all steps ([group][row tiles][kv
+// The shared tokens: a CTA an SM takes an equal share of all steps ([group][row tiles][kv
 // head][128 keys]), one or more stretches of keys of row tiles; a row tile's
 // parts are the CTAs that had some of its steps. (Grids of parts of a fixed size
 // ended in a wave of few CTAs: ragged questions on two documents of 8k to 16k
-// tokens 234 us for the whole call, this 212.) A step takes 2500 clocks with one tile,
+// tokens 234 us for the whole call, this 213.) A step takes 2500 clocks with one tile,
 // 4600 with two, 6300 to 7200 at head_dim 128 with two planes of P; a stretch's start and
 // end 30000 to 50000, most of it code that is fetched as it first runs. Measured: 64 rows x
-// 4 heads against 32k tokens, 8 kv heads of 128, fp16: 85 us. Otherwise the own tokens: y is the kv head and x [sequence][row
-// tiles][part].
-template <int DH, int QP, int PP, int TILES>
+// 4 heads against 32k tokens, 8 kv heads of 128, fp16: 85 us.
+// OWN: the own tokens; y is the kv head and x [sequence][row tiles][part]. (One body
+// that chooses at run time spills more: 226 us for the questions.)
+template <int DH, int QP, int PP, int TILES, bool OWN>
 __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
     kv8_group_kernel(KV8 c, int dtype, const int32_t* __restrict__ counts, int T, int G, int flags,
                      KV8Work w, GroupQ pq, KV8Groups gr) {
@@ -220,13 +221,13 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (gr.tiles > 0 || !gr.paired) pdl_wait();
+  if (!OWN) pdl_wait();
   pdl_launch_dependents();  // every CTA that runs holds its TMEM by now
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
   int64_t at = 0, stop = 1, share = 1;   // this CTA's steps of the shared tokens
   int stretch = 0;                       // stretches of keys done
   int4 begin_g = make_int4(0, 0, 0, 0), begin = begin_g;
-  if (gr.tiles > 0) {
+  if constexpr (!OWN) {
     begin_g = __ldg(gr.record + 2 * blockIdx.x);
     begin = __ldg(gr.record + 2 * blockIdx.x + 1);
     const int64_t all = __ldg(gr.work + gr.N);
@@ -235,13 +236,13 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
     at = blockIdx.x * share;
     stop = min(at + share, all);
   }
-  bool more = gr.tiles == 0 || at < stop;
+  bool more = OWN || at < stop;
   while (more) {
   int b, h, chunk, row0, rows;   // b: whose table row has the pages (the group's first with a new token)
   int end, k0, k1;
   int2 seq = make_int2(0, 0);    // the group's sequences from b on
   bool last_part = false;        // no CTA has later keys of this tile
-  if (gr.tiles > 0) {
+  if constexpr (!OWN) {
     int4 g = begin_g;
     int item = begin.x, step = begin.y, steps = begin.z;
     chunk = begin.w;
@@ -283,12 +284,12 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
     b = i / gr.own_tiles;
     row0 = (i - b * gr.own_tiles) * Cfg::ROWS;
     rows = w.rows;
-    const int shared = kv8_shared_of(c, gr, counts, T, b);
+    const int shared = __ldg(gr.of_seq + b);
     const int len = kv8_len(c, b);
     const int count = kv8_count(c, counts, b, T);
     end = kv8_end(c, len, count);
-    if (count > 0 && end - shared > gr.max_own) {
-      if (tid == 0) record_device_status(KF_DEV_BAD_KV_PAGE);
+    if (end - shared > gr.max_own) {
+      if (tid == 0 && count > 0) record_device_status(KF_DEV_BAD_KV_PAGE);
       end = shared + gr.max_own;
     }
     const int last_row = min(row0 + Cfg::ROWS, rows) - 1;
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
   // Sequence (from b on) and row within it of a row, and where its numbers are:
   // [B * H][rows of a sequence].
   auto row_of = [&](int row) -> int2 {
-    return gr.tiles > 0 ? kv8_group_row(gr, seq, w.rows, G, row) : make_int2(0, row);
+    return !OWN ? kv8_group_row(gr, seq, w.rows, G, row) : make_int2(0, row);
   };
   auto spot_of = [&](int2 at) -> int64_t {
     return static_cast<int64_t>((b + at.x) * c.H + h) * w.rows + at.y;
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
   const int n_steps = (k1 - k0 + BN - 1) / BN;
 
   float vmax = 0.f;  // the largest V scale of the range
-  if (stretch) {
+  if (!OWN && stretch) {
     if (tid == 0) set_up_barriers();
     __syncthreads();
   }
@@ -654,7 +655,7 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
       const int tok = my_seq.y / G;
       // Rows that are not there take all keys of a group like the others (their q is
       // 0): masks cost a third of a step, and nothing of them is written.
-      if (gr.tiles > 0)
+      if (!OWN)
         limit = end;
       else if (live)
         limit = causal ? min(kv8_len(c, b) + tok + 1, end) : end;
@@ -833,7 +834,9 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
       float f = vmax;  // not used where sum is 0
       if (nan_v) f = nan;
       const bool have_m = QP == 2 && n_steps > Cfg::FLUSH;
-#pragma unroll
+      // (head_dim 64: rolled, since it runs once a stretch and its code has to be fetched,
+      // 216 -> 213 us for questions on two documents; at 128 121 -> 124 for a long one)
+#pragma unroll(DH > 64 ? 4 : 1)
       for (int cc = 0; cc < (DH + 31) / 32; ++cc) {
         float o[32];
         tmem_ld32(t_o + cc * 32, o);
@@ -886,7 +889,7 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
     __syncwarp();
     tmem_dealloc(*tmem_slot, 512);
   }
-  kv8_end_of_pair(gr);
+  if (OWN) pdl_wait();
 }
 
 }  // namespace kf
