@@ -70,6 +70,8 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 // scheduled, and waits for its predecessor grid to complete (memory
 // visible) before it reads anything the predecessor wrote. The next
 // kernel's launch and set-up then overlap this kernel's tail.
+// One kernel differs: that of a group's own tokens (kv8_begin_of_pair) waits at its
+// end, and the kernel before it signals only after its own wait.
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

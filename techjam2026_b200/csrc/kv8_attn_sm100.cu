@@ -87,7 +87,6 @@ struct KV8Groups {
   const int32_t* of_seq;  // [B]: tokens that a sequence shares
   int32_t* used;          // [B * H][rows]: parts of the shared tokens that a row has
   int least;              // steps of a part, at least
-  bool paired;            // the kernel of the own tokens follows that of the shared ones
 };
 
 // The sequences of group n; none (recorded) where starts is out of order.
@@ -198,11 +197,26 @@ __device__ __forceinline__ int kv8_shared_of(const KV8& c, const KV8Groups& gr,
   return 0;
 }
 
-// The kernel of the own tokens starts without waiting for that of the shared
-// ones, which waited for everything earlier before it let it start. It ends
-// after it, so that the join has to wait for one kernel.
-__device__ __forceinline__ void kv8_end_of_pair(const KV8Groups& gr) {
-  if (gr.tiles == 0 && gr.paired) pdl_wait();
+// The kernel of the own tokens (gr.tiles = 0) runs beside that of the shared ones: it
+// begins without waiting for it, and ends after it, so that the join has to wait for
+// one kernel. What it reads besides is complete by then: the shared kernel's CTAs
+// signal only after their own wait, when all that ran before (the groups' lists, q,
+// the cache) has ended and is visible to them, and the own kernel's CTAs start after
+// all of those signals. A grid is promised to see such writes at its wait only, so
+// each of its threads begins with a fence at the GPU's scope, which leaves nothing
+// older in its SM's L1 cache for its reads, and not with a wait, which
+// would run the two kernels one after the other (64 samples 30.6 -> 36.4 us, uneven
+// groups 94 -> 100, questions 222 -> 234; the fence costs 0.3 us of the 64 samples' 31,
+// and nothing that shows elsewhere).
+__device__ __forceinline__ void kv8_begin_of_pair(bool own) {
+  if (own)
+    __threadfence();
+  else
+    pdl_wait();
+  pdl_launch_dependents();   // (only now: see above)
+}
+__device__ __forceinline__ void kv8_end_of_pair(bool own) {
+  if (own) pdl_wait();
 }
 // Empty parts in the places of the shared tokens, or none, for rows that share
 // nothing.
@@ -461,14 +475,11 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
   extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ float s_ref[4][KV8_ROWS], s_sum[4][KV8_ROWS];
   __shared__ int2 s_row[SH ? KV8_ROWS : 1];
-  // The kernel of the own tokens alone runs beside that of the shared ones
-  // (kv8_end_of_pair).
   if constexpr (!SH) {
     pdl_launch_dependents();
     pdl_wait();
   } else {
-    if (gr.tiles > 0 || !gr.paired) pdl_wait();
-    pdl_launch_dependents();
+    kv8_begin_of_pair(gr.tiles == 0);
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
@@ -585,7 +596,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
         w.ref[at] = -INFINITY;
         w.sum[at] = 0.f;
       }
-    if constexpr (SH) kv8_end_of_pair(gr);
+    if constexpr (SH) kv8_end_of_pair(gr.tiles == 0);
     return;
   }
   const int j0 = k0 >> c.p_shift;
@@ -851,7 +862,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
       }
     }
   }
-  if constexpr (SH) kv8_end_of_pair(gr);
+  if constexpr (SH) kv8_end_of_pair(gr.tiles == 0);
 }
 
 // ---------------------------------------------------------------- join

@@ -437,7 +437,6 @@ static int kv8_shared_plan(const char* what, const KV8& c, int dtype, int64_t T,
   w->rows = static_cast<int>(per);
   w->ld_score = 0;
   w->prompt = false;       // (no planes: the kernel reads q itself)
-  gr->paired = true;
   if (tiles * gr->chunks + c.B * own_tiles * own_chunks > INT32_MAX) {
     set_last_error("%s: too many rows and keys for one call", what);
     return KF_E_UNSUPPORTED;

@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
   uint64_t* rk_full = bars + 18;  // [RS] raw codes of K, of V: their bytes
   uint64_t* rv_full = bars + 20;  // [RS]
   uint64_t* s_free = bars + 22;   // [2] S read into registers (P apart), 4 warps
-  uint64_t* rk_empty = bars + 24; // [RS] raw codes expanded by the three warps
+  uint64_t* rk_empty = bars + 24; // [RS] raw codes expanded by the loading warps
   uint64_t* rv_empty = bars + 26; // [RS]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -221,8 +221,7 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (!OWN) pdl_wait();
-  pdl_launch_dependents();  // every CTA that runs holds its TMEM by now
+  kv8_begin_of_pair(OWN);   // (every CTA that runs holds its TMEM by now)
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
   int64_t at = 0, stop = 1, share = 1;   // this CTA's steps of the shared tokens
   int stretch = 0;                       // stretches of keys done
@@ -889,7 +888,7 @@ __global__ void __launch_bounds__(GroupCfg<DH, QP, PP, TILES>::THREADS, 1)
     __syncwarp();
     tmem_dealloc(*tmem_slot, 512);
   }
-  if (OWN) pdl_wait();
+  kv8_end_of_pair(OWN);
 }
 
 }  // namespace kf

@@ -348,6 +348,53 @@ def test_repeated_calls_graphs_and_streams_give_the_same_bits(members, T):
     assert status() == 0
 
 
+@pytest.mark.parametrize("members,T,group", [(5, 1, 1), (5, 3, 8), (40, 1, 4), (40, 2, 2), (3, 50, 2)])
+def test_what_is_written_just_before_a_call_is_read_by_all_of_its_kernels(members, T, group):
+    """q, lengths, counts, table, scales and groups change between calls that nothing
+    waits between; each is as the same call alone."""
+    cache, starts, shared = make_groups([members, 4], [640, 64], [30 + b % 9 for b in range(members + 4)],
+                                        block=16, room=T)
+    append(cache, T)
+    B = members + 4
+    g = torch.Generator().manual_seed(7)
+    own = cache.table[:, 40:].clone()
+    counts = ints([T] * B)
+    q = queries(cache, group, T, BF16)
+    held = [t.clone() for t in (q, cache.lens, cache.table, cache.scale)]
+    states = []
+    for i in range(12):
+        lens = cache.lens - torch.randint(0, 25, (B,), generator=g, dtype=torch.int32).cuda()
+        table = cache.table.clone()
+        order = torch.randperm(members, generator=g).cuda()
+        table[:members, 40:] = own[order]
+        scale = cache.scale * (0.5 + torch.rand(cache.scale.shape, generator=g).cuda())
+        cut = int(torch.randint(0, members + 1, (1,), generator=g))
+        states.append((q * (1 + i % 3), lens, table, scale,
+                       torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32).cuda(),
+                       ints([0, cut, B if i % 2 else members]), ints([640, 64 if i % 2 else 320])))
+    live = (q, cache.lens, cache.table, cache.scale, counts, starts, shared)
+
+    def call(state):
+        for to, x in zip(live, state):
+            to.copy_(x)
+        return ops.kv8_attention_shared(q, cache, starts, shared, counts=counts, return_lse=True)
+
+    alone = []
+    for state in states:
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in call(state)])
+        torch.cuda.synchronize()
+    for _ in range(3):
+        got = [call(state) for state in states]
+        for (out, lse), (want, want_lse) in zip(got, alone):
+            # (bits, since a row of the table may name a page that was never written, NaN)
+            assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+            assert torch.equal(lse.view(torch.int32), want_lse.view(torch.int32))
+    for to, x in zip(live, held):
+        to.copy_(x)
+    assert status() == 0
+
+
 def test_refusals():
     cache, starts, shared = make_groups([2], [16], [1, 2], block=16, heads=2)
     q = queries(cache, 1, 1)
