@@ -156,6 +156,45 @@ def test_waits_that_run_out_end_the_call_and_the_next_is_right(members, T, kind,
     assert status() == 0
 
 
+@pytest.mark.parametrize("kind,dim", [(BF16, 64), (BF16, 128), (F16, 32), (F16, 128), (F32, 64),
+                                      (F32, 128)])
+@pytest.mark.parametrize("sizes,T", [([80, 3], 1), ([150, 3], 1), ([6, 3], 100),
+                                     ([70, 1, 40, 0, 55, 64], 4)])
+def test_waits_that_run_out_are_recorded(sizes, T, kind, dim):
+    """With a limit of one cycle some wait gives up in every configuration of the
+    tensor-memory kernel (more than 64 rows a group on average, of one tile, of two,
+    of ragged chunks); with longer ones it is one of a later step, or of a later
+    stretch of a CTA that has several (the last sizes: 16 heads of 230 sequences are
+    more tiles than processors). The next call is right."""
+    L = _lib.lib()
+    many = len(sizes) > 2
+    shared = [640, 576, 64, 128, 64, 1280] if many else [1216, 640]
+    B = sum(sizes)
+    cache, starts, shared = make_groups(sizes, shared, [b % 19 for b in range(B)], dim=dim, block=64,
+                                        dtype=F8, heads=16 if many else 3, room=T)
+    append(cache, T)
+    q = queries(cache, 2, T, kind)
+    good = ops.kv8_attention_shared(q, cache, starts, shared)
+    assert status() == 0
+    seen = {}
+    try:
+        for limit in (1, 1, 1, 500, 3000, 10000, 40000):
+            _lib.check(L.kf_set_wait_limit(limit), "kf_set_wait_limit")
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            ops.kv8_attention_shared(q, cache, starts, shared)
+            end.record()
+            torch.cuda.synchronize()
+            assert begin.elapsed_time(end) < 1000
+            seen.setdefault(limit, set()).add(status())
+    finally:
+        L.kf_set_wait_limit(0)
+    assert all(codes <= {0, 1, 2, 4} for codes in seen.values()), seen
+    assert seen[1] & {1, 2, 4}, seen
+    assert torch.equal(ops.kv8_attention_shared(q, cache, starts, shared), good)
+    assert status() == 0
+
+
 def test_what_counts_as_shared_is_cut():
     """shared is cut to whole pages, to the shortest of the group's lens and to
     max_shared; the result is that of kv8_attention whatever it says."""
