@@ -496,10 +496,12 @@ int64_t kf_kv8_copy_workspace_bytes(const kf_kv8_cache* from, const kf_kv8_cache
  * with the logarithm's sum in fp32 and the rest in fp64. A beam with
  * ended[b, k] != 0 (uint8, may be null) has one candidate: (k, pad) with its
  * score unchanged. Per row the n largest candidates, largest first (of equal
- * ones the lowest k * V + v): out_score fp32, out_beam and out_token int32
+ * ones the lowest k * V + v; but a beam's own n best tokens are chosen by their logits,
+ * so where two differ by less than the candidates' last place, the larger one is among
+ * them): out_score fp32, out_beam and out_token int32
  * [batch, n]. Candidates that are -inf or NaN are none (a logit of +inf or NaN
  * makes its beam's candidates NaN); entries without a candidate get -inf, -1, -1. 1 <= n <= 128, beams <=
- * 1024, vocab < 2^31. `workspace`: at least kf_beam_select_workspace_bytes bytes,
+ * 1024, batch * beams <= 65535, vocab < 2^31. `workspace`: at least kf_beam_select_workspace_bytes bytes,
  * 16-byte aligned; calls that overlap on the GPU must not share it. No
  * reference counterpart. */
 int kf_beam_select(const void* logits, int64_t l_sb, int64_t l_sk, int dtype, const float* scores,

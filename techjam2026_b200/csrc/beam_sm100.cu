@@ -105,11 +105,15 @@ __device__ __forceinline__ void beam_best(Key* list, int count, int n, Put&& put
 // of the others stays short without any barrier in the loop. Where it does not
 // (many equal logits, or logits that grow along the slice), the slice is read
 // again in small rounds that cut the list as it fills.
-// What bounds it: issue. A logit takes four instructions of the sum (and an
-// exponential, 16 a clock and SM); as many more go to 16-byte runs that hold a token above
-// the bound, 2 % of them, which is every second run of a warp. Measured: 64 x 8 rows
-// of 128000 bf16 logits, 62 us for 124 MB (floor 19; with a barrier and a list of all
-// candidates in every round 138); 24 x 8 rows of 50021 fp32 logits, 35 MB, about 20 us.
+// What bounds it: latency. 64 x 8 rows of 128000 bf16 logits take 62 us for 124 MB (floor
+// 19; with a barrier and a list of all candidates in every round 138): a quarter
+// of the copy rate, 58 % of the issue slots while an SM has work (17 instructions
+// a logit: four and an exponential of its sum, the rest the appends of 16-byte runs
+// with a token above the bound, 2 % of the runs but every second one of a warp, with 22
+// of 32 lanes active) and 35 % of the exponentials' pipe. Six warps a scheduler
+// wait 2.5 cycles an issue on fixed latencies and 2.4 on loads: a round's are asked for
+// when the last one is summed, not before. 512 CTAs on 148 SMs leave some with three
+// of four. 24 x 8 rows of 50021 fp32 logits, 35 MB, about 20 us.
 
 template <int DT>
 __device__ __forceinline__ void beam_load(const void* logits, int64_t base, int64_t i, int64_t last,

@@ -344,7 +344,7 @@ struct KV8SharedPlan {
   KV8Work w;
   bool tc_shared, tc_own;  // the tensor-memory kernel takes the shared, the own tokens
   int tiles, own_tiles;    // its tiles of 128 rows a CTA
-  bool packed;             // the rows of new tokens are listed first (kv8_live_kernel)
+  bool packed;             // the rows of new tokens are listed first (kv8_groups_kernel)
 };
 
 static int kv8_shared_plan(const char* what, const KV8& c, int dtype, int64_t T, int64_t q_heads,

@@ -330,7 +330,8 @@ class CachedStack:
             kv8_append(cache, k, v, counts=new)
             ctx = torch.empty((B, T, self.heads, self.head_dim), device=x.device)
             if groups is not None:
-                # (cut by the shortest sequence, so its other tokens may be more than `own`)
+                # (every sequence of a group holds all that it shares: only full pages are
+                # common, so nothing is cut and `own` bounds the rest)
                 kv8_attention_shared(q, cache, groups[0], groups[1], counts=new,
                                      max_shared=max(groups[2]), max_own=own,
                                      out=ctx.permute(0, 2, 1, 3))

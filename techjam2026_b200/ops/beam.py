@@ -38,7 +38,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
 
     Returns (scores [B, n] float32, beams [B, n] int32, tokens [B, n] int32),
     best first; of equal candidates the one of the lowest beam, then token. They
-    are compared in 64 bits (the softmax's sum is one of float32 values).
+    are compared in 64 bits (the softmax's sum is one of float32 values). Which
+    tokens of a beam are among its n best is decided by their logits: of two that
+    differ but give equal candidates, the larger logit comes first there.
     Candidates that are -inf or NaN are none; a logit of +inf or NaN leaves its beam
     without candidates. Where there are fewer than n, the rest is (-inf, -1, -1)."""
     what = "beam_select"
