@@ -581,10 +581,12 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
       chunk += gr.chunks;
     }
   }
-  // Where a row's numbers are: [B * H][rows of a sequence]
-  auto spot = [&](int row) -> int64_t {
-    if constexpr (!SH) return static_cast<int64_t>(blockIdx.z) * w.rows + row;
-    const int2 at = s_row[SH ? row - row0 : 0];
+  // Where a row's numbers are: [B * H][rows of a sequence]. The row comes in parts, each
+  // added in 64 bits: with sums in 32 the compiler holds other values, and a token of 64
+  // ragged sequences with the record takes 43.1 us instead of 42.5.
+  auto spot = [&](auto... row) -> int64_t {
+    if constexpr (!SH) return (static_cast<int64_t>(blockIdx.z) * w.rows + ... + row);
+    const int2 at = s_row[SH ? (row + ...) - row0 : 0];
     return static_cast<int64_t>((b + at.x) * c.H + h) * w.rows + at.y;
   };
   const bool alone = w.chunks == 1;
@@ -592,7 +594,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     // nothing here: the join reads this chunk's sums all the same
     for (int r = tid; r < KV8_ROWS; r += 128)
       if (row0 + r < rows) {
-        const int64_t at = spot(row0 + r) * w.chunks + chunk;
+        const int64_t at = spot(row0, r) * w.chunks + chunk;
         w.ref[at] = -INFINITY;
         w.sum[at] = 0.f;
       }
@@ -703,7 +705,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
 #pragma unroll
       for (int r = 0; r < RH; ++r)
         if (row0 + g + 8 * r < w.rows) {
-          float* sp = w.score + spot(row0 + g + 8 * r) * w.ld_score + key + 2 * t;
+          float* sp = w.score + spot(row0, g, 8 * r) * w.ld_score + key + 2 * t;
           *reinterpret_cast<float2*>(sp) = make_float2(f[0][2 * r], f[0][2 * r + 1]);
           *reinterpret_cast<float2*>(sp + 8) = make_float2(f[1][2 * r], f[1][2 * r + 1]);
         }
