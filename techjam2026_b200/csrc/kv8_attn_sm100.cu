@@ -457,16 +457,23 @@ __device__ __forceinline__ void score_tile(const QFrag<DH, QP, RH>& q, const KBy
   }
 }
 
-// QP, PP: fp16 planes of q and of P. SH: the call has groups; y is then the kv head,
-// and the CTAs (x) are [row tile of a group][part of its shared tokens] (none if
-// gr.tiles is 0), then [sequence][row tile][part of its own tokens].
-template <int DH, int FMT, int QP, int PP, int RH, bool SH>
+template <class T>
+__device__ __forceinline__ const T& kv8_the(const T& one) {
+  return one;
+}
+
+// QP, PP: fp16 planes of q and of P. SH: the call has groups, one KV8Groups (a pack, since
+// a parameter that plain calls do not need costs each 0.3 us of host); y is then the kv
+// head, and the CTAs (x) are [row tile of a group][part of its shared tokens] (none if
+// its tiles are 0), then [sequence][row tile][part of its own tokens].
+template <int DH, int FMT, int QP, int PP, int RH, class... Groups>
 __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     kv8_split_kernel(KV8 c, const void* __restrict__ q, int64_t q_sb, int64_t q_sh, int64_t q_st,
                      void* __restrict__ out, int64_t o_sb, int64_t o_sh, int64_t o_st, int dtype,
                      int vec, const int32_t* __restrict__ counts, int T, int G, int max_len,
                      float scale_log2, int flags, float* __restrict__ lse_out, KV8Work w,
-                     KV8Groups gr) {
+                     Groups... groups) {
+  constexpr bool SH = sizeof...(Groups) > 0;
   constexpr int NT = DH / 8;  // n8 tiles of the output
   __shared__ int s_page[KV8_CHUNK_MAX / 16];
   __shared__ float s_ks[KV8_CHUNK_MAX / 16];
@@ -479,7 +486,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     pdl_launch_dependents();
     pdl_wait();
   } else {
-    kv8_begin_of_pair(gr.tiles == 0);
+    kv8_begin_of_pair(kv8_the(groups...).tiles == 0);
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const bool causal = (flags & KF_KV8_CAUSAL) != 0;
@@ -520,6 +527,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
     k0 = chunk * w.chunk;
     k1 = min(k0 + w.chunk, reach);
   } else {
+    const KV8Groups& gr = kv8_the(groups...);
     h = blockIdx.y;
     int i = blockIdx.x;
     if (i < gr.tiles * gr.chunks) {
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
         w.ref[at] = -INFINITY;
         w.sum[at] = 0.f;
       }
-    if constexpr (SH) kv8_end_of_pair(gr.tiles == 0);
+    if constexpr (SH) kv8_end_of_pair(kv8_the(groups...).tiles == 0);
     return;
   }
   const int j0 = k0 >> c.p_shift;
@@ -864,7 +872,7 @@ __global__ void __launch_bounds__(128, SplitCfg<DH>::min_blocks(QP))
       }
     }
   }
-  if constexpr (SH) kv8_end_of_pair(gr.tiles == 0);
+  if constexpr (SH) kv8_end_of_pair(kv8_the(groups...).tiles == 0);
 }
 
 // ---------------------------------------------------------------- join

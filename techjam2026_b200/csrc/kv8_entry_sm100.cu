@@ -150,9 +150,9 @@ struct KV8Call {
   KV8Groups gr;                      // N = 0: no groups
 };
 
-template <int DH, int FMT, int QP, int PP, int RH, bool SH>
-static cudaError_t kv8_split(const KV8& c, const KV8Call& a, const KV8Work& w) {
-  auto kern = kv8_split_kernel<DH, FMT, QP, PP, RH, SH>;
+template <int DH, int FMT, int QP, int PP, int RH, class... Groups>
+static cudaError_t kv8_split(const KV8& c, const KV8Call& a, const KV8Work& w, const Groups&... gr) {
+  auto kern = kv8_split_kernel<DH, FMT, QP, PP, RH, Groups...>;
   constexpr int smem = SplitCfg<DH>::SMEM;
   static DeviceOnce once;
   cudaError_t attr = cudaSuccess;
@@ -164,21 +164,20 @@ static cudaError_t kv8_split(const KV8& c, const KV8Call& a, const KV8Work& w) {
   dim3 grid(static_cast<unsigned>(w.chunks),
             static_cast<unsigned>((w.rows + KV8_ROWS - 1) / KV8_ROWS),
             static_cast<unsigned>(c.B * c.H));
-  if constexpr (SH)
+  if constexpr (sizeof...(Groups) > 0)
     grid = dim3(static_cast<unsigned>(a.gr.tiles * a.gr.chunks +
                                       c.B * a.gr.own_tiles * (w.chunks - a.gr.chunks)),
                 static_cast<unsigned>(c.H));
   return launch_chained(kern, grid, dim3(128), smem, a.st, c, a.q, a.q_sb, a.q_sh, a.q_st, a.out,
                         a.o_sb, a.o_sh, a.o_st, a.dtype, a.q_vec, a.counts, a.T, a.G, a.max_len,
-                        a.scale_log2, a.flags, a.lse, w, a.gr);
+                        a.scale_log2, a.flags, a.lse, w, gr...);
 }
 template <int DH, int FMT, int QP, int PP>
 static cudaError_t kv8_split_rows(const KV8& c, const KV8Call& a, const KV8Work& w, bool half) {
   if (a.gr.N > 0)
-    return half ? kv8_split<DH, FMT, QP, PP, 1, true>(c, a, w)
-                : kv8_split<DH, FMT, QP, PP, 2, true>(c, a, w);
-  return half ? kv8_split<DH, FMT, QP, PP, 1, false>(c, a, w)
-              : kv8_split<DH, FMT, QP, PP, 2, false>(c, a, w);
+    return half ? kv8_split<DH, FMT, QP, PP, 1>(c, a, w, a.gr)
+                : kv8_split<DH, FMT, QP, PP, 2>(c, a, w, a.gr);
+  return half ? kv8_split<DH, FMT, QP, PP, 1>(c, a, w) : kv8_split<DH, FMT, QP, PP, 2>(c, a, w);
 }
 // fp16 outputs show one plane's rounding of P (1.4 times their own error), bf16
 // ones do not. The second plane costs (us, one / two): a token of 4 rows a kv
